@@ -224,6 +224,78 @@ NxrtStatus nxrt_rocm_matmul_nbits_set_block_acc_probe(NxrtRocmMatMulNBits* kerne
  * keeps until it is released, because a HIP graph recorded earlier may still replay through them. */
 uint64_t nxrt_rocm_matmul_nbits_retired_buffers(const NxrtRocmMatMulNBits* kernel);
 
+/* ---- operators beside MatMulNBits: what stands between the quantized products of a decoder layer ---- */
+
+/* One node of one of the operators below. The contract is that of a MatMulNBits kernel: tensors contiguous and on the provider's GPU, an absent optional
+ * tensor has data = NULL, calls run on the provider's stream in call order, one call at a time per node. No node copies or remembers its weights. Outputs may not overlap inputs unless said so. A node
+ * keeps a reference on its provider. Calls may be recorded into a graph; a call that needs scratch takes the caller's workspace or the node's own,
+ * which an eager call of that height has to have made before (nothing is allocated while a capture is open). Outgrown scratch stays until the node is released. */
+typedef struct NxrtRocmNode NxrtRocmNode;
+
+/* com.microsoft::QMoE with activation_type "swiglu" (or "silu" with fc3): a mixture-of-experts layer over 4-bit weights, from router logits to the weighted sum.
+ *   inputs: 0 input [.., H] Float16 / BFloat16; 1 router_probs [.., E] logits of any float type; 2 fc1_experts_weights [E, F, kb, block_size / 2] (or
+ *           [E, F, kb * block_size / 2]) Uint8, 3 fc1_scales [E, F, kb], 4 fc1_experts_bias [E, F] or absent; 5, 6, 7 the same of fc2 ([E, H, ..] over I);
+ *           8, 9, 10 of fc3 or absent; 11, 12, 13 zero points [E, F, ceil(kb / 2)] of fc1, fc2, fc3 or absent (8; fc1's come with fc3's).
+ *           Packing is MatMulNBits's; scales of the input's type or Float32, all alike, as are the biases.
+ *   output: [.., H] of the input's type.
+ *   swiglu_fusion 1: F = 2 I, gate and up rows alternate; 2: I gate rows, then I up rows; 0: F = I, gate in fc1 and up in fc3.
+ * For token t: p = softmax(logits); S = the k experts of the largest logits, the lowest index first among equal ones, without those whose p is 0; w = p, or p over
+ * its sum on S with normalize_routing_weights. h = g sigmoid(activation_alpha g) (u + activation_beta), g <= swiglu_limit, |u| <= swiglu_limit (g, u: the
+ * products with bias), rounded to the input's type; y = sum over S of w (fc2 h + bias), summed in f32. A row whose logits are all -inf (padding) gives zeros and
+ * reads no expert; a NaN or +inf among a row's logits gives NaN. An infinity or NaN in a row of `input` gives no finite value in that row.
+ * block_size: a power of two >= 32. E <= 1024, k <= 64. Weights start at multiples of 16 bytes. */
+typedef struct NxrtRocmQMoEAttrs {
+  uint32_t struct_size;
+  uint32_t present;      /* bit i: 0 k (default 1), 1 block_size (required), 2 expert_weight_bits (4), 3 normalize_routing_weights (0), 4 swiglu_fusion (0),
+                            5 activation_alpha (1), 6 activation_beta (0), 7 swiglu_limit (none) */
+  int64_t k, block_size, expert_weight_bits, normalize_routing_weights, swiglu_fusion;
+  double activation_alpha, activation_beta, swiglu_limit;
+} NxrtRocmQMoEAttrs;
+int nxrt_rocm_ep_supports_qmoe(const NxrtRocmEp* ep, const NxrtRocmQMoEAttrs* attrs, const NxrtTensorDesc* inputs, uint32_t n_inputs, char* reason, size_t reason_len);
+NxrtStatus nxrt_rocm_qmoe_create(NxrtRocmEp* ep, const NxrtRocmQMoEAttrs* attrs, NxrtRocmNode** out_node);
+
+/* MatMulInt8: Y = (codes of A) B^T with a scale per token and per output channel.
+ *   inputs: 0 A [.., K] Float32 / Float16 / BFloat16, or its Int8 codes; 1 B [N, K] Int8; 2 b_scale [N] of a float type; 3 a_scale [rows] Float32: with codes, and
+ *           only then; 4 bias, absent, [N], or of Y's shape (a residual), of a float type.
+ *   output: Y [.., N] of a float type.
+ * Codes of a row: scale = max|a| / 127, code = a / scale to the nearest, ties to even; a row of zeros has scale 0. A row that holds an infinity or a NaN gives NaN.
+ * Integer sums are exact. K < 131072. B starts at a multiple of 16 bytes where K is one of 16, else anywhere. */
+typedef struct NxrtRocmMatMulInt8Attrs {
+  uint32_t struct_size;
+  uint32_t present;      /* bit i: 0 K, 1 N: both required */
+  int64_t K, N;
+} NxrtRocmMatMulInt8Attrs;
+int nxrt_rocm_ep_supports_matmul_int8(const NxrtRocmEp* ep, const NxrtRocmMatMulInt8Attrs* attrs, const NxrtTensorDesc* inputs, uint32_t n_inputs, char* reason, size_t reason_len);
+NxrtStatus nxrt_rocm_matmul_int8_create(NxrtRocmEp* ep, const NxrtRocmMatMulInt8Attrs* attrs, NxrtRocmNode** out_node);
+
+/* GatedResidualNorm: the norm behind a block, its gate, the scaled residual stream, and the norm before the next block.
+ *   inputs: 0 residual [.., H] Float32 / Float16 / BFloat16; 1 block [.., H] of the same type, or absent; 2 post_gamma [H] or absent (then no norm behind the
+ *           block); 3 gate [H], or [G, H] with G dividing the rows (row r has gate r / (rows / G)), or absent; 4 pre_gamma [H] or absent (1); 5 pre_beta [H] or
+ *           absent; 6 post_beta [H] or absent. Weights of the residual's type or Float32.
+ *   outputs: 0 Z [.., H] of the residual's type or absent; 1 N [.., H] of that type, or Int8, or absent; 2 n_scale [rows] Float32: with Int8 N.
+ *   p = post_gamma ? unit(block) * post_gamma + post_beta : block;  Z = residual_scale * residual + block_scale * gate * p;  N = unit(Z) * pre_gamma + pre_beta
+ *   unit(x) = x / sqrt(mean(x^2) + epsilon), with layer_norm (x - mean) / sqrt(mean((x - mean)^2) + epsilon)
+ * All in f32 (N from Z before its rounding), each output rounded once; Int8 N are codes as MatMulInt8 makes them. Z and a float N may be written over residual or
+ * block. H <= 32768. */
+typedef struct NxrtRocmGatedResidualNormAttrs {
+  uint32_t struct_size;
+  uint32_t present;      /* bit i: 0 epsilon (default 1e-5), 1 residual_scale (1), 2 block_scale (1), 3 layer_norm (0) */
+  double epsilon, residual_scale, block_scale;
+  int64_t layer_norm;
+} NxrtRocmGatedResidualNormAttrs;
+int nxrt_rocm_ep_supports_gated_residual_norm(const NxrtRocmEp* ep, const NxrtRocmGatedResidualNormAttrs* attrs, const NxrtTensorDesc* inputs, uint32_t n_inputs, char* reason,
+                                              size_t reason_len);
+NxrtStatus nxrt_rocm_gated_residual_norm_create(NxrtRocmEp* ep, const NxrtRocmGatedResidualNormAttrs* attrs, NxrtRocmNode** out_node);
+
+/* As the functions of the same names for MatMulNBits. */
+void nxrt_rocm_node_set_constant_inputs(NxrtRocmNode* node, const uint8_t* is_constant, uint32_t n);
+NxrtStatus nxrt_rocm_node_workspace_requirement(const NxrtRocmNode* node, const NxrtTensorDesc* inputs, uint32_t n_inputs, NxrtRocmWorkspaceRequirement* out);
+NxrtStatus nxrt_rocm_node_execute(NxrtRocmNode* node, const NxrtRocmTensorView* inputs, uint32_t n_inputs, NxrtRocmTensorView* outputs, uint32_t n_outputs,
+                                  void* workspace_device, uint64_t workspace_bytes);
+const char* nxrt_rocm_node_last_variant(const NxrtRocmNode* node);
+uint64_t nxrt_rocm_node_retired_buffers(const NxrtRocmNode* node);
+void nxrt_rocm_node_release(NxrtRocmNode* node);
+
 /* ---- timing on the provider's stream (HIP events) ---------------------------------------------- */
 
 typedef struct NxrtRocmEvent NxrtRocmEvent;

@@ -34,8 +34,12 @@ HIP_SOURCES = [
     "kernels/swiglu.hip",
     "kernels/acc4.hip",
     "kernels/acc4_mfma.hip",
+    "kernels/gated_norm.hip",
+    "kernels/int8_gemm.hip",
+    "kernels/moe_route.hip",
+    "kernels/moe_rows.hip",
 ]
-HOST_SOURCES = ["ep/provider.cpp", "ep/matmul_nbits.cpp", "ep/nxrt_plugin.cpp", "ep/nxmem_plugin.cpp", "ep/ort_plugin.cpp"]
+HOST_SOURCES = ["ep/provider.cpp", "ep/matmul_nbits.cpp", "ep/nodes.cpp", "ep/nxrt_plugin.cpp", "ep/nxmem_plugin.cpp", "ep/ort_plugin.cpp"]
 
 # packed-fp32 VALU forms are kept off for all device code; the first fourteen dwords of a kernel's plain arguments are in scalar registers when its waves start
 DEVICE_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -329,6 +329,83 @@ int rocm_launch_acc4_packed(const RocmMatMulNBitsArgs* args, const void* packed,
  * wave, register sets (1 or 2). -1: the shape does not take this route. */
 int rocm_acc4_packed_plan(const RocmMatMulNBitsArgs* args, int waves, int compute_units, int* waves_out, int* groups_per_wave, int* register_sets);
 
+/* ---- operators beside MatMulNBits ------------------------------------------------------------------------------------ */
+
+enum { ROCM_DT_I8 = 3 };
+
+/* GatedResidualNorm (kernels/gated_norm.hip). residual, block, z and n [rows, hidden] of `dtype`; block NULL: z = residual_scale * residual. With n_scale,
+ * n is int8 codes and n_scale [rows]. z or n may be NULL. z and n may lie where residual or block do (codes may not). Any alignment of whole elements. */
+enum { ROCM_GATED_NORM_MAX_HIDDEN = 32768 };
+typedef struct RocmGatedNormArgs {
+  const void* residual;
+  const void* block;
+  const void* post_gamma;   /* read with `post`; each weight is of `dtype` or f32, or NULL */
+  const void* post_beta;
+  const void* gate;         /* [rows / rows_per_gate, hidden] */
+  const void* pre_gamma;
+  const void* pre_beta;
+  void* z;
+  void* n;
+  float* n_scale;
+  int64_t rows, hidden, rows_per_gate;
+  int dtype, post_gamma_dtype, post_beta_dtype, gate_dtype, pre_gamma_dtype, pre_beta_dtype;
+  int post, layer;
+  float epsilon, residual_scale, block_scale;
+} RocmGatedNormArgs;
+int rocm_launch_gated_norm(const RocmGatedNormArgs* args, rocm_stream_t stream);
+
+/* MatMulInt8 (kernels/int8_gemm.hip). Rows of codes are lda bytes apart with zeros from k to the next multiple of 128, lda and their address multiples of 16;
+ * rows of b are ldb bytes apart. k < ROCM_INT8_MAX_K, for which int32 holds every sum. */
+enum { ROCM_INT8_MAX_K = 131072 };
+typedef struct RocmInt8Args {
+  const int8_t* a;
+  const float* a_scale;     /* [m] */
+  const int8_t* b;
+  const void* b_scale;      /* [n] */
+  const void* bias;         /* as RocmMatMulNBitsArgs::bias */
+  void* y;
+  int32_t* partial;         /* rocm_int8_scratch_bytes() of device memory */
+  int64_t m, n, k, lda, ldb;
+  int b_scale_dtype, bias_dtype, y_dtype;
+} RocmInt8Args;
+/* Of m, n and k alone: whether B has to be handed over in padded rows (rocm_launch_pad_codes; else ldb = k and any address for k no multiple of 16, one of
+ * 16 bytes otherwise), and what the sums of slices of K take. */
+int rocm_int8_pads_b(const RocmInt8Args* args);
+uint64_t rocm_int8_scratch_bytes(const RocmInt8Args* args);
+/* Codes [m, k rounded up to 128] and scales [m] of a [m, k] (f32, f16, bf16). */
+int rocm_launch_quantize_rows(const void* a, int dtype, int64_t m, int64_t k, int8_t* codes, float* scales, rocm_stream_t stream);
+/* [rows, k] -> [rows, k rounded up to 128], zeros behind k. */
+int rocm_launch_pad_codes(const int8_t* from, int64_t rows, int64_t k, int8_t* to, rocm_stream_t stream);
+const char* rocm_int8_variant(const RocmInt8Args* args);
+int rocm_launch_int8(const RocmInt8Args* args, rocm_stream_t stream);
+
+/* QMoE (kernels/moe_*.hip). Weights as RocmMatMulNBitsArgs has them, 4 bits, one expert behind the other; scales and biases of `scale_dtype` / `bias_dtype`.
+ * gate and up: column j of expert e is row e * up_expert_step + j * up_row_step of theirs. block_size a power of two >= 32; x, logits, y any alignment of whole
+ * elements, weights of 16 bytes. */
+enum { ROCM_MOE_MAX_EXPERTS = 1024, ROCM_MOE_MAX_CHOICES = 64 };
+typedef struct RocmMoeWeights {
+  const uint8_t* b;
+  const void* scales;
+  const uint8_t* zp;        /* or NULL: 8 */
+  const void* bias;         /* or NULL */
+} RocmMoeWeights;
+typedef struct RocmMoeArgs {
+  const void* x;            /* [rows, hidden] f16 or bf16 */
+  const void* logits;       /* [rows, experts] */
+  void* y;                  /* [rows, hidden] */
+  RocmMoeWeights gate, up, down;
+  int64_t up_expert_step;
+  int up_row_step;
+  int64_t rows, hidden, inter;
+  int experts, k, block_size, normalize;
+  int dtype, logits_dtype, scale_dtype, bias_dtype;
+  float alpha, beta, limit;
+} RocmMoeArgs;
+uint64_t rocm_moe_workspace_bytes(const RocmMoeArgs* args);
+const char* rocm_moe_variant(const RocmMoeArgs* args);
+/* workspace: rocm_moe_workspace_bytes() of device memory, 256-byte aligned, contents of no interest before or after. */
+int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

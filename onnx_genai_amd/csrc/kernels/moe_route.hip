@@ -1,0 +1,193 @@
+// QMoE, from router logits to the experts' rows.
+//
+// A token's k experts are those of its largest logits, the lowest index first among equal ones. Its weights are the softmax over all experts, or, normalized,
+// over the chosen ones. An expert of weight 0 (a logit of -inf, or one so far below the largest that exp gives 0) is not chosen; a row of -inf has none, and
+// its result is 0. A NaN or +inf among a token's logits makes its result NaN.
+// The (token, expert) pairs are then sorted by expert, and each expert's pairs are cut into tiles of rows. The order of an expert's rows follows from atomics
+// and differs from run to run; each row's result does not depend on where it lies.
+#include "moe.hiph"
+#include "rows.hiph"
+
+namespace mnb {
+namespace {
+
+__device__ __forceinline__ uint32_t ordered(float v)
+{
+    const uint32_t u = __float_as_uint(v + 0.0f);            // (-0 as 0: they tie)
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key); }
+
+// One wave a token. NL: experts a lane looks at.
+template <int NL>
+__global__ __launch_bounds__(256) void moe_top_k_kernel(const void* logits, int dtype, int64_t rows, int experts, int k, int normalize, MoeRoute r)
+{
+    const int lane = threadIdx.x & 63;
+    const int64_t token = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (token >= rows) return;
+    uint32_t key[NL];
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+        const int e = j * 64 + lane;
+        const float v = e < experts ? load_as_f32(logits, dtype, token * experts + e) : -INFINITY;
+        bad |= !(v < INFINITY);
+        key[j] = ordered(v);
+    }
+    bad = __any(bad);
+    const uint32_t none = ordered(-INFINITY);
+    auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    auto smaller = [](uint32_t a, uint32_t b) { return a < b ? a : b; };
+    float peak = 0.f, all = 0.f, mine = 0.f;
+    int my_expert = -1;
+    for (int i = 0; i < k && !bad; ++i) {
+        uint32_t best = 0;
+#pragma unroll
+        for (int j = 0; j < NL; ++j) best = larger(best, key[j]);
+        best = over_wave(best, larger);
+        if (best <= none) break;
+        uint32_t at = 0xffffffffu;
+#pragma unroll
+        for (int j = NL - 1; j >= 0; --j)
+            if (key[j] == best) at = j * 64 + lane;
+        at = over_wave(at, smaller);
+        const float v = value_of(best);
+        if (i == 0) {
+            peak = v;
+#pragma unroll
+            for (int j = 0; j < NL; ++j) all += key[j] > none ? expf(value_of(key[j]) - peak) : 0.f;
+            all = over_wave(all, [](float a, float b) { return a + b; });
+        }
+        if (lane == i) {
+            mine = expf(v - peak);
+            my_expert = static_cast<int>(at);
+        }
+#pragma unroll
+        for (int j = 0; j < NL; ++j)
+            if (at == static_cast<uint32_t>(j * 64 + lane)) key[j] = 0;
+    }
+    const float chosen = over_wave(mine, [](float a, float b) { return a + b; });
+    const float weight = my_expert >= 0 ? mine / (normalize ? chosen : all) : 0.f;
+    if (lane < k) {
+        r.expert[token * k + lane] = weight > 0.f ? my_expert : -1;
+        r.weight[token * k + lane] = weight;
+    }
+    if (lane == 0) r.base[token] = bad ? NAN : 0.f;
+}
+
+// One workgroup sorts the pairs and cuts the tiles.
+__global__ __launch_bounds__(1024) void moe_plan_kernel(int pairs, int experts, int k, int tile_rows, int max_tiles, MoeRoute r)
+{
+    __shared__ int count[1024], rows_to[1024], tiles_to[1024];
+    const int t = threadIdx.x;
+    count[t] = 0;
+    __syncthreads();
+    for (int p = t; p < pairs; p += 1024) {
+        const int e = r.expert[p];
+        if (e >= 0) r.pair_row[p] = atomicAdd(&count[e], 1);
+    }
+    __syncthreads();
+    const int own = count[t], own_tiles = (own + tile_rows - 1) / tile_rows;
+    rows_to[t] = own;
+    tiles_to[t] = own_tiles;
+    __syncthreads();
+    for (int d = 1; d < 1024; d *= 2) {
+        const int a = t >= d ? rows_to[t - d] : 0, b = t >= d ? tiles_to[t - d] : 0;
+        __syncthreads();
+        rows_to[t] += a;
+        tiles_to[t] += b;
+        __syncthreads();
+    }
+    const int row0 = rows_to[t] - own, tile0 = tiles_to[t] - own_tiles;
+    for (int i = 0; i < own_tiles; ++i) r.tiles[tile0 + i] = make_int4(t, row0 + i * tile_rows, min(tile_rows, own - i * tile_rows), 0);
+    for (int i = tiles_to[1023] + t; i < max_tiles; i += 1024) r.tiles[i] = make_int4(0, 0, 0, 0);
+    for (int p = t; p < pairs; p += 1024) {
+        const int e = r.expert[p];
+        int row = -1;
+        if (e >= 0) {
+            row = rows_to[e] - count[e] + r.pair_row[p];
+            r.token[row] = p / k;
+        }
+        r.pair_row[p] = row;
+    }
+}
+
+// y = base + sum over a token's experts, in the order of their logits, of weight * (out + bias).
+template <typename T, bool BF16>
+__global__ __launch_bounds__(256) void moe_combine_kernel(RocmMoeArgs a, MoeRoute r, const float* __restrict__ out)
+{
+    const unsigned parts = static_cast<unsigned>((a.hidden + 2047) / 2048);
+    const int64_t token = blockIdx.x / parts;
+    const int64_t h = (static_cast<int64_t>(blockIdx.x % parts) * 256 + threadIdx.x) * 8;
+    const int left = static_cast<int>(a.hidden - h < 8 ? a.hidden - h : 8);
+    if (left <= 0) return;
+    float sum[8];
+    const float base = r.base[token];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = base;
+    for (int j = 0; j < a.k; ++j) {
+        const int row = r.pair_row[token * a.k + j];
+        if (row < 0) continue;
+        const float w = r.weight[token * a.k + j];
+        const float* const from = out + static_cast<int64_t>(row) * a.hidden + h;
+        const int64_t bias_at = static_cast<int64_t>(r.expert[token * a.k + j]) * a.hidden + h;
+        Eight<float, false> v;
+        if (left == 8) v.load(from);
+        else v.load_first(from, left);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] = fmaf(w, v.raw[e] + (a.down.bias && e < left ? load_as_f32(a.down.bias, a.bias_dtype, bias_at + e) : 0.f), sum[e]);
+    }
+    Eight<T, BF16> o;
+    o.set(sum);
+    T* const to = static_cast<T*>(a.y) + token * a.hidden + h;
+    if (left == 8) o.store(to);
+    else o.store_first(to, left);
+}
+
+// Rows of `k` elements -> rows of `kp`, zeros behind: for rows that do not begin at a multiple of 16 bytes.
+__global__ __launch_bounds__(256) void moe_pad_rows_kernel(const uint16_t* __restrict__ from, int64_t k, int64_t kp, uint16_t* __restrict__ to)
+{
+    const unsigned parts = static_cast<unsigned>((kp + 2047) / 2048);
+    const int64_t row = blockIdx.x / parts, i = (static_cast<int64_t>(blockIdx.x % parts) * 256 + threadIdx.x) * 8;
+    if (i >= kp) return;
+    Eight<uint16_t, false> e;
+    const int64_t left = k - i;
+    if (left >= 8) e.load(from + row * k + i);
+    else e.load_first(from + row * k + i, left > 0 ? static_cast<int>(left) : 0);
+    e.store(to + row * kp + i);
+}
+
+}  // namespace
+
+int launch_moe_top_k(const RocmMoeArgs& a, const MoeRoute& r, hipStream_t s)
+{
+    const dim3 grid(static_cast<unsigned>((a.rows + 3) / 4));
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a.logits, a.logits_dtype, a.rows, a.experts, a.k, a.normalize, r);
+        return static_cast<int>(hipGetLastError());
+    };
+    return a.experts <= 64 ? go(moe_top_k_kernel<1>) : a.experts <= 128 ? go(moe_top_k_kernel<2>) : a.experts <= 256 ? go(moe_top_k_kernel<4>) : go(moe_top_k_kernel<16>);
+}
+
+int launch_moe_plan(const RocmMoeArgs& a, int tile_rows, int max_tiles, const MoeRoute& r, hipStream_t s)
+{
+    hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, s, static_cast<int>(a.rows * a.k), a.experts, a.k, tile_rows, max_tiles, r);
+    return static_cast<int>(hipGetLastError());
+}
+
+int launch_moe_combine(const RocmMoeArgs& a, const MoeRoute& r, const float* out, hipStream_t s)
+{
+    const dim3 grid(static_cast<unsigned>((a.hidden + 2047) / 2048 * a.rows));
+    if (a.dtype == ROCM_DT_BF16) hipLaunchKernelGGL((moe_combine_kernel<uint16_t, true>), grid, dim3(256), 0, s, a, r, out);
+    else hipLaunchKernelGGL((moe_combine_kernel<uint16_t, false>), grid, dim3(256), 0, s, a, r, out);
+    return static_cast<int>(hipGetLastError());
+}
+
+int launch_moe_pad_rows(const void* from, int64_t rows, int64_t k, int64_t kp, void* to, hipStream_t s)
+{
+    hipLaunchKernelGGL(moe_pad_rows_kernel, dim3(static_cast<unsigned>((kp + 2047) / 2048 * rows)), dim3(256), 0, s, static_cast<const uint16_t*>(from), k, kp,
+                       static_cast<uint16_t*>(to));
+    return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace mnb

@@ -69,6 +69,24 @@ class WorkspaceRequirement(C.Structure):
     _fields_ = [("bytes", C.c_uint64), ("alignment", C.c_uint64)]
 
 
+class QMoEAttrs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("present", C.c_uint32), ("k", C.c_int64), ("block_size", C.c_int64), ("expert_weight_bits", C.c_int64),
+                ("normalize_routing_weights", C.c_int64), ("swiglu_fusion", C.c_int64), ("activation_alpha", C.c_double), ("activation_beta", C.c_double),
+                ("swiglu_limit", C.c_double)]
+
+
+class MatMulInt8Attrs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("present", C.c_uint32), ("K", C.c_int64), ("N", C.c_int64)]
+
+
+class GatedResidualNormAttrs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("present", C.c_uint32), ("epsilon", C.c_double), ("residual_scale", C.c_double), ("block_scale", C.c_double),
+                ("layer_norm", C.c_int64)]
+
+
+# operators beside MatMulNBits: their attributes (bit i of `present` = the i-th of them) and the name in their entry points
+_NODE_OPS = {"QMoE": (QMoEAttrs, "qmoe"), "MatMulInt8": (MatMulInt8Attrs, "matmul_int8"), "GatedResidualNorm": (GatedResidualNormAttrs, "gated_residual_norm")}
+
 _ATTR_BITS = {"K": 0, "N": 1, "bits": 2, "block_size": 3, "accuracy_level": 4, "weight_prepacked": 5, "folded_bias": 6, "gate_up_swiglu": 7,
               "decomposed_silu": 8, "rmsnorm_prologue": 9, "rmsnorm_epsilon": 10}
 _lib = None
@@ -168,7 +186,25 @@ def load_library() -> C.CDLL:
     L.nxrt_rocm_ep_kernel_launch_count.argtypes = [v]
     L.nxrt_rocm_live_provider_count.restype = u64
     L.nxrt_rocm_live_provider_count.argtypes = []
+    for attrs, name in _NODE_OPS.values():
+        supports, create = getattr(L, f"nxrt_rocm_ep_supports_{name}"), getattr(L, f"nxrt_rocm_{name}_create")
+        supports.restype, create.restype = C.c_int, S
+        supports.argtypes = [v, C.POINTER(attrs), C.POINTER(NxrtTensorDesc), u32, C.c_char_p, sz]
+        create.argtypes = [v, C.POINTER(attrs), C.POINTER(v)]
+    L.nxrt_rocm_node_set_constant_inputs.restype = None
+    L.nxrt_rocm_node_set_constant_inputs.argtypes = [v, C.POINTER(C.c_uint8), u32]
+    L.nxrt_rocm_node_workspace_requirement.restype = S
+    L.nxrt_rocm_node_workspace_requirement.argtypes = [v, C.POINTER(NxrtTensorDesc), u32, C.POINTER(WorkspaceRequirement)]
+    L.nxrt_rocm_node_execute.restype = S
+    L.nxrt_rocm_node_execute.argtypes = [v, v, u32, v, u32, v, u64]
+    L.nxrt_rocm_node_last_variant.restype = C.c_char_p
+    L.nxrt_rocm_node_last_variant.argtypes = [v]
+    L.nxrt_rocm_node_retired_buffers.restype = u64
+    L.nxrt_rocm_node_retired_buffers.argtypes = [v]
+    L.nxrt_rocm_node_release.restype = None
+    L.nxrt_rocm_node_release.argtypes = [v]
     L.execute_at = C.cast(L.nxrt_rocm_matmul_nbits_execute, v).value
+    L.node_execute_at = C.cast(L.nxrt_rocm_node_execute, v).value
     _lib = L
     return L
 
@@ -182,6 +218,25 @@ def make_attrs(**kw) -> Attrs:
             continue
         a.present |= 1 << _ATTR_BITS[name]
         setattr(a, name, float(value) if name == "rmsnorm_epsilon" else int(value))
+    return a
+
+
+def make_node_attrs(op_type: str, attrs: dict):
+    """The attribute struct of an operator beside MatMulNBits; only the names passed are marked present."""
+    if op_type not in _NODE_OPS:
+        raise ValueError(f"unknown operator {op_type!r}: this provider has MatMulNBits, " + ", ".join(_NODE_OPS))
+    struct_type, _ = _NODE_OPS[op_type]
+    a = struct_type()
+    a.struct_size = C.sizeof(struct_type)
+    fields = {name: (i, kind) for i, (name, kind) in enumerate(struct_type._fields_[2:])}
+    for name, value in attrs.items():
+        if name not in fields:
+            raise ValueError(f"{op_type} has no attribute {name!r}")
+        if value is None:
+            continue
+        i, kind = fields[name]
+        a.present |= 1 << i
+        setattr(a, name, float(value) if kind is C.c_double else int(value))
     return a
 
 
@@ -346,19 +401,24 @@ class RocmExecutionProvider:
         return out
 
     # -- operator ---------------------------------------------------------------------------------
-    def supports_op(self, attrs: dict, inputs=None):
+    def supports_op(self, attrs: dict, inputs=None, op_type: str = "MatMulNBits"):
         """-> (True, "") or (False, reason). inputs: [(shape or None, dtype)] for A, B, scales, ..."""
-        a = make_attrs(**attrs)
+        if op_type == "MatMulNBits":
+            a, supports = make_attrs(**attrs), self.lib.nxrt_rocm_ep_supports_matmul_nbits
+        else:
+            a = make_node_attrs(op_type, attrs)
+            supports = getattr(self.lib, f"nxrt_rocm_ep_supports_{_NODE_OPS[op_type][1]}")
         reason = C.create_string_buffer(512)
         if inputs is None:
-            ok = self.lib.nxrt_rocm_ep_supports_matmul_nbits(self.handle, C.byref(a), None, 0, reason, 512)
+            ok = supports(self.handle, C.byref(a), None, 0, reason, 512)
         else:
             descs, keep = make_descs(inputs)
-            ok = self.lib.nxrt_rocm_ep_supports_matmul_nbits(self.handle, C.byref(a), descs, len(inputs), reason, 512)
+            ok = supports(self.handle, C.byref(a), descs, len(inputs), reason, 512)
         return bool(ok), reason.value.decode()
 
-    def get_kernel(self, attrs: dict, input_shapes=None) -> "MatMulNBitsKernel":
-        return MatMulNBitsKernel(self, attrs, input_shapes)
+    def get_kernel(self, attrs: dict, input_shapes=None, op_type: str = "MatMulNBits"):
+        """A kernel object for one node: MatMulNBits, or QMoE, MatMulInt8, GatedResidualNorm (include/nxrt_ep_rocm.h says what each takes)."""
+        return MatMulNBitsKernel(self, attrs, input_shapes) if op_type == "MatMulNBits" else NodeKernel(self, op_type, attrs)
 
     # -- pieces -----------------------------------------------------------------------------------
     def dequantize(self, b: DeviceBuffer, scales: DeviceBuffer, scale_dtype: int, zp: DeviceBuffer | None, n, k, bs, out: DeviceBuffer, bits: int = 4) -> None:
@@ -521,6 +581,55 @@ class MatMulNBitsKernel:
             pass
 
 
+class NodeKernel:
+    """One node of an operator beside MatMulNBits; the same calls as MatMulNBitsKernel's."""
+
+    def __init__(self, ep: RocmExecutionProvider, op_type: str, attrs: dict):
+        self.ep, self.lib, self.op_type = ep, ep.lib, op_type
+        a = make_node_attrs(op_type, attrs)
+        h = C.c_void_p()
+        getattr(self.lib, f"nxrt_rocm_{_NODE_OPS[op_type][1]}_create")(ep.handle, C.byref(a), C.byref(h)).check()
+        self.handle = h
+
+    def set_constant_inputs(self, flags) -> None:
+        arr = (C.c_uint8 * max(len(flags), 1))(*[1 if f else 0 for f in flags])
+        self.lib.nxrt_rocm_node_set_constant_inputs(self.handle, arr, len(flags))
+
+    def workspace_requirement(self, input_shapes) -> tuple[int, int]:
+        descs, keep = make_descs(input_shapes)
+        out = WorkspaceRequirement()
+        self.lib.nxrt_rocm_node_workspace_requirement(self.handle, descs, len(input_shapes), C.byref(out)).check()
+        return out.bytes, out.alignment
+
+    def execute(self, inputs, outputs, workspace: DeviceBuffer | None = None) -> None:
+        if _calls is not None and self.handle:
+            failed = _calls.execute(self.lib.node_execute_at, self.handle.value, inputs, outputs, workspace.ptr if workspace else 0, workspace.nbytes if workspace else 0)
+            if failed is None:
+                return
+            if failed:
+                raise EpError(failed[0], failed[1].decode("utf-8", "replace"))
+        buf, at = _packed_views((*inputs, *outputs))
+        self.lib.nxrt_rocm_node_execute(self.handle, at, len(inputs), at + _VIEW_BYTES * len(inputs), len(outputs),
+                                        workspace.ptr if workspace else None, workspace.nbytes if workspace else 0).check()
+
+    def last_variant(self) -> str:
+        return self.lib.nxrt_rocm_node_last_variant(self.handle).decode()
+
+    def retired_buffers(self) -> int:
+        return self.lib.nxrt_rocm_node_retired_buffers(self.handle)
+
+    def release(self) -> None:
+        if self.handle:
+            self.lib.nxrt_rocm_node_release(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.release()
+        except Exception:
+            pass
+
+
 _NP = {F32: np.float32, F16: np.float16, BF16: np.uint16, U8: np.uint8, I8: np.int8, I32: np.int32}
 
 
@@ -659,5 +768,5 @@ def gate_up_swiglu(ep, a, a_dtype, gate, up, scale_dtype, n, k, bs, *, decompose
     return y, variant
 
 
-__all__ = ["RocmExecutionProvider", "GateUpOperands", "gate_up_swiglu", "MatMulNBitsKernel", "TensorView", "DeviceBuffer", "DeviceOperands", "EpError", "matmul_nbits",
-           "load_library", "make_attrs", "make_descs", "synth", "F32", "U8", "I8", "I32", "F16", "BF16"]
+__all__ = ["RocmExecutionProvider", "GateUpOperands", "gate_up_swiglu", "MatMulNBitsKernel", "NodeKernel", "TensorView", "DeviceBuffer", "DeviceOperands", "EpError", "matmul_nbits",
+           "load_library", "make_attrs", "make_node_attrs", "make_descs", "synth", "F32", "U8", "I8", "I32", "F16", "BF16"]
