@@ -1,0 +1,130 @@
+// QMoE: which launches a call is.
+//
+//   up to 4 tokens      gate/up (every workgroup routes for itself), down with the sum over experts
+//   up to 16 tokens     routing, gate/up, down with the sum over experts
+//   more                top-k, sorting by expert, gate/up, down, sum over each token's experts
+#include "moe.hiph"
+
+namespace mnb {
+namespace {
+
+constexpr int kTileRows = 16;
+
+struct MoePlan {
+    int where;                 // kMoeFused, kMoeTable, kMoeTiles
+    int slots;                 // experts that can be active, or tiles
+    int64_t kp, ip, pairs;
+    uint64_t table, expert, weight, pair_row, token, base, tiles, x, h, out, total;
+};
+
+MoePlan plan_of(const RocmMoeArgs& a)
+{
+    MoePlan l{};
+    l.pairs = a.rows * a.k;
+    l.where = a.rows <= 4 && l.pairs <= kFewPairs ? kMoeFused : a.rows <= kFewTokens && l.pairs <= kFewPairs ? kMoeTable : kMoeTiles;
+    l.slots = static_cast<int>((l.where == kMoeTiles ? l.pairs / kTileRows : 0) + (l.pairs < a.experts ? l.pairs : a.experts));
+    l.kp = (a.hidden + 7) / 8 * 8;
+    l.ip = (a.inter + 127) / 128 * 128;
+    auto part = [&](uint64_t bytes) {
+        const uint64_t here = l.total;
+        l.total += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const bool tiled = l.where == kMoeTiles;
+    l.table = part(tiled ? 0 : sizeof(MoeFewTable));
+    l.expert = part(tiled ? l.pairs * 4 : 0);
+    l.weight = part(tiled ? l.pairs * 4 : 0);
+    l.pair_row = part(tiled ? l.pairs * 4 : 0);
+    l.token = part(tiled ? l.pairs * 4 : 0);
+    l.base = part(tiled ? a.rows * 4 : 0);
+    l.tiles = part(tiled ? static_cast<uint64_t>(l.slots) * 16 : 0);
+    // rows that do not begin at multiples of 16 bytes are copied: the address may be any
+    l.x = part(a.rows * l.kp * 2);
+    const int64_t rows_of_h = tiled ? l.pairs : l.slots * (l.where == kMoeFused ? 4 : 16);
+    l.h = part(rows_of_h * l.ip * 4);
+    l.out = part(tiled ? l.pairs * a.hidden * 4 : 0);
+    return l;
+}
+
+MoeMatrix matrix_of(const RocmMoeArgs& a, const RocmMoeWeights& w, const RocmMoeWeights* second, int64_t k, int64_t n, int64_t expert_step, int row_step)
+{
+    MoeMatrix m{};
+    m.w[0] = w;
+    if (second) m.w[1] = *second;
+    m.expert_step = expert_step;
+    m.row_step = row_step;
+    m.n = static_cast<int>(n);
+    m.kb = static_cast<int>((k + a.block_size - 1) / a.block_size);
+    m.block_size = a.block_size;
+    m.row_bytes = static_cast<int64_t>(m.kb) * a.block_size / 2;
+    m.zp_row = (m.kb + 1) / 2;
+    m.scale_dtype = a.scale_dtype;
+    m.bias_dtype = a.bias_dtype;
+    return m;
+}
+
+}  // namespace
+}  // namespace mnb
+
+extern "C" uint64_t rocm_moe_workspace_bytes(const RocmMoeArgs* args) { return mnb::plan_of(*args).total; }
+extern "C" const char* rocm_moe_variant(const RocmMoeArgs* args)
+{
+    const int where = mnb::plan_of(*args).where;
+    return where == mnb::kMoeFused ? "moe_few" : where == mnb::kMoeTable ? "moe_table" : "moe_tiles";
+}
+
+extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_stream_t stream)
+{
+    using namespace mnb;
+    const RocmMoeArgs& a = *args;
+    if (a.rows <= 0) return 0;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const MoePlan l = plan_of(a);
+    uint8_t* const ws = static_cast<uint8_t*>(workspace);
+    auto at = [&](uint64_t offset) { return reinterpret_cast<int32_t*>(ws + offset); };
+    const MoeRoute route{at(l.expert), reinterpret_cast<float*>(ws + l.weight), at(l.pair_row), at(l.token), reinterpret_cast<float*>(ws + l.base), reinterpret_cast<int4*>(ws + l.tiles)};
+    MoeFewTable* const table = reinterpret_cast<MoeFewTable*>(ws + l.table);
+    int rc = 0;
+    if (l.where == kMoeTable) rc = launch_moe_route_few(a, table, s);
+    if (l.where == kMoeTiles) {
+        rc = launch_moe_top_k(a, route, s);
+        if (rc == 0) rc = launch_moe_plan(a, kTileRows, l.slots, route, s);
+    }
+    const void* x = a.x;
+    if (rc == 0 && (l.kp != a.hidden || reinterpret_cast<uintptr_t>(a.x) % 16 != 0)) {
+        rc = launch_moe_pad_rows(a.x, a.rows, a.hidden, l.kp, ws + l.x, s);
+        x = ws + l.x;
+    }
+    if (rc != 0) return rc;
+    MoeUpCall up{};
+    up.m = matrix_of(a, a.gate, &a.up, a.hidden, a.inter, a.up_expert_step, a.up_row_step);
+    up.x = static_cast<const uint16_t*>(x);
+    up.ldx = l.kp;
+    up.h = reinterpret_cast<uint16_t*>(ws + l.h);
+    up.ip = l.ip;
+    up.alpha = a.alpha;
+    up.beta = a.beta;
+    up.limit = a.limit;
+    up.route = route;
+    up.table = table;
+    up.logits = a.logits;
+    up.logits_dtype = a.logits_dtype;
+    up.rows = static_cast<int>(a.rows);
+    up.experts = a.experts;
+    up.k = a.k;
+    up.normalize = a.normalize;
+    MoeDownCall down{};
+    down.m = matrix_of(a, a.down, nullptr, a.inter, a.hidden, a.hidden, 1);
+    down.h = up.h;
+    down.ip = l.ip;
+    down.route = route;
+    down.table = table;
+    down.rows = up.rows;
+    down.y = a.y;
+    down.out = reinterpret_cast<float*>(ws + l.out);
+    if (l.where == kMoeFused) return launch_moe_few(a, up, down, l.slots, s);
+    rc = launch_moe_gate_up(a, up, l.where, l.slots, s);
+    if (rc == 0) rc = launch_moe_down(a, down, l.where, l.slots, s);
+    if (rc == 0 && l.where == kMoeTiles) rc = launch_moe_combine(a, route, down.out, s);
+    return rc;
+}

@@ -5,74 +5,30 @@
 // its result is 0. A NaN or +inf among a token's logits makes its result NaN.
 // The (token, expert) pairs are then sorted by expert, and each expert's pairs are cut into tiles of rows. The order of an expert's rows follows from atomics
 // and differs from run to run; each row's result does not depend on where it lies.
-#include "moe.hiph"
-#include "rows.hiph"
+#include "moe_route.hiph"
 
 namespace mnb {
 namespace {
 
-__device__ __forceinline__ uint32_t ordered(float v)
-{
-    const uint32_t u = __float_as_uint(v + 0.0f);            // (-0 as 0: they tie)
-    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key); }
-
-// One wave a token. NL: experts a lane looks at.
 template <int NL>
 __global__ __launch_bounds__(256) void moe_top_k_kernel(const void* logits, int dtype, int64_t rows, int experts, int k, int normalize, MoeRoute r)
 {
     const int lane = threadIdx.x & 63;
     const int64_t token = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (token >= rows) return;
-    uint32_t key[NL];
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < NL; ++j) {
-        const int e = j * 64 + lane;
-        const float v = e < experts ? load_as_f32(logits, dtype, token * experts + e) : -INFINITY;
-        bad |= !(v < INFINITY);
-        key[j] = ordered(v);
-    }
-    bad = __any(bad);
-    const uint32_t none = ordered(-INFINITY);
-    auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
-    auto smaller = [](uint32_t a, uint32_t b) { return a < b ? a : b; };
-    float peak = 0.f, all = 0.f, mine = 0.f;
-    int my_expert = -1;
-    for (int i = 0; i < k && !bad; ++i) {
-        uint32_t best = 0;
-#pragma unroll
-        for (int j = 0; j < NL; ++j) best = larger(best, key[j]);
-        best = over_wave(best, larger);
-        if (best <= none) break;
-        uint32_t at = 0xffffffffu;
-#pragma unroll
-        for (int j = NL - 1; j >= 0; --j)
-            if (key[j] == best) at = j * 64 + lane;
-        at = over_wave(at, smaller);
-        const float v = value_of(best);
-        if (i == 0) {
-            peak = v;
-#pragma unroll
-            for (int j = 0; j < NL; ++j) all += key[j] > none ? expf(value_of(key[j]) - peak) : 0.f;
-            all = over_wave(all, [](float a, float b) { return a + b; });
-        }
-        if (lane == i) {
-            mine = expf(v - peak);
-            my_expert = static_cast<int>(at);
-        }
-#pragma unroll
-        for (int j = 0; j < NL; ++j)
-            if (at == static_cast<uint32_t>(j * 64 + lane)) key[j] = 0;
-    }
-    const float chosen = over_wave(mine, [](float a, float b) { return a + b; });
-    const float weight = my_expert >= 0 ? mine / (normalize ? chosen : all) : 0.f;
+    const MoeChoice c = choose_experts<NL>(logits, dtype, token, experts, k, normalize);
     if (lane < k) {
-        r.expert[token * k + lane] = weight > 0.f ? my_expert : -1;
-        r.weight[token * k + lane] = weight;
+        r.expert[token * k + lane] = c.expert;
+        r.weight[token * k + lane] = c.weight;
     }
-    if (lane == 0) r.base[token] = bad ? NAN : 0.f;
+    if (lane == 0) r.base[token] = c.base;
+}
+
+__global__ __launch_bounds__(1024) void moe_route_few_kernel(const void* logits, int dtype, int rows, int experts, int k, int normalize, MoeFewTable* table)
+{
+    __shared__ MoeFewRouting routing;
+    route_few(routing, logits, dtype, rows, experts, k, normalize);
+    write_table(routing, rows, k, table);
 }
 
 // One workgroup sorts the pairs and cuts the tiles.
@@ -167,6 +123,12 @@ int launch_moe_top_k(const RocmMoeArgs& a, const MoeRoute& r, hipStream_t s)
         return static_cast<int>(hipGetLastError());
     };
     return a.experts <= 64 ? go(moe_top_k_kernel<1>) : a.experts <= 128 ? go(moe_top_k_kernel<2>) : a.experts <= 256 ? go(moe_top_k_kernel<4>) : go(moe_top_k_kernel<16>);
+}
+
+int launch_moe_route_few(const RocmMoeArgs& a, MoeFewTable* table, hipStream_t s)
+{
+    hipLaunchKernelGGL(moe_route_few_kernel, dim3(1), dim3(1024), 0, s, a.logits, a.logits_dtype, static_cast<int>(a.rows), a.experts, a.k, a.normalize, table);
+    return static_cast<int>(hipGetLastError());
 }
 
 int launch_moe_plan(const RocmMoeArgs& a, int tile_rows, int max_tiles, const MoeRoute& r, hipStream_t s)
