@@ -17,6 +17,7 @@ namespace {
 struct GatedNormParams {
     RocmGatedNormArgs a;
     int vectors;               // pieces of eight elements in a row, the last one perhaps short
+    int per_gate;              // rows of a gate
 };
 
 __device__ __forceinline__ float add(float a, float b) { return a + b; }
@@ -32,8 +33,10 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_kernel(GatedNorm
     __shared__ uint32_t slots_max[16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = WAVE ? 1 : blockDim.x >> 6;
-    const int64_t row = WAVE ? static_cast<int64_t>(blockIdx.x) * 4 + wave : static_cast<int64_t>(blockIdx.x);
-    if (row >= a.rows) return;                                   // (whole waves: no barrier is left behind where WAVE)
+    // rows of one gate along x, gates along y: no division for the gate
+    const int in_gate = WAVE ? static_cast<int>(blockIdx.x) * 4 + wave : static_cast<int>(blockIdx.x);
+    if (in_gate >= p.per_gate) return;                           // (whole waves, and no barrier is left behind where WAVE)
+    const int64_t row = static_cast<int64_t>(blockIdx.y) * p.per_gate + in_gate;
     const int first = WAVE ? threadIdx.x & 63 : threadIdx.x, step = WAVE ? 64 : blockDim.x;
     const int h = static_cast<int>(a.hidden);
     const int64_t at = row * h;
@@ -101,7 +104,7 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_kernel(GatedNorm
     if (block) {
         float mean = 0.f, rstd = 1.f;
         if (a.post) moments(z, slots[0], mean, rstd);
-        const int64_t gate_at = a.gate ? row / a.rows_per_gate * h : 0;
+        const int64_t gate_at = static_cast<int64_t>(blockIdx.y) * h;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int i = first + j * step;
@@ -205,12 +208,27 @@ extern "C" int rocm_launch_gated_norm(const RocmGatedNormArgs* args, rocm_stream
     if (args->rows <= 0 || args->hidden <= 0) return 0;
     if (args->hidden > ROCM_GATED_NORM_MAX_HIDDEN || args->rows > 0x7fffffff) return static_cast<int>(hipErrorInvalidValue);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    GatedNormParams p{*args, static_cast<int>((args->hidden + 7) / 8)};
+    const int64_t gates = args->gate ? args->rows / args->rows_per_gate : 1;
+    GatedNormParams p{*args, static_cast<int>((args->hidden + 7) / 8), static_cast<int>(args->rows / gates)};
     auto go = [&](auto kernel, unsigned grid, unsigned threads) {
-        hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, s, p);
-        return static_cast<int>(hipGetLastError());
+        // a grid has 65535 rows: further gates go in further launches
+        for (int64_t g = 0; g < gates; g += 65535) {
+            GatedNormParams part = p;
+            const int64_t first = g * p.per_gate, item = args->dtype == ROCM_DT_F32 ? 4 : 2, skip = first * args->hidden;
+            auto on = [&](auto* x, int64_t bytes) { return x ? reinterpret_cast<decltype(x)>(reinterpret_cast<uintptr_t>(x) + static_cast<uintptr_t>(bytes)) : x; };
+            part.a.residual = on(args->residual, skip * item);
+            part.a.block = on(args->block, skip * item);
+            part.a.z = on(args->z, skip * item);
+            part.a.n = on(args->n, skip * (args->n_scale ? 1 : item));
+            part.a.n_scale = on(args->n_scale, first * 4);
+            part.a.gate = on(args->gate, g * args->hidden * (args->gate_dtype == ROCM_DT_F32 ? 4 : 2));
+            hipLaunchKernelGGL(kernel, dim3(grid, static_cast<unsigned>(gates - g < 65535 ? gates - g : 65535)), dim3(threads), 0, s, part);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return static_cast<int>(e);
+        }
+        return 0;
     };
-    const unsigned rows = static_cast<unsigned>(args->rows);
+    const unsigned rows = static_cast<unsigned>(p.per_gate);
     auto typed = [&](auto t, auto bf) {
         using T = decltype(t);
         constexpr bool BF16 = decltype(bf)::value;

@@ -21,7 +21,8 @@ MoePlan plan_of(const RocmMoeArgs& a)
 {
     MoePlan l{};
     l.pairs = a.rows * a.k;
-    l.where = a.rows <= 4 && l.pairs <= kFewPairs ? kMoeFused : a.rows <= kFewTokens && l.pairs <= kFewPairs ? kMoeTable : kMoeTiles;
+    // (the rows of x lie in the 48 KiB of LDS that a kernel gets without asking beside its tables)
+    l.where = a.rows <= 4 && a.experts <= 256 && l.pairs <= kFewPairs && a.rows * ((a.hidden + 2047) / 2048) <= 12 ? kMoeFused : a.rows <= kFewTokens && l.pairs <= kFewPairs ? kMoeTable : kMoeTiles;
     l.slots = static_cast<int>((l.where == kMoeTiles ? l.pairs / kTileRows : 0) + (l.pairs < a.experts ? l.pairs : a.experts));
     l.kp = (a.hidden + 7) / 8 * 8;
     l.ip = (a.inter + 127) / 128 * 128;
@@ -106,6 +107,7 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     up.beta = a.beta;
     up.limit = a.limit;
     up.route = route;
+    up.tiles = static_cast<unsigned>(l.slots);
     up.table = table;
     up.logits = a.logits;
     up.logits_dtype = a.logits_dtype;
@@ -118,6 +120,7 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     down.h = up.h;
     down.ip = l.ip;
     down.route = route;
+    down.tiles = up.tiles;
     down.table = table;
     down.rows = up.rows;
     down.y = a.y;

@@ -37,7 +37,7 @@ __global__ __launch_bounds__(512) void moe_down_few_kernel(MoeDownCall p)
     };
     moe_pipeline<typename Dot::Step>(begin, end,
                                      [&](typename Dot::Step& s, int item) {
-                                         const int at = item / steps;
+                                         const int at = static_cast<int>(static_cast<unsigned>(item) / static_cast<unsigned>(steps));
                                          const MoeTile<1> tile = moe_tile<ST, ZP, 1>(p.m, __builtin_amdgcn_readfirstlane(experts[at]), n0, live);
                                          dot.template load<false>(s, tile, item - at * steps, p.h + (static_cast<int64_t>(at) * kRows + dot.col) * (2 * p.ip), dot.col < p.rows, p.ip, 0);
                                      },
@@ -68,12 +68,12 @@ __global__ __launch_bounds__(256) void moe_down_tiles_kernel(MoeDownCall p)
 {
     using Dot = MoeDot<BF16, BS, ST, ZP, 1, 2>;
     __shared__ float sums[4][256];
-    const unsigned col_tiles = static_cast<unsigned>(p.m.n + 15) / 16;
-    const unsigned index = blockIdx.x / col_tiles;
+    const unsigned index = blockIdx.z * gridDim.y + blockIdx.y;
+    if (index >= p.tiles) return;
     const int4 tile_at = p.route.tiles[index];
     if (tile_at.z == 0) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = static_cast<int>(blockIdx.x - index * col_tiles) * 16, live = min(p.m.n - n0, 16);
+    const int n0 = static_cast<int>(blockIdx.x) * 16, live = min(p.m.n - n0, 16);
     const Dot dot(p.m, live);
     const MoeTile<1> tile = moe_tile<ST, ZP, 1>(p.m, tile_at.x, n0, live);
     const uint16_t* const h = p.h + static_cast<int64_t>(tile_at.y + (dot.col < tile_at.z ? dot.col : 0)) * (2 * p.ip);
@@ -102,7 +102,7 @@ int launch_moe_down(const RocmMoeArgs& a, const MoeDownCall& p, int where, int t
         using ST = decltype(st);
         const unsigned n = static_cast<unsigned>(p.m.n);
         if (where == kMoeTable) hipLaunchKernelGGL((moe_down_few_kernel<BF16, BS, ST, ZP>), dim3((n + 15) / 16), dim3(512), 0, s, p);
-        else hipLaunchKernelGGL((moe_down_tiles_kernel<BF16, BS, ST, ZP>), dim3((n + 15) / 16 * static_cast<unsigned>(tiles)), dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((moe_down_tiles_kernel<BF16, BS, ST, ZP>), moe_grid((n + 15) / 16, tiles), dim3(256), 0, s, p);
         return static_cast<int>(hipGetLastError());
     });
 }

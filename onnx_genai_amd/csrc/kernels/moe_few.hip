@@ -33,33 +33,49 @@ struct Elements32 {
     // `count` of them are there (a multiple of 8), the rest is zero
     __device__ __forceinline__ void load(const uint16_t* x, int count)
     {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put(j, j * 8 < count ? *reinterpret_cast<const uint4*>(x + j * 8) : make_uint4(0, 0, 0, 0));
+    }
+    __device__ __forceinline__ void put(int j, const uint4& d)
+    {
+        v[4 * j] = d.x;
+        v[4 * j + 1] = d.y;
+        v[4 * j + 2] = d.z;
+        v[4 * j + 3] = d.w;
+    }
+    __device__ __forceinline__ void order()
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put(j, ordered(make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3])));
+        add_up();
+    }
+    __device__ __forceinline__ void add_up()
+    {
         constexpr uint32_t kOnes = BF16 ? 0x3f803f80u : 0x3c003c00u;
-        sum = 0.f;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint4 d = make_uint4(0, 0, 0, 0);
-            if (j * 8 < count) d = *reinterpret_cast<const uint4*>(x + j * 8);
-            v[4 * j] = __builtin_amdgcn_perm(d.z, d.x, 0x05040100u);           // 0 | 4
-            v[4 * j + 1] = __builtin_amdgcn_perm(d.z, d.x, 0x07060302u);       // 1 | 5
-            v[4 * j + 2] = __builtin_amdgcn_perm(d.w, d.y, 0x05040100u);
-            v[4 * j + 3] = __builtin_amdgcn_perm(d.w, d.y, 0x07060302u);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum = dot2<BF16>(v[4 * j + i], kOnes, sum);
-        }
+        for (int i = 0; i < 16; ++i) s[i & 3] = dot2<BF16>(v[i], kOnes, s[i & 3]);
+        sum = (s[0] + s[1]) + (s[2] + s[3]);
+    }
+    static __device__ __forceinline__ uint4 ordered(const uint4& d)
+    {
+        return make_uint4(__builtin_amdgcn_perm(d.z, d.x, 0x05040100u), __builtin_amdgcn_perm(d.z, d.x, 0x07060302u), __builtin_amdgcn_perm(d.w, d.y, 0x05040100u),
+                          __builtin_amdgcn_perm(d.w, d.y, 0x07060302u));
     }
 };
 
+// `mask`: 0x000f000f in a vector register, which leaves room for the magic in a scalar one, so that each pair but the first is a shift and one and-or.
 template <bool BF16>
-__device__ __forceinline__ void nibbles32(const uint4& w, uint32_t (&out)[16])
+__device__ __forceinline__ void nibbles32(const uint4& w, uint32_t mask, uint32_t (&out)[16])
 {
-    constexpr uint32_t kMagic = BF16 ? 0x43004300u : 0x64006400u;
+    const uint32_t magic = opaque_scalar(BF16 ? 0x43004300u : 0x64006400u);
     uint32_t d[4] = {w.x, w.y, w.z, w.w};
     // unpacked for each row anew: kept for the next row, the nibbles of a wave's columns take 128 registers
     asm volatile("" : "+v"(d[0]), "+v"(d[1]), "+v"(d[2]), "+v"(d[3]));
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out[4 * j + i] = ((d[j] >> (4 * i)) & 0x000f000fu) | kMagic;
+        for (int i = 0; i < 4; ++i) out[4 * j + i] = ((d[j] >> (4 * i)) & mask) | magic;
 }
 
 // start + sum a (magic + q), in four chains
@@ -77,20 +93,22 @@ template <typename ST, bool ZP, int NU, int LPC>
 struct FewColumns {
     uint4 w[NU];
     typename ScaleIo<ST>::raw_t s[NU];
-    uint8_t z[NU];
+    uint32_t z[NU];
 
-    __device__ __forceinline__ void load(const MoeMatrix& m, const MoeTile<1>& t, int live, int k, int kl)
+    // k: the lane's first element. Columns that are not there lie beyond the tile's range and read as zeros; so may, or may not, what lies behind a row, whose
+    // activations are zero.
+    __device__ __forceinline__ void load(const MoeMatrix& m, const MoeTile<1>& t, int k, int shift)
     {
         const int group = (threadIdx.x & 63) / LPC;
-        const uint32_t block = static_cast<uint32_t>(min(k / m.block_size, m.kb - 1));
+        const uint32_t block = static_cast<uint32_t>(min(k >> shift, m.kb - 1));
+        const uint32_t first = static_cast<uint32_t>(group * m.row_step), step = static_cast<uint32_t>(64 / LPC * m.row_step);
+        const uint32_t row_bytes = static_cast<uint32_t>(m.row_bytes), kb = static_cast<uint32_t>(m.kb), zp_row = static_cast<uint32_t>(m.zp_row);
+        const uint32_t w_at = first * row_bytes + static_cast<uint32_t>(k) / 2, s_at = (first * kb + block) * static_cast<uint32_t>(sizeof(ST)), z_at = first * zp_row + block / 2;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            const int col = u * (64 / LPC) + group;
-            const uint32_t row = static_cast<uint32_t>(col) * static_cast<uint32_t>(m.row_step);
-            const bool is = col < live && kl >= 0;
-            w[u] = load16(t.w[0], is ? row * static_cast<uint32_t>(m.row_bytes) + static_cast<uint32_t>(k) / 2 : kOutOfRange, 0);
-            s[u] = ScaleIo<ST>::load_raw(t.s[0], is ? (row * static_cast<uint32_t>(m.kb) + block) * static_cast<uint32_t>(sizeof(ST)) : kOutOfRange, 0);
-            if constexpr (ZP) z[u] = __builtin_amdgcn_raw_buffer_load_b8(t.z[0], static_cast<int>(is ? row * static_cast<uint32_t>(m.zp_row) + block / 2 : kOutOfRange), 0, 0);
+            w[u] = load16(t.w[0], w_at + u * (step * row_bytes), 0);
+            s[u] = ScaleIo<ST>::load_raw(t.s[0], s_at + u * (step * kb * static_cast<uint32_t>(sizeof(ST))), 0);
+            if constexpr (ZP) z[u] = __builtin_amdgcn_raw_buffer_load_b8(t.z[0], static_cast<int>(z_at + u * (step * zp_row)), 0, 0);
         }
     }
 };
@@ -103,12 +121,14 @@ __device__ __forceinline__ void few_multiply(const FewColumns<ST, ZP, NU, LPC>& 
     float sum = a[0].sum;
     if constexpr (NH == 2) sum += a[1].sum;
     const float plain = -(kMagic + 8.f) * sum;
+    uint32_t mask = 0x000f000fu;
+    asm volatile("" : "+v"(mask));
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
         uint32_t q[16];
-        nibbles32<BF16>(c.w[u], q);
+        nibbles32<BF16>(c.w[u], mask, q);
         float start = plain;
-        if constexpr (ZP) start = (-kMagic - static_cast<float>(odd ? c.z[u] >> 4 : c.z[u] & 15)) * sum;
+        if constexpr (ZP) start = (-kMagic - static_cast<float>((c.z[u] >> odd) & 15u)) * sum;
         float d = dot32<BF16>(a[0].v, q, start);
         if constexpr (NH == 2) d += dot32<BF16>(a[1].v, q, 0.f);
         acc[u] = fmaf(factor * ScaleIo<ST>::to_f32(c.s[u], BF16), d, acc[u]);
@@ -121,108 +141,213 @@ __device__ __forceinline__ float over_lanes(float v)
 {
     auto add = [](float a, float b) { return a + b; };
     if constexpr (LPC == 64) return over_wave(v, add);
-    v += __shfl_xor(v, 8, 64);
-    v += __shfl_xor(v, 4, 64);
-    v += __shfl_xor(v, 2, 64);
-    v += __shfl_xor(v, 1, 64);
-    if constexpr (LPC == 32) v += __shfl_xor(v, 16, 64);
+    v = over_row(v, add);
+    if constexpr (LPC == 32) {
+        const uint32_t bits = __float_as_uint(v);
+        const auto s = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
     return v;
 }
 
 constexpr int kFewRows = 4;
 
 // What is known before the call's other arguments are read: in scalar registers when a wave starts.
-#define MOE_FEW_FIRST const void *logits, const uint16_t *x, int logits_dtype, int rows, int experts, int k, int normalize, unsigned col_tiles
+#define MOE_FEW_FIRST const void *logits, const uint16_t *x, int logits_dtype, int rows, int experts, int k, int normalize, int width
 
-// A wave has NU times 64 / LPC columns of gate and up, a workgroup four times as many.
+// A wave has NU times 64 / LPC columns of gate and up of one expert at a time; the tiles of all active experts, one behind the other, go round the waves of the
+// grid. The rows of x lie in LDS, in the order of the nibbles, a pass's first eight elements of each lane side by side, then the second eight ..., so that a read
+// meets every bank once.
 template <bool BF16, typename ST, bool ZP, int LPC>
 __global__ __launch_bounds__(256) void moe_few_up_kernel(MOE_FEW_FIRST, MoeUpCall p)
 {
-    constexpr int NU = 4, kCols = NU * 64 / LPC;
+    constexpr int NU = 4, kCols = NU * 64 / LPC, kPass = LPC * 32;
+    using Columns = FewColumns<ST, ZP, NU, LPC>;
     __shared__ MoeFewRouting routing;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const unsigned slot = blockIdx.x / col_tiles;
-    const int n0 = (static_cast<int>(blockIdx.x - slot * col_tiles) * 4 + wave) * kCols;
-    route_few(routing, logits, logits_dtype, rows, experts, k, normalize);
-    if (blockIdx.x == 0) write_table(routing, rows, k, p.table);
-    if (static_cast<int>(slot) >= routing.active || n0 >= p.ip) return;
-    const int expert = __builtin_amdgcn_readfirstlane(routing.chosen[slot]);
-    const int live = min(p.m.n - n0, kCols);
-    float g[kFewRows][NU] = {}, u[kFewRows][NU] = {};
-    unsigned chose = 0;
+    __shared__ int32_t chose_of[kFewPairs];                              // bit t: token t chose it
+    extern __shared__ __attribute__((aligned(16))) uint4 staged[];      // [rows][pass][4][LPC]
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, kl = lane % LPC;
+    const int passes = static_cast<unsigned>(width + kPass - 1) / kPass;
+    const unsigned pieces = passes * (kPass / 8);
+    const bool ranks = ranks_few(rows, experts);
+    const float logit = ranks ? few_logit(logits, logits_dtype, rows, experts) : 0.f;
     for (int t = 0; t < rows; ++t)
-        for (int j = 0; j < k; ++j) chose |= static_cast<unsigned>(routing.expert[t * k + j] == expert) << t;
-    chose = __builtin_amdgcn_readfirstlane(chose);
-    if (live > 0) {
-        MoeMatrix up = p.m;
-        up.w[0] = p.m.w[1];
-        const MoeTile<1> tg = moe_tile<ST, ZP, 1>(p.m, expert, n0, live), tu = moe_tile<ST, ZP, 1>(up, expert, n0, live);
-        const int kl = lane % LPC, width = static_cast<int>(p.ldx);
-        FewColumns<ST, ZP, NU, LPC> cg, cu;
-        for (int k0 = 0; k0 < width; k0 += LPC * 32) {
-            const int at = k0 + kl * 32, count = width - at;
-            cg.load(p.m, tg, live, at, count > 0 ? kl : -1);
-            cu.load(p.m, tu, live, at, count > 0 ? kl : -1);
-            const int odd = (at / p.m.block_size) & 1;
-#pragma unroll
-            for (int t = 0; t < kFewRows; ++t) {
-                if (!(chose >> t & 1)) continue;
-                Elements32<BF16> a[1];
-                a[0].load(x + t * p.ldx + at, count);
-                few_multiply<BF16, ST, ZP, NU, LPC, 1>(cg, a, odd, 1.f, g[t]);
-                few_multiply<BF16, ST, ZP, NU, LPC, 1>(cu, a, odd, 1.f, u[t]);
-            }
+        for (unsigned piece = threadIdx.x; piece < pieces; piece += 256) {
+            const unsigned l = piece / 4;
+            const uint4 d = piece * 8 < static_cast<unsigned>(width) ? *reinterpret_cast<const uint4*>(x + static_cast<int64_t>(t) * width + piece * 8) : make_uint4(0, 0, 0, 0);
+            staged[((t * passes + l / LPC) * 4 + piece % 4) * LPC + l % LPC] = Elements32<BF16>::ordered(d);
         }
+    if (ranks) rank_few(routing, logit, rows, experts, k, normalize);
+    else route_few<4>(routing, logits, logits_dtype, rows, experts, k, normalize);
+    if (blockIdx.x == 0) write_table(routing, rows, k, p.table);
+    if (rows > 1) {
+        for (int i = threadIdx.x; i < routing.active; i += 256) {
+            int bits = 0;
+            for (int t = 0; t < rows; ++t)
+                for (int j = 0; j < k; ++j) bits |= (routing.expert[t * k + j] == routing.chosen[i]) << t;
+            chose_of[i] = bits;
+        }
+        __syncthreads();
     }
-    // lane u of a column's lanes keeps column u's result
-    const int mine = lane % LPC, col = n0 + mine * (64 / LPC) + lane / LPC;
-#pragma unroll
-    for (int t = 0; t < kFewRows; ++t) {
-        if (!(chose >> t & 1)) continue;
-        float gate = 0.f, upv = 0.f;
-#pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            const float a = over_lanes<LPC>(g[t][i]), b = over_lanes<LPC>(u[t][i]);
-            if (mine == i) {
-                gate = a;
-                upv = b;
-            }
+
+    const int shift = 31 - __builtin_clz(p.m.block_size);
+    MoeMatrix up = p.m;
+    up.w[0] = p.m.w[1];
+    // A unit is a pass over a tile's K. No division: a wave counts its way through units, and an integer division is forty instructions.
+    const int tiles = static_cast<int>((static_cast<unsigned>(p.ip) + kCols - 1) / kCols), step = static_cast<int>(gridDim.x) * 4, active = routing.active;
+    struct Place {
+        int slot, tile, pass;
+    };
+    auto settle = [&](Place& at) {
+        while (at.tile >= tiles) {
+            at.tile -= tiles;
+            ++at.slot;
         }
-        if (mine < NU && col < p.ip) store_h<BF16>(p, static_cast<int64_t>(slot) * kFewRows + t, col, col < p.m.n ? moe_gated(p, expert, col, gate, upv) : 0.f);
+    };
+    auto next = [&](Place& at) {
+        if (++at.pass < passes) return;
+        at.pass = 0;
+        at.tile += step;
+        settle(at);
+    };
+    Place ahead{0, static_cast<int>(blockIdx.x) * 4 + wave, 0};
+    settle(ahead);
+    Place now = ahead;
+    float g[kFewRows][NU] = {}, u[kFewRows][NU] = {};
+    Columns cg[2], cu[2];
+    auto load = [&](Columns& to_g, Columns& to_u) {
+        const int at = ahead.pass * kPass + kl * 32;
+        const bool is = ahead.slot < active;
+        const int expert = __builtin_amdgcn_readfirstlane(routing.chosen[is ? ahead.slot : 0]);
+        // (a tile of columns behind the last, whose h is zero, reads the last column)
+        const int n0 = is ? min(ahead.tile * kCols, p.m.n - 1) : 0, live = is ? min(p.m.n - n0, kCols) : 0;
+        to_g.load(p.m, moe_tile<ST, ZP, 1>(p.m, expert, n0, live), at, shift);
+        to_u.load(p.m, moe_tile<ST, ZP, 1>(up, expert, n0, live), at, shift);
+        next(ahead);
+    };
+    auto multiply = [&](const Columns& of_g, const Columns& of_u) {
+        const int pass = now.pass, slot = now.slot, odd = ((pass * kPass + kl * 32) >> shift & 1) * 4;
+        const int chose = rows > 1 ? __builtin_amdgcn_readfirstlane(chose_of[slot]) : 1;
+#pragma unroll
+        for (int t = 0; t < kFewRows; ++t) {
+            if (!(chose >> t & 1)) continue;
+            Elements32<BF16> a[1];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[0].put(j, staged[((t * passes + pass) * 4 + j) * LPC + kl]);
+            a[0].add_up();
+            few_multiply<BF16, ST, ZP, NU, LPC, 1>(of_g, a, odd, 1.f, g[t]);
+            few_multiply<BF16, ST, ZP, NU, LPC, 1>(of_u, a, odd, 1.f, u[t]);
+        }
+        if (pass != static_cast<int>(passes) - 1) return next(now);
+        // the tile's sums; lane i of a column's lanes keeps column i's
+        const int expert = __builtin_amdgcn_readfirstlane(routing.chosen[slot]), col = now.tile * kCols + kl * (64 / LPC) + lane / LPC;
+#pragma unroll
+        for (int t = 0; t < kFewRows; ++t) {
+            if (!(chose >> t & 1)) continue;
+            float gate = 0.f, upv = 0.f;
+#pragma unroll
+            for (int i = 0; i < NU; ++i) {
+                const float a = over_lanes<LPC>(g[t][i]), b = over_lanes<LPC>(u[t][i]);
+                if (kl == i) {
+                    gate = a;
+                    upv = b;
+                }
+                g[t][i] = u[t][i] = 0.f;
+            }
+            if (kl < NU && col < p.ip) store_h<BF16>(p, static_cast<int64_t>(slot) * kFewRows + t, col, col < p.m.n ? moe_gated(p, expert, col, gate, upv) : 0.f);
+        }
+        next(now);
+    };
+    // two units' loads in flight; those behind the last read nothing (a tile of no columns), but are asked for all the same: a branch would have every load waited for
+    if (now.slot >= active) return;
+    load(cg[0], cu[0]);
+    while (true) {
+        load(cg[1], cu[1]);
+        multiply(cg[0], cu[0]);
+        if (now.slot >= active) break;
+        load(cg[0], cu[0]);
+        multiply(cg[1], cu[1]);
+        if (now.slot >= active) break;
     }
 }
 
-// A wave has eight columns and a share of the experts' K; a workgroup's waves have the same columns.
+// A wave has eight columns and a share of the experts' K; a workgroup's waves have the same columns. An item is one pass over one expert's K; its weights and
+// the first row that it meets are asked for one item ahead.
 template <bool BF16, typename ST, bool ZP, int LPC>
-__global__ __launch_bounds__(512) void moe_few_down_kernel(MoeDownCall p)
+__global__ __launch_bounds__(512) void moe_few_down_kernel(const MoeFewTable* table, int slots, MoeDownCall p)
 {
-    constexpr int NU = LPC / 8, kCols = 8;
+    constexpr int NU = LPC / 8, kCols = 8, kPass = LPC * 32;
+    struct Item {
+        FewColumns<ST, ZP, NU, LPC> c;
+        Elements32<BF16> a[2];
+    };
     __shared__ float sums[8][kFewRows][kCols];
     __shared__ float weight[kFewPairs][kFewRows];
     __shared__ int32_t chosen[kFewPairs];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63;
-    const int n0 = static_cast<int>(blockIdx.x) * kCols, live = min(p.m.n - n0, kCols);
-    const int active = p.table->active;
-    for (int i = threadIdx.x; i < active * kFewRows; i += blockDim.x) weight[i / kFewRows][i % kFewRows] = p.table->weight[i / kFewRows][i % kFewRows];
-    for (int i = threadIdx.x; i < active; i += blockDim.x) chosen[i] = p.table->expert[i];
+    __shared__ float base[kFewRows];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63, kl = lane % LPC;
+    if (threadIdx.x < kFewRows) base[threadIdx.x] = table->base[threadIdx.x];
+    for (int i = threadIdx.x; i < slots * kFewRows; i += blockDim.x) weight[i / kFewRows][i % kFewRows] = table->weight[i / kFewRows][i % kFewRows];
+    for (int i = threadIdx.x; i < slots; i += blockDim.x) chosen[i] = table->expert[i];
+    const int active = table->active;
     __syncthreads();
-    const int kl = lane % LPC, width = static_cast<int>(p.ip), passes = (width + LPC * 32 - 1) / (LPC * 32);
+    const int n0 = static_cast<int>(blockIdx.x) * kCols, live = min(p.m.n - n0, kCols);
+    const int shift = 31 - __builtin_clz(p.m.block_size), width = static_cast<int>(p.ip), passes = static_cast<int>(static_cast<unsigned>(width + kPass - 1) / kPass);
+    struct Place {
+        int slot, pass;
+    };
+    auto settle = [&](Place& at) {
+        while (at.pass >= passes) {
+            at.pass -= passes;
+            ++at.slot;
+        }
+    };
+    Place ahead{0, wave};
+    settle(ahead);
+    Place now = ahead;
     float acc[kFewRows][NU] = {};
-    for (int item = wave; item < active * passes; item += waves) {
-        const int slot = item / passes, at = (item - slot * passes) * (LPC * 32) + kl * 32, count = width - at;
-        const MoeTile<1> tile = moe_tile<ST, ZP, 1>(p.m, __builtin_amdgcn_readfirstlane(chosen[slot]), n0, live);
-        FewColumns<ST, ZP, NU, LPC> c;
-        c.load(p.m, tile, live, at, count > 0 ? kl : -1);
-        const int odd = (at / p.m.block_size) & 1;
+    auto first_row = [&](int slot) {
+        int t = 0;
+        while (t < kFewRows - 1 && !(weight[slot][t] > 0.f)) ++t;
+        return __builtin_amdgcn_readfirstlane(t);
+    };
+    auto rows_of = [&](int slot, int t, int at, Elements32<BF16> (&a)[2]) {
+        const uint16_t* const h = p.h + (static_cast<int64_t>(slot) * kFewRows + t) * (2 * p.ip) + at;
+        a[0].load(h, width - at);
+        a[1].load(h + p.ip, width - at);
+    };
+    auto load = [&](Item& to) {
+        const bool is = ahead.slot < active;
+        const int slot = is ? ahead.slot : 0, at = ahead.pass * kPass + kl * 32;
+        to.c.load(p.m, moe_tile<ST, ZP, 1>(p.m, __builtin_amdgcn_readfirstlane(chosen[slot]), n0, is ? live : 0), at, shift);
+        rows_of(slot, p.rows > 1 ? first_row(slot) : 0, at, to.a);
+        ahead.pass += waves;
+        settle(ahead);
+    };
+    auto multiply = [&](Item& of) {
+        const int slot = now.slot, at = now.pass * kPass + kl * 32, odd = (at >> shift & 1) * 4, first = p.rows > 1 ? first_row(slot) : 0;
+        now.pass += waves;
+        settle(now);
 #pragma unroll
         for (int t = 0; t < kFewRows; ++t) {
             const float w = weight[slot][t];
             if (!(w > 0.f)) continue;
-            const uint16_t* const h = p.h + (static_cast<int64_t>(slot) * kFewRows + t) * (2 * p.ip) + at;
-            Elements32<BF16> a[2];
-            a[0].load(h, count);
-            a[1].load(h + p.ip, count);
-            few_multiply<BF16, ST, ZP, NU, LPC, 2>(c, a, odd, w, acc[t]);
+            if (t != first) rows_of(slot, t, at, of.a);
+            of.a[0].order();
+            of.a[1].order();
+            few_multiply<BF16, ST, ZP, NU, LPC, 2>(of.c, of.a, odd, w, acc[t]);
+        }
+    };
+    if (now.slot < active) {
+        Item one, two;
+        load(one);
+        while (true) {
+            load(two);
+            multiply(one);
+            if (now.slot >= active) break;
+            load(one);
+            multiply(two);
+            if (now.slot >= active) break;
         }
     }
 #pragma unroll
@@ -235,11 +360,12 @@ __global__ __launch_bounds__(512) void moe_few_down_kernel(MoeDownCall p)
         }
     }
     __syncthreads();
-    const int row = threadIdx.x / kCols, c = threadIdx.x % kCols;
-    if (row >= p.rows || c >= live) return;
-    float v = p.table->base[row];
-    for (int w = 0; w < waves; ++w) v += sums[w][row][c];
-    const int64_t col = n0 + c;
+    const int row = static_cast<int>(threadIdx.x) / kCols, col_in = static_cast<int>(threadIdx.x) % kCols;
+    if (row >= p.rows || col_in >= live) return;
+    float v = base[row];
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += w < waves ? sums[w][row][col_in] : 0.f;
+    const int64_t col = n0 + col_in;
     if (p.m.w[0].bias)
         for (int i = 0; i < active; ++i) {
             const float f = weight[i][row];
@@ -280,14 +406,20 @@ int launch_moe_few(const RocmMoeArgs& a, const MoeUpCall& up, const MoeDownCall&
 {
     int rc = few_build(a, a.gate.zp != nullptr, lanes_per_column(up.ldx), [&](auto bf, auto st, auto zp, auto lanes) {
         constexpr int LPC = decltype(lanes)::value;
-        const unsigned col_tiles = static_cast<unsigned>((up.ip + 1024 / LPC - 1) / (1024 / LPC));
-        hipLaunchKernelGGL((moe_few_up_kernel<decltype(bf)::value, decltype(st), decltype(zp)::value, LPC>), dim3(col_tiles * static_cast<unsigned>(slots)), dim3(256), 0, s, up.logits, up.x,
-                           up.logits_dtype, up.rows, up.experts, up.k, up.normalize, col_tiles, up);
+        // each workgroup routes first, which takes it 3 us: no more of them than run at once
+        const int64_t waves = slots * ((up.ip + 256 / LPC - 1) / (256 / LPC));
+        const unsigned grid = static_cast<unsigned>((waves + 3) / 4 < 2 * rocm_ffi_compute_units() ? (waves + 3) / 4 : 2 * rocm_ffi_compute_units());
+        const size_t lds = static_cast<size_t>(up.rows) * ((up.ldx + LPC * 32 - 1) / (LPC * 32)) * (LPC * 64);
+        auto kernel = moe_few_up_kernel<decltype(bf)::value, decltype(st), decltype(zp)::value, LPC>;
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), lds, s, up.logits, up.x, up.logits_dtype, up.rows, up.experts, up.k, up.normalize,
+                           static_cast<int>(up.ldx), up);
         return static_cast<int>(hipGetLastError());
     });
     if (rc != 0) return rc;
     return few_build(a, a.down.zp != nullptr, lanes_per_column(down.ip), [&](auto bf, auto st, auto zp, auto lanes) {
-        hipLaunchKernelGGL((moe_few_down_kernel<decltype(bf)::value, decltype(st), decltype(zp)::value, decltype(lanes)::value>), dim3(static_cast<unsigned>(down.m.n + 7) / 8), dim3(512), 0, s, down);
+        const unsigned grid = static_cast<unsigned>(down.m.n + 7) / 8, threads = grid <= static_cast<unsigned>(rocm_ffi_compute_units()) ? 512 : 256;
+        auto kernel = moe_few_down_kernel<decltype(bf)::value, decltype(st), decltype(zp)::value, decltype(lanes)::value>;
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, s, down.table, slots, down);
         return static_cast<int>(hipGetLastError());
     });
 }

@@ -14,9 +14,9 @@ __global__ __launch_bounds__(256) void moe_gate_up_kernel(MoeUpCall p)
     using Dot = MoeDot<BF16, BS, ST, ZP, 2, 1>;
     __shared__ float sums[4][2][256];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const unsigned col_tiles = static_cast<unsigned>(p.ip) / 16;
-    const unsigned slot = blockIdx.x / col_tiles;
-    const int n0 = static_cast<int>(blockIdx.x - slot * col_tiles) * 16;
+    const unsigned slot = blockIdx.z * gridDim.y + blockIdx.y;
+    const int n0 = static_cast<int>(blockIdx.x) * 16;
+    if (!TABLE && slot >= p.tiles) return;
     int expert, rows;
     int64_t h_row;
     if constexpr (TABLE) {
@@ -82,7 +82,7 @@ int launch_moe_gate_up(const RocmMoeArgs& a, const MoeUpCall& p, int where, int 
         constexpr bool BF16 = decltype(bf)::value, ZP = decltype(zp)::value;
         constexpr int BS = decltype(bs)::value;
         using ST = decltype(st);
-        const dim3 grid(static_cast<unsigned>(p.ip / 16) * static_cast<unsigned>(slots));
+        const dim3 grid = moe_grid(static_cast<unsigned>(p.ip / 16), slots);
         if (where == kMoeTable) hipLaunchKernelGGL((moe_gate_up_kernel<BF16, BS, ST, ZP, true>), grid, dim3(256), 0, s, p);
         else hipLaunchKernelGGL((moe_gate_up_kernel<BF16, BS, ST, ZP, false>), grid, dim3(256), 0, s, p);
         return static_cast<int>(hipGetLastError());

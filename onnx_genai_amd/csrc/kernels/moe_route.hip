@@ -27,7 +27,7 @@ __global__ __launch_bounds__(256) void moe_top_k_kernel(const void* logits, int 
 __global__ __launch_bounds__(1024) void moe_route_few_kernel(const void* logits, int dtype, int rows, int experts, int k, int normalize, MoeFewTable* table)
 {
     __shared__ MoeFewRouting routing;
-    route_few(routing, logits, dtype, rows, experts, k, normalize);
+    route_few<16>(routing, logits, dtype, rows, experts, k, normalize);
     write_table(routing, rows, k, table);
 }
 
@@ -72,9 +72,9 @@ __global__ __launch_bounds__(1024) void moe_plan_kernel(int pairs, int experts, 
 template <typename T, bool BF16>
 __global__ __launch_bounds__(256) void moe_combine_kernel(RocmMoeArgs a, MoeRoute r, const float* __restrict__ out)
 {
-    const unsigned parts = static_cast<unsigned>((a.hidden + 2047) / 2048);
-    const int64_t token = blockIdx.x / parts;
-    const int64_t h = (static_cast<int64_t>(blockIdx.x % parts) * 256 + threadIdx.x) * 8;
+    const int64_t token = static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y;
+    if (token >= a.rows) return;
+    const int64_t h = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8;
     const int left = static_cast<int>(a.hidden - h < 8 ? a.hidden - h : 8);
     if (left <= 0) return;
     float sum[8];
@@ -101,11 +101,10 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(RocmMoeArgs a, MoeRout
 }
 
 // Rows of `k` elements -> rows of `kp`, zeros behind: for rows that do not begin at a multiple of 16 bytes.
-__global__ __launch_bounds__(256) void moe_pad_rows_kernel(const uint16_t* __restrict__ from, int64_t k, int64_t kp, uint16_t* __restrict__ to)
+__global__ __launch_bounds__(256) void moe_pad_rows_kernel(const uint16_t* __restrict__ from, int64_t rows, int64_t k, int64_t kp, uint16_t* __restrict__ to)
 {
-    const unsigned parts = static_cast<unsigned>((kp + 2047) / 2048);
-    const int64_t row = blockIdx.x / parts, i = (static_cast<int64_t>(blockIdx.x % parts) * 256 + threadIdx.x) * 8;
-    if (i >= kp) return;
+    const int64_t row = static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y, i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8;
+    if (i >= kp || row >= rows) return;
     Eight<uint16_t, false> e;
     const int64_t left = k - i;
     if (left >= 8) e.load(from + row * k + i);
@@ -139,7 +138,7 @@ int launch_moe_plan(const RocmMoeArgs& a, int tile_rows, int max_tiles, const Mo
 
 int launch_moe_combine(const RocmMoeArgs& a, const MoeRoute& r, const float* out, hipStream_t s)
 {
-    const dim3 grid(static_cast<unsigned>((a.hidden + 2047) / 2048 * a.rows));
+    const dim3 grid = moe_grid(static_cast<unsigned>((a.hidden + 2047) / 2048), static_cast<int>(a.rows));
     if (a.dtype == ROCM_DT_BF16) hipLaunchKernelGGL((moe_combine_kernel<uint16_t, true>), grid, dim3(256), 0, s, a, r, out);
     else hipLaunchKernelGGL((moe_combine_kernel<uint16_t, false>), grid, dim3(256), 0, s, a, r, out);
     return static_cast<int>(hipGetLastError());
@@ -147,7 +146,7 @@ int launch_moe_combine(const RocmMoeArgs& a, const MoeRoute& r, const float* out
 
 int launch_moe_pad_rows(const void* from, int64_t rows, int64_t k, int64_t kp, void* to, hipStream_t s)
 {
-    hipLaunchKernelGGL(moe_pad_rows_kernel, dim3(static_cast<unsigned>((kp + 2047) / 2048 * rows)), dim3(256), 0, s, static_cast<const uint16_t*>(from), k, kp,
+    hipLaunchKernelGGL(moe_pad_rows_kernel, moe_grid(static_cast<unsigned>((kp + 2047) / 2048), static_cast<int>(rows)), dim3(256), 0, s, static_cast<const uint16_t*>(from), rows, k, kp,
                        static_cast<uint16_t*>(to));
     return static_cast<int>(hipGetLastError());
 }
