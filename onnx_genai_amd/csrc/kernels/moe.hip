@@ -8,13 +8,15 @@
 namespace mnb {
 namespace {
 
-constexpr int kTileRows = 16;
+// Pairs an expert from which tiles have 128 rows.
+constexpr int64_t kTallPairs = 48;
 
 struct MoePlan {
     int where;                 // kMoeFused, kMoeTable, kMoeTiles
     int slots;                 // experts that can be active, or tiles
-    int64_t kp, ip, pairs;
-    uint64_t table, expert, weight, pair_row, token, base, tiles, x, h, out, total;
+    int tile_rows;
+    int64_t kp, ip, pairs, eight_bytes;
+    uint64_t table, eights, expert, weight, pair_row, token, base, tiles, x, h, out, total;
 };
 
 MoePlan plan_of(const RocmMoeArgs& a)
@@ -23,9 +25,10 @@ MoePlan plan_of(const RocmMoeArgs& a)
     l.pairs = a.rows * a.k;
     // (the rows of x lie in the 48 KiB of LDS that a kernel gets without asking beside its tables)
     l.where = a.rows <= 4 && a.experts <= 256 && l.pairs <= kFewPairs && a.rows * ((a.hidden + 2047) / 2048) <= 12 ? kMoeFused : a.rows <= kFewTokens && l.pairs <= kFewPairs ? kMoeTable : kMoeTiles;
-    l.slots = static_cast<int>((l.where == kMoeTiles ? l.pairs / kTileRows : 0) + (l.pairs < a.experts ? l.pairs : a.experts));
+    l.tile_rows = l.pairs >= kTallPairs * a.experts ? 128 : 32;
+    l.slots = static_cast<int>((l.where == kMoeTiles ? l.pairs / l.tile_rows : 0) + (l.pairs < a.experts ? l.pairs : a.experts));
     l.kp = (a.hidden + 7) / 8 * 8;
-    l.ip = (a.inter + 127) / 128 * 128;
+    l.ip = (a.inter + 127) / 128 * 128;      // (steps of 64 and 128)
     auto part = [&](uint64_t bytes) {
         const uint64_t here = l.total;
         l.total += (bytes + 255) / 256 * 256;
@@ -41,8 +44,10 @@ MoePlan plan_of(const RocmMoeArgs& a)
     l.tiles = part(tiled ? static_cast<uint64_t>(l.slots) * 16 : 0);
     // rows that do not begin at multiples of 16 bytes are copied: the address may be any
     l.x = part(a.rows * l.kp * 2);
-    const int64_t rows_of_h = tiled ? l.pairs : l.slots * (l.where == kMoeFused ? 4 : 16);
-    l.h = part(rows_of_h * l.ip * 4);
+    l.eight_bytes = tiled && (!a.gate.zp || !a.down.zp) ? ((l.kp > l.ip ? l.kp : l.ip) + 63) / 64 + 1 : 0;
+    l.eights = part(l.eight_bytes);
+    // (few tokens: two parts of every value of h)
+    l.h = part(tiled ? l.pairs * l.ip * 2 : l.slots * (l.where == kMoeFused ? 4 : 16) * l.ip * 4);
     l.out = part(tiled ? l.pairs * a.hidden * 4 : 0);
     return l;
 }
@@ -71,7 +76,7 @@ extern "C" uint64_t rocm_moe_workspace_bytes(const RocmMoeArgs* args) { return m
 extern "C" const char* rocm_moe_variant(const RocmMoeArgs* args)
 {
     const int where = mnb::plan_of(*args).where;
-    return where == mnb::kMoeFused ? "moe_few" : where == mnb::kMoeTable ? "moe_table" : "moe_tiles";
+    return where == mnb::kMoeFused ? "moe_few" : where == mnb::kMoeTable ? "moe_table" : mnb::plan_of(*args).tile_rows == 128 ? "moe_tall_tiles" : "moe_tiles";
 }
 
 extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_stream_t stream)
@@ -89,7 +94,7 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     if (l.where == kMoeTable) rc = launch_moe_route_few(a, table, s);
     if (l.where == kMoeTiles) {
         rc = launch_moe_top_k(a, route, s);
-        if (rc == 0) rc = launch_moe_plan(a, kTileRows, l.slots, route, s);
+        if (rc == 0) rc = launch_moe_plan(a, l.tile_rows, l.slots, route, ws + l.eights, static_cast<int>(l.eight_bytes), s);
     }
     const void* x = a.x;
     if (rc == 0 && (l.kp != a.hidden || reinterpret_cast<uintptr_t>(a.x) % 16 != 0)) {
@@ -106,8 +111,6 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     up.alpha = a.alpha;
     up.beta = a.beta;
     up.limit = a.limit;
-    up.route = route;
-    up.tiles = static_cast<unsigned>(l.slots);
     up.table = table;
     up.logits = a.logits;
     up.logits_dtype = a.logits_dtype;
@@ -119,15 +122,37 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     down.m = matrix_of(a, a.down, nullptr, a.inter, a.hidden, a.hidden, 1);
     down.h = up.h;
     down.ip = l.ip;
-    down.route = route;
-    down.tiles = up.tiles;
     down.table = table;
     down.rows = up.rows;
     down.y = a.y;
     down.out = reinterpret_cast<float*>(ws + l.out);
     if (l.where == kMoeFused) return launch_moe_few(a, up, down, l.slots, s);
-    rc = launch_moe_gate_up(a, up, l.where, l.slots, s);
-    if (rc == 0) rc = launch_moe_down(a, down, l.where, l.slots, s);
-    if (rc == 0 && l.where == kMoeTiles) rc = launch_moe_combine(a, route, down.out, s);
-    return rc;
+    if (l.where == kMoeTable) {
+        rc = launch_moe_gate_up(a, up, l.slots, s);
+        return rc != 0 ? rc : launch_moe_down(a, down, s);
+    }
+    auto tiled = [&](const MoeMatrix& m, const uint16_t* rows, int64_t ldx) {
+        MoeTileCall t{};
+        t.m = m;
+        if (!m.w[0].zp) {
+            t.m.w[0].zp = t.m.w[1].zp = ws + l.eights;
+            t.m.zp_row = 0;
+        }
+        t.x = rows;
+        t.ldx = ldx;
+        t.tiles = route.tiles;
+        t.count = static_cast<unsigned>(l.slots);
+        t.h = up.h;
+        t.ldh = l.ip;
+        t.out = down.out;
+        t.alpha = a.alpha;
+        t.beta = a.beta;
+        t.limit = a.limit;
+        return t;
+    };
+    MoeTileCall first = tiled(up.m, up.x, up.ldx), second = tiled(down.m, up.h, l.ip);
+    first.token = route.token;
+    rc = launch_moe_tile(a, first, true, l.tile_rows, s);
+    if (rc == 0) rc = launch_moe_tile(a, second, false, l.tile_rows, s);
+    return rc != 0 ? rc : launch_moe_combine(a, route, down.out, s);
 }

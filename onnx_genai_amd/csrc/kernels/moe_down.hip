@@ -62,47 +62,16 @@ __global__ __launch_bounds__(512) void moe_down_few_kernel(MoeDownCall p)
     store_from_f32(p.y, BF16 ? ROCM_DT_BF16 : ROCM_DT_F16, row * static_cast<int64_t>(p.m.n) + col, v);
 }
 
-// Tiles of up to 16 pairs: out[pair] = h W2^T, in f32. A workgroup has 16 columns, K split over its waves.
-template <bool BF16, int BS, typename ST, bool ZP>
-__global__ __launch_bounds__(256) void moe_down_tiles_kernel(MoeDownCall p)
-{
-    using Dot = MoeDot<BF16, BS, ST, ZP, 1, 2>;
-    __shared__ float sums[4][256];
-    const unsigned index = blockIdx.z * gridDim.y + blockIdx.y;
-    if (index >= p.tiles) return;
-    const int4 tile_at = p.route.tiles[index];
-    if (tile_at.z == 0) return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = static_cast<int>(blockIdx.x) * 16, live = min(p.m.n - n0, 16);
-    const Dot dot(p.m, live);
-    const MoeTile<1> tile = moe_tile<ST, ZP, 1>(p.m, tile_at.x, n0, live);
-    const uint16_t* const h = p.h + static_cast<int64_t>(tile_at.y + (dot.col < tile_at.z ? dot.col : 0)) * (2 * p.ip);
-    const int steps = static_cast<int>(p.ip / 128);
-    f32x4_t total[1] = {};
-    moe_pipeline<typename Dot::Step>(steps * wave / 4, steps * (wave + 1) / 4, [&](typename Dot::Step& s, int t) { dot.template load<false>(s, tile, t, h, dot.col < tile_at.z, p.ip, 0); },
-                                     [&](const typename Dot::Step& s, int) { dot.multiply(s, total); });
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sums[wave][(dot.g * 4 + i) * 16 + dot.col] = total[0][i];
-    __syncthreads();
-    const int row = threadIdx.x >> 4, c = threadIdx.x & 15;
-    if (row >= tile_at.z || c >= live) return;
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) v += sums[w][threadIdx.x];
-    p.out[static_cast<int64_t>(tile_at.y + row) * p.m.n + n0 + c] = v;
-}
-
 }  // namespace
 
-int launch_moe_down(const RocmMoeArgs& a, const MoeDownCall& p, int where, int tiles, hipStream_t s)
+int launch_moe_down(const RocmMoeArgs& a, const MoeDownCall& p, hipStream_t s)
 {
     return moe_build(a, a.down.zp != nullptr, [&](auto bf, auto bs, auto st, auto zp) {
         constexpr bool BF16 = decltype(bf)::value, ZP = decltype(zp)::value;
         constexpr int BS = decltype(bs)::value;
         using ST = decltype(st);
         const unsigned n = static_cast<unsigned>(p.m.n);
-        if (where == kMoeTable) hipLaunchKernelGGL((moe_down_few_kernel<BF16, BS, ST, ZP>), dim3((n + 15) / 16), dim3(512), 0, s, p);
-        else hipLaunchKernelGGL((moe_down_tiles_kernel<BF16, BS, ST, ZP>), moe_grid((n + 15) / 16, tiles), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((moe_down_few_kernel<BF16, BS, ST, ZP>), dim3((n + 15) / 16), dim3(512), 0, s, p);
         return static_cast<int>(hipGetLastError());
     });
 }

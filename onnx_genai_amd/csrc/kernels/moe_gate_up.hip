@@ -6,41 +6,25 @@
 namespace mnb {
 namespace {
 
-// TABLE: up to 16 tokens, every active expert with a row for each, zero where the token did not choose it; else tiles of up to 16 pairs sorted by expert.
-// A workgroup has 16 columns of gate and of up, K split over its waves.
-template <bool BF16, int BS, typename ST, bool ZP, bool TABLE>
+// Up to 16 tokens: every active expert has a row for each, zero where the token did not choose it. A workgroup has 16 columns of gate and of up, K split over
+// its waves.
+template <bool BF16, int BS, typename ST, bool ZP>
 __global__ __launch_bounds__(256) void moe_gate_up_kernel(MoeUpCall p)
 {
     using Dot = MoeDot<BF16, BS, ST, ZP, 2, 1>;
     __shared__ float sums[4][2][256];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const unsigned slot = blockIdx.z * gridDim.y + blockIdx.y;
-    const int n0 = static_cast<int>(blockIdx.x) * 16;
-    if (!TABLE && slot >= p.tiles) return;
-    int expert, rows;
-    int64_t h_row;
-    if constexpr (TABLE) {
-        if (static_cast<int>(slot) >= p.table->active) return;
-        expert = p.table->expert[slot];
-        rows = p.rows;
-        h_row = static_cast<int64_t>(slot) * kFewTokens;
-    } else {
-        const int4 tile = p.route.tiles[slot];
-        if (tile.z == 0) return;
-        expert = tile.x;
-        h_row = tile.y;
-        rows = tile.z;
-    }
+    const int slot = static_cast<int>(blockIdx.y), n0 = static_cast<int>(blockIdx.x) * 16;
+    if (slot >= p.table->active) return;
+    const int expert = p.table->expert[slot];
+    const int64_t h_row = static_cast<int64_t>(slot) * kFewTokens;
     const int live = min(p.m.n - n0, 16);
     if (live > 0) {
         f32x4_t total[2] = {};
         const Dot dot(p.m, live);
         const MoeTile<2> tile = moe_tile<ST, ZP, 2>(p.m, expert, n0, live);
-        bool has = dot.col < rows;
-        if constexpr (TABLE) has = has && p.table->weight[slot][dot.col] > 0.f;
-        int64_t token = has ? dot.col : 0;
-        if constexpr (!TABLE) token = p.route.token[h_row + token];
-        const uint16_t* const x = p.x + token * p.ldx;
+        const bool has = p.table->weight[slot][dot.col] > 0.f;
+        const uint16_t* const x = p.x + (has ? dot.col : 0) * p.ldx;
         const int steps = static_cast<int>((p.ldx + 127) / 128), whole = static_cast<int>(p.ldx / 128);
         const int begin = steps * wave / 4, end = steps * (wave + 1) / 4;
         moe_pipeline<typename Dot::Step>(begin, min(end, whole), [&](typename Dot::Step& s, int t) { dot.template load<false>(s, tile, t, x, has, 0, 0); },
@@ -58,11 +42,8 @@ __global__ __launch_bounds__(256) void moe_gate_up_kernel(MoeUpCall p)
     }
     __syncthreads();
     const int row = threadIdx.x >> 4, col = n0 + (threadIdx.x & 15);
-    if (row >= (TABLE ? static_cast<int>(kFewTokens) : rows)) return;
-    bool chose = row < rows;
-    if constexpr (TABLE) chose = p.table->weight[slot][row] > 0.f;
     float v = 0.f;
-    if (chose && col < p.m.n) {
+    if (p.table->weight[slot][row] > 0.f && col < p.m.n) {
         float g = 0.f, u = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -76,15 +57,13 @@ __global__ __launch_bounds__(256) void moe_gate_up_kernel(MoeUpCall p)
 
 }  // namespace
 
-int launch_moe_gate_up(const RocmMoeArgs& a, const MoeUpCall& p, int where, int slots, hipStream_t s)
+int launch_moe_gate_up(const RocmMoeArgs& a, const MoeUpCall& p, int slots, hipStream_t s)
 {
     return moe_build(a, a.gate.zp != nullptr, [&](auto bf, auto bs, auto st, auto zp) {
         constexpr bool BF16 = decltype(bf)::value, ZP = decltype(zp)::value;
         constexpr int BS = decltype(bs)::value;
         using ST = decltype(st);
-        const dim3 grid = moe_grid(static_cast<unsigned>(p.ip / 16), slots);
-        if (where == kMoeTable) hipLaunchKernelGGL((moe_gate_up_kernel<BF16, BS, ST, ZP, true>), grid, dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((moe_gate_up_kernel<BF16, BS, ST, ZP, false>), grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL((moe_gate_up_kernel<BF16, BS, ST, ZP>), dim3(static_cast<unsigned>(p.ip / 16), static_cast<unsigned>(slots)), dim3(256), 0, s, p);
         return static_cast<int>(hipGetLastError());
     });
 }

@@ -32,10 +32,11 @@ __global__ __launch_bounds__(1024) void moe_route_few_kernel(const void* logits,
 }
 
 // One workgroup sorts the pairs and cuts the tiles.
-__global__ __launch_bounds__(1024) void moe_plan_kernel(int pairs, int experts, int k, int tile_rows, int max_tiles, MoeRoute r)
+__global__ __launch_bounds__(1024) void moe_plan_kernel(int pairs, int k, int tile_rows, int max_tiles, MoeRoute r, uint8_t* eights, int eight_bytes)
 {
     __shared__ int count[1024], rows_to[1024], tiles_to[1024];
     const int t = threadIdx.x;
+    for (int i = t; i < eight_bytes; i += 1024) eights[i] = 0x88;
     count[t] = 0;
     __syncthreads();
     for (int p = t; p < pairs; p += 1024) {
@@ -130,9 +131,9 @@ int launch_moe_route_few(const RocmMoeArgs& a, MoeFewTable* table, hipStream_t s
     return static_cast<int>(hipGetLastError());
 }
 
-int launch_moe_plan(const RocmMoeArgs& a, int tile_rows, int max_tiles, const MoeRoute& r, hipStream_t s)
+int launch_moe_plan(const RocmMoeArgs& a, int tile_rows, int max_tiles, const MoeRoute& r, uint8_t* eights, int eight_bytes, hipStream_t s)
 {
-    hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, s, static_cast<int>(a.rows * a.k), a.experts, a.k, tile_rows, max_tiles, r);
+    hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, s, static_cast<int>(a.rows * a.k), a.k, tile_rows, max_tiles, r, eights, eight_bytes);
     return static_cast<int>(hipGetLastError());
 }
 

@@ -1,0 +1,199 @@
+// QMoE over tiles of pairs sorted by expert, on v_mfma_f32_32x32x16_{f16,bf16}: 32 TM rows by 64 columns of gate and of up, or by 128 of down.
+//
+// A wave has all rows of the tile and 32 columns of weights that no other wave has (16 of gate beside 16 of up), so that it unpacks them for itself, from
+// registers into the matrix core; only activations go through LDS, in the order in which a dword's nibbles come out (0 4 1 5 2 6 3 7 of each eight).
+// Weights enter the matrix core as q - zp, which is exact in 16 bits, and each block's sum is scaled in f32: no weight is rounded.
+// TM = 4 (prompts): the matrix cores and the vector instructions beside them bound it, 64 to scale a block's sums and 72 (bf16: 152) to unpack 64 k for 512
+// cycles of products. TM = 1 (a few rows an expert): the weights' bytes.
+// h is rounded to the activations' type here (as a graph of separate nodes has it): a second part of it would be half again as many products in the second half.
+#include "moe.hiph"
+#include "prefill_common.hiph"
+#include "rows.hiph"
+
+namespace mnb {
+namespace {
+
+template <bool BF16, int BS, typename ST, bool UP, int TM>
+__global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileCall p)
+{
+    constexpr int kPitch = 9;                                            // pieces of 16 bytes from a row of 64 elements in LDS to the next
+    constexpr int kScales = BS == 32 ? 2 : 1;                            // blocks of a step
+    __shared__ uint4 staged[2][TM * 32 * kPitch];
+    const unsigned index = blockIdx.z * gridDim.y + blockIdx.y;
+    if (index >= p.count) return;
+    const int4 tile = p.tiles[index];
+    if (tile.z == 0) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, g = lane >> 5;
+    const int col = UP ? static_cast<int>(blockIdx.x) * 64 + wave * 16 + (c & 15) : static_cast<int>(blockIdx.x) * 128 + wave * 32 + c;
+    const int which = UP ? c >> 4 : 0;
+    const int64_t at = tile.x * p.m.expert_step + static_cast<int64_t>(min(col, p.m.n - 1)) * p.m.row_step;       // (columns that are not there repeat the last)
+    const uint8_t* const b = (which ? p.m.w[1].b : p.m.w[0].b) + at * p.m.row_bytes;
+    const ST* const s = static_cast<const ST*>(which ? p.m.w[1].scales : p.m.w[0].scales) + at * p.m.kb;
+    const uint8_t* const z = (which ? p.m.w[1].zp : p.m.w[0].zp) + at * p.m.zp_row;
+    const int width = static_cast<int>(p.ldx), steps = (width + 63) >> 6, shift = 31 - __builtin_clz(p.m.block_size), row_bytes = static_cast<int>(p.m.row_bytes);
+
+    const int piece = threadIdx.x & 7;
+    const uint16_t* x[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int64_t row = tile.y + min(static_cast<int>(threadIdx.x >> 3) + i * 32, tile.z - 1);                // (nor are rows)
+        x[i] = p.x + (p.token ? p.token[row] : row) * p.ldx + piece * 8;
+    }
+    struct Weights {
+        uint4 w;
+        ST s[kScales];
+        uint32_t z;
+    };
+    auto load_w = [&](int t, Weights& to) {
+        const int byte = t * 32 + g * 16;
+        to.w = *reinterpret_cast<const uint4*>(b + (byte < row_bytes ? byte : 0));                                // (behind a row's end its activations are zero)
+        const int block = min(t * 64 >> shift, p.m.kb - 1);
+#pragma unroll
+        for (int i = 0; i < kScales; ++i) to.s[i] = s[min(block + i, p.m.kb - 1)];
+        to.z = z[block >> 1];
+    };
+    auto load_x = [&](int t, uint4 (&to)[TM]) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) to[i] = t * 64 + piece * 8 < width ? *reinterpret_cast<const uint4*>(x[i] + t * 64) : make_uint4(0, 0, 0, 0);
+    };
+    auto stage = [&](int t, const uint4 (&from)[TM]) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const uint4 d = from[i];
+            staged[t & 1][((threadIdx.x >> 3) + i * 32) * kPitch + piece] =
+                make_uint4(__builtin_amdgcn_perm(d.z, d.x, 0x05040100u), __builtin_amdgcn_perm(d.z, d.x, 0x07060302u), __builtin_amdgcn_perm(d.w, d.y, 0x05040100u),
+                           __builtin_amdgcn_perm(d.w, d.y, 0x07060302u));
+        }
+    };
+    uint32_t mask = 0x000f000fu;
+    asm volatile("" : "+v"(mask));
+    const uint32_t magic = opaque_scalar(0x64006400u);
+
+    float16_t total[TM] = {}, sum[TM] = {};
+    const float16_t none = {};
+    auto scale_of = [&](ST raw) {
+        if constexpr (sizeof(ST) == 4) return static_cast<float>(raw);
+        else return BF16 ? bf16_bits_to_f32(static_cast<uint16_t>(raw)) : f16_bits_to_f32(static_cast<uint16_t>(raw));
+    };
+    auto add_up = [&](float scale) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) total[i][e] = fmaf(scale, sum[i][e], total[i][e]);
+    };
+    // eight elements of each of the two lane groups, at pieces `at_piece` of the rows
+    auto product = [&](int t, uint32_t q, uint32_t zero, int at_piece, bool first) {
+        const uint4 w = plain_nibbles<BF16>(q, zero, mask, magic);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) sum[i] = mfma32<BF16>(staged[t & 1][(i * 32 + c) * kPitch + at_piece], w, first ? none : sum[i]);
+    };
+    // FIRST, LAST: the step begins, ends a block (of 64 or more)
+    auto step = [&](int t, Weights& now, Weights& next, bool first, bool last) {
+        uint4 ahead[TM];
+        const int to = min(t + 1, steps - 1);
+        load_w(to, next);
+        load_x(to, ahead);
+        uint4 w = now.w;
+        if constexpr (BS == 32) {
+            // lane group h has block h; afterwards x and z hold block 0 of both groups, y and w block 1
+            const auto lo = __builtin_amdgcn_permlane32_swap(w.x, w.y, false, false), hi = __builtin_amdgcn_permlane32_swap(w.z, w.w, false, false);
+            const uint32_t z0 = now.z & 15u, z1 = now.z >> 4;
+            product(t, lo[0], z0, g, true);
+            product(t, hi[0], z0, 2 + g, false);
+            add_up(scale_of(now.s[0]));
+            product(t, lo[1], z1, 4 + g, true);
+            product(t, hi[1], z1, 6 + g, false);
+            add_up(scale_of(now.s[kScales - 1]));
+        } else {
+            const uint32_t zero = now.z >> ((min(t * 64 >> shift, p.m.kb - 1) & 1) * 4) & 15u;
+            product(t, w.x, zero, g * 4, first);
+            product(t, w.y, zero, g * 4 + 1, false);
+            product(t, w.z, zero, g * 4 + 2, false);
+            product(t, w.w, zero, g * 4 + 3, false);
+            if (last) add_up(scale_of(now.s[0]));
+        }
+        stage(t + 1, ahead);
+        __syncthreads();
+    };
+
+    Weights one, two;
+    {
+        uint4 begin[TM];
+        load_w(0, one);
+        load_x(0, begin);
+        stage(0, begin);
+    }
+    __syncthreads();
+    for (int t = 0; t < steps; t += 2) {
+        const bool pair = t + 1 < steps;
+        if constexpr (BS == 128) {
+            if (pair) {
+                step(t, one, two, true, false);
+                step(t + 1, two, one, false, true);
+            } else {
+                step(t, one, two, true, true);
+            }
+        } else {
+            step(t, one, two, true, true);
+            if (pair) step(t + 1, two, one, true, true);
+        }
+    }
+
+    // a lane has column c and rows 8 (e / 4) + 4 g + e % 4 of each 32
+    auto row_of = [&](int i, int e) { return i * 32 + (e >> 2) * 8 + g * 4 + (e & 3); };
+    if constexpr (UP) {
+        float bias_g = 0.f, bias_u = 0.f;
+        const bool is = col < p.m.n;
+        if (p.m.w[0].bias && is) {
+            bias_g = load_as_f32(p.m.w[0].bias, p.m.bias_dtype, at);
+            bias_u = load_as_f32(p.m.w[1].bias, p.m.bias_dtype, at);
+        }
+        // lanes with gate take the even rows, lanes with up the odd ones
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(total[i][e]), __float_as_uint(total[i][e]), false, false);
+                const auto o = __builtin_amdgcn_permlane16_swap(__float_as_uint(total[i][e + 1]), __float_as_uint(total[i][e + 1]), false, false);
+                const float gate = __uint_as_float(which ? o[0] : a[0]) + bias_g, up = __uint_as_float(which ? o[1] : a[1]) + bias_u;
+                const int row = row_of(i, e + which);
+                if (row >= tile.z || col >= p.ldh) continue;
+                const float v = is ? moe_activation(gate, up, p.alpha, p.beta, p.limit) : 0.f;
+                p.h[(tile.y + row) * p.ldh + col] = BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
+            }
+    } else {
+        if (col >= p.m.n) return;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int row = row_of(i, e);
+                if (row < tile.z) p.out[static_cast<int64_t>(tile.y + row) * p.m.n + col] = total[i][e];
+            }
+    }
+}
+
+}  // namespace
+
+int launch_moe_tile(const RocmMoeArgs& a, const MoeTileCall& p, bool up, int tile_rows, hipStream_t s)
+{
+    auto go = [&](auto bf, auto bs, auto st, auto half) {
+        constexpr bool BF16 = decltype(bf)::value, UP = decltype(half)::value;
+        constexpr int BS = decltype(bs)::value;
+        using ST = decltype(st);
+        const dim3 grid = moe_grid(UP ? static_cast<unsigned>((p.ldh + 63) / 64) : static_cast<unsigned>(p.m.n + 127) / 128, static_cast<int>(p.count));
+        if (tile_rows == 128) hipLaunchKernelGGL((moe_tile_kernel<BF16, BS, ST, UP, 4>), grid, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((moe_tile_kernel<BF16, BS, ST, UP, 1>), grid, dim3(256), 0, s, p);
+        return static_cast<int>(hipGetLastError());
+    };
+    auto halved = [&](auto bf, auto bs, auto st) { return up ? go(bf, bs, st, std::true_type{}) : go(bf, bs, st, std::false_type{}); };
+    auto scaled = [&](auto bf, auto bs) { return a.scale_dtype == ROCM_DT_F32 ? halved(bf, bs, float{}) : halved(bf, bs, uint16_t{}); };
+    auto typed = [&](auto bf) {
+        if (a.block_size == 32) return scaled(bf, std::integral_constant<int, 32>{});
+        if (a.block_size == 64) return scaled(bf, std::integral_constant<int, 64>{});
+        return scaled(bf, std::integral_constant<int, 128>{});
+    };
+    return a.dtype == ROCM_DT_BF16 ? typed(std::true_type{}) : typed(std::false_type{});
+}
+
+}  // namespace mnb
