@@ -446,7 +446,7 @@ struct Int8Node final : NxrtRocmNode {
     struct Layout {
         uint64_t codes = 0, scales = 0, b = 0, partial = 0, partial_bytes = 0, total = 0;
     };
-    Layout layout(int64_t rows, bool makes_codes, bool pads_codes) const
+    Layout layout(int64_t rows, uint32_t a_dtype, bool pads_codes) const
     {
         Layout l;
         auto part = [&](uint64_t bytes) {
@@ -458,6 +458,8 @@ struct Int8Node final : NxrtRocmNode {
         a.m = rows;
         a.n = s.n;
         a.k = s.k;
+        a.a_dtype = static_cast<int>(a_dtype);
+        const bool makes_codes = a_dtype != NXRT_DT_INT8 && !rocm_int8_fuses_quantizer(&a);
         l.codes = part(makes_codes || pads_codes ? static_cast<uint64_t>(rows * kp()) : 0);
         l.scales = part(makes_codes ? static_cast<uint64_t>(rows) * 4 : 0);
         l.b = part(rocm_int8_pads_b(&a) ? static_cast<uint64_t>(s.n * kp()) : 0);
@@ -469,8 +471,7 @@ struct Int8Node final : NxrtRocmNode {
     {
         int64_t rows = 0, last = 0;
         if (!static_matrix(in, n, 0, &rows, &last)) return make_status(NXRT_INVALID_ARGUMENT, err("workspace_requirement needs the shape of A"));
-        const bool given = in[0].dtype == NXRT_DT_INT8;
-        *bytes = rows ? layout(rows, !given, given).total : 0;
+        *bytes = rows ? layout(rows, in[0].dtype, in[0].dtype == NXRT_DT_INT8).total : 0;
         return ok();
     }
     NxrtStatus execute(const NxrtRocmTensorView* in, uint32_t n_in, NxrtRocmTensorView* out, uint32_t n_out, void* ws, uint64_t ws_bytes) override
@@ -510,7 +511,7 @@ struct Int8Node final : NxrtRocmNode {
         NxrtStatus st = ep->bind();
         if (st.code != NXRT_OK) return st;
         const bool pads_codes = codes && (s.k % 128 != 0 || reinterpret_cast<uintptr_t>(at(*a)) % 16 != 0);
-        const Layout l = layout(static_cast<int64_t>(rows), !codes, pads_codes);
+        const Layout l = layout(static_cast<int64_t>(rows), a->dtype, pads_codes);
         void* scratch_at = nullptr;
         st = find_scratch(l.total, ws, ws_bytes, &scratch_at);
         if (st.code != NXRT_OK) return st;
@@ -529,6 +530,7 @@ struct Int8Node final : NxrtRocmNode {
             args.ldb = kp();
         }
         args.lda = kp();
+        args.a_dtype = static_cast<int>(a->dtype);
         if (codes) {
             args.a = reinterpret_cast<const int8_t*>(at(*a));
             args.a_scale = reinterpret_cast<const float*>(at(*sa));
@@ -536,6 +538,8 @@ struct Int8Node final : NxrtRocmNode {
                 if (rc == 0) rc = rocm_launch_pad_codes(args.a, args.m, s.k, reinterpret_cast<int8_t*>(w + l.codes), ep->stream);
                 args.a = reinterpret_cast<const int8_t*>(w + l.codes);
             }
+        } else if (rocm_int8_fuses_quantizer(&args)) {
+            args.a_float = at(*a);
         } else {
             if (rc == 0) rc = rocm_launch_quantize_rows(at(*a), static_cast<int>(a->dtype), args.m, s.k, reinterpret_cast<int8_t*>(w + l.codes), reinterpret_cast<float*>(w + l.scales), ep->stream);
             ep->launches.fetch_add(1);

@@ -359,6 +359,7 @@ int rocm_launch_gated_norm(const RocmGatedNormArgs* args, rocm_stream_t stream);
 enum { ROCM_INT8_MAX_K = 131072 };
 typedef struct RocmInt8Args {
   const int8_t* a;
+  const void* a_float;      /* instead of a and a_scale where rocm_int8_fuses_quantizer(): [m, k] of a_dtype, any alignment of whole elements */
   const float* a_scale;     /* [m] */
   const int8_t* b;
   const void* b_scale;      /* [n] */
@@ -366,10 +367,11 @@ typedef struct RocmInt8Args {
   void* y;
   int32_t* partial;         /* rocm_int8_scratch_bytes() of device memory */
   int64_t m, n, k, lda, ldb;
-  int b_scale_dtype, bias_dtype, y_dtype;
+  int a_dtype, b_scale_dtype, bias_dtype, y_dtype;
 } RocmInt8Args;
-/* Of m, n and k alone: whether B has to be handed over in padded rows (rocm_launch_pad_codes; else ldb = k and any address for k no multiple of 16, one of
+/* Of m, n, k and a_dtype (f16 and bf16: codes are wanted) alone: whether the kernel makes the codes itself; of m, n and k: whether B has to be handed over in padded rows (rocm_launch_pad_codes; else ldb = k and any address for k no multiple of 16, one of
  * 16 bytes otherwise), and what the sums of slices of K take. */
+int rocm_int8_fuses_quantizer(const RocmInt8Args* args);
 int rocm_int8_pads_b(const RocmInt8Args* args);
 uint64_t rocm_int8_scratch_bytes(const RocmInt8Args* args);
 /* Codes [m, k rounded up to 128] and scales [m] of a [m, k] (f32, f16, bf16). */

@@ -88,101 +88,330 @@ __device__ __forceinline__ void store_scaled(const Int8Params& p, int64_t row, i
     store_from_f32(p.y, p.y_dtype, row * p.n + col, with_bias(v, p.bias, p.bias_dtype, row, p.n, col, p.y_dtype));
 }
 
-// Few rows: a workgroup has 16 columns, its waves split K. v_mfma_i32_16x16x64_i8: lane l holds 16 bytes of k of row (or column) l % 16, k from (l / 16) * 16.
-// RT: tiles of 16 rows.
-template <int RT>
-__global__ __launch_bounds__(512) void int8_rows_kernel(Int8Params p)
+// Few rows: a workgroup has 16 CT columns, its waves split K; B's bytes bound it. v_mfma_i32_16x16x64_i8: lane l holds 16 bytes of k of row (or column) l % 16, k
+// from (l / 16) * 16. RT: tiles of 16 rows; lanes whose row is not there load no codes (a CU's vector memory path is 64 bytes a cycle, and 16 rows are as many
+// bytes as 16 columns). Two steps' loads are in flight.
+// FUSED (up to four rows of at most 32 KiB of codes): a is [m, k] of type T, and every workgroup makes the codes for itself, in LDS, while its first weights are on
+// their way: a launch of its own takes longer than a row's second and third trip from L2.
+template <int RT, int CT, typename T, bool BF16, bool FUSED>
+__global__ __launch_bounds__(512) void int8_rows_kernel(const int8_t* b_base, const void* a_base, int m, int n, int k, int steps, Int8Params p)
 {
-    __shared__ int32_t sums[8][RT * 4][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int c = lane & 15, g = lane >> 4;
-    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
-    const int64_t cols = p.n - n0 < 16 ? p.n - n0 : 16;
-    const auto srd_b = make_srd(p.b + n0 * p.ldb, static_cast<uint64_t>(cols * p.ldb));
-    const auto srd_a = make_srd(p.a, static_cast<uint64_t>(p.m * p.lda));
-    const int per_wave = (p.steps + waves - 1) / waves;
-    const int begin = wave * per_wave, end = min(begin + per_wave, p.steps);
-    const uint32_t b_at = c < cols ? static_cast<uint32_t>(c * p.ldb + g * 16) : kOutOfRange;
-    uint32_t a_at[RT];
-    i32x4_t acc[RT] = {};
+    __shared__ int32_t sums[8][RT * CT * 4][64];
+    extern __shared__ __attribute__((aligned(16))) uint8_t coded[];                     // FUSED: rows of kp codes
+    __shared__ float row_scale[4];
+    __shared__ uint32_t slots[16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4, kp = steps * 128;
+    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (16 * CT);
+    const int cols = static_cast<int>(n - n0 < 16 * CT ? n - n0 : 16 * CT);
+    const auto srd_b = make_srd(b_base + n0 * p.ldb, static_cast<uint64_t>(cols * p.ldb));
+    const auto srd_a = make_srd(a_base, FUSED ? 0 : static_cast<uint64_t>(m) * p.lda);
+    const int begin = steps * wave >> 3, end = steps * (wave + 1) >> 3;                // (eight waves)
+    uint32_t b_at[CT], a_at[RT];
+    i32x4_t acc[RT][CT] = {};
 #pragma unroll
-    for (int r = 0; r < RT; ++r) a_at[r] = r * 16 + c < p.m ? static_cast<uint32_t>((r * 16 + c) * p.lda + g * 16) : kOutOfRange;
-#pragma unroll 2
-    for (int t = begin; t < end; ++t) {
+    for (int j = 0; j < CT; ++j) b_at[j] = j * 16 + c < cols ? static_cast<uint32_t>((j * 16 + c) * p.ldb + g * 16) : kOutOfRange;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) a_at[r] = r * 16 + c < m ? static_cast<uint32_t>((r * 16 + c) * p.lda + g * 16) : kOutOfRange;
+    struct Step {
+        uint4 b[CT][2], a[FUSED ? 1 : RT][2];
+    };
+    auto load = [&](int t, Step& s) {
+        // (behind the wave's last step nothing is read, but asked for all the same: a branch would have every load waited for)
+        const uint32_t at = t < end ? static_cast<uint32_t>(t) * 128u : 0u, off = t < end ? 0u : kOutOfRange;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t k = static_cast<uint32_t>(t) * 128u + h * 64u;
-            const i32x4_t b = __builtin_bit_cast(i32x4_t, load16(srd_b, b_at + k, 0));
 #pragma unroll
-            for (int r = 0; r < RT; ++r) acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, load16(srd_a, a_at[r] + k, 0)), b, acc[r], 0, 0, 0);
+            for (int j = 0; j < CT; ++j) s.b[j][h] = load16(srd_b, off ? off : b_at[j] + at + h * 64, 0);
+            if constexpr (!FUSED)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) s.a[r][h] = load16(srd_a, off ? off : a_at[r] + at + h * 64, 0);
         }
+    };
+    auto multiply = [&](int t, const Step& s) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            i32x4_t fused = {};
+            if constexpr (FUSED) {
+                if (c < m) fused = *reinterpret_cast<const i32x4_t*>(coded + c * kp + t * 128 + h * 64 + g * 16);
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int j = 0; j < CT; ++j)
+                    acc[r][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(FUSED ? fused : __builtin_bit_cast(i32x4_t, s.a[FUSED ? 0 : r][h]), __builtin_bit_cast(i32x4_t, s.b[j][h]), acc[r][j], 0, 0, 0);
+        }
+    };
+    Step one, two;
+    load(begin, one);
+    load(begin + 1, two);
+    if constexpr (FUSED) {
+        using V8 = Eight<T, BF16>;
+        const int pieces = kp / 8;
+        constexpr int kHeld = 2;                                                       // pieces a thread holds between the two passes
+        for (int t = 0; t < m; ++t) {
+            const T* const x = static_cast<const T*>(a_base) + static_cast<int64_t>(t) * k;
+            auto piece = [&](int i, V8& e) {
+                const int left = k - i * 8;
+                if (left >= 8) e.load(x + i * 8);
+                else if (left > 0) e.load_first(x + i * 8, left);
+                else e.zero();
+            };
+            V8 held[kHeld];
+            uint32_t amax = 0;
+            auto look = [&](const V8& e) {
+                float v[8];
+                e.get(v);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) amax = larger(amax, __float_as_uint(v[q]) & 0x7fffffffu);
+            };
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j) {
+                const int i = threadIdx.x + j * 512;
+                if (i < pieces) piece(i, held[j]);
+                else held[j].zero();
+            }
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j) look(held[j]);
+            for (int i = threadIdx.x + kHeld * 512; i < pieces; i += 512) {
+                V8 e;
+                piece(i, e);
+                look(e);
+            }
+            __syncthreads();                                                           // (the slots of the row before are read)
+            const RowScale scale(over_workgroup(amax, slots, wave, 8, larger));
+            if (threadIdx.x == 0) row_scale[t] = scale.scale;
+            auto code = [&](int i, const V8& e) {
+                float v[8];
+                e.get(v);
+                uint32_t d[2] = {0, 0};
+#pragma unroll
+                for (int q = 0; q < 8; ++q) d[q >> 2] |= static_cast<uint32_t>(scale.code(v[q]) & 0xff) << (8 * (q & 3));
+                *reinterpret_cast<uint2*>(coded + t * kp + i * 8) = make_uint2(d[0], d[1]);
+            };
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j)
+                if (static_cast<int>(threadIdx.x) + j * 512 < pieces) code(threadIdx.x + j * 512, held[j]);
+            for (int i = threadIdx.x + kHeld * 512; i < pieces; i += 512) {
+                V8 e;
+                piece(i, e);
+                code(i, e);
+            }
+        }
+        __syncthreads();
+    }
+    for (int t = begin; t < end; t += 2) {
+        multiply(t, one);
+        load(t + 2, one);
+        if (t + 1 < end) multiply(t + 1, two);
+        load(t + 3, two);
     }
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sums[wave][r * 4 + i][lane] = acc[r][i];
+        for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[wave][(r * CT + j) * 4 + i][lane] = acc[r][j][i];
     __syncthreads();
-    const int64_t col = n0 + c;
-    if (c >= cols) return;
-    const float sb = load_as_f32(p.b_scale, p.b_scale_dtype, col);
-    for (int j = wave; j < RT * 4; j += waves) {
-        const int64_t row = (j >> 2) * 16 + g * 4 + (j & 3);
-        if (row >= p.m) continue;
+    for (int q = wave; q < RT * CT * 4; q += 8) {
+        const int tile = q >> 2, r = tile / CT, j = tile % CT;
+        const int64_t row = r * 16 + g * 4 + (q & 3), col = n0 + j * 16 + c;
+        if (row >= m || j * 16 + c >= cols) continue;
         int32_t sum = 0;
-        for (int w = 0; w < waves; ++w) sum += sums[w][j][lane];
-        store_scaled(p, row, col, sum, p.a_scale[row], sb);
+#pragma unroll
+        for (int w = 0; w < 8; ++w) sum += sums[w][q][lane];
+        store_scaled(p, row, col, sum, FUSED ? row_scale[row] : p.a_scale[row], load_as_f32(p.b_scale, p.b_scale_dtype, col));
     }
 }
 
-// Tall calls: 128 x 128 tiles.
-__global__ __launch_bounds__(256) void int8_tile_kernel(Int8Params p)
+// Tall calls: tiles of 64 W x 64 W, four waves of 32 W x 32 W each on v_mfma_i32_32x32x32_i8, BK bytes of K a step, both operands from memory straight into LDS.
+//
+// A step's pieces of 16 bytes lie in LDS in the order in which the loads leave them (a wave's 64 lanes side by side), rows of BK bytes; which piece of its row a lane
+// asks for is turned round by its row, so that the 32 rows of an operand read meet each bank as often as it takes and no more.
+// One barrier a step: before the step's last products the next step has arrived, its first operands are read while those products run, and the loads of the step
+// after it go where this step's operands were, which all are in registers by then.
+// W = 4 (256 x 256): 256 accumulators a lane, one wave a SIMD; a piece read from LDS meets four others (128 KiB of LDS reads for 2,048 cycles of products and
+// 64 KiB of K). W = 2 (128 x 128): two workgroups a CU, for grids that would not cover the chip.
+template <int W, int BK>
+struct Int8Tile {
+    static constexpr int kRows = 64 * W, kPieces = BK / 16, kStage = 2 * kRows * BK;     // bytes of a step: A, then B
+    static constexpr int kLoads = kStage / 1024 / 4;                                     // of a wave
+    static constexpr int kRowsPerLoad = 1024 / BK, kSteps = BK / 32;
+
+    static __device__ __forceinline__ int turned(int row, int piece)
+    {
+        if constexpr (kPieces == 8) return piece ^ (row & 7);
+        return piece ^ (row >> 1 & 3);
+    }
+};
+
+typedef __attribute__((ext_vector_type(4))) uint32_t srd_t;
+__device__ __forceinline__ srd_t plain_srd(const void* base, uint32_t bytes)
 {
-    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * 128 * 144];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 128, n0 = static_cast<int64_t>(blockIdx.x) * 128;
-    const int64_t rows = p.m - m0 < 128 ? p.m - m0 : 128, cols = p.n - n0 < 128 ? p.n - n0 : 128;
-    const auto srd_a = make_srd(p.a + m0 * p.lda, static_cast<uint64_t>(rows * p.lda));
-    const auto srd_b = make_srd(p.b + n0 * p.ldb, static_cast<uint64_t>(cols * p.ldb));
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-    i32x16_t acc[2][2] = {};
-    for (int t = 0; t < p.steps; ++t) {
-        __syncthreads();
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    srd_t s;
+    s.x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
+    s.y = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32));
+    s.z = __builtin_amdgcn_readfirstlane(bytes);
+    s.w = 0x00020000u;
+    return s;
+}
+
+template <int W, int BK, bool SLICED>
+__global__ __launch_bounds__(256, W == 4 ? 1 : 2) void int8_tile_kernel(Int8Params p, unsigned tiles_m, unsigned tiles_n)
+{
+    using Tile = Int8Tile<W, BK>;
+    constexpr int kWave = 32 * W, kStage = Tile::kStage, kSteps = Tile::kSteps;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStage];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, g = lane >> 5;
+
+    // Workgroups go round the eight XCDs; each takes a run of tiles, eight row blocks by all columns at a time, so that its L2 sees an operand more than once.
+    const unsigned all = tiles_m * tiles_n, per = (all + 7) / 8, linear = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= per || linear >= all) return;
+    const unsigned band = linear / (8 * tiles_n), in_band = linear - band * 8 * tiles_n, rows_here = min(8u, tiles_m - band * 8);
+    const int64_t m0 = static_cast<int64_t>(band * 8 + in_band % rows_here) * Tile::kRows, n0 = static_cast<int64_t>(in_band / rows_here) * Tile::kRows;
+    const int rows = static_cast<int>(p.m - m0 < Tile::kRows ? p.m - m0 : Tile::kRows), cols = static_cast<int>(p.n - n0 < Tile::kRows ? p.n - n0 : Tile::kRows);
+    const int slice = static_cast<int>(blockIdx.y), total = p.steps * (128 / BK), share = p.steps_per_slice * (128 / BK);
+    const int begin = slice * share, end = min(begin + share, total), count = end - begin;
+
+    // Load i of a wave brings kRowsPerLoad rows; rows that are not there repeat the last. The range ends with the operand's last row, and moves on with K.
+    uint32_t at[Tile::kLoads];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int id = threadIdx.x + i * 256, r = id >> 3, ch = id & 7;
-            const uint4 va = load16(srd_a, r < rows ? static_cast<uint32_t>(r * p.lda + ch * 16 + t * 128) : kOutOfRange, 0);
-            const uint4 vb = load16(srd_b, r < cols ? static_cast<uint32_t>(r * p.ldb + ch * 16 + t * 128) : kOutOfRange, 0);
-            *reinterpret_cast<uint4*>(smem + r * 144 + ch * 16) = va;
-            *reinterpret_cast<uint4*>(smem + 128 * 144 + r * 144 + ch * 16) = vb;
+    for (int i = 0; i < Tile::kLoads; ++i) {
+        const bool of_b = i >= Tile::kLoads / 2;
+        const int row = (wave * (Tile::kLoads / 2) + i % (Tile::kLoads / 2)) * Tile::kRowsPerLoad + lane / Tile::kPieces;
+        const int from = min(row, (of_b ? cols : rows) - 1);
+        at[i] = static_cast<uint32_t>(from * static_cast<int>(of_b ? p.ldb : p.lda) + Tile::turned(row, lane % Tile::kPieces) * 16);
+    }
+    const int8_t* const a = p.a + m0 * p.lda;
+    const int8_t* const b = p.b + n0 * p.ldb;
+    const uint32_t a_bytes = static_cast<uint32_t>(rows * p.lda), b_bytes = static_cast<uint32_t>(cols * p.ldb);
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+    auto fetch = [&](int t) {                                    // step `begin + t` into its half of LDS
+        const uint32_t k = static_cast<uint32_t>(begin + t) * BK, to = lds + (t & 1) * kStage + wave * (kStage / 8);
+        // (behind the slice's last step: nothing, into a half that nobody reads any more)
+        const bool is = t < count;
+        const srd_t sa = plain_srd(a + k, is ? a_bytes - k : 0u), sb = plain_srd(b + k, is && b_bytes > k ? b_bytes - k : 0u);
+#pragma unroll
+        for (int i = 0; i < Tile::kLoads; ++i) {
+            const bool of_b = i >= Tile::kLoads / 2;
+            const uint32_t dst = __builtin_amdgcn_readfirstlane(to + (of_b ? kStage / 2 : 0) + i % (Tile::kLoads / 2) * 1024);
+            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(at[i]), "s"(of_b ? sb : sa) : "memory");
         }
-        __syncthreads();
+    };
+    const int wm = (wave & 1) * kWave, wn = (wave >> 1) * kWave;
+    i32x4_t fa[2][W], fb[2][W];
+    auto operands = [&](int t, int s, i32x4_t (&xa)[W], i32x4_t (&xb)[W]) {
+        const uint8_t* const half = smem + (t & 1) * kStage;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            i32x4_t a[2], b[2];
+        for (int i = 0; i < W; ++i) {
+            const int ra = wm + i * 32 + c, rb = wn + i * 32 + c;
+            xa[i] = *reinterpret_cast<const i32x4_t*>(half + ra * BK + Tile::turned(ra, s * 2 + g) * 16);
+            xb[i] = *reinterpret_cast<const i32x4_t*>(half + kStage / 2 + rb * BK + Tile::turned(rb, s * 2 + g) * 16);
+        }
+    };
+    i32x16_t acc[W][W] = {};
+    auto products = [&](const i32x4_t (&xa)[W], const i32x4_t (&xb)[W]) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                a[i] = *reinterpret_cast<const i32x4_t*>(smem + (wm + i * 32 + (lane & 31)) * 144 + s * 32 + (lane >> 5) * 16);
-                b[i] = *reinterpret_cast<const i32x4_t*>(smem + 128 * 144 + (wn + i * 32 + (lane & 31)) * 144 + s * 32 + (lane >> 5) * 16);
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xa[i], xb[j], acc[i][j], 0, 0, 0);
+    };
+    auto arrived = [&] {                                         // own loads into LDS and reads from it are done, and everyone's
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    fetch(0);                                                    // (no slice is empty)
+    arrived();
+    operands(0, 0, fa[0], fb[0]);
+    fetch(1);
+    for (int t = 0; t < count; ++t) {
+#pragma unroll
+        for (int s = 0; s < kSteps - 1; ++s) {
+            operands(t, s + 1, fa[(s + 1) & 1], fb[(s + 1) & 1]);
+            products(fa[s & 1], fb[s & 1]);
+        }
+        arrived();
+        operands(t + 1, 0, fa[0], fb[0]);                        // (behind the last step: whatever lies there, for no product)
+        fetch(t + 2);
+        products(fa[1], fb[1]);
+    }
+
+    // A lane has column c and rows 8 (e / 4) + 4 g + e % 4 of each 32 x 32, and leaves with 16 columns of row lane / 2: each tile is turned round in the wave's own
+    // piece of LDS. (One form takes the accumulators out, whatever becomes of them: with one for each kind of result the compiler moves all 256 at once, and spills.)
+    constexpr int kTurn = 36;                                    // dwords from a row to the next
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (what was fetched behind the end has to be in before LDS is used for something else)
+    __syncthreads();
+    int32_t* const turn = reinterpret_cast<int32_t*>(smem) + wave * (32 * kTurn);
+    const bool wide = p.y_dtype != ROCM_DT_F32 && (p.n & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && !(p.bias_dtype & ROCM_BIAS_PER_ROW);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        const int64_t first = n0 + wn + j * 32 + (lane & 1) * 16;
+        float sb[16];
+        if constexpr (!SLICED)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) sb[q] = load_as_f32(p.b_scale, p.b_scale_dtype, first + q < p.n ? first + q : p.n - 1);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) turn[((e >> 2) * 8 + g * 4 + (e & 3)) * kTurn + c] = acc[i][j][e];
+            lds_order();
+            const int64_t row = m0 + wm + i * 32 + (lane >> 1);
+            int32_t* const mine = turn + (lane >> 1) * kTurn + (lane & 1) * 16;
+            if (row < p.m) {
+                if constexpr (SLICED) {
+                    int32_t* const part = p.partial + (static_cast<int64_t>(slice) * p.m + row) * p.n;
+                    for (int q = 0; q < 16 && first + q < p.n; ++q) part[first + q] = mine[q];
+                } else {
+                    const float sa = p.a_scale[row];
+                    float v[16];
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) v[q] = static_cast<float>(mine[q]) * sa * sb[q];
+                    if (wide) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int64_t at = first + h * 8;
+                            if (at >= p.n) continue;
+                            float w[8];
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) w[q] = v[h * 8 + q];
+                            if (p.bias)
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) w[q] += load_as_f32(p.bias, p.bias_dtype, at + q);
+                            uint16_t* const y = static_cast<uint16_t*>(p.y) + row * p.n + at;
+                            if (p.y_dtype == ROCM_DT_BF16) {
+                                Eight<uint16_t, true> o;
+                                o.set(w);
+                                *reinterpret_cast<uint4*>(y) = make_uint4(o.raw.x, o.raw.y, o.raw.z, o.raw.w);
+                            } else {
+                                Eight<uint16_t, false> o;
+                                o.set(w);
+                                *reinterpret_cast<uint4*>(y) = make_uint4(o.raw.x, o.raw.y, o.raw.z, o.raw.w);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) mine[q] = __float_as_int(v[q]);       // (a run-time index, so through LDS)
+#pragma unroll 1
+                        for (int q = 0; q < 16 && first + q < p.n; ++q)
+                            store_from_f32(p.y, p.y_dtype, row * p.n + first + q, with_bias(__int_as_float(mine[q]), p.bias, p.bias_dtype, row, p.n, first + q, p.y_dtype));
+                    }
+                }
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
+            lds_order();
         }
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int64_t col = n0 + wn + j * 32 + (lane & 31);
-        if (col >= p.n) continue;
-        const float sb = load_as_f32(p.b_scale, p.b_scale_dtype, col);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int64_t row = m0 + wm + i * 32 + (e >> 2) * 8 + (lane >> 5) * 4 + (e & 3);
-                if (row < p.m) store_scaled(p, row, col, acc[i][j][e], p.a_scale[row], sb);
-            }
-    }
+}
+
+// y from the sums of slices of K.
+__global__ __launch_bounds__(256) void int8_reduce_kernel(Int8Params p, int slices)
+{
+    const int64_t row = static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y, col = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (row >= p.m || col >= p.n) return;
+    int32_t sum = 0;
+    for (int i = 0; i < slices; ++i) sum += p.partial[(i * p.m + row) * p.n + col];
+    store_scaled(p, row, col, sum, p.a_scale[row], load_as_f32(p.b_scale, p.b_scale_dtype, col));
 }
 
 Int8Params params_of(const RocmInt8Args* a)
@@ -237,24 +466,90 @@ extern "C" int rocm_launch_pad_codes(const int8_t* from, int64_t rows, int64_t k
     return 0;
 }
 
+namespace mnb {
+namespace {
+
+constexpr int64_t kFewRows = 64;              // rows up to which a call streams B
+
+// What a call is launched as.
+struct Int8Plan {
+    int tile;                   // 0: rows
+    int slices;
+};
+Int8Plan plan_of(const RocmInt8Args& a)
+{
+    Int8Plan p{0, 1};
+    if (a.m <= kFewRows) return p;
+    auto tiles = [&](int64_t t) { return (a.m + t - 1) / t * ((a.n + t - 1) / t); };
+    const int64_t cus = rocm_ffi_compute_units(), steps = (a.k + 127) / 128;
+    p.tile = tiles(256) >= cus * 3 / 4 ? 256 : 128;
+    if (p.tile == 128) {
+        // slices of K until two workgroups for each CU are there, none of less than 16 steps
+        int64_t s = 2 * cus / tiles(128);
+        if (s > steps / 16) s = steps / 16;
+        s = s < 1 ? 1 : s > 16 ? 16 : s;
+        const int64_t share = (steps + s - 1) / s;
+        p.slices = static_cast<int>((steps + share - 1) / share);
+    }
+    return p;
+}
+bool fuses(const RocmInt8Args& a) { return a.m <= 4 && (a.a_dtype == ROCM_DT_F16 || a.a_dtype == ROCM_DT_BF16) && a.m * ((a.k + 127) / 128 * 128) <= 32768; }
+
+}  // namespace
+}  // namespace mnb
+
 extern "C" int rocm_int8_pads_b(const RocmInt8Args* args) { return args->k % 16 != 0; }
-extern "C" uint64_t rocm_int8_scratch_bytes(const RocmInt8Args*) { return 0; }
-extern "C" const char* rocm_int8_variant(const RocmInt8Args* args) { return args->m <= 64 ? "int8_rows" : "int8_tile"; }
+extern "C" uint64_t rocm_int8_scratch_bytes(const RocmInt8Args* args)
+{
+    const mnb::Int8Plan p = mnb::plan_of(*args);
+    return p.slices > 1 ? static_cast<uint64_t>(p.slices) * args->m * args->n * 4 : 0;
+}
+extern "C" int rocm_int8_fuses_quantizer(const RocmInt8Args* args) { return mnb::fuses(*args); }
+extern "C" const char* rocm_int8_variant(const RocmInt8Args* args)
+{
+    const mnb::Int8Plan p = mnb::plan_of(*args);
+    if (p.tile == 0) return args->a_float ? "int8_rows_fused" : "int8_rows";
+    return p.tile == 256 ? "int8_tile_256" : p.slices > 1 ? "int8_tile_128_sliced" : "int8_tile_128";
+}
 
 extern "C" int rocm_launch_int8(const RocmInt8Args* args, rocm_stream_t stream)
 {
     using namespace mnb;
     if (args->m <= 0 || args->n <= 0) return 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const Int8Params p = params_of(args);
-    if (args->m <= 64) {
-        const unsigned grid = static_cast<unsigned>((p.n + 15) / 16), threads = 512;
-        auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, s, p);
+    Int8Params p = params_of(args);
+    const Int8Plan plan = plan_of(*args);
+    if (plan.tile == 0) {
+        const unsigned wide = static_cast<unsigned>((p.n + 31) / 32), cus = static_cast<unsigned>(rocm_ffi_compute_units());
+        auto go = [&](auto kernel, unsigned grid, const void* a, size_t lds) {
+            hipLaunchKernelGGL(kernel, dim3(grid), dim3(512), lds, s, p.b, a, static_cast<int>(p.m), static_cast<int>(p.n), static_cast<int>(args->k), p.steps, p);
             return static_cast<int>(hipGetLastError());
         };
-        return p.m <= 16 ? go(int8_rows_kernel<1>) : p.m <= 32 ? go(int8_rows_kernel<2>) : go(int8_rows_kernel<4>);
+        // two tiles of columns share a row's codes where the chip is covered all the same
+        const unsigned narrow = static_cast<unsigned>((p.n + 15) / 16);
+        auto columns = [&](auto one, auto two, const void* a, size_t lds) { return wide >= 2 * cus ? go(two, wide, a, lds) : go(one, narrow, a, lds); };
+        if (args->a_float) {
+            if (!fuses(*args)) return static_cast<int>(hipErrorInvalidValue);
+            const size_t lds = static_cast<size_t>(p.m) * p.steps * 128;
+            if (args->a_dtype == ROCM_DT_BF16) return columns(int8_rows_kernel<1, 1, uint16_t, true, true>, int8_rows_kernel<1, 2, uint16_t, true, true>, args->a_float, lds);
+            return columns(int8_rows_kernel<1, 1, uint16_t, false, true>, int8_rows_kernel<1, 2, uint16_t, false, true>, args->a_float, lds);
+        }
+        if (p.m <= 16) return columns(int8_rows_kernel<1, 1, float, false, false>, int8_rows_kernel<1, 2, float, false, false>, p.a, 0);
+        if (p.m <= 32) return columns(int8_rows_kernel<2, 1, float, false, false>, int8_rows_kernel<2, 2, float, false, false>, p.a, 0);
+        return go(int8_rows_kernel<4, 1, float, false, false>, narrow, p.a, 0);
     }
-    hipLaunchKernelGGL(int8_tile_kernel, dim3(static_cast<unsigned>((p.n + 127) / 128), static_cast<unsigned>((p.m + 127) / 128)), dim3(256), 0, s, p);
-    return static_cast<int>(hipGetLastError());
+    p.steps_per_slice = (p.steps + plan.slices - 1) / plan.slices;
+    p.partial = plan.slices > 1 ? args->partial : nullptr;
+    const unsigned tm = static_cast<unsigned>((p.m + plan.tile - 1) / plan.tile), tn = static_cast<unsigned>((p.n + plan.tile - 1) / plan.tile);
+    const dim3 grid((tm * tn + 7) / 8 * 8, static_cast<unsigned>(plan.slices));
+    if (plan.tile == 256) hipLaunchKernelGGL((int8_tile_kernel<4, 64, false>), grid, dim3(256), 0, s, p, tm, tn);
+    else if (p.partial) hipLaunchKernelGGL((int8_tile_kernel<2, 128, true>), grid, dim3(256), 0, s, p, tm, tn);
+    else hipLaunchKernelGGL((int8_tile_kernel<2, 128, false>), grid, dim3(256), 0, s, p, tm, tn);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && p.partial) {
+        const unsigned y = static_cast<unsigned>(p.m < 32768 ? p.m : 32768);
+        hipLaunchKernelGGL(int8_reduce_kernel, dim3(static_cast<unsigned>((p.n + 255) / 256), y, static_cast<unsigned>((p.m + y - 1) / y)), dim3(256), 0, s, p, plan.slices);
+        e = hipGetLastError();
+    }
+    return static_cast<int>(e);
 }
