@@ -228,12 +228,13 @@ __global__ __launch_bounds__(512) void int8_rows_kernel(const int8_t* b_base, co
 //
 // A step's pieces of 16 bytes lie in LDS in the order in which the loads leave them (a wave's 64 lanes side by side), rows of BK bytes; which piece of its row a lane
 // asks for is turned round by its row, so that the 32 rows of an operand read meet each bank as often as it takes and no more.
-// One barrier a step: before the step's last products the next step has arrived, its first operands are read while those products run, and the loads of the step
-// after it go where this step's operands were, which all are in registers by then.
-// W = 4 (256 x 256): 256 accumulators a lane, one wave a SIMD; a piece read from LDS meets four others (128 KiB of LDS reads for 2,048 cycles of products and
-// 64 KiB of K). W = 2 (128 x 128): two workgroups a CU, for grids that would not cover the chip.
+// Four steps are in LDS or on their way. One barrier a step: before the step's last products the next step has arrived, its first operands are read while those
+// products run, and the loads of the step four on go where this step's operands were, which all are in registers by then.
+// W = 4 (256 x 256): 256 accumulators a lane, one wave a SIMD; a piece read from LDS meets four others. W = 2 (128 x 128): two workgroups a CU, for grids that would
+// not cover the chip.
 template <int W, int BK>
 struct Int8Tile {
+    static constexpr int kStages = 4;
     static constexpr int kRows = 64 * W, kPieces = BK / 16, kStage = 2 * kRows * BK;     // bytes of a step: A, then B
     static constexpr int kLoads = kStage / 1024 / 4;                                     // of a wave
     static constexpr int kRowsPerLoad = 1024 / BK, kSteps = BK / 32;
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void int8_tile_kernel(Int8Para
 {
     using Tile = Int8Tile<W, BK>;
     constexpr int kWave = 32 * W, kStage = Tile::kStage, kSteps = Tile::kSteps;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStage];
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];           // four steps
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, g = lane >> 5;
 
     // Workgroups go round the eight XCDs; each takes a run of tiles, eight row blocks by all columns at a time, so that its L2 sees an operand more than once.
@@ -287,9 +288,9 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void int8_tile_kernel(Int8Para
     const int8_t* const b = p.b + n0 * p.ldb;
     const uint32_t a_bytes = static_cast<uint32_t>(rows * p.lda), b_bytes = static_cast<uint32_t>(cols * p.ldb);
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
-    auto fetch = [&](int t) {                                    // step `begin + t` into its half of LDS
-        const uint32_t k = static_cast<uint32_t>(begin + t) * BK, to = lds + (t & 1) * kStage + wave * (kStage / 8);
-        // (behind the slice's last step: nothing, into a half that nobody reads any more)
+    auto fetch = [&](int t) {                                    // step `begin + t` into its quarter of LDS
+        const uint32_t k = static_cast<uint32_t>(begin + t) * BK, to = lds + (t & 3) * kStage + wave * (kStage / 8);
+        // (behind the slice's last step: nothing, into a quarter that nobody reads any more)
         const bool is = t < count;
         const srd_t sa = plain_srd(a + k, is ? a_bytes - k : 0u), sb = plain_srd(b + k, is && b_bytes > k ? b_bytes - k : 0u);
 #pragma unroll
@@ -302,7 +303,7 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void int8_tile_kernel(Int8Para
     const int wm = (wave & 1) * kWave, wn = (wave >> 1) * kWave;
     i32x4_t fa[2][W], fb[2][W];
     auto operands = [&](int t, int s, i32x4_t (&xa)[W], i32x4_t (&xb)[W]) {
-        const uint8_t* const half = smem + (t & 1) * kStage;
+        const uint8_t* const half = smem + (t & 3) * kStage;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             const int ra = wm + i * 32 + c, rb = wn + i * 32 + c;
@@ -311,31 +312,49 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void int8_tile_kernel(Int8Para
         }
     };
     i32x16_t acc[W][W] = {};
-    auto products = [&](const i32x4_t (&xa)[W], const i32x4_t (&xb)[W]) {
+    auto products = [&](const i32x4_t (&xa)[W], const i32x4_t (&xb)[W], int first, int last) {
 #pragma unroll
         for (int i = 0; i < W; ++i)
+            if (i >= first && i < last)
 #pragma unroll
-            for (int j = 0; j < W; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xa[i], xb[j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < W; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xa[i], xb[j], acc[i][j], 0, 0, 0);
     };
-    auto arrived = [&] {                                         // own loads into LDS and reads from it are done, and everyone's
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // A read of an operand after each product while there are any. (The compiler would put them where they are used, and wait.)
+    auto interleave = [&] {
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+    };
+    // own loads but those of the steps behind the next are in, own reads done, and everyone's
+    auto arrived = [&] {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * Tile::kLoads) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
     fetch(0);                                                    // (no slice is empty)
+    fetch(1);
+    fetch(2);
     arrived();
     operands(0, 0, fa[0], fb[0]);
-    fetch(1);
+    fetch(3);
     for (int t = 0; t < count; ++t) {
 #pragma unroll
         for (int s = 0; s < kSteps - 1; ++s) {
             operands(t, s + 1, fa[(s + 1) & 1], fb[(s + 1) & 1]);
-            products(fa[s & 1], fb[s & 1]);
+            products(fa[s & 1], fb[s & 1], 0, W);
+            interleave();
+            __builtin_amdgcn_sched_barrier(0);
         }
         arrived();
         operands(t + 1, 0, fa[0], fb[0]);                        // (behind the last step: whatever lies there, for no product)
-        fetch(t + 2);
-        products(fa[1], fb[1]);
+        products(fa[1], fb[1], 0, W / 2);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(t + 4);
+        __builtin_amdgcn_sched_barrier(0);
+        products(fa[1], fb[1], W / 2, W);
+        __builtin_amdgcn_sched_barrier(0);
     }
 
     // A lane has column c and rows 8 (e / 4) + 4 g + e % 4 of each 32 x 32, and leaves with 16 columns of row lane / 2: each tile is turned round in the wave's own
@@ -542,10 +561,18 @@ extern "C" int rocm_launch_int8(const RocmInt8Args* args, rocm_stream_t stream)
     p.partial = plan.slices > 1 ? args->partial : nullptr;
     const unsigned tm = static_cast<unsigned>((p.m + plan.tile - 1) / plan.tile), tn = static_cast<unsigned>((p.n + plan.tile - 1) / plan.tile);
     const dim3 grid((tm * tn + 7) / 8 * 8, static_cast<unsigned>(plan.slices));
-    if (plan.tile == 256) hipLaunchKernelGGL((int8_tile_kernel<4, 64, false>), grid, dim3(256), 0, s, p, tm, tn);
-    else if (p.partial) hipLaunchKernelGGL((int8_tile_kernel<2, 128, true>), grid, dim3(256), 0, s, p, tm, tn);
-    else hipLaunchKernelGGL((int8_tile_kernel<2, 128, false>), grid, dim3(256), 0, s, p, tm, tn);
-    hipError_t e = hipGetLastError();
+    auto tiled = [&](auto kernel, size_t lds) {
+        if (lds > 65536) {           // more than a kernel gets without asking
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+            if (e != hipSuccess) return e;
+        }
+        hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, p, tm, tn);
+        return hipGetLastError();
+    };
+    constexpr size_t kLds256 = 4 * Int8Tile<4, 64>::kStage, kLds128 = 4 * Int8Tile<2, 64>::kStage;
+    hipError_t e = plan.tile == 256 ? tiled(int8_tile_kernel<4, 64, false>, kLds256)
+                   : p.partial      ? tiled(int8_tile_kernel<2, 64, true>, kLds128)
+                                    : tiled(int8_tile_kernel<2, 64, false>, kLds128);
     if (e == hipSuccess && p.partial) {
         const unsigned y = static_cast<unsigned>(p.m < 32768 ? p.m : 32768);
         hipLaunchKernelGGL(int8_reduce_kernel, dim3(static_cast<unsigned>((p.n + 255) / 256), y, static_cast<unsigned>((p.m + y - 1) / y)), dim3(256), 0, s, p, plan.slices);

@@ -26,7 +26,7 @@ def run(ep, m, n, k, dtype, *, y_dtype=None, bias=None, codes=False, scale_dtype
     bias_np = None
     if bias is not None:
         bias_np = synth.to_dtype(rng.standard_normal(n if bias == "column" else (m, n)).astype(np.float32), y_dtype)
-    product = (q.astype(np.int64) @ b.astype(np.int64).T).astype(np.float64) * sa.astype(np.float64)[:, None] * as64(sb, scale_dtype)
+    product = (q.astype(np.float64) @ b.astype(np.float64).T) * sa.astype(np.float64)[:, None] * as64(sb, scale_dtype)
     want = product + (as64(bias_np, y_dtype) if bias_np is not None else 0)
     dev = Device(ep)
     kernel = ep.get_kernel({"K": k, "N": n}, op_type="MatMulInt8")
@@ -109,6 +109,17 @@ def test_the_largest_sums(ep, m):
 @pytest.mark.parametrize("m,n,k", [(500, 512, 18944), (300, 384, 4096), (1000, 3584, 1024), (600, 2000, 896)])
 def test_tall(ep, m, n, k):
     run(ep, m, n, k, E.BF16, bias="column", workspace=True)
+
+
+@pytest.mark.parametrize("k", [64, 65, 128, 192, 208, 256, 320, 1040])
+def test_tiles_of_256(ep, k):
+    """Enough tiles for the largest ones, their last rows and columns partial, from one step of K to many."""
+    assert run(ep, 2050, 6200, k, E.F16, bias="column") == "int8_tile_256"
+
+
+@pytest.mark.parametrize("y_dtype,bias,n", [(E.F32, "row", 6200), (E.BF16, "row", 6200), (E.BF16, "column", 6201), (E.F32, None, 6203)])
+def test_results_of_tiles_of_256(ep, y_dtype, bias, n):
+    assert run(ep, 2050, n, 128, E.BF16, y_dtype=y_dtype, bias=bias) == "int8_tile_256"
 
 
 @pytest.mark.parametrize("m", [1, 5, 20, 150])
