@@ -357,69 +357,84 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void int8_tile_kernel(Int8Para
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // A lane has column c and rows 8 (e / 4) + 4 g + e % 4 of each 32 x 32, and leaves with 16 columns of row lane / 2: each tile is turned round in the wave's own
-    // piece of LDS. (One form takes the accumulators out, whatever becomes of them: with one for each kind of result the compiler moves all 256 at once, and spills.)
-    constexpr int kTurn = 36;                                    // dwords from a row to the next
+    // A lane has column c and rows 8 (e / 4) + 4 g + e % 4 of each 32 x 32; 32 rows of all of the wave's columns are turned round in the wave's own piece of LDS, and
+    // a lane leaves with eight columns, the same ones in all of its rows: whole lines of y. (One form takes the accumulators out, whatever becomes of them: with one
+    // for each kind of result the compiler moves all 256 at once, and spills.)
+    constexpr int kTurn = kWave + 8, kAcross = kWave / 8, kDown = 64 / kAcross;          // dwords from a row to the next; lanes to a row, rows of a wave
+    static_assert(32 % kDown == 0 && 4 * (4 * 32 * kTurn) <= 4 * kStage);
+    const int64_t first = n0 + wn + lane % kAcross * 8;
+    const int64_t left = p.n - first;                            // columns from here on
+    const int mine = lane / kAcross;
+    float sb[8] = {}, bias[8] = {};
+    bool wide = false;                                           // whole eights go out at once
+    if constexpr (SLICED) {
+        wide = (p.n & 3) == 0 && left >= 8;
+    } else {
+        const bool row_bias = p.bias && (p.bias_dtype & ROCM_BIAS_PER_ROW);
+        wide = !row_bias && left >= 8 && (p.n & (p.y_dtype == ROCM_DT_F32 ? 3 : 7)) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const int64_t col = q < left ? first + q : p.n - 1;
+            sb[q] = load_as_f32(p.b_scale, p.b_scale_dtype, col);
+            if (p.bias && !row_bias) bias[q] = load_as_f32(p.bias, p.bias_dtype, col);
+        }
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (what was fetched behind the end has to be in before LDS is used for something else)
     __syncthreads();
     int32_t* const turn = reinterpret_cast<int32_t*>(smem) + wave * (32 * kTurn);
-    const bool wide = p.y_dtype != ROCM_DT_F32 && (p.n & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && !(p.bias_dtype & ROCM_BIAS_PER_ROW);
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-        const int64_t first = n0 + wn + j * 32 + (lane & 1) * 16;
-        float sb[16];
-        if constexpr (!SLICED)
+    for (int i = 0; i < W; ++i) {
 #pragma unroll
-            for (int q = 0; q < 16; ++q) sb[q] = load_as_f32(p.b_scale, p.b_scale_dtype, first + q < p.n ? first + q : p.n - 1);
+        for (int j = 0; j < W; ++j)
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) turn[((e >> 2) * 8 + g * 4 + (e & 3)) * kTurn + c] = acc[i][j][e];
-            lds_order();
-            const int64_t row = m0 + wm + i * 32 + (lane >> 1);
-            int32_t* const mine = turn + (lane >> 1) * kTurn + (lane & 1) * 16;
-            if (row < p.m) {
-                if constexpr (SLICED) {
-                    int32_t* const part = p.partial + (static_cast<int64_t>(slice) * p.m + row) * p.n;
-                    for (int q = 0; q < 16 && first + q < p.n; ++q) part[first + q] = mine[q];
+            for (int e = 0; e < 16; ++e) turn[((e >> 2) * 8 + g * 4 + (e & 3)) * kTurn + j * 32 + c] = acc[i][j][e];
+        lds_order();
+#pragma unroll 2
+        for (int d = 0; d < 32; d += kDown) {
+            const int64_t row = m0 + wm + i * 32 + d + mine;
+            if (row >= p.m || left <= 0) continue;
+            const int32_t* const from = turn + (d + mine) * kTurn + lane % kAcross * 8;
+            const int4 lo = *reinterpret_cast<const int4*>(from), hi = *reinterpret_cast<const int4*>(from + 4);
+            if constexpr (SLICED) {
+                int32_t* const part = p.partial + (static_cast<int64_t>(slice) * p.m + row) * p.n + first;
+                if (wide) {
+                    reinterpret_cast<int4*>(part)[0] = lo;
+                    reinterpret_cast<int4*>(part)[1] = hi;
                 } else {
-                    const float sa = p.a_scale[row];
-                    float v[16];
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) v[q] = static_cast<float>(mine[q]) * sa * sb[q];
-                    if (wide) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int64_t at = first + h * 8;
-                            if (at >= p.n) continue;
-                            float w[8];
-#pragma unroll
-                            for (int q = 0; q < 8; ++q) w[q] = v[h * 8 + q];
-                            if (p.bias)
-#pragma unroll
-                                for (int q = 0; q < 8; ++q) w[q] += load_as_f32(p.bias, p.bias_dtype, at + q);
-                            uint16_t* const y = static_cast<uint16_t*>(p.y) + row * p.n + at;
-                            if (p.y_dtype == ROCM_DT_BF16) {
-                                Eight<uint16_t, true> o;
-                                o.set(w);
-                                *reinterpret_cast<uint4*>(y) = make_uint4(o.raw.x, o.raw.y, o.raw.z, o.raw.w);
-                            } else {
-                                Eight<uint16_t, false> o;
-                                o.set(w);
-                                *reinterpret_cast<uint4*>(y) = make_uint4(o.raw.x, o.raw.y, o.raw.z, o.raw.w);
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) mine[q] = __float_as_int(v[q]);       // (a run-time index, so through LDS)
 #pragma unroll 1
-                        for (int q = 0; q < 16 && first + q < p.n; ++q)
-                            store_from_f32(p.y, p.y_dtype, row * p.n + first + q, with_bias(__int_as_float(mine[q]), p.bias, p.bias_dtype, row, p.n, first + q, p.y_dtype));
+                    for (int q = 0; q < 8 && q < left; ++q) part[q] = from[q];
+                }
+            } else {
+                const float sa = p.a_scale[row];
+                if (!wide) {
+#pragma unroll 1
+                    for (int q = 0; q < 8 && q < left; ++q) store_scaled(p, row, first + q, from[q], sa, load_as_f32(p.b_scale, p.b_scale_dtype, first + q));
+                    continue;
+                }
+                const int32_t sum[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                float v[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[q] = static_cast<float>(sum[q]) * sa * sb[q] + bias[q];
+                const int64_t at = row * p.n + first;
+                if (p.y_dtype == ROCM_DT_F32) {
+                    float4* const y = reinterpret_cast<float4*>(static_cast<float*>(p.y) + at);
+                    y[0] = make_float4(v[0], v[1], v[2], v[3]);
+                    y[1] = make_float4(v[4], v[5], v[6], v[7]);
+                } else {
+                    uint4* const y = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + at);
+                    Eight<uint16_t, true> wide_range;
+                    Eight<uint16_t, false> half;
+                    if (p.y_dtype == ROCM_DT_BF16) {
+                        wide_range.set(v);
+                        *y = make_uint4(wide_range.raw.x, wide_range.raw.y, wide_range.raw.z, wide_range.raw.w);
+                    } else {
+                        half.set(v);
+                        *y = make_uint4(half.raw.x, half.raw.y, half.raw.z, half.raw.w);
                     }
                 }
             }
-            lds_order();
         }
+        lds_order();
     }
 }
 
