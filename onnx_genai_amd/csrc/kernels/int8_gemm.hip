@@ -18,40 +18,70 @@ typedef __attribute__((ext_vector_type(16))) int i32x16_t;
 
 __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
-// One workgroup a row: the largest magnitude, then the codes from a second read, which comes from L2. Memory bounds it.
-template <typename T, bool BF16>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ a, int64_t k, int64_t kp, int8_t* __restrict__ codes, float* __restrict__ scales)
+// One workgroup of WAVES waves a row: the largest magnitude, then the codes. The first HELD eights of a thread stay in registers, all loaded before any is looked
+// at; what lies behind them is read again. Memory bounds it.
+template <typename T, bool BF16, int WAVES, int HELD>
+__global__ __launch_bounds__(WAVES * 64) void quantize_rows_kernel(const T* __restrict__ a, int64_t k, int64_t kp, int8_t* __restrict__ codes, float* __restrict__ scales)
 {
     using V8 = Eight<T, BF16>;
-    __shared__ uint32_t slots[16];
+    constexpr int kThreads = WAVES * 64;
+    __shared__ uint32_t slots[WAVES];
     const int64_t row = blockIdx.x;
     const T* const x = a + row * k;
-    const int vectors = static_cast<int>(kp / 8);
+    const int vectors = static_cast<int>(kp / 8), whole = static_cast<int>(k / 8), rest = static_cast<int>(k & 7);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    V8 held[HELD];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const int i = threadIdx.x + h * kThreads;
+        held[h].zero();
+        if (i < whole) held[h].load(x + i * 8);
+    }
+    if (rest)
+#pragma unroll
+        for (int h = 0; h < HELD; ++h)
+            if (static_cast<int>(threadIdx.x) + h * kThreads == whole) held[h].load_first(x + whole * 8, rest);
     auto piece = [&](int i, float (&v)[8]) {
         V8 e;
-        const int left = static_cast<int>(k) - i * 8;
-        if (left >= 8) e.load(x + i * 8);
-        else if (left > 0) e.load_first(x + i * 8, left);
+        if (i < whole) e.load(x + i * 8);
+        else if (i == whole && rest) e.load_first(x + i * 8, rest);
         else e.zero();
         e.get(v);
     };
     uint32_t amax = 0;
-    for (int i = threadIdx.x; i < vectors; i += 256) {
-        float v[8];
-        piece(i, v);
+    float v[8];
+    auto look = [&] {
 #pragma unroll
         for (int e = 0; e < 8; ++e) amax = larger(amax, __float_as_uint(v[e]) & 0x7fffffffu);
+    };
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        held[h].get(v);
+        look();
     }
-    const RowScale scale(over_workgroup(amax, slots, wave, 4, larger));
-    if (threadIdx.x == 0) scales[row] = scale.scale;
-    for (int i = threadIdx.x; i < vectors; i += 256) {
-        float v[8];
+    for (int i = threadIdx.x + HELD * kThreads; i < vectors; i += kThreads) {
         piece(i, v);
+        look();
+    }
+    const RowScale scale(over_workgroup(amax, slots, wave, WAVES, larger));
+    if (threadIdx.x == 0) scales[row] = scale.scale;
+    auto put = [&](int i) {
         uint32_t d[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < 8; ++e) d[e >> 2] |= static_cast<uint32_t>(scale.code(v[e]) & 0xff) << (8 * (e & 3));
         *reinterpret_cast<uint2*>(codes + row * kp + i * 8) = make_uint2(d[0], d[1]);
+    };
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const int i = threadIdx.x + h * kThreads;
+        if (i < vectors) {
+            held[h].get(v);
+            put(i);
+        }
+    }
+    for (int i = threadIdx.x + HELD * kThreads; i < vectors; i += kThreads) {
+        piece(i, v);
+        put(i);
     }
 }
 
@@ -259,21 +289,22 @@ __device__ __forceinline__ srd_t plain_srd(const void* base, uint32_t bytes)
 }
 
 template <int W, int BK, bool SLICED>
-__global__ __launch_bounds__(256, W == 4 ? 1 : 2) void int8_tile_kernel(Int8Params p, unsigned tiles_m, unsigned tiles_n)
+__global__ __launch_bounds__(256, W == 4 ? 1 : 2) void int8_tile_kernel(Int8Params p, unsigned tiles_m, unsigned tiles_n, unsigned slices)
 {
     using Tile = Int8Tile<W, BK>;
     constexpr int kWave = 32 * W, kStage = Tile::kStage, kSteps = Tile::kSteps;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];           // four steps
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, g = lane >> 5;
 
-    // Workgroups go round the eight XCDs; each takes a run of tiles, eight row blocks by all columns at a time, so that its L2 sees an operand more than once.
-    const unsigned all = tiles_m * tiles_n, per = (all + 7) / 8, linear = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    // Workgroups go round the eight XCDs; each takes a run of one slice's tiles, eight row blocks by all columns at a time, so that its L2 sees an operand more than once.
+    const unsigned of_slice = tiles_m * tiles_n, all = SLICED ? of_slice * slices : of_slice, per = (all + 7) / 8, linear = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((blockIdx.x >> 3) >= per || linear >= all) return;
-    const unsigned band = linear / (8 * tiles_n), in_band = linear - band * 8 * tiles_n, rows_here = min(8u, tiles_m - band * 8);
+    const unsigned slice = SLICED ? linear / of_slice : 0, tile = linear - slice * of_slice;
+    const unsigned band = tile / (8 * tiles_n), in_band = tile - band * 8 * tiles_n, rows_here = min(8u, tiles_m - band * 8);
     const int64_t m0 = static_cast<int64_t>(band * 8 + in_band % rows_here) * Tile::kRows, n0 = static_cast<int64_t>(in_band / rows_here) * Tile::kRows;
     const int rows = static_cast<int>(p.m - m0 < Tile::kRows ? p.m - m0 : Tile::kRows), cols = static_cast<int>(p.n - n0 < Tile::kRows ? p.n - n0 : Tile::kRows);
-    const int slice = static_cast<int>(blockIdx.y), total = p.steps * (128 / BK), share = p.steps_per_slice * (128 / BK);
-    const int begin = slice * share, end = min(begin + share, total), count = end - begin;
+    const int total = p.steps * (128 / BK), share = p.steps_per_slice * (128 / BK);
+    const int begin = static_cast<int>(slice) * share, end = min(begin + share, total), count = end - begin;
 
     // Load i of a wave brings kRowsPerLoad rows; rows that are not there repeat the last. The range ends with the operand's last row, and moves on with K.
     uint32_t at[Tile::kLoads];
@@ -438,14 +469,24 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void int8_tile_kernel(Int8Para
     }
 }
 
-// y from the sums of slices of K.
+// y from the sums of slices of K: four columns a thread where rows of n begin at a multiple of four.
+template <int FOUR>
 __global__ __launch_bounds__(256) void int8_reduce_kernel(Int8Params p, int slices)
 {
-    const int64_t row = static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y, col = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t row = static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y, col = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * FOUR;
     if (row >= p.m || col >= p.n) return;
-    int32_t sum = 0;
-    for (int i = 0; i < slices; ++i) sum += p.partial[(i * p.m + row) * p.n + col];
-    store_scaled(p, row, col, sum, p.a_scale[row], load_as_f32(p.b_scale, p.b_scale_dtype, col));
+    int32_t sum[FOUR] = {};
+    for (int i = 0; i < slices; ++i) {
+        const int32_t* const from = p.partial + (i * p.m + row) * p.n + col;
+        if constexpr (FOUR == 4) {
+            const int4 v = *reinterpret_cast<const int4*>(from);
+            sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+        } else {
+            sum[0] += *from;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < FOUR; ++q) store_scaled(p, row, col + q, sum[q], p.a_scale[row], load_as_f32(p.b_scale, p.b_scale_dtype, col + q));
 }
 
 Int8Params params_of(const RocmInt8Args* a)
@@ -478,13 +519,14 @@ extern "C" int rocm_launch_quantize_rows(const void* a, int dtype, int64_t m, in
     if (m > 0x7fffffff || k >= ROCM_INT8_MAX_K) return static_cast<int>(hipErrorInvalidValue);
     const int64_t kp = (k + 127) / 128 * 128;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    auto go = [&](auto kernel, auto* x) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(m)), dim3(256), 0, s, x, k, kp, codes, scales);
+    auto go = [&](auto kernel, unsigned threads, auto* x) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(m)), dim3(threads), 0, s, x, k, kp, codes, scales);
         return static_cast<int>(hipGetLastError());
     };
-    if (dtype == ROCM_DT_F32) return go(quantize_rows_kernel<float, false>, static_cast<const float*>(a));
-    if (dtype == ROCM_DT_BF16) return go(quantize_rows_kernel<uint16_t, true>, static_cast<const uint16_t*>(a));
-    return go(quantize_rows_kernel<uint16_t, false>, static_cast<const uint16_t*>(a));
+    auto held = [&](auto four_waves, auto sixteen_waves, auto* x) { return kp <= 8192 ? go(four_waves, 256u, x) : go(sixteen_waves, 1024u, x); };
+    if (dtype == ROCM_DT_F32) return held(quantize_rows_kernel<float, false, 4, 4>, quantize_rows_kernel<float, false, 16, 3>, static_cast<const float*>(a));
+    if (dtype == ROCM_DT_BF16) return held(quantize_rows_kernel<uint16_t, true, 4, 4>, quantize_rows_kernel<uint16_t, true, 16, 3>, static_cast<const uint16_t*>(a));
+    return held(quantize_rows_kernel<uint16_t, false, 4, 4>, quantize_rows_kernel<uint16_t, false, 16, 3>, static_cast<const uint16_t*>(a));
 }
 
 extern "C" int rocm_launch_pad_codes(const int8_t* from, int64_t rows, int64_t k, int8_t* to, rocm_stream_t stream)
@@ -575,13 +617,14 @@ extern "C" int rocm_launch_int8(const RocmInt8Args* args, rocm_stream_t stream)
     p.steps_per_slice = (p.steps + plan.slices - 1) / plan.slices;
     p.partial = plan.slices > 1 ? args->partial : nullptr;
     const unsigned tm = static_cast<unsigned>((p.m + plan.tile - 1) / plan.tile), tn = static_cast<unsigned>((p.n + plan.tile - 1) / plan.tile);
-    const dim3 grid((tm * tn + 7) / 8 * 8, static_cast<unsigned>(plan.slices));
+    const unsigned slices = static_cast<unsigned>(plan.slices);
+    const dim3 grid((tm * tn * slices + 7) / 8 * 8);
     auto tiled = [&](auto kernel, size_t lds) {
         if (lds > 65536) {           // more than a kernel gets without asking
             const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
             if (e != hipSuccess) return e;
         }
-        hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, p, tm, tn);
+        hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, p, tm, tn, slices);
         return hipGetLastError();
     };
     constexpr size_t kLds256 = 4 * Int8Tile<4, 64>::kStage, kLds128 = 4 * Int8Tile<2, 64>::kStage;
@@ -590,7 +633,9 @@ extern "C" int rocm_launch_int8(const RocmInt8Args* args, rocm_stream_t stream)
                                     : tiled(int8_tile_kernel<2, 64, false>, kLds128);
     if (e == hipSuccess && p.partial) {
         const unsigned y = static_cast<unsigned>(p.m < 32768 ? p.m : 32768);
-        hipLaunchKernelGGL(int8_reduce_kernel, dim3(static_cast<unsigned>((p.n + 255) / 256), y, static_cast<unsigned>((p.m + y - 1) / y)), dim3(256), 0, s, p, plan.slices);
+        const bool four = p.n % 4 == 0;
+        const int64_t across = four ? p.n / 4 : p.n;
+        hipLaunchKernelGGL(four ? int8_reduce_kernel<4> : int8_reduce_kernel<1>, dim3(static_cast<unsigned>((across + 255) / 256), y, static_cast<unsigned>((p.m + y - 1) / y)), dim3(256), 0, s, p, plan.slices);
         e = hipGetLastError();
     }
     return static_cast<int>(e);
