@@ -15,6 +15,7 @@ struct MoePlan {
     int where;                 // kMoeFused, kMoeTable, kMoeTiles
     int slots;                 // experts that can be active, or tiles
     int tile_rows;
+    bool tall;                 // tiles of 128 pairs, weights rounded to f16
     int64_t kp, ip, pairs, eight_bytes;
     uint64_t table, eights, expert, weight, pair_row, token, base, tiles, x, h, out, total;
 };
@@ -27,7 +28,11 @@ MoePlan plan_of(const RocmMoeArgs& a)
     l.where = a.rows <= 4 && a.experts <= 256 && l.pairs <= kFewPairs && a.rows * ((a.hidden + 2047) / 2048) <= 12 ? kMoeFused : a.rows <= kFewTokens && l.pairs <= kFewPairs ? kMoeTable : kMoeTiles;
     l.tile_rows = l.pairs >= kTallPairs * a.experts ? 128 : 32;
     l.slots = static_cast<int>((l.where == kMoeTiles ? l.pairs / l.tile_rows : 0) + (l.pairs < a.experts ? l.pairs : a.experts));
-    l.kp = (a.hidden + 7) / 8 * 8;
+    // Weights are scaled in f16 where activations and scales are f16: rounding them to bf16 would double y's error, and f32 scales may lie outside of f16's range.
+    // (Those tiles address an expert's weights and the rows in 32 bits.)
+    const int64_t most = 1ll << 31, columns = a.hidden > 2 * a.inter ? a.hidden : 2 * a.inter, deepest = (a.hidden > a.inter ? a.hidden : a.inter) + 128;
+    l.tall = l.where == kMoeTiles && l.tile_rows == 128 && a.dtype == ROCM_DT_F16 && a.scale_dtype == ROCM_DT_F16 && columns * deepest / 2 < most && a.rows * (a.hidden + 64) * 2 < most;
+    l.kp = l.where == kMoeTiles ? (a.hidden + 63) / 64 * 64 : (a.hidden + 7) / 8 * 8;        // (tiles read whole steps of 64)
     l.ip = (a.inter + 127) / 128 * 128;      // (steps of 64 and 128)
     auto part = [&](uint64_t bytes) {
         const uint64_t here = l.total;
@@ -75,8 +80,8 @@ MoeMatrix matrix_of(const RocmMoeArgs& a, const RocmMoeWeights& w, const RocmMoe
 extern "C" uint64_t rocm_moe_workspace_bytes(const RocmMoeArgs* args) { return mnb::plan_of(*args).total; }
 extern "C" const char* rocm_moe_variant(const RocmMoeArgs* args)
 {
-    const int where = mnb::plan_of(*args).where;
-    return where == mnb::kMoeFused ? "moe_few" : where == mnb::kMoeTable ? "moe_table" : mnb::plan_of(*args).tile_rows == 128 ? "moe_tall_tiles" : "moe_tiles";
+    const mnb::MoePlan l = mnb::plan_of(*args);
+    return l.where == mnb::kMoeFused ? "moe_few" : l.where == mnb::kMoeTable ? "moe_table" : l.tall ? "moe_tall_tiles" : l.tile_rows == 128 ? "moe_tiles_128" : "moe_tiles_32";
 }
 
 extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_stream_t stream)
@@ -152,7 +157,8 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     };
     MoeTileCall first = tiled(up.m, up.x, up.ldx), second = tiled(down.m, up.h, l.ip);
     first.token = route.token;
-    rc = launch_moe_tile(a, first, true, l.tile_rows, s);
-    if (rc == 0) rc = launch_moe_tile(a, second, false, l.tile_rows, s);
+    auto half = [&](const MoeTileCall& t, bool is_up) { return l.tall ? launch_moe_tall(t, is_up, s) : launch_moe_tile(a, t, is_up, l.tile_rows, s); };
+    rc = half(first, true);
+    if (rc == 0) rc = half(second, false);
     return rc != 0 ? rc : launch_moe_combine(a, route, down.out, s);
 }

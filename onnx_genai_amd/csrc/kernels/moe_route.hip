@@ -39,9 +39,17 @@ __global__ __launch_bounds__(1024) void moe_plan_kernel(int pairs, int k, int ti
     for (int i = t; i < eight_bytes; i += 1024) eights[i] = 0x88;
     count[t] = 0;
     __syncthreads();
-    for (int p = t; p < pairs; p += 1024) {
-        const int e = r.expert[p];
-        if (e >= 0) r.pair_row[p] = atomicAdd(&count[e], 1);
+    // (kBatch pairs a thread at once: one at a time the trips to memory alone are 1.5 us for each 1024 pairs)
+    constexpr int kBatch = 8;
+    for (int p = t; p < pairs; p += kBatch * 1024) {
+        int e[kBatch], place[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) e[i] = r.expert[min(p + i * 1024, pairs - 1)];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) place[i] = p + i * 1024 < pairs && e[i] >= 0 ? atomicAdd(&count[e[i]], 1) : 0;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (p + i * 1024 < pairs) r.pair_row[p + i * 1024] = place[i];
     }
     __syncthreads();
     const int own = count[t], own_tiles = (own + tile_rows - 1) / tile_rows;
@@ -58,14 +66,22 @@ __global__ __launch_bounds__(1024) void moe_plan_kernel(int pairs, int k, int ti
     const int row0 = rows_to[t] - own, tile0 = tiles_to[t] - own_tiles;
     for (int i = 0; i < own_tiles; ++i) r.tiles[tile0 + i] = make_int4(t, row0 + i * tile_rows, min(tile_rows, own - i * tile_rows), 0);
     for (int i = tiles_to[1023] + t; i < max_tiles; i += 1024) r.tiles[i] = make_int4(0, 0, 0, 0);
-    for (int p = t; p < pairs; p += 1024) {
-        const int e = r.expert[p];
-        int row = -1;
-        if (e >= 0) {
-            row = rows_to[e] - count[e] + r.pair_row[p];
-            r.token[row] = p / k;
+    for (int p = t; p < pairs; p += kBatch * 1024) {
+        int e[kBatch], place[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int at = min(p + i * 1024, pairs - 1);
+            e[i] = r.expert[at];
+            place[i] = r.pair_row[at];
         }
-        r.pair_row[p] = row;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int at = p + i * 1024;
+            if (at >= pairs) break;
+            const int row = e[i] >= 0 ? rows_to[e[i]] - count[e[i]] + place[i] : -1;
+            if (row >= 0) r.token[row] = at / k;
+            r.pair_row[at] = row;
+        }
     }
 }
 

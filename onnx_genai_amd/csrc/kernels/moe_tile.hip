@@ -3,8 +3,9 @@
 // A wave has all rows of the tile and 32 columns of weights that no other wave has (16 of gate beside 16 of up), so that it unpacks them for itself, from
 // registers into the matrix core; only activations go through LDS, in the order in which a dword's nibbles come out (0 4 1 5 2 6 3 7 of each eight).
 // Weights enter the matrix core as q - zp, which is exact in 16 bits, and each block's sum is scaled in f32: no weight is rounded.
-// TM = 4 (prompts): the matrix cores and the vector instructions beside them bound it, 64 to scale a block's sums and 72 (bf16: 152) to unpack 64 k for 512
-// cycles of products. TM = 1 (a few rows an expert): the weights' bytes.
+// TM = 4 (prompts that are not scaled in f16): the matrix cores and the vector instructions beside them bound it, 64 to scale a block's sums and 44 (bf16: 76) to
+// unpack 64 k for 512 cycles of products. TM = 1 (a few rows an expert): the weights' bytes, and a CU's path to memory, where 64 columns' scales take as long as
+// their weights.
 // h is rounded to the activations' type here (as a graph of separate nodes has it): a second part of it would be half again as many products in the second half.
 #include "moe.hiph"
 #include "prefill_common.hiph"
@@ -18,6 +19,7 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
 {
     constexpr int kPitch = 9;                                            // pieces of 16 bytes from a row of 64 elements in LDS to the next
     constexpr int kScales = BS == 32 ? 2 : 1;                            // blocks of a step
+    constexpr int kAhead = 2;                                            // steps whose weights are in registers or on their way
     __shared__ uint4 staged[2][TM * 32 * kPitch];
     const unsigned index = blockIdx.z * gridDim.y + blockIdx.y;
     if (index >= p.count) return;
@@ -30,7 +32,7 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
     const uint8_t* const b = (which ? p.m.w[1].b : p.m.w[0].b) + at * p.m.row_bytes;
     const ST* const s = static_cast<const ST*>(which ? p.m.w[1].scales : p.m.w[0].scales) + at * p.m.kb;
     const uint8_t* const z = (which ? p.m.w[1].zp : p.m.w[0].zp) + at * p.m.zp_row;
-    const int width = static_cast<int>(p.ldx), steps = (width + 63) >> 6, shift = 31 - __builtin_clz(p.m.block_size), row_bytes = static_cast<int>(p.m.row_bytes);
+    const int steps = static_cast<int>(p.ldx) >> 6, shift = 31 - __builtin_clz(p.m.block_size), row_bytes = static_cast<int>(p.m.row_bytes), last_block = p.m.kb - 1;
 
     const int piece = threadIdx.x & 7;
     const uint16_t* x[TM];
@@ -42,24 +44,25 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
     struct Weights {
         uint4 w;
         ST s[kScales];
-        uint32_t z;
+        uint16_t z;
     };
     auto load_w = [&](int t, Weights& to) {
         const int byte = t * 32 + g * 16;
         to.w = *reinterpret_cast<const uint4*>(b + (byte < row_bytes ? byte : 0));                                // (behind a row's end its activations are zero)
-        const int block = min(t * 64 >> shift, p.m.kb - 1);
+        const int block = min(t * 64 >> shift, last_block);
 #pragma unroll
-        for (int i = 0; i < kScales; ++i) to.s[i] = s[min(block + i, p.m.kb - 1)];
+        for (int i = 0; i < kScales; ++i) to.s[i] = s[min(block + i, last_block)];
         to.z = z[block >> 1];
     };
-    auto load_x = [&](int t, uint4 (&to)[TM]) {
+    uint4 ahead[TM];
+    auto load_x = [&](int t) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) to[i] = t * 64 + piece * 8 < width ? *reinterpret_cast<const uint4*>(x[i] + t * 64) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < TM; ++i) ahead[i] = *reinterpret_cast<const uint4*>(x[i] + t * 64);
     };
-    auto stage = [&](int t, const uint4 (&from)[TM]) {
+    auto stage = [&](int t) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            const uint4 d = from[i];
+            const uint4 d = ahead[i];
             staged[t & 1][((threadIdx.x >> 3) + i * 32) * kPitch + piece] =
                 make_uint4(__builtin_amdgcn_perm(d.z, d.x, 0x05040100u), __builtin_amdgcn_perm(d.z, d.x, 0x07060302u), __builtin_amdgcn_perm(d.w, d.y, 0x05040100u),
                            __builtin_amdgcn_perm(d.w, d.y, 0x07060302u));
@@ -71,9 +74,21 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
 
     float16_t total[TM] = {}, sum[TM] = {};
     const float16_t none = {};
+    // (The instructions that first touch what was loaded are pinned: the compiler would widen it, and wait for it, a step before.)
     auto scale_of = [&](ST raw) {
-        if constexpr (sizeof(ST) == 4) return static_cast<float>(raw);
-        else return BF16 ? bf16_bits_to_f32(static_cast<uint16_t>(raw)) : f16_bits_to_f32(static_cast<uint16_t>(raw));
+        if constexpr (sizeof(ST) == 4) {
+            return static_cast<float>(raw);
+        } else {
+            float v;
+            if constexpr (BF16) asm volatile("v_lshlrev_b32 %0, 16, %1" : "=v"(v) : "v"(raw));
+            else asm volatile("v_cvt_f32_f16 %0, %1" : "=v"(v) : "v"(raw));
+            return v;
+        }
+    };
+    auto zero_of = [&](uint16_t two, int which) {
+        uint32_t v;
+        asm volatile("v_bfe_u32 %0, %1, %2, 4" : "=v"(v) : "v"(two), "s"(which * 4));
+        return v;
     };
     auto add_up = [&](float scale) {
 #pragma unroll
@@ -87,17 +102,18 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
 #pragma unroll
         for (int i = 0; i < TM; ++i) sum[i] = mfma32<BF16>(staged[t & 1][(i * 32 + c) * kPitch + at_piece], w, first ? none : sum[i]);
     };
+    // A step stages the next one's activations, asks for those of the one behind it, multiplies, and asks for the weights kAhead steps on, where its own were.
     // FIRST, LAST: the step begins, ends a block (of 64 or more)
-    auto step = [&](int t, Weights& now, Weights& next, bool first, bool last) {
-        uint4 ahead[TM];
-        const int to = min(t + 1, steps - 1);
-        load_w(to, next);
-        load_x(to, ahead);
-        uint4 w = now.w;
+    auto step = [&](int t, Weights& now, bool first, bool last) {
+        stage(t + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        load_x(min(t + 2, steps - 1));
+        __builtin_amdgcn_sched_barrier(0);
+        const uint4 w = now.w;
         if constexpr (BS == 32) {
             // lane group h has block h; afterwards x and z hold block 0 of both groups, y and w block 1
             const auto lo = __builtin_amdgcn_permlane32_swap(w.x, w.y, false, false), hi = __builtin_amdgcn_permlane32_swap(w.z, w.w, false, false);
-            const uint32_t z0 = now.z & 15u, z1 = now.z >> 4;
+            const uint32_t z0 = zero_of(now.z, 0), z1 = zero_of(now.z, 1);
             product(t, lo[0], z0, g, true);
             product(t, hi[0], z0, 2 + g, false);
             add_up(scale_of(now.s[0]));
@@ -105,39 +121,34 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
             product(t, hi[1], z1, 6 + g, false);
             add_up(scale_of(now.s[kScales - 1]));
         } else {
-            const uint32_t zero = now.z >> ((min(t * 64 >> shift, p.m.kb - 1) & 1) * 4) & 15u;
+            const uint32_t zero = zero_of(now.z, min(t * 64 >> shift, last_block) & 1);
             product(t, w.x, zero, g * 4, first);
             product(t, w.y, zero, g * 4 + 1, false);
             product(t, w.z, zero, g * 4 + 2, false);
             product(t, w.w, zero, g * 4 + 3, false);
             if (last) add_up(scale_of(now.s[0]));
         }
-        stage(t + 1, ahead);
-        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+        load_w(min(t + kAhead, steps - 1), now);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
 
-    Weights one, two;
-    {
-        uint4 begin[TM];
-        load_w(0, one);
-        load_x(0, begin);
-        stage(0, begin);
-    }
+    Weights ring[kAhead];
+    load_x(0);
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) load_w(min(r, steps - 1), ring[r]);
+    stage(0);
+    load_x(min(1, steps - 1));
     __syncthreads();
-    for (int t = 0; t < steps; t += 2) {
-        const bool pair = t + 1 < steps;
-        if constexpr (BS == 128) {
-            if (pair) {
-                step(t, one, two, true, false);
-                step(t + 1, two, one, false, true);
-            } else {
-                step(t, one, two, true, true);
-            }
-        } else {
-            step(t, one, two, true, true);
-            if (pair) step(t + 1, two, one, true, true);
-        }
-    }
+    int t = 0;
+    for (; t + kAhead <= steps; t += kAhead)                             // (with branches between the steps the compiler waits for all loads there)
+#pragma unroll
+        for (int r = 0; r < kAhead; ++r) step(t + r, ring[r], BS != 128 || r % 2 == 0, BS != 128 || r % 2 == 1);
+#pragma unroll
+    for (int r = 0; r < kAhead - 1; ++r)
+        if (t + r < steps) step(t + r, ring[r], BS != 128 || r % 2 == 0, BS != 128 || r % 2 == 1 || t + r + 1 == steps);
 
     // a lane has column c and rows 8 (e / 4) + 4 g + e % 4 of each 32
     auto row_of = [&](int i, int e) { return i * 32 + (e >> 2) * 8 + g * 4 + (e & 3); };
