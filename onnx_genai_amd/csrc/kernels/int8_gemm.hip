@@ -109,6 +109,7 @@ struct Int8Params {
     int64_t m, n, lda, ldb;
     int steps;                 // of 128 k
     int steps_per_slice;
+    int columns;               // of a workgroup: few rows
     int b_scale_dtype, bias_dtype, y_dtype;
 };
 
@@ -118,7 +119,7 @@ __device__ __forceinline__ void store_scaled(const Int8Params& p, int64_t row, i
     store_from_f32(p.y, p.y_dtype, row * p.n + col, with_bias(v, p.bias, p.bias_dtype, row, p.n, col, p.y_dtype));
 }
 
-// Few rows: a workgroup has 16 CT columns, its waves split K; B's bytes bound it. v_mfma_i32_16x16x64_i8: lane l holds 16 bytes of k of row (or column) l % 16, k
+// Few rows: a workgroup has up to 16 CT columns, its waves split K; B's bytes bound it. v_mfma_i32_16x16x64_i8: lane l holds 16 bytes of k of row (or column) l % 16, k
 // from (l / 16) * 16. RT: tiles of 16 rows; lanes whose row is not there load no codes (a CU's vector memory path is 64 bytes a cycle, and 16 rows are as many
 // bytes as 16 columns). Two steps' loads are in flight.
 // FUSED (up to four rows of at most 32 KiB of codes): a is [m, k] of type T, and every workgroup makes the codes for itself, in LDS, while its first weights are on
@@ -132,8 +133,8 @@ __global__ __launch_bounds__(512) void int8_rows_kernel(const int8_t* b_base, co
     __shared__ uint32_t slots[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4, kp = steps * 128;
-    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (16 * CT);
-    const int cols = static_cast<int>(n - n0 < 16 * CT ? n - n0 : 16 * CT);
+    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * p.columns;
+    const int cols = static_cast<int>(n - n0 < p.columns ? n - n0 : p.columns);
     const auto srd_b = make_srd(b_base + n0 * p.ldb, static_cast<uint64_t>(cols * p.ldb));
     const auto srd_a = make_srd(a_base, FUSED ? 0 : static_cast<uint64_t>(m) * p.lda);
     const int begin = steps * wave >> 3, end = steps * (wave + 1) >> 3;                // (eight waves)
@@ -545,7 +546,9 @@ extern "C" int rocm_launch_pad_codes(const int8_t* from, int64_t rows, int64_t k
 namespace mnb {
 namespace {
 
-constexpr int64_t kFewRows = 64;              // rows up to which a call streams B
+// Rows up to which a call streams B, and up to which it does if B is small: 24 rows of 4096 -> 8192 take 10.7 us so and 15.3 in tiles with a sum over slices,
+// 24 rows of 18944 -> 3584 (65 MiB) 25 and 19, 60 rows of 4096 -> 14336 (56 MiB) 31 and 19.
+constexpr int64_t kFewRows = 16, kSomeRows = 32, kSmallBytes = 52 << 20;
 
 // What a call is launched as.
 struct Int8Plan {
@@ -555,7 +558,7 @@ struct Int8Plan {
 Int8Plan plan_of(const RocmInt8Args& a)
 {
     Int8Plan p{0, 1};
-    if (a.m <= kFewRows) return p;
+    if (a.m <= kFewRows || (a.m <= kSomeRows && a.n * ((a.k + 127) / 128 * 128) <= kSmallBytes)) return p;
     auto tiles = [&](int64_t t) { return (a.m + t - 1) / t * ((a.n + t - 1) / t); };
     const int64_t cus = rocm_ffi_compute_units(), steps = (a.k + 127) / 128;
     p.tile = tiles(256) >= cus * 3 / 4 ? 256 : 128;
@@ -596,23 +599,27 @@ extern "C" int rocm_launch_int8(const RocmInt8Args* args, rocm_stream_t stream)
     Int8Params p = params_of(args);
     const Int8Plan plan = plan_of(*args);
     if (plan.tile == 0) {
-        const unsigned wide = static_cast<unsigned>((p.n + 31) / 32), cus = static_cast<unsigned>(rocm_ffi_compute_units());
-        auto go = [&](auto kernel, unsigned grid, const void* a, size_t lds) {
+        // As many columns a workgroup, up to 48, as make the grid one, two ... times the CUs: tiles of whole 16s left 5 us of 24 to the few that came last
+        // (24 rows of 3584 -> 18944), and more workgroups read the rows more often (24 rows of 4096 -> 8192: 13.4 us with 16 columns each, 10.7 with 32).
+        const int64_t cus = rocm_ffi_compute_units(), most = 48;
+        int64_t times = (p.n + cus * most - 1) / (cus * most);
+        p.columns = static_cast<int>((p.n + cus * times - 1) / (cus * times));
+        if (p.columns < 16) p.columns = 16;
+        const unsigned grid = static_cast<unsigned>((p.n + p.columns - 1) / p.columns);
+        auto go = [&](auto kernel, const void* a, size_t lds) {
             hipLaunchKernelGGL(kernel, dim3(grid), dim3(512), lds, s, p.b, a, static_cast<int>(p.m), static_cast<int>(p.n), static_cast<int>(args->k), p.steps, p);
             return static_cast<int>(hipGetLastError());
         };
-        // two tiles of columns share a row's codes where the chip is covered all the same
-        const unsigned narrow = static_cast<unsigned>((p.n + 15) / 16);
-        auto columns = [&](auto one, auto two, const void* a, size_t lds) { return wide >= 2 * cus ? go(two, wide, a, lds) : go(one, narrow, a, lds); };
+        auto columns = [&](auto one, auto two, auto three, const void* a, size_t lds) { return p.columns <= 16 ? go(one, a, lds) : p.columns <= 32 ? go(two, a, lds) : go(three, a, lds); };
         if (args->a_float) {
             if (!fuses(*args)) return static_cast<int>(hipErrorInvalidValue);
             const size_t lds = static_cast<size_t>(p.m) * p.steps * 128;
-            if (args->a_dtype == ROCM_DT_BF16) return columns(int8_rows_kernel<1, 1, uint16_t, true, true>, int8_rows_kernel<1, 2, uint16_t, true, true>, args->a_float, lds);
-            return columns(int8_rows_kernel<1, 1, uint16_t, false, true>, int8_rows_kernel<1, 2, uint16_t, false, true>, args->a_float, lds);
+            if (args->a_dtype == ROCM_DT_BF16)
+                return columns(int8_rows_kernel<1, 1, uint16_t, true, true>, int8_rows_kernel<1, 2, uint16_t, true, true>, int8_rows_kernel<1, 3, uint16_t, true, true>, args->a_float, lds);
+            return columns(int8_rows_kernel<1, 1, uint16_t, false, true>, int8_rows_kernel<1, 2, uint16_t, false, true>, int8_rows_kernel<1, 3, uint16_t, false, true>, args->a_float, lds);
         }
-        if (p.m <= 16) return columns(int8_rows_kernel<1, 1, float, false, false>, int8_rows_kernel<1, 2, float, false, false>, p.a, 0);
-        if (p.m <= 32) return columns(int8_rows_kernel<2, 1, float, false, false>, int8_rows_kernel<2, 2, float, false, false>, p.a, 0);
-        return go(int8_rows_kernel<4, 1, float, false, false>, narrow, p.a, 0);
+        if (p.m <= 16) return columns(int8_rows_kernel<1, 1, float, false, false>, int8_rows_kernel<1, 2, float, false, false>, int8_rows_kernel<1, 3, float, false, false>, p.a, 0);
+        return columns(int8_rows_kernel<2, 1, float, false, false>, int8_rows_kernel<2, 2, float, false, false>, int8_rows_kernel<2, 3, float, false, false>, p.a, 0);
     }
     p.steps_per_slice = (p.steps + plan.slices - 1) / plan.slices;
     p.partial = plan.slices > 1 ? args->partial : nullptr;
