@@ -18,8 +18,6 @@ template <bool BF16, int BS, typename ST, bool UP, int TM>
 __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileCall p)
 {
     constexpr int kPitch = 9;                                            // pieces of 16 bytes from a row of 64 elements in LDS to the next
-    constexpr int kScales = BS == 32 ? 2 : 1;                            // blocks of a step
-    constexpr int kAhead = 2;                                            // steps whose weights are in registers or on their way
     __shared__ uint4 staged[2][TM * 32 * kPitch];
     const unsigned index = blockIdx.z * gridDim.y + blockIdx.y;
     if (index >= p.count) return;
@@ -41,18 +39,20 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
         const int64_t row = tile.y + min(static_cast<int>(threadIdx.x >> 3) + i * 32, tile.z - 1);                // (nor are rows)
         x[i] = p.x + (p.token ? p.token[row] : row) * p.ldx + piece * 8;
     }
-    struct Weights {
-        uint4 w;
-        ST s[kScales];
+    auto load_w = [&](int t, uint4& to) {
+        const int byte = t * 32 + g * 16;
+        to = *reinterpret_cast<const uint4*>(b + (byte < row_bytes ? byte : 0));                                  // (behind a row's end its activations are zero)
+    };
+    // Scales of two blocks at once, one in each lane group, and their zero points: 32 columns' scales take a CU's path to memory as long as their weights of a step,
+    // however few bytes they are. (Two steps are one block of 128.)
+    struct Scales {
+        ST s;
         uint16_t z;
     };
-    auto load_w = [&](int t, Weights& to) {
-        const int byte = t * 32 + g * 16;
-        to.w = *reinterpret_cast<const uint4*>(b + (byte < row_bytes ? byte : 0));                                // (behind a row's end its activations are zero)
-        const int block = min(t * 64 >> shift, last_block);
-#pragma unroll
-        for (int i = 0; i < kScales; ++i) to.s[i] = s[min(block + i, last_block)];
-        to.z = z[block >> 1];
+    auto load_s = [&](int t, Scales& to) {
+        const int block = t * 64 >> shift;
+        to.s = s[min(block + (BS == 128 ? 0 : g), last_block)];
+        to.z = z[min(block, last_block) >> 1];
     };
     uint4 ahead[TM];
     auto load_x = [&](int t) {
@@ -75,20 +75,24 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
     float16_t total[TM] = {}, sum[TM] = {};
     const float16_t none = {};
     // (The instructions that first touch what was loaded are pinned: the compiler would widen it, and wait for it, a step before.)
-    auto scale_of = [&](ST raw) {
-        if constexpr (sizeof(ST) == 4) {
-            return static_cast<float>(raw);
-        } else {
-            float v;
-            if constexpr (BF16) asm volatile("v_lshlrev_b32 %0, 16, %1" : "=v"(v) : "v"(raw));
-            else asm volatile("v_cvt_f32_f16 %0, %1" : "=v"(v) : "v"(raw));
-            return v;
-        }
-    };
-    auto zero_of = [&](uint16_t two, int which) {
+    float scale[2];
+    uint32_t zero[2];
+    auto take = [&](int t, const Scales& from) {
         uint32_t v;
-        asm volatile("v_bfe_u32 %0, %1, %2, 4" : "=v"(v) : "v"(two), "s"(which * 4));
-        return v;
+        if constexpr (sizeof(ST) == 4) v = __float_as_uint(from.s);
+        else if constexpr (BF16) asm volatile("v_lshlrev_b32 %0, 16, %1" : "=v"(v) : "v"(from.s));
+        else asm volatile("v_cvt_f32_f16 %0, %1" : "=v"(v) : "v"(from.s));
+        if constexpr (BS == 128) {
+            scale[0] = scale[1] = __uint_as_float(v);
+            asm volatile("v_bfe_u32 %0, %1, %2, 4" : "=v"(zero[0]) : "v"(from.z), "s"((min(t * 64 >> shift, last_block) & 1) * 4));
+            zero[1] = zero[0];
+        } else {
+            const auto both = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+            scale[0] = __uint_as_float(both[0]);
+            scale[1] = __uint_as_float(both[1]);
+            asm volatile("v_bfe_u32 %0, %1, 0, 4" : "=v"(zero[0]) : "v"(from.z));
+            asm volatile("v_bfe_u32 %0, %1, 4, 4" : "=v"(zero[1]) : "v"(from.z));
+        }
     };
     auto add_up = [&](float scale) {
 #pragma unroll
@@ -102,53 +106,63 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
 #pragma unroll
         for (int i = 0; i < TM; ++i) sum[i] = mfma32<BF16>(staged[t & 1][(i * 32 + c) * kPitch + at_piece], w, first ? none : sum[i]);
     };
-    // A step stages the next one's activations, asks for those of the one behind it, multiplies, and asks for the weights kAhead steps on, where its own were.
-    // FIRST, LAST: the step begins, ends a block (of 64 or more)
-    auto step = [&](int t, Weights& now, bool first, bool last) {
+    // A step stages the next one's activations, asks for those of the one behind it, multiplies, and asks for the weights two steps on, where its own were.
+    // FIRST, LAST: the step begins, ends a block (of 64 or more), the one of scale[which]
+    auto step = [&](int t, uint4& now, int which, bool first, bool last) {
         stage(t + 1);
         __builtin_amdgcn_sched_barrier(0);
         load_x(min(t + 2, steps - 1));
         __builtin_amdgcn_sched_barrier(0);
-        const uint4 w = now.w;
+        const uint4 w = now;
         if constexpr (BS == 32) {
             // lane group h has block h; afterwards x and z hold block 0 of both groups, y and w block 1
             const auto lo = __builtin_amdgcn_permlane32_swap(w.x, w.y, false, false), hi = __builtin_amdgcn_permlane32_swap(w.z, w.w, false, false);
-            const uint32_t z0 = zero_of(now.z, 0), z1 = zero_of(now.z, 1);
-            product(t, lo[0], z0, g, true);
-            product(t, hi[0], z0, 2 + g, false);
-            add_up(scale_of(now.s[0]));
-            product(t, lo[1], z1, 4 + g, true);
-            product(t, hi[1], z1, 6 + g, false);
-            add_up(scale_of(now.s[kScales - 1]));
+            product(t, lo[0], zero[0], g, true);
+            product(t, hi[0], zero[0], 2 + g, false);
+            add_up(scale[0]);
+            product(t, lo[1], zero[1], 4 + g, true);
+            product(t, hi[1], zero[1], 6 + g, false);
+            add_up(scale[1]);
         } else {
-            const uint32_t zero = zero_of(now.z, min(t * 64 >> shift, last_block) & 1);
-            product(t, w.x, zero, g * 4, first);
-            product(t, w.y, zero, g * 4 + 1, false);
-            product(t, w.z, zero, g * 4 + 2, false);
-            product(t, w.w, zero, g * 4 + 3, false);
-            if (last) add_up(scale_of(now.s[0]));
+            product(t, w.x, zero[which], g * 4, first);
+            product(t, w.y, zero[which], g * 4 + 1, false);
+            product(t, w.z, zero[which], g * 4 + 2, false);
+            product(t, w.w, zero[which], g * 4 + 3, false);
+            if (last) add_up(scale[which]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        load_w(min(t + kAhead, steps - 1), now);
+        load_w(min(t + 2, steps - 1), now);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);                               // (nothing that waits for loads comes before)
     };
 
-    Weights ring[kAhead];
+    uint4 one, two;
+    Scales sa, sb;                                                       // (blocks of 32: of a step each; else sa of both)
     load_x(0);
-#pragma unroll
-    for (int r = 0; r < kAhead; ++r) load_w(min(r, steps - 1), ring[r]);
+    load_s(0, sa);
+    load_w(0, one);
+    if (BS == 32) load_s(1, sb);
+    load_w(min(1, steps - 1), two);
     stage(0);
     load_x(min(1, steps - 1));
     __syncthreads();
     int t = 0;
-    for (; t + kAhead <= steps; t += kAhead)                             // (with branches between the steps the compiler waits for all loads there)
-#pragma unroll
-        for (int r = 0; r < kAhead; ++r) step(t + r, ring[r], BS != 128 || r % 2 == 0, BS != 128 || r % 2 == 1);
-#pragma unroll
-    for (int r = 0; r < kAhead - 1; ++r)
-        if (t + r < steps) step(t + r, ring[r], BS != 128 || r % 2 == 0, BS != 128 || r % 2 == 1 || t + r + 1 == steps);
+    for (; t + 2 <= steps; t += 2) {                                     // (with a branch between the two the compiler waits for all loads there)
+        take(t, sa);
+        load_s(t + 2, sa);
+        step(t, one, 0, true, BS != 128);
+        if constexpr (BS == 32) {
+            take(t + 1, sb);
+            load_s(t + 3, sb);
+        }
+        step(t + 1, two, 1, BS != 128, true);
+    }
+    if (t < steps) {
+        take(t, sa);
+        step(t, one, 0, true, true);
+    }
 
     // a lane has column c and rows 8 (e / 4) + 4 g + e % 4 of each 32
     auto row_of = [&](int i, int e) { return i * 32 + (e >> 2) * 8 + g * 4 + (e & 3); };
