@@ -17,7 +17,7 @@ struct MoePlan {
     int tile_rows;
     bool tall;                 // tiles of 128 pairs, weights rounded to f16
     int64_t kp, ip, pairs, eight_bytes;
-    uint64_t table, eights, expert, weight, pair_row, token, base, tiles, x, h, out, total;
+    uint64_t table, eights, expert, weight, pair_row, token, base, tiles, counts, x, h, out, total;
 };
 
 MoePlan plan_of(const RocmMoeArgs& a)
@@ -47,6 +47,7 @@ MoePlan plan_of(const RocmMoeArgs& a)
     l.token = part(tiled ? l.pairs * 4 : 0);
     l.base = part(tiled ? a.rows * 4 : 0);
     l.tiles = part(tiled ? static_cast<uint64_t>(l.slots) * 16 : 0);
+    l.counts = part(tiled && a.rows > 64 ? kMoeGroups * static_cast<uint64_t>(a.experts) * 4 : 0);
     // rows that do not begin at multiples of 16 bytes are copied: the address may be any
     l.x = part(a.rows * l.kp * 2);
     l.eight_bytes = tiled && (!a.gate.zp || !a.down.zp) ? ((l.kp > l.ip ? l.kp : l.ip) + 63) / 64 + 1 : 0;
@@ -93,14 +94,11 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     const MoePlan l = plan_of(a);
     uint8_t* const ws = static_cast<uint8_t*>(workspace);
     auto at = [&](uint64_t offset) { return reinterpret_cast<int32_t*>(ws + offset); };
-    const MoeRoute route{at(l.expert), reinterpret_cast<float*>(ws + l.weight), at(l.pair_row), at(l.token), reinterpret_cast<float*>(ws + l.base), reinterpret_cast<int4*>(ws + l.tiles)};
+    const MoeRoute route{at(l.expert), reinterpret_cast<float*>(ws + l.weight), at(l.pair_row), at(l.token), reinterpret_cast<float*>(ws + l.base), reinterpret_cast<int4*>(ws + l.tiles), at(l.counts)};
     MoeFewTable* const table = reinterpret_cast<MoeFewTable*>(ws + l.table);
     int rc = 0;
     if (l.where == kMoeTable) rc = launch_moe_route_few(a, table, s);
-    if (l.where == kMoeTiles) {
-        rc = launch_moe_top_k(a, route, s);
-        if (rc == 0) rc = launch_moe_plan(a, l.tile_rows, l.slots, route, ws + l.eights, static_cast<int>(l.eight_bytes), s);
-    }
+    if (l.where == kMoeTiles) rc = launch_moe_plan(a, l.tile_rows, l.slots, route, ws + l.eights, static_cast<int>(l.eight_bytes), s);
     const void* x = a.x;
     if (rc == 0 && (l.kp != a.hidden || reinterpret_cast<uintptr_t>(a.x) % 16 != 0)) {
         rc = launch_moe_pad_rows(a.x, a.rows, a.hidden, l.kp, ws + l.x, s);

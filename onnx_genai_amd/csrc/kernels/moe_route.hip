@@ -10,18 +10,87 @@
 namespace mnb {
 namespace {
 
-template <int NL>
-__global__ __launch_bounds__(256) void moe_top_k_kernel(const void* logits, int dtype, int64_t rows, int experts, int k, int normalize, MoeRoute r)
+// What the sum over the threads before a thread is, for two values at once: rows and tiles of the experts before its own.
+__device__ __forceinline__ int2 sums_before(int a, int b, int2* of_wave, int2& all)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t token = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (token >= rows) return;
-    const MoeChoice c = choose_experts<NL>(logits, dtype, token, experts, k, normalize);
-    if (lane < k) {
-        r.expert[token * k + lane] = c.expert;
-        r.weight[token * k + lane] = c.weight;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int2 v = make_int2(a, b);
+    for (int d = 1; d < 64; d *= 2) {
+        const int x = __shfl_up(v.x, d), y = __shfl_up(v.y, d);
+        if (lane >= d) v = make_int2(v.x + x, v.y + y);
     }
-    if (lane == 0) r.base[token] = c.base;
+    if (lane == 63) of_wave[wave] = v;
+    __syncthreads();
+    int2 before = make_int2(0, 0);
+    all = before;
+    for (int w = 0; w < 16; ++w) {
+        const int2 x = of_wave[w];
+        if (w < wave) before = make_int2(before.x + x.x, before.y + x.y);
+        all = make_int2(all.x + x.x, all.y + x.y);
+    }
+    return make_int2(before.x + v.x - a, before.y + v.y - b);
+}
+
+struct MoePlanCall {
+    int tile_rows, max_tiles;
+    uint8_t* eights;
+    int eight_bytes;
+};
+
+// By 1024 threads, a thread an expert: `own` pairs in all, `before` of them in the workgroups before. The experts' rows and tiles; row0[e]: where this workgroup's
+// pairs of e begin.
+__device__ __forceinline__ void cut_tiles(int own, int before, int* row0, bool write, const MoePlanCall& c, const MoeRoute& r)
+{
+    __shared__ int2 of_wave[16];
+    const int t = threadIdx.x, tiles = (own + c.tile_rows - 1) / c.tile_rows;
+    int2 all;
+    const int2 to = sums_before(own, tiles, of_wave, all);
+    row0[t] = to.x + before;
+    if (write) {
+        for (int i = 0; i < tiles; ++i) r.tiles[to.y + i] = make_int4(t, to.x + i * c.tile_rows, min(c.tile_rows, own - i * c.tile_rows), 0);
+        for (int i = all.y + t; i < c.max_tiles; i += 1024) r.tiles[i] = make_int4(0, 0, 0, 0);
+        for (int i = t; i < c.eight_bytes; i += 1024) c.eights[i] = 0x88;
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ void place_pairs(int first, int end, int k, const int* row0, const MoeRoute& r)
+{
+    for (int p = first + static_cast<int>(threadIdx.x); p < end; p += 1024) {
+        const int e = r.expert[p], row = e >= 0 ? row0[e] + r.pair_row[p] : -1;
+        if (row >= 0) r.token[row] = p / k;
+        r.pair_row[p] = row;
+    }
+}
+
+// A workgroup chooses for `share` tokens and counts their experts; a pair's place among its workgroup's of that expert goes where its row will stand. The only
+// workgroup of a short call cuts the tiles at once.
+template <int NL>
+__global__ __launch_bounds__(1024) void moe_top_k_kernel(const void* logits, int dtype, int rows, int experts, int k, int normalize, int share, MoePlanCall c, MoeRoute r)
+{
+    __shared__ int count[1024];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    count[threadIdx.x] = 0;
+    __syncthreads();
+    const int first = blockIdx.x * share, end = min(first + share, rows);
+    for (int token = first + wave; token < end; token += 16) {
+        const MoeChoice choice = choose_experts<NL>(logits, dtype, token, experts, k, normalize);
+        if (lane < k) {
+            r.expert[token * k + lane] = choice.expert;
+            r.weight[token * k + lane] = choice.weight;
+            if (choice.expert >= 0) r.pair_row[token * k + lane] = atomicAdd(&count[choice.expert], 1);
+        }
+        if (lane == 0) r.base[token] = choice.base;
+    }
+    __syncthreads();
+    const int own = count[threadIdx.x];
+    if (gridDim.x > 1) {
+        if (static_cast<int>(threadIdx.x) < experts) r.counts[blockIdx.x * experts + threadIdx.x] = own;
+        return;
+    }
+    __syncthreads();
+    cut_tiles(own, 0, count, true, c, r);
+    place_pairs(0, rows * k, k, count, r);
 }
 
 __global__ __launch_bounds__(1024) void moe_route_few_kernel(const void* logits, int dtype, int rows, int experts, int k, int normalize, MoeFewTable* table)
@@ -31,58 +100,21 @@ __global__ __launch_bounds__(1024) void moe_route_few_kernel(const void* logits,
     write_table(routing, rows, k, table);
 }
 
-// One workgroup sorts the pairs and cuts the tiles.
-__global__ __launch_bounds__(1024) void moe_plan_kernel(int pairs, int k, int tile_rows, int max_tiles, MoeRoute r, uint8_t* eights, int eight_bytes)
+// The rows of the pairs of workgroup blockIdx.x of the launch before. (One workgroup for all, counting again, took 50 us for 32768 pairs.)
+__global__ __launch_bounds__(1024) void moe_plan_kernel(int rows, int experts, int k, int share, MoePlanCall c, MoeRoute r)
 {
-    __shared__ int count[1024], rows_to[1024], tiles_to[1024];
-    const int t = threadIdx.x;
-    for (int i = t; i < eight_bytes; i += 1024) eights[i] = 0x88;
-    count[t] = 0;
-    __syncthreads();
-    // (kBatch pairs a thread at once: one at a time the trips to memory alone are 1.5 us for each 1024 pairs)
-    constexpr int kBatch = 8;
-    for (int p = t; p < pairs; p += kBatch * 1024) {
-        int e[kBatch], place[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) e[i] = r.expert[min(p + i * 1024, pairs - 1)];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) place[i] = p + i * 1024 < pairs && e[i] >= 0 ? atomicAdd(&count[e[i]], 1) : 0;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-            if (p + i * 1024 < pairs) r.pair_row[p + i * 1024] = place[i];
-    }
-    __syncthreads();
-    const int own = count[t], own_tiles = (own + tile_rows - 1) / tile_rows;
-    rows_to[t] = own;
-    tiles_to[t] = own_tiles;
-    __syncthreads();
-    for (int d = 1; d < 1024; d *= 2) {
-        const int a = t >= d ? rows_to[t - d] : 0, b = t >= d ? tiles_to[t - d] : 0;
-        __syncthreads();
-        rows_to[t] += a;
-        tiles_to[t] += b;
-        __syncthreads();
-    }
-    const int row0 = rows_to[t] - own, tile0 = tiles_to[t] - own_tiles;
-    for (int i = 0; i < own_tiles; ++i) r.tiles[tile0 + i] = make_int4(t, row0 + i * tile_rows, min(tile_rows, own - i * tile_rows), 0);
-    for (int i = tiles_to[1023] + t; i < max_tiles; i += 1024) r.tiles[i] = make_int4(0, 0, 0, 0);
-    for (int p = t; p < pairs; p += kBatch * 1024) {
-        int e[kBatch], place[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int at = min(p + i * 1024, pairs - 1);
-            e[i] = r.expert[at];
-            place[i] = r.pair_row[at];
+    __shared__ int row0[1024];
+    const int t = threadIdx.x, groups = static_cast<int>(gridDim.x), group = static_cast<int>(blockIdx.x);
+    int own = 0, before = 0;
+    if (t < experts)
+#pragma unroll 16
+        for (int i = 0; i < groups; ++i) {
+            const int n = r.counts[i * experts + t];
+            own += n;
+            before += i < group ? n : 0;
         }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int at = p + i * 1024;
-            if (at >= pairs) break;
-            const int row = e[i] >= 0 ? rows_to[e[i]] - count[e[i]] + place[i] : -1;
-            if (row >= 0) r.token[row] = at / k;
-            r.pair_row[at] = row;
-        }
-    }
+    cut_tiles(own, before, row0, group == 0, c, r);
+    place_pairs(group * share * k, min((group + 1) * share, rows) * k, k, row0, r);
 }
 
 // y = base + sum over a token's experts, in the order of their logits, of weight * (out + bias).
@@ -131,25 +163,24 @@ __global__ __launch_bounds__(256) void moe_pad_rows_kernel(const uint16_t* __res
 
 }  // namespace
 
-int launch_moe_top_k(const RocmMoeArgs& a, const MoeRoute& r, hipStream_t s)
+int launch_moe_plan(const RocmMoeArgs& a, int tile_rows, int max_tiles, const MoeRoute& r, uint8_t* eights, int eight_bytes, hipStream_t s)
 {
-    const dim3 grid(static_cast<unsigned>((a.rows + 3) / 4));
+    // up to kMoeGroups workgroups of 32 tokens or more (a wave's tokens follow one another, 1.5 us each), but one for up to 64, which saves a launch
+    const int rows = static_cast<int>(a.rows), share = rows <= 64 ? 64 : rows <= 32 * kMoeGroups ? 32 : (rows + kMoeGroups - 1) / kMoeGroups, groups = (rows + share - 1) / share;
+    const MoePlanCall c{tile_rows, max_tiles, eights, eight_bytes};
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a.logits, a.logits_dtype, a.rows, a.experts, a.k, a.normalize, r);
+        hipLaunchKernelGGL(kernel, dim3(groups), dim3(1024), 0, s, a.logits, a.logits_dtype, rows, a.experts, a.k, a.normalize, share, c, r);
         return static_cast<int>(hipGetLastError());
     };
-    return a.experts <= 64 ? go(moe_top_k_kernel<1>) : a.experts <= 128 ? go(moe_top_k_kernel<2>) : a.experts <= 256 ? go(moe_top_k_kernel<4>) : go(moe_top_k_kernel<16>);
+    const int rc = a.experts <= 64 ? go(moe_top_k_kernel<1>) : a.experts <= 128 ? go(moe_top_k_kernel<2>) : a.experts <= 256 ? go(moe_top_k_kernel<4>) : go(moe_top_k_kernel<16>);
+    if (rc != 0 || groups == 1) return rc;
+    hipLaunchKernelGGL(moe_plan_kernel, dim3(groups), dim3(1024), 0, s, rows, a.experts, a.k, share, c, r);
+    return static_cast<int>(hipGetLastError());
 }
 
 int launch_moe_route_few(const RocmMoeArgs& a, MoeFewTable* table, hipStream_t s)
 {
     hipLaunchKernelGGL(moe_route_few_kernel, dim3(1), dim3(1024), 0, s, a.logits, a.logits_dtype, static_cast<int>(a.rows), a.experts, a.k, a.normalize, table);
-    return static_cast<int>(hipGetLastError());
-}
-
-int launch_moe_plan(const RocmMoeArgs& a, int tile_rows, int max_tiles, const MoeRoute& r, uint8_t* eights, int eight_bytes, hipStream_t s)
-{
-    hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, s, static_cast<int>(a.rows * a.k), a.k, tile_rows, max_tiles, r, eights, eight_bytes);
     return static_cast<int>(hipGetLastError());
 }
 
