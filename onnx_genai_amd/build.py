@@ -38,9 +38,8 @@ HIP_SOURCES = [
     "kernels/int8_gemm.hip",
     "kernels/moe_route.hip",
     "kernels/moe_few.hip",
-    "kernels/moe_gate_up.hip",
-    "kernels/moe_down.hip",
-    "kernels/moe_tile.hip", "kernels/moe_tall.hip",
+    "kernels/moe_tile.hip",
+    "kernels/moe_tall.hip",
     "kernels/moe.hip",
 ]
 HOST_SOURCES = ["ep/provider.cpp", "ep/matmul_nbits.cpp", "ep/nodes.cpp", "ep/nxrt_plugin.cpp", "ep/nxmem_plugin.cpp", "ep/ort_plugin.cpp"]

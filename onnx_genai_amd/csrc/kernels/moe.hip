@@ -1,22 +1,24 @@
 // QMoE: which launches a call is.
 //
 //   up to 4 tokens      gate/up (every workgroup routes for itself), down with the sum over experts
-//   up to 16 tokens     routing, gate/up, down with the sum over experts
-//   more                top-k, sorting by expert, gate/up, down, sum over each token's experts
+//   more                top-k and sorting by expert (one launch up to 64 tokens, then two), gate/up, down, sum over each token's experts
 #include "moe.hiph"
 
 namespace mnb {
 namespace {
 
-// Pairs an expert from which tiles have 128 rows.
-constexpr int64_t kTallPairs = 48;
+// Pairs an expert from which tiles have 128 rows. With weights scaled in f16, 16 experts of 2880: 38 pairs 155 us so and 201 in tiles of 32 rows, 25 pairs 153 and 129
+// (8 experts of 4096 and 14336: 32 pairs 577 and 585, 16 pairs 574 and 427). With exact weights, 64 experts of 2048 and 1024: 96 pairs 165 and 216, 64 pairs
+// 148 and 151, 48 pairs 146 and 130.
+constexpr int64_t kTallPairs = 32, kTallExactPairs = 64;
 
 struct MoePlan {
-    int where;                 // kMoeFused, kMoeTable, kMoeTiles
+    bool tiled;                // or few tokens
     int slots;                 // experts that can be active, or tiles
     int tile_rows;
     bool tall;                 // tiles of 128 pairs, weights rounded to f16
     int64_t kp, ip, pairs, eight_bytes;
+    int slices, steps_per_slice;         // of down's K
     uint64_t table, eights, expert, weight, pair_row, token, base, tiles, counts, x, h, out, total;
 };
 
@@ -25,21 +27,33 @@ MoePlan plan_of(const RocmMoeArgs& a)
     MoePlan l{};
     l.pairs = a.rows * a.k;
     // (the rows of x lie in the 48 KiB of LDS that a kernel gets without asking beside its tables)
-    l.where = a.rows <= 4 && a.experts <= 256 && l.pairs <= kFewPairs && a.rows * ((a.hidden + 2047) / 2048) <= 12 ? kMoeFused : a.rows <= kFewTokens && l.pairs <= kFewPairs ? kMoeTable : kMoeTiles;
-    l.tile_rows = l.pairs >= kTallPairs * a.experts ? 128 : 32;
-    l.slots = static_cast<int>((l.where == kMoeTiles ? l.pairs / l.tile_rows : 0) + (l.pairs < a.experts ? l.pairs : a.experts));
+    l.tiled = !(a.rows <= kFewTokens && a.experts <= 256 && l.pairs <= kFewPairs && a.rows * ((a.hidden + 2047) / 2048) <= 12);
     // Weights are scaled in f16 where activations and scales are f16: rounding them to bf16 would double y's error, and f32 scales may lie outside of f16's range.
     // (Those tiles address an expert's weights and the rows in 32 bits.)
     const int64_t most = 1ll << 31, columns = a.hidden > 2 * a.inter ? a.hidden : 2 * a.inter, deepest = (a.hidden > a.inter ? a.hidden : a.inter) + 128;
-    l.tall = l.where == kMoeTiles && l.tile_rows == 128 && a.dtype == ROCM_DT_F16 && a.scale_dtype == ROCM_DT_F16 && columns * deepest / 2 < most && a.rows * (a.hidden + 64) * 2 < most;
-    l.kp = l.where == kMoeTiles ? (a.hidden + 63) / 64 * 64 : (a.hidden + 7) / 8 * 8;        // (tiles read whole steps of 64)
+    const bool in_f16 = l.tiled && a.dtype == ROCM_DT_F16 && a.scale_dtype == ROCM_DT_F16 && columns * deepest / 2 < most && a.rows * (a.hidden + 64) * 2 < most;
+    l.tall = in_f16 && l.pairs >= kTallPairs * a.experts;
+    l.tile_rows = l.tall || (!in_f16 && l.pairs >= kTallExactPairs * a.experts) ? 128 : 32;
+    l.slots = static_cast<int>((l.tiled ? l.pairs / l.tile_rows : 0) + (l.pairs < a.experts ? l.pairs : a.experts));
+    l.kp = l.tiled ? (a.hidden + 63) / 64 * 64 : (a.hidden + 7) / 8 * 8;        // (tiles read whole steps of 64)
     l.ip = (a.inter + 127) / 128 * 128;      // (steps of 64 and 128)
+    // Down in slices of its K, of 16 steps or more, until four workgroups for each CU are there: one after the other its steps are trips to memory.
+    l.slices = 1;
+    const int steps = static_cast<int>(l.ip / 64);
+    if (l.tiled && !l.tall) {
+        const int64_t grid = (a.hidden + 127) / 128 * l.slots, wanted = 4 * rocm_ffi_compute_units() / grid;
+        const int64_t most = steps / 16 < 8 ? steps / 16 : 8;
+        l.slices = static_cast<int>(wanted < most ? wanted : most);
+        if (l.slices < 1) l.slices = 1;
+    }
+    l.steps_per_slice = ((steps + l.slices - 1) / l.slices + 1) / 2 * 2;
+    l.slices = (steps + l.steps_per_slice - 1) / l.steps_per_slice;
     auto part = [&](uint64_t bytes) {
         const uint64_t here = l.total;
         l.total += (bytes + 255) / 256 * 256;
         return here;
     };
-    const bool tiled = l.where == kMoeTiles;
+    const bool tiled = l.tiled;
     l.table = part(tiled ? 0 : sizeof(MoeFewTable));
     l.expert = part(tiled ? l.pairs * 4 : 0);
     l.weight = part(tiled ? l.pairs * 4 : 0);
@@ -53,8 +67,8 @@ MoePlan plan_of(const RocmMoeArgs& a)
     l.eight_bytes = tiled && (!a.gate.zp || !a.down.zp) ? ((l.kp > l.ip ? l.kp : l.ip) + 63) / 64 + 1 : 0;
     l.eights = part(l.eight_bytes);
     // (few tokens: two parts of every value of h)
-    l.h = part(tiled ? l.pairs * l.ip * 2 : l.slots * (l.where == kMoeFused ? 4 : 16) * l.ip * 4);
-    l.out = part(tiled ? l.pairs * a.hidden * 4 : 0);
+    l.h = part(tiled ? l.pairs * l.ip * 2 : l.slots * kFewTokens * l.ip * 4);
+    l.out = part(tiled ? l.slices * l.pairs * a.hidden * 4 : 0);
     return l;
 }
 
@@ -82,7 +96,7 @@ extern "C" uint64_t rocm_moe_workspace_bytes(const RocmMoeArgs* args) { return m
 extern "C" const char* rocm_moe_variant(const RocmMoeArgs* args)
 {
     const mnb::MoePlan l = mnb::plan_of(*args);
-    return l.where == mnb::kMoeFused ? "moe_few" : l.where == mnb::kMoeTable ? "moe_table" : l.tall ? "moe_tall_tiles" : l.tile_rows == 128 ? "moe_tiles_128" : "moe_tiles_32";
+    return !l.tiled ? "moe_few" : l.tall ? "moe_tall_tiles" : l.tile_rows == 128 ? "moe_tiles_128" : "moe_tiles_32";
 }
 
 extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_stream_t stream)
@@ -97,8 +111,7 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     const MoeRoute route{at(l.expert), reinterpret_cast<float*>(ws + l.weight), at(l.pair_row), at(l.token), reinterpret_cast<float*>(ws + l.base), reinterpret_cast<int4*>(ws + l.tiles), at(l.counts)};
     MoeFewTable* const table = reinterpret_cast<MoeFewTable*>(ws + l.table);
     int rc = 0;
-    if (l.where == kMoeTable) rc = launch_moe_route_few(a, table, s);
-    if (l.where == kMoeTiles) rc = launch_moe_plan(a, l.tile_rows, l.slots, route, ws + l.eights, static_cast<int>(l.eight_bytes), s);
+    if (l.tiled) rc = launch_moe_plan(a, l.tile_rows, l.slots, route, ws + l.eights, static_cast<int>(l.eight_bytes), s);
     const void* x = a.x;
     if (rc == 0 && (l.kp != a.hidden || reinterpret_cast<uintptr_t>(a.x) % 16 != 0)) {
         rc = launch_moe_pad_rows(a.x, a.rows, a.hidden, l.kp, ws + l.x, s);
@@ -129,11 +142,7 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     down.rows = up.rows;
     down.y = a.y;
     down.out = reinterpret_cast<float*>(ws + l.out);
-    if (l.where == kMoeFused) return launch_moe_few(a, up, down, l.slots, s);
-    if (l.where == kMoeTable) {
-        rc = launch_moe_gate_up(a, up, l.slots, s);
-        return rc != 0 ? rc : launch_moe_down(a, down, s);
-    }
+    if (!l.tiled) return launch_moe_few(a, up, down, l.slots, s);
     auto tiled = [&](const MoeMatrix& m, const uint16_t* rows, int64_t ldx) {
         MoeTileCall t{};
         t.m = m;
@@ -148,6 +157,9 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
         t.h = up.h;
         t.ldh = l.ip;
         t.out = down.out;
+        t.slices = l.slices;
+        t.steps_per_slice = l.steps_per_slice;
+        t.slice_elements = l.pairs * a.hidden;
         t.alpha = a.alpha;
         t.beta = a.beta;
         t.limit = a.limit;
@@ -158,5 +170,5 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     auto half = [&](const MoeTileCall& t, bool is_up) { return l.tall ? launch_moe_tall(t, is_up, s) : launch_moe_tile(a, t, is_up, l.tile_rows, s); };
     rc = half(first, true);
     if (rc == 0) rc = half(second, false);
-    return rc != 0 ? rc : launch_moe_combine(a, route, down.out, s);
+    return rc != 0 ? rc : launch_moe_combine(a, route, down.out, l.slices, s);
 }

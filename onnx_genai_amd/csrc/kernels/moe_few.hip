@@ -6,13 +6,34 @@
 // The weights' bytes bound it once there are enough of them, and before that the way to them: arguments, logits and weights are reached one after the other.
 // A lane holds 32 elements of K of a row of x in registers, in 16 dot products of two with 32 nibbles of each of several columns (v_dot2_f32_f16, v_dot2_f32_bf16:
 // 46 instructions for 16 bytes of weights and one row; the matrix core wants the nibbles turned between lanes and takes 71 with its corrections, for up to 16 rows).
-// A nibble q is the 16-bit float magic + q (moe_dot.hiph), and the products' sum starts from -(magic + zp) times the lane's sum of x.
+// A nibble q is the 16-bit float magic + q (magic = 1024 in f16, 128 in bf16; exact), and the products' sum starts from -(magic + zp) times the lane's sum of x.
 // LPC lanes stand side by side on K and read 16 LPC bytes of a column's row as the caller holds it; 64 / LPC columns are read at once.
-#include "moe_dot.hiph"
 #include "moe_route.hiph"
 
 namespace mnb {
 namespace {
+
+// What a step reads of its tile of columns: wave-uniform.
+template <int NM>
+struct MoeTile {
+    __amdgpu_buffer_rsrc_t w[NM], s[NM], z[NM];
+};
+
+// Columns [n0, n0 + live) of an expert; with none, every load reads as zeros and goes to no memory.
+template <typename ST, bool ZP, int NM>
+__device__ __forceinline__ MoeTile<NM> moe_tile(const MoeMatrix& m, int expert, int n0, int live)
+{
+    MoeTile<NM> t;
+    const int64_t row = expert * m.expert_step + static_cast<int64_t>(n0) * m.row_step;
+    const uint64_t rows = live > 0 ? static_cast<uint64_t>(live - 1) * m.row_step + 1 : 0;
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+        t.w[i] = make_srd(m.w[i].b + row * m.row_bytes, rows * m.row_bytes);
+        t.s[i] = make_srd(static_cast<const ST*>(m.w[i].scales) + row * m.kb, rows * m.kb * sizeof(ST));
+        t.z[i] = ZP ? make_srd(m.w[i].zp + row * m.zp_row, rows * m.zp_row) : t.w[i];
+    }
+    return t;
+}
 
 typedef __attribute__((ext_vector_type(2))) _Float16 moe_half2_t;
 typedef __attribute__((ext_vector_type(2))) __bf16 moe_bf16x2_t;

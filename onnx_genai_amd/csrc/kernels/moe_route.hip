@@ -93,13 +93,6 @@ __global__ __launch_bounds__(1024) void moe_top_k_kernel(const void* logits, int
     place_pairs(0, rows * k, k, count, r);
 }
 
-__global__ __launch_bounds__(1024) void moe_route_few_kernel(const void* logits, int dtype, int rows, int experts, int k, int normalize, MoeFewTable* table)
-{
-    __shared__ MoeFewRouting routing;
-    route_few<16>(routing, logits, dtype, rows, experts, k, normalize);
-    write_table(routing, rows, k, table);
-}
-
 // The rows of the pairs of workgroup blockIdx.x of the launch before. (One workgroup for all, counting again, took 50 us for 32768 pairs.)
 __global__ __launch_bounds__(1024) void moe_plan_kernel(int rows, int experts, int k, int share, MoePlanCall c, MoeRoute r)
 {
@@ -117,9 +110,9 @@ __global__ __launch_bounds__(1024) void moe_plan_kernel(int rows, int experts, i
     place_pairs(group * share * k, min((group + 1) * share, rows) * k, k, row0, r);
 }
 
-// y = base + sum over a token's experts, in the order of their logits, of weight * (out + bias).
+// y = base + sum over a token's experts, in the order of their logits, of weight * (out + bias), out the sum of its slices.
 template <typename T, bool BF16>
-__global__ __launch_bounds__(256) void moe_combine_kernel(RocmMoeArgs a, MoeRoute r, const float* __restrict__ out)
+__global__ __launch_bounds__(256) void moe_combine_kernel(RocmMoeArgs a, MoeRoute r, const float* __restrict__ out, int slices)
 {
     const int64_t token = static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y;
     if (token >= a.rows) return;
@@ -139,6 +132,13 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(RocmMoeArgs a, MoeRout
         Eight<float, false> v;
         if (left == 8) v.load(from);
         else v.load_first(from, left);
+        for (int i = 1; i < slices; ++i) {
+            Eight<float, false> more;
+            if (left == 8) more.load(from + i * (a.rows * a.k * a.hidden));
+            else more.load_first(from + i * (a.rows * a.k * a.hidden), left);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v.raw[e] += more.raw[e];
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] = fmaf(w, v.raw[e] + (a.down.bias && e < left ? load_as_f32(a.down.bias, a.bias_dtype, bias_at + e) : 0.f), sum[e]);
     }
@@ -178,17 +178,11 @@ int launch_moe_plan(const RocmMoeArgs& a, int tile_rows, int max_tiles, const Mo
     return static_cast<int>(hipGetLastError());
 }
 
-int launch_moe_route_few(const RocmMoeArgs& a, MoeFewTable* table, hipStream_t s)
-{
-    hipLaunchKernelGGL(moe_route_few_kernel, dim3(1), dim3(1024), 0, s, a.logits, a.logits_dtype, static_cast<int>(a.rows), a.experts, a.k, a.normalize, table);
-    return static_cast<int>(hipGetLastError());
-}
-
-int launch_moe_combine(const RocmMoeArgs& a, const MoeRoute& r, const float* out, hipStream_t s)
+int launch_moe_combine(const RocmMoeArgs& a, const MoeRoute& r, const float* out, int slices, hipStream_t s)
 {
     const dim3 grid = moe_grid(static_cast<unsigned>((a.hidden + 2047) / 2048), static_cast<int>(a.rows));
-    if (a.dtype == ROCM_DT_BF16) hipLaunchKernelGGL((moe_combine_kernel<uint16_t, true>), grid, dim3(256), 0, s, a, r, out);
-    else hipLaunchKernelGGL((moe_combine_kernel<uint16_t, false>), grid, dim3(256), 0, s, a, r, out);
+    if (a.dtype == ROCM_DT_BF16) hipLaunchKernelGGL((moe_combine_kernel<uint16_t, true>), grid, dim3(256), 0, s, a, r, out, slices);
+    else hipLaunchKernelGGL((moe_combine_kernel<uint16_t, false>), grid, dim3(256), 0, s, a, r, out, slices);
     return static_cast<int>(hipGetLastError());
 }
 

@@ -19,7 +19,8 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
 {
     constexpr int kPitch = 9;                                            // pieces of 16 bytes from a row of 64 elements in LDS to the next
     __shared__ uint4 staged[2][TM * 32 * kPitch];
-    const unsigned index = blockIdx.z * gridDim.y + blockIdx.y;
+    // (slices of down's K along z; without them z goes on where y ends)
+    const unsigned slice = !UP && p.slices > 1 ? blockIdx.z : 0u, index = (slice ? 0u : blockIdx.z) * gridDim.y + blockIdx.y;
     if (index >= p.count) return;
     const int4 tile = p.tiles[index];
     if (tile.z == 0) return;
@@ -30,7 +31,9 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
     const uint8_t* const b = (which ? p.m.w[1].b : p.m.w[0].b) + at * p.m.row_bytes;
     const ST* const s = static_cast<const ST*>(which ? p.m.w[1].scales : p.m.w[0].scales) + at * p.m.kb;
     const uint8_t* const z = (which ? p.m.w[1].zp : p.m.w[0].zp) + at * p.m.zp_row;
-    const int steps = static_cast<int>(p.ldx) >> 6, shift = 31 - __builtin_clz(p.m.block_size), row_bytes = static_cast<int>(p.m.row_bytes), last_block = p.m.kb - 1;
+    const int from = UP ? 0 : static_cast<int>(slice) * p.steps_per_slice, all_steps = static_cast<int>(p.ldx) >> 6;
+    const int steps = UP || p.slices == 1 ? all_steps : min(from + p.steps_per_slice, all_steps);             // where the slice ends
+    const int shift = 31 - __builtin_clz(p.m.block_size), row_bytes = static_cast<int>(p.m.row_bytes), last_block = p.m.kb - 1;
 
     const int piece = threadIdx.x & 7;
     const uint16_t* x[TM];
@@ -140,15 +143,15 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
 
     uint4 one, two;
     Scales sa, sb;                                                       // (blocks of 32: of a step each; else sa of both)
-    load_x(0);
-    load_s(0, sa);
-    load_w(0, one);
-    if (BS == 32) load_s(1, sb);
-    load_w(min(1, steps - 1), two);
-    stage(0);
-    load_x(min(1, steps - 1));
+    load_x(from);
+    load_s(from, sa);
+    load_w(from, one);
+    if (BS == 32) load_s(from + 1, sb);
+    load_w(min(from + 1, steps - 1), two);
+    stage(from);
+    load_x(min(from + 1, steps - 1));
     __syncthreads();
-    int t = 0;
+    int t = from;                                                        // (even)
     for (; t + 2 <= steps; t += 2) {                                     // (with a branch between the two the compiler waits for all loads there)
         take(t, sa);
         load_s(t + 2, sa);
@@ -188,12 +191,13 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
             }
     } else {
         if (col >= p.m.n) return;
+        float* const out = p.out + slice * p.slice_elements;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int row = row_of(i, e);
-                if (row < tile.z) p.out[static_cast<int64_t>(tile.y + row) * p.m.n + col] = total[i][e];
+                if (row < tile.z) out[static_cast<int64_t>(tile.y + row) * p.m.n + col] = total[i][e];
             }
     }
 }
@@ -206,7 +210,8 @@ int launch_moe_tile(const RocmMoeArgs& a, const MoeTileCall& p, bool up, int til
         constexpr bool BF16 = decltype(bf)::value, UP = decltype(half)::value;
         constexpr int BS = decltype(bs)::value;
         using ST = decltype(st);
-        const dim3 grid = moe_grid(UP ? static_cast<unsigned>((p.ldh + 63) / 64) : static_cast<unsigned>(p.m.n + 127) / 128, static_cast<int>(p.count));
+        dim3 grid = moe_grid(UP ? static_cast<unsigned>((p.ldh + 63) / 64) : static_cast<unsigned>(p.m.n + 127) / 128, static_cast<int>(p.count));
+        if (!UP && p.slices > 1) grid.z = static_cast<unsigned>(p.slices);
         if (tile_rows == 128) hipLaunchKernelGGL((moe_tile_kernel<BF16, BS, ST, UP, 4>), grid, dim3(256), 0, s, p);
         else hipLaunchKernelGGL((moe_tile_kernel<BF16, BS, ST, UP, 1>), grid, dim3(256), 0, s, p);
         return static_cast<int>(hipGetLastError());

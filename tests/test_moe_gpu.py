@@ -194,6 +194,20 @@ def test_elements_anywhere_and_callers_workspace(ep, rows):
     run(ep, rows, 4, 2, 136, 72, 32, E.F16, offset=3, bias=True, zero_points=True, workspace=True)
 
 
+@pytest.mark.parametrize("block,inter", [(32, 2176), (64, 4224), (128, 3000), (256, 2049)])
+@pytest.mark.parametrize("rows", [5, 17, 90])
+def test_down_in_slices_of_its_k(ep, rows, block, inter):
+    run(ep, rows, 4, 2, 200, inter, block, E.BF16, zero_points=True, again=True)
+    run(ep, rows, 4, 2, 200, inter, block, E.F16, scale_dtype=E.F32, bias=True)
+
+
+@pytest.mark.parametrize("block", [32, 64, 128])
+@pytest.mark.parametrize("dtype,scale_dtype", [(E.F16, E.F32), (E.BF16, E.F32), (E.BF16, E.BF16), (E.F16, E.F16)])
+def test_tiles_of_128_pairs(ep, block, dtype, scale_dtype):
+    _, variant = run(ep, 333, 3, 2, 192, 160, block, dtype, scale_dtype=scale_dtype, zero_points=block == 64, bias=True)
+    assert variant == ("moe_tall_tiles" if scale_dtype == E.F16 else "moe_tiles_128")
+
+
 def test_leading_dimensions(ep):
     run(ep, 12, 4, 2, 64, 32, 32, E.F16, shape=(2, 3, 2))
 
