@@ -19,7 +19,8 @@ typedef __attribute__((ext_vector_type(16))) int i32x16_t;
 __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
 // One workgroup of WAVES waves a row: the largest magnitude, then the codes. The first HELD eights of a thread stay in registers, all loaded before any is looked
-// at; what lies behind them is read again. Memory bounds it.
+// at; what lies behind them is read again. Memory bounds it: 8192 rows of 4096 in bf16 take 26 us (3.9 TB/s), 500 of 18944 take 9 (3.2 TB/s; one read of the row
+// after the other took 14).
 template <typename T, bool BF16, int WAVES, int HELD>
 __global__ __launch_bounds__(WAVES * 64) void quantize_rows_kernel(const T* __restrict__ a, int64_t k, int64_t kp, int8_t* __restrict__ codes, float* __restrict__ scales)
 {
@@ -124,6 +125,8 @@ __device__ __forceinline__ void store_scaled(const Int8Params& p, int64_t row, i
 // bytes as 16 columns). Two steps' loads are in flight.
 // FUSED (up to four rows of at most 32 KiB of codes): a is [m, k] of type T, and every workgroup makes the codes for itself, in LDS, while its first weights are on
 // their way: a launch of its own takes longer than a row's second and third trip from L2.
+// Measured: one row of 4096 -> 6144 with the quantizer inside 8.1 us (25 MB: 3.1 TB/s, an empty launch is 2 of them), 8 rows of 4096 -> 28672 23.5 us (5.0 TB/s),
+// 24 rows of 4096 -> 12288 13.7 us (3.7 TB/s).
 template <int RT, int CT, typename T, bool BF16, bool FUSED>
 __global__ __launch_bounds__(512) void int8_rows_kernel(const int8_t* b_base, const void* a_base, int m, int n, int k, int steps, Int8Params p)
 {
@@ -262,7 +265,9 @@ __global__ __launch_bounds__(512) void int8_rows_kernel(const int8_t* b_base, co
 // Four steps are in LDS or on their way. One barrier a step: before the step's last products the next step has arrived, its first operands are read while those
 // products run, and the loads of the step four on go where this step's operands were, which all are in registers by then.
 // W = 4 (256 x 256): 256 accumulators a lane, one wave a SIMD; a piece read from LDS meets four others. W = 2 (128 x 128): two workgroups a CU, for grids that would
-// not cover the chip.
+// not cover the chip; with slices of K, which make one workgroup a CU, BK = 128 instead of 64, whole lines (500 rows of 18944 -> 3584: 50 us instead of 59).
+// Measured: 8192 rows of 4096 -> 14336 520-540 us (1.8 POP/s; a product of twice the K reaches 2.0, so that some 130 us are the first loads and the last stores of
+// seven rounds of tiles, one workgroup a CU), 500 rows of 18944 -> 3584 in two slices 50 us and 7.5 for their sum (1.2 POP/s).
 template <int W, int BK>
 struct Int8Tile {
     static constexpr int kStages = 4;
@@ -561,10 +566,13 @@ Int8Plan plan_of(const RocmInt8Args& a)
     if (a.m <= kFewRows || (a.m <= kSomeRows && a.n * ((a.k + 127) / 128 * 128) <= kSmallBytes)) return p;
     auto tiles = [&](int64_t t) { return (a.m + t - 1) / t * ((a.n + t - 1) / t); };
     const int64_t cus = rocm_ffi_compute_units(), steps = (a.k + 127) / 128;
+    // 256 x 256 from tiles for three quarters of the CUs on. K 4096, us in tiles of 256 and of 128: 1024 x 8192 (128 tiles of 256) 65 and 48, 1024 x 10240 (160) 67 and
+    // 66, 1500 x 8192 (192) 69 and 74, 1024 x 14336 (224) 74 and 92.
     p.tile = tiles(256) >= cus * 3 / 4 ? 256 : 128;
     if (p.tile == 128) {
-        // slices of K until two workgroups for each CU are there, none of less than 16 steps
-        int64_t s = 2 * cus / tiles(128);
+        // Slices of K until a workgroup for each CU is there, none of less than 16 steps. 500 rows of 18944 -> 3584 (112 tiles): 80 us without, 54 with two, 59 with four,
+        // 64 with six; 100 rows of them (28 tiles): 76 without, 23 with nine or sixteen.
+        int64_t s = cus / tiles(128);
         if (s > steps / 16) s = steps / 16;
         s = s < 1 ? 1 : s > 16 ? 16 : s;
         const int64_t share = (steps + s - 1) / s;
@@ -634,9 +642,9 @@ extern "C" int rocm_launch_int8(const RocmInt8Args* args, rocm_stream_t stream)
         hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, p, tm, tn, slices);
         return hipGetLastError();
     };
-    constexpr size_t kLds256 = 4 * Int8Tile<4, 64>::kStage, kLds128 = 4 * Int8Tile<2, 64>::kStage;
+    constexpr size_t kLds256 = 4 * Int8Tile<4, 64>::kStage, kLds128 = 4 * Int8Tile<2, 64>::kStage, kLdsSlices = 4 * Int8Tile<2, 128>::kStage;
     hipError_t e = plan.tile == 256 ? tiled(int8_tile_kernel<4, 64, false>, kLds256)
-                   : p.partial      ? tiled(int8_tile_kernel<2, 64, true>, kLds128)
+                   : p.partial      ? tiled(int8_tile_kernel<2, 128, true>, kLdsSlices)
                                     : tiled(int8_tile_kernel<2, 64, false>, kLds128);
     if (e == hipSuccess && p.partial) {
         const unsigned y = static_cast<unsigned>(p.m < 32768 ? p.m : 32768);
