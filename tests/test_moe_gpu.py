@@ -5,7 +5,7 @@ import pytest
 from onnx_genai_amd import ep as E
 from onnx_genai_amd import synth
 
-from .node_helpers import EPS, Device, Experts, as64, moe64_noises
+from .node_helpers import EPS, Device, Experts, as64, moe64
 
 pytestmark = pytest.mark.gpu
 
@@ -14,8 +14,7 @@ def check(got, want, noise, dtype, what):
     """Two roundings to the type lie between input and result, of h and of y. A rounding of a value v is off by at most half a step of its binade: evenly spread,
     at most eps / 2 |v| / sqrt(3) in the mean square. h's roundings are independent, so that they are off in y by that times sqrt(noise), noise = sum w^2 h^2 W2^2
     (not by that times |y|: what the experts add may cancel). So each row's error has a mean square of at most (eps / 2)^2 / 3 times |y|^2 + noise; it is
-    held to three times that (sqrt(3) in the norm), one element to y's half step and six deviations. The f32 sums before h are off by 2^-16 of their terms' size.
-    The tiles of 128 pairs round each weight to the type too: noise then holds what that does to y, by the same mean square."""
+    held to three times that (sqrt(3) in the norm), one element to y's half step and six deviations. The f32 sums before h are off by 2^-16 of their terms' size."""
     half = EPS[dtype] / 2
     nan = np.isnan(want).any(-1)
     assert np.isnan(got[nan]).all(), what
@@ -47,7 +46,7 @@ def run(ep, rows, experts, k, hidden, inter, block, dtype, *, fusion=1, zero_poi
     extra = {"alpha": 1.702, "beta": 1.0, "limit": 1.5} if clamped else {}
     if clamped:
         attrs.update(activation_alpha=1.702, activation_beta=1.0, swiglu_limit=1.5)
-    want, noise, of_weights = moe64_noises(as64(x, dtype), as64(logits, logits_dtype), fc1, fc2, third, k=k, normalize=normalize, fusion=fusion, **extra)
+    want, noise = moe64(as64(x, dtype), as64(logits, logits_dtype), fc1, fc2, third, k=k, normalize=normalize, fusion=fusion, **extra)
     dev = Device(ep)
     kernel = ep.get_kernel(attrs, op_type="QMoE")
     lead = shape or (rows,)
@@ -73,8 +72,6 @@ def run(ep, rows, experts, k, hidden, inter, block, dtype, *, fusion=1, zero_poi
     finally:
         dev.free()
         kernel.release()
-    if variant == "moe_tall_tiles":
-        noise = noise + of_weights
     check(as64(got, dtype), want, noise, dtype, (variant, rows, experts, k, hidden, inter, block))
     return got, variant
 
@@ -205,7 +202,7 @@ def test_down_in_slices_of_its_k(ep, rows, block, inter):
 @pytest.mark.parametrize("dtype,scale_dtype", [(E.F16, E.F32), (E.BF16, E.F32), (E.BF16, E.BF16), (E.F16, E.F16)])
 def test_tiles_of_128_pairs(ep, block, dtype, scale_dtype):
     _, variant = run(ep, 333, 3, 2, 192, 160, block, dtype, scale_dtype=scale_dtype, zero_points=block == 64, bias=True)
-    assert variant == ("moe_tall_tiles" if scale_dtype == E.F16 else "moe_tiles_128")
+    assert variant == "moe_tiles_128"
 
 
 def test_leading_dimensions(ep):
