@@ -471,6 +471,8 @@ struct Int8Node final : NxrtRocmNode {
     {
         int64_t rows = 0, last = 0;
         if (!static_matrix(in, n, 0, &rows, &last)) return make_status(NXRT_INVALID_ARGUMENT, err("workspace_requirement needs the shape of A"));
+        const NxrtStatus st = ep->bind();          // (the plan goes by the GPU's CUs)
+        if (st.code != NXRT_OK) return st;
         *bytes = rows ? layout(rows, in[0].dtype, in[0].dtype == NXRT_DT_INT8).total : 0;
         return ok();
     }
@@ -610,6 +612,10 @@ struct MoeNode final : NxrtRocmNode {
         a.experts = static_cast<int>(experts);
         a.k = static_cast<int>(s.k);
         a.block_size = static_cast<int>(s.block_size);
+        if (hidden < 1 || hidden > (1 << 20) || a.inter < 1 || a.inter > (1 << 20) || experts < 1 || experts > ROCM_MOE_MAX_EXPERTS || rows * s.k >= (int64_t{1} << 24))
+            return make_status(NXRT_INVALID_ARGUMENT, err("workspace_requirement got shapes that no call takes"));
+        const NxrtStatus st = ep->bind();          // (the plan goes by the GPU's CUs)
+        if (st.code != NXRT_OK) return st;
         *bytes = rocm_moe_workspace_bytes(&a);
         return ok();
     }

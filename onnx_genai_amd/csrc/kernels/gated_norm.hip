@@ -210,35 +210,39 @@ extern "C" int rocm_launch_gated_norm(const RocmGatedNormArgs* args, rocm_stream
     if (args->rows <= 0 || args->hidden <= 0) return 0;
     if (args->hidden > ROCM_GATED_NORM_MAX_HIDDEN || args->rows > 0x7fffffff) return static_cast<int>(hipErrorInvalidValue);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int64_t gates = args->gate ? args->rows / args->rows_per_gate : 1;
-    GatedNormParams p{*args, static_cast<int>((args->hidden + 7) / 8), static_cast<int>(args->rows / gates)};
-    auto go = [&](auto kernel, unsigned grid, unsigned threads) {
-        // a grid has 65535 rows: further gates go in further launches
-        for (int64_t g = 0; g < gates; g += 65535) {
-            GatedNormParams part = p;
-            const int64_t first = g * p.per_gate, item = args->dtype == ROCM_DT_F32 ? 4 : 2, skip = first * args->hidden;
-            auto on = [&](auto* x, int64_t bytes) { return x ? reinterpret_cast<decltype(x)>(reinterpret_cast<uintptr_t>(x) + static_cast<uintptr_t>(bytes)) : x; };
-            part.a.residual = on(args->residual, skip * item);
-            part.a.block = on(args->block, skip * item);
-            part.a.z = on(args->z, skip * item);
-            part.a.n = on(args->n, skip * (args->n_scale ? 1 : item));
-            part.a.n_scale = on(args->n_scale, first * 4);
-            part.a.gate = on(args->gate, g * args->hidden * (args->gate_dtype == ROCM_DT_F32 ? 4 : 2));
-            hipLaunchKernelGGL(kernel, dim3(grid, static_cast<unsigned>(gates - g < 65535 ? gates - g : 65535)), dim3(threads), 0, s, part);
-            const hipError_t e = hipGetLastError();
-            if (e != hipSuccess) return static_cast<int>(e);
-        }
+    const int64_t gates = args->gate ? args->rows / args->rows_per_gate : 1, per_gate = args->rows / gates;
+    // A grid has 65535 rows and fewer than 2^32 threads: further gates, and further rows of a gate, go in further launches.
+    constexpr int64_t kMostGates = 65535, kMostRows = 1 << 21;
+    auto go = [&](auto kernel, unsigned rows_of_block, unsigned threads) {
+        const int64_t gates_at_once = per_gate > kMostRows ? 1 : kMostGates, rows_at_once = per_gate > kMostRows ? kMostRows : per_gate;
+        for (int64_t g = 0; g < gates; g += gates_at_once)
+            for (int64_t r = 0; r < per_gate; r += rows_at_once) {
+                const int64_t rows = per_gate - r < rows_at_once ? per_gate - r : rows_at_once, first = g * per_gate + r;
+                GatedNormParams part{*args, static_cast<int>((args->hidden + 7) / 8), static_cast<int>(rows)};
+                const int64_t item = args->dtype == ROCM_DT_F32 ? 4 : 2, skip = first * args->hidden;
+                auto on = [&](auto* x, int64_t bytes) { return x ? reinterpret_cast<decltype(x)>(reinterpret_cast<uintptr_t>(x) + static_cast<uintptr_t>(bytes)) : x; };
+                part.a.residual = on(args->residual, skip * item);
+                part.a.block = on(args->block, skip * item);
+                part.a.z = on(args->z, skip * item);
+                part.a.n = on(args->n, skip * (args->n_scale ? 1 : item));
+                part.a.n_scale = on(args->n_scale, first * 4);
+                part.a.gate = on(args->gate, g * args->hidden * (args->gate_dtype == ROCM_DT_F32 ? 4 : 2));
+                const dim3 grid(static_cast<unsigned>((rows + rows_of_block - 1) / rows_of_block), static_cast<unsigned>(gates - g < gates_at_once ? gates - g : gates_at_once));
+                hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, part);
+                const hipError_t e = hipGetLastError();
+                if (e != hipSuccess) return static_cast<int>(e);
+            }
         return 0;
     };
-    const unsigned rows = static_cast<unsigned>(p.per_gate);
+    const int vectors = static_cast<int>((args->hidden + 7) / 8);
     auto typed = [&](auto t, auto bf) {
         using T = decltype(t);
         constexpr bool BF16 = decltype(bf)::value;
-        if (p.vectors <= 64) return go(gated_norm_kernel<T, BF16, 1, true>, (rows + 3) / 4, 256);
-        const unsigned threads = static_cast<unsigned>(p.vectors + 63) / 64 * 64;
-        if (threads <= 1024) return go(gated_norm_kernel<T, BF16, 1, false>, rows, threads);
-        if (threads <= 2048) return go(gated_norm_kernel<T, BF16, 2, false>, rows, (threads / 2 + 63) / 64 * 64);
-        return go(gated_norm_kernel<T, BF16, 4, false>, rows, 1024);
+        if (vectors <= 64) return go(gated_norm_kernel<T, BF16, 1, true>, 4, 256);
+        const unsigned threads = static_cast<unsigned>(vectors + 63) / 64 * 64;
+        if (threads <= 1024) return go(gated_norm_kernel<T, BF16, 1, false>, 1, threads);
+        if (threads <= 2048) return go(gated_norm_kernel<T, BF16, 2, false>, 1, (threads / 2 + 63) / 64 * 64);
+        return go(gated_norm_kernel<T, BF16, 4, false>, 1, 1024);
     };
     if (args->dtype == ROCM_DT_F32) return typed(float{}, std::false_type{});
     if (args->dtype == ROCM_DT_BF16) return typed(uint16_t{}, std::true_type{});

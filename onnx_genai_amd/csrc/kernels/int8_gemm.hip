@@ -526,8 +526,13 @@ extern "C" int rocm_launch_quantize_rows(const void* a, int dtype, int64_t m, in
     const int64_t kp = (k + 127) / 128 * 128;
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto go = [&](auto kernel, unsigned threads, auto* x) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(m)), dim3(threads), 0, s, x, k, kp, codes, scales);
-        return static_cast<int>(hipGetLastError());
+        constexpr int64_t kMost = 1 << 21;                   // rows of a launch: a grid has fewer than 2^32 threads
+        for (int64_t r = 0; r < m; r += kMost) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(m - r < kMost ? m - r : kMost)), dim3(threads), 0, s, x + r * k, k, kp, codes + r * kp, scales + r);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return static_cast<int>(e);
+        }
+        return 0;
     };
     auto held = [&](auto four_waves, auto sixteen_waves, auto* x) { return kp <= 8192 ? go(four_waves, 256u, x) : go(sixteen_waves, 1024u, x); };
     if (dtype == ROCM_DT_F32) return held(quantize_rows_kernel<float, false, 4, 4>, quantize_rows_kernel<float, false, 16, 3>, static_cast<const float*>(a));

@@ -234,3 +234,14 @@ def test_scratch(host_only, provider):  # noqa: F811
     with pytest.raises(E.EpError):
         k.workspace_requirement([((-1, 32), E.F16)])
     k.release()
+
+
+@pytest.mark.parametrize("x,logits,w1", [((3, 0), (3, 4), (4, 64, 1, 16)), ((3, 32), (3, 0), (0, 64, 1, 16)), ((3, 32), (3, 4), (4, 0, 1, 16)), ((3, 32), (3, 4), (4, 1, 1, 16)),
+                                         ((3, 32), (3, 2048), (2048, 64, 1, 16)), ((2 ** 23, 32), (2 ** 23, 4), (4, 64, 1, 16))])
+def test_scratch_of_shapes_that_no_call_takes(provider, x, logits, w1):
+    k = provider.get_kernel({"k": 2, "block_size": 32, "swiglu_fusion": 1}, op_type="QMoE")
+    with pytest.raises(E.EpError) as err:
+        k.workspace_requirement([(x, E.F16), (logits, E.F32), (w1, E.U8)])
+    assert err.value.code == 3 and "shapes that no call takes" in err.value.message
+    assert k.workspace_requirement([((0, 32), E.F16), ((0, 4), E.F32), ((4, 64, 1, 16), E.U8)])[1] == 256
+    k.release()
