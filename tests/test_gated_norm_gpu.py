@@ -177,3 +177,8 @@ def test_graph_replays(ep):
     finally:
         dev.free()
         kernel.release()
+
+
+@pytest.mark.parametrize("rows,h,gates,outputs", [(2 ** 21 + 5, 8, 1, "zn"), (2 * (2 ** 21 + 3), 4, 2, "zc")])
+def test_more_rows_than_one_launch_takes(ep, rows, h, gates, outputs):
+    run(ep, rows, h, E.F16, gates=gates, outputs=outputs)

@@ -195,3 +195,7 @@ def test_graph_replays(ep, m, k):
     finally:
         dev.free()
         kernel.release()
+
+
+def test_more_rows_than_one_launch_quantizes(ep):
+    run(ep, 2 ** 21 + 3, 1, 16, E.F16)
