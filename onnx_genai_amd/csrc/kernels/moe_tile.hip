@@ -6,11 +6,12 @@
 // TM = 4 (prompts): the matrix cores and the vector instructions beside them bound it, 64 to scale a block's sums and 44 (bf16: 76) to
 // unpack 64 k for 512 cycles of products. TM = 1 (a few rows an expert): the weights' bytes, and a CU's path to memory, where 64 columns' scales take as long as
 // their weights.
-// Measured: TM = 1, 48 tokens of 8 out of 64 experts of 2048 and 1024, blocks of 64, 53 us up and 28 down (2.7 TB/s); TM = 4, 4096 tokens of those, blocks of 128, 414 us
-// up and 223 down (0.66 and 0.62 PFLOP/s; vector and matrix instructions together fill the issue slots, at 2.0 GHz).
-// Weights rounded to 16 bits before the product save the scaling and half of the accumulators, so that a wave has 64 columns (777 tokens of 4 out of 16 experts of 2880 in
-// f16: 191 us up instead of 252, 124 down instead of 142; 4096 tokens in bf16 349 instead of 414, 188 instead of 223), and put y off by up to twice its own rounding:
-// they stay exact.
+// Measured: TM = 1, 48 tokens of 8 out of 64 experts of 2048 and 1024, blocks of 64, 52 us up and 28 down (2.7 TB/s); TM = 4, 4096 tokens of those, blocks of 128, 405 us
+// up and 222 down (0.68 and 0.62 PFLOP/s; vector and matrix instructions together fill the issue slots, at 2.0 GHz), 777 tokens of 4 out of 16 experts of 2880, f16,
+// blocks of 32, 230 us up and 121 down (0.45 and 0.43 PFLOP/s; its tiles are 128 and 66 rows, a quarter of them absent). With a step's reads and unpacking in front of
+// its products, as the compiler places them, those were 414, 223, 252 and 142.
+// Weights rounded to 16 bits before the product save the scaling and half of the accumulators, so that a wave has 64 columns (777 tokens: 191 us up and 124 down; 4096
+// tokens in bf16: 349 and 188), and put y off by up to twice its own rounding: they stay exact.
 // h is rounded to the activations' type here (as a graph of separate nodes has it): a second part of it would be half again as many products in the second half.
 #include "moe.hiph"
 #include "prefill_common.hiph"
@@ -18,6 +19,21 @@
 
 namespace mnb {
 namespace {
+
+// Nibbles 0 and 4 of `bits` as q - zp: plain_nibbles for two of its eight.
+template <bool BF16>
+__device__ __forceinline__ uint32_t tile_pair(uint32_t bits, uint32_t z, uint32_t mask, uint32_t magic)
+{
+    const half2p_t h = __builtin_bit_cast(half2p_t, (bits & mask) | magic);
+    if constexpr (BF16) {
+        const float off = -1024.0f - static_cast<float>(z);
+        float one = 1.0f;
+        asm("" : "+v"(one));                                   // (a factor the compiler knows to be one would make it a conversion and an add)
+        return __builtin_amdgcn_perm(__float_as_uint(fmaf(static_cast<float>(h.y), one, off)), __float_as_uint(fmaf(static_cast<float>(h.x), one, off)), 0x07060302u);
+    } else {
+        return __builtin_bit_cast(uint32_t, h + __builtin_bit_cast(half2p_t, 0xE400E400u | (z * 0x00010001u)));
+    }
+}
 
 template <bool BF16, int BS, typename ST, bool UP, int TM>
 __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileCall p)
@@ -67,14 +83,10 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
 #pragma unroll
         for (int i = 0; i < TM; ++i) ahead[i] = *reinterpret_cast<const uint4*>(x[i] + t * 64);
     };
-    auto stage = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const uint4 d = ahead[i];
-            staged[t & 1][((threadIdx.x >> 3) + i * 32) * kPitch + piece] =
-                make_uint4(__builtin_amdgcn_perm(d.z, d.x, 0x05040100u), __builtin_amdgcn_perm(d.z, d.x, 0x07060302u), __builtin_amdgcn_perm(d.w, d.y, 0x05040100u),
-                           __builtin_amdgcn_perm(d.w, d.y, 0x07060302u));
-        }
+    auto stage = [&](int t, int i) {
+        const uint4 d = ahead[i];
+        staged[t & 1][((threadIdx.x >> 3) + i * 32) * kPitch + piece] = make_uint4(__builtin_amdgcn_perm(d.z, d.x, 0x05040100u), __builtin_amdgcn_perm(d.z, d.x, 0x07060302u),
+                                                                                   __builtin_amdgcn_perm(d.w, d.y, 0x05040100u), __builtin_amdgcn_perm(d.w, d.y, 0x07060302u));
     };
     uint32_t mask = 0x000f000fu;
     asm volatile("" : "+v"(mask));
@@ -102,75 +114,100 @@ __global__ __launch_bounds__(256, TM == 4 ? 2 : 4) void moe_tile_kernel(MoeTileC
             asm volatile("v_bfe_u32 %0, %1, 4, 4" : "=v"(zero[1]) : "v"(from.z));
         }
     };
-    auto add_up = [&](float scale) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) total[i][e] = fmaf(scale, sum[i][e], total[i][e]);
-    };
-    // eight elements of each of the two lane groups, at pieces `at_piece` of the rows
-    auto product = [&](int t, uint32_t q, uint32_t zero, int at_piece, bool first) {
-        const uint4 w = plain_nibbles<BF16>(q, zero, mask, magic);
-#pragma unroll
-        for (int i = 0; i < TM; ++i) sum[i] = mfma32<BF16>(staged[t & 1][(i * 32 + c) * kPitch + at_piece], w, first ? none : sum[i]);
-    };
-    // A step stages the next one's activations, asks for those of the one behind it, multiplies, and asks for the weights two steps on, where its own were.
-    // FIRST, LAST: the step begins, ends a block (of 64 or more), the one of scale[which]
-    auto step = [&](int t, uint4& now, int which, bool first, bool last) {
-        stage(t + 1);
-        __builtin_amdgcn_sched_barrier(0);
-        load_x(min(t + 2, steps - 1));
-        __builtin_amdgcn_sched_barrier(0);
-        const uint4 w = now;
+    // A step is four parts of 16 k. Behind a part's product of 32 rows come the next part's read of them and a share of its weights' unpacking, so that they run beside
+    // the products; the last part's come from the next step, whose activations all waves have staged by then: the step's only barrier. A block's sum is scaled where
+    // the next block's first product overwrites it.
+    uint4 rows[TM];
+    uint32_t weights[2][4];
+    float pending = 0.f;                                                 // the scale of the block whose sum this is
+    auto read = [&](int t, int part, int i) { return staged[t & 1][(i * 32 + c) * kPitch + (BS == 32 ? part * 2 + g : g * 4 + part)]; };
+    // BS 32: lane group h has block h; afterwards x and y hold block 0 of both groups, z and w block 1
+    auto arrange = [&](uint4& w) {
         if constexpr (BS == 32) {
-            // lane group h has block h; afterwards x and z hold block 0 of both groups, y and w block 1
             const auto lo = __builtin_amdgcn_permlane32_swap(w.x, w.y, false, false), hi = __builtin_amdgcn_permlane32_swap(w.z, w.w, false, false);
-            product(t, lo[0], zero[0], g, true);
-            product(t, hi[0], zero[0], 2 + g, false);
-            add_up(scale[0]);
-            product(t, lo[1], zero[1], 4 + g, true);
-            product(t, hi[1], zero[1], 6 + g, false);
-            add_up(scale[1]);
-        } else {
-            product(t, w.x, zero[which], g * 4, first);
-            product(t, w.y, zero[which], g * 4 + 1, false);
-            product(t, w.z, zero[which], g * 4 + 2, false);
-            product(t, w.w, zero[which], g * 4 + 3, false);
-            if (last) add_up(scale[which]);
+            w = make_uint4(lo[0], hi[0], lo[1], hi[1]);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        load_w(min(t + 2, steps - 1), now);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);                               // (nothing that waits for loads comes before)
+    };
+    auto unpack = [&](const uint4& w, int part, int two, uint32_t zp) {
+        const uint32_t q = part == 0 ? w.x : part == 1 ? w.y : part == 2 ? w.z : w.w;
+        return tile_pair<BF16>(q >> (4 * two), zp, mask, magic);
+    };
+    // FIRST: the step begins a block (of 64 or more). which: its scale, next_which: that of the next step, whose scales are taken before the last part.
+    auto step = [&](int t, uint4& now, uint4& next, int which, int next_which, bool first, auto take_next) {
+        float of_block[2] = {BS == 32 ? scale[0] : scale[which], scale[1]};
+        uint32_t zp = BS == 32 ? zero[0] : zero[which], zp1 = zero[1];
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {
+            if (part == 3) {
+                take_next();
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                load_w(min(t + 2, steps - 1), now);
+                arrange(next);
+            }
+            if (part == 1) load_x(min(t + 2, steps - 1));
+            __builtin_amdgcn_sched_barrier(0);
+            const bool begins = BS == 32 ? part % 2 == 0 : part == 0 && first;
+            const float done = pending;
+            if (begins) pending = of_block[part / 2];
+            const int coming = (part + 1) & 3;
+            const uint32_t coming_zp = part == 3 ? (BS == 32 ? zero[0] : zero[next_which]) : BS == 32 && part >= 1 ? zp1 : zp;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                if (begins)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) total[i][e] = fmaf(done, sum[i][e], total[i][e]);
+                const uint32_t(&w)[4] = weights[part & 1];
+                sum[i] = mfma32<BF16>(rows[i], make_uint4(w[0], w[1], w[2], w[3]), begins ? none : sum[i]);
+                rows[i] = read(part == 3 ? t + 1 : t, coming, i);
+#pragma unroll
+                for (int two = i * 4 / TM; two < (i + 1) * 4 / TM; ++two) weights[(part + 1) & 1][two] = unpack(part == 3 ? next : now, coming, two, coming_zp);
+                if (part == 0) stage(t + 1, i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
     };
 
-    uint4 one, two;
+    uint4 one, two_w;
     Scales sa, sb;                                                       // (blocks of 32: of a step each; else sa of both)
     load_x(from);
     load_s(from, sa);
     load_w(from, one);
     if (BS == 32) load_s(from + 1, sb);
-    load_w(min(from + 1, steps - 1), two);
-    stage(from);
+    load_w(min(from + 1, steps - 1), two_w);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) stage(from, i);
     load_x(min(from + 1, steps - 1));
     __syncthreads();
+    take(from, sa);
+    load_s(from + 2, sa);
+    arrange(one);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) rows[i] = read(from, 0, i);
+#pragma unroll
+    for (int two = 0; two < 4; ++two) weights[0][two] = unpack(one, 0, two, zero[0]);
+    auto none_taken = [] {};
     int t = from;                                                        // (even)
     for (; t + 2 <= steps; t += 2) {                                     // (with a branch between the two the compiler waits for all loads there)
-        take(t, sa);
-        load_s(t + 2, sa);
-        step(t, one, 0, true, BS != 128);
         if constexpr (BS == 32) {
-            take(t + 1, sb);
-            load_s(t + 3, sb);
+            step(t, one, two_w, 0, 0, true, [&] {
+                take(t + 1, sb);
+                load_s(t + 3, sb);
+            });
+        } else {
+            step(t, one, two_w, 0, 1, true, none_taken);
         }
-        step(t + 1, two, 1, BS != 128, true);
+        step(t + 1, two_w, one, 1, 0, BS != 128, [&] {
+            take(t + 2, sa);
+            load_s(t + 4, sa);
+        });
     }
-    if (t < steps) {
-        take(t, sa);
-        step(t, one, 0, true, true);
-    }
+    if (t < steps) step(t, one, two_w, 0, 0, true, none_taken);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) total[i][e] = fmaf(pending, sum[i][e], total[i][e]);
 
     // a lane has column c and rows 8 (e / 4) + 4 g + e % 4 of each 32
     auto row_of = [&](int i, int e) { return i * 32 + (e >> 2) * 8 + g * 4 + (e & 3); };
