@@ -77,7 +77,6 @@ MoeMatrix matrix_of(const RocmMoeArgs& a, const RocmMoeWeights& w, const RocmMoe
     m.block_size = a.block_size;
     m.row_bytes = static_cast<int64_t>(m.kb) * a.block_size / 2;
     m.zp_row = (m.kb + 1) / 2;
-    m.scale_dtype = a.scale_dtype;
     m.bias_dtype = a.bias_dtype;
     return m;
 }
@@ -134,7 +133,6 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     down.table = table;
     down.rows = up.rows;
     down.y = a.y;
-    down.out = reinterpret_cast<float*>(ws + l.out);
     if (!l.tiled) return launch_moe_few(a, up, down, l.slots, s);
     auto tiled = [&](const MoeMatrix& m, const uint16_t* rows, int64_t ldx) {
         MoeTileCall t{};
@@ -149,7 +147,7 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
         t.count = static_cast<unsigned>(l.slots);
         t.h = up.h;
         t.ldh = l.ip;
-        t.out = down.out;
+        t.out = reinterpret_cast<float*>(ws + l.out);
         t.slices = l.slices;
         t.steps_per_slice = l.steps_per_slice;
         t.slice_elements = l.pairs * a.hidden;
@@ -162,5 +160,5 @@ extern "C" int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_st
     first.token = route.token;
     rc = launch_moe_tile(a, first, true, l.tile_rows, s);
     if (rc == 0) rc = launch_moe_tile(a, second, false, l.tile_rows, s);
-    return rc != 0 ? rc : launch_moe_combine(a, route, down.out, l.slices, s);
+    return rc != 0 ? rc : launch_moe_combine(a, route, reinterpret_cast<const float*>(ws + l.out), l.slices, s);
 }
