@@ -25,21 +25,19 @@ struct GatedNormParams {
 __device__ __forceinline__ float add(float a, float b) { return a + b; }
 __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
-// NV: pieces a thread holds. WAVE: a wave has a row of its own (rows of at most NV * 512 elements), else the workgroup.
-template <typename T, bool BF16, int NV, bool WAVE>
-__global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_kernel(GatedNormParams p)
+// A workgroup has a row; NV: pieces a thread holds. (Four rows of at most 512 elements to a workgroup, a wave each, were level: 32768 rows of 512 23.4 us.)
+template <typename T, bool BF16, int NV>
+__global__ __launch_bounds__(1024) void gated_norm_kernel(GatedNormParams p)
 {
     using V8 = Eight<T, BF16>;
     const RocmGatedNormArgs& a = p.a;
     __shared__ float slots[4][16];
     __shared__ uint32_t slots_max[16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int waves = WAVE ? 1 : blockDim.x >> 6;
+    const int waves = blockDim.x >> 6;
     // rows of one gate along x, gates along y: no division for the gate
-    const int in_gate = WAVE ? static_cast<int>(blockIdx.x) * 4 + wave : static_cast<int>(blockIdx.x);
-    if (in_gate >= p.per_gate) return;                           // (whole waves, and no barrier is left behind where WAVE)
-    const int64_t row = static_cast<int64_t>(blockIdx.y) * p.per_gate + in_gate;
-    const int first = WAVE ? threadIdx.x & 63 : threadIdx.x, step = WAVE ? 64 : blockDim.x;
+    const int64_t row = static_cast<int64_t>(blockIdx.y) * p.per_gate + blockIdx.x;
+    const int first = threadIdx.x, step = blockDim.x;
     const int h = static_cast<int>(a.hidden);
     const int64_t at = row * h;
     const float inv_h = 1.0f / static_cast<float>(h);
@@ -213,7 +211,7 @@ extern "C" int rocm_launch_gated_norm(const RocmGatedNormArgs* args, rocm_stream
     const int64_t gates = args->gate ? args->rows / args->rows_per_gate : 1, per_gate = args->rows / gates;
     // A grid has 65535 rows and fewer than 2^32 threads: further gates, and further rows of a gate, go in further launches.
     constexpr int64_t kMostGates = 65535, kMostRows = 1 << 21;
-    auto go = [&](auto kernel, unsigned rows_of_block, unsigned threads) {
+    auto go = [&](auto kernel, unsigned threads) {
         const int64_t gates_at_once = per_gate > kMostRows ? 1 : kMostGates, rows_at_once = per_gate > kMostRows ? kMostRows : per_gate;
         for (int64_t g = 0; g < gates; g += gates_at_once)
             for (int64_t r = 0; r < per_gate; r += rows_at_once) {
@@ -227,7 +225,7 @@ extern "C" int rocm_launch_gated_norm(const RocmGatedNormArgs* args, rocm_stream
                 part.a.n = on(args->n, skip * (args->n_scale ? 1 : item));
                 part.a.n_scale = on(args->n_scale, first * 4);
                 part.a.gate = on(args->gate, g * args->hidden * (args->gate_dtype == ROCM_DT_F32 ? 4 : 2));
-                const dim3 grid(static_cast<unsigned>((rows + rows_of_block - 1) / rows_of_block), static_cast<unsigned>(gates - g < gates_at_once ? gates - g : gates_at_once));
+                const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(gates - g < gates_at_once ? gates - g : gates_at_once));
                 hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, part);
                 const hipError_t e = hipGetLastError();
                 if (e != hipSuccess) return static_cast<int>(e);
@@ -238,11 +236,10 @@ extern "C" int rocm_launch_gated_norm(const RocmGatedNormArgs* args, rocm_stream
     auto typed = [&](auto t, auto bf) {
         using T = decltype(t);
         constexpr bool BF16 = decltype(bf)::value;
-        if (vectors <= 64) return go(gated_norm_kernel<T, BF16, 1, true>, 4, 256);
         const unsigned threads = static_cast<unsigned>(vectors + 63) / 64 * 64;
-        if (threads <= 1024) return go(gated_norm_kernel<T, BF16, 1, false>, 1, threads);
-        if (threads <= 2048) return go(gated_norm_kernel<T, BF16, 2, false>, 1, (threads / 2 + 63) / 64 * 64);
-        return go(gated_norm_kernel<T, BF16, 4, false>, 1, 1024);
+        if (threads <= 1024) return go(gated_norm_kernel<T, BF16, 1>, threads);
+        if (threads <= 2048) return go(gated_norm_kernel<T, BF16, 2>, (threads / 2 + 63) / 64 * 64);
+        return go(gated_norm_kernel<T, BF16, 4>, 1024);
     };
     if (args->dtype == ROCM_DT_F32) return typed(float{}, std::false_type{});
     if (args->dtype == ROCM_DT_BF16) return typed(uint16_t{}, std::true_type{});

@@ -24,6 +24,7 @@ MoePlan plan_of(const RocmMoeArgs& a)
 {
     MoePlan l{};
     l.pairs = a.rows * a.k;
+    // Few tokens in dot products, or in tiles: 64 experts of 2048 and 1024, 1 token 16 us and 40, 4 tokens 47 and 55; 8 experts of 4096 and 14336, 51 and 84, 156 and 342.
     // (the rows of x lie in the 48 KiB of LDS that a kernel gets without asking beside its tables)
     l.tiled = !(a.rows <= kFewTokens && a.experts <= 256 && l.pairs <= kFewPairs && a.rows * ((a.hidden + 2047) / 2048) <= 12);
     l.tile_rows = l.pairs >= kTallPairs * a.experts ? 128 : 32;

@@ -440,6 +440,7 @@ int launch_moe_few(const RocmMoeArgs& a, const MoeUpCall& up, const MoeDownCall&
     });
     if (rc != 0) return rc;
     return few_build(a, a.down.zp != nullptr, lanes_per_column(down.ip), [&](auto bf, auto st, auto zp, auto lanes) {
+        // (4 tokens, 2048 columns: 47 us with 512 threads, 51 with 256; 1 token, 4096 columns: 56 and 51)
         const unsigned grid = static_cast<unsigned>(down.m.n + 7) / 8, threads = grid <= static_cast<unsigned>(rocm_ffi_compute_units()) ? 512 : 256;
         auto kernel = moe_few_down_kernel<decltype(bf)::value, decltype(st), decltype(zp)::value, decltype(lanes)::value>;
         hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, s, down.table, slots, down);
