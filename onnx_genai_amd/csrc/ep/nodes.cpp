@@ -616,7 +616,7 @@ struct MoeNode final : NxrtRocmNode {
             return make_status(NXRT_INVALID_ARGUMENT, err("workspace_requirement got shapes that no call takes"));
         const NxrtStatus st = ep->bind();          // (the plan goes by the GPU's CUs)
         if (st.code != NXRT_OK) return st;
-        *bytes = rocm_moe_workspace_bytes(&a);
+        *bytes = rows ? rocm_moe_workspace_bytes(&a) : 0;
         return ok();
     }
     NxrtStatus execute(const NxrtRocmTensorView* in, uint32_t n_in, NxrtRocmTensorView* out, uint32_t n_out, void* ws, uint64_t ws_bytes) override

@@ -23,6 +23,7 @@ struct MoePlan {
 MoePlan plan_of(const RocmMoeArgs& a)
 {
     MoePlan l{};
+    if (a.rows <= 0) return l;               // (no rows: no tiles to divide the chip by)
     l.pairs = a.rows * a.k;
     // Few tokens in dot products, or in tiles: 64 experts of 2048 and 1024, 1 token 16 us and 40, 4 tokens 47 and 55; 8 experts of 4096 and 14336, 51 and 84, 156 and 342.
     // (the rows of x lie in the 48 KiB of LDS that a kernel gets without asking beside its tables)
