@@ -98,7 +98,8 @@ __global__ __launch_bounds__(1024) void lds_probe_kernel(unsigned long long* cyc
             for (int j = 0; j < 8; ++j) {
                 const uint32_t lds = __builtin_amdgcn_readfirstlane((((j + wave) & 7) * 4096 + ((it & 1) << 10)) & 0xffff);
                 const uint32_t soff = (j * 1024 + wave * 8192 + blockIdx.x * 131072) & 0xfffff;
-                asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(srd), "s"(soff) : "memory");
+                // (a load into LDS needs a wait state behind the write of M0, which the compiler does not put into an asm block)
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(srd), "s"(soff) : "memory");
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }

@@ -340,12 +340,15 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void int8_tile_kernel(Int8Para
         const uint32_t k = static_cast<uint32_t>(begin + t) * BK, to = lds + (t & 3) * kStage + wave * (kStage / 8);
         // (behind the slice's last step: nothing, into a quarter that nobody reads any more)
         const bool is = t < count;
-        const srd_t sa = plain_srd(a + k, is ? a_bytes - k : 0u), sb = plain_srd(b + k, is && b_bytes > k ? b_bytes - k : 0u);
+        // The compiler puts no wait states in front of what stands in an asm block. A load needs five behind a vector instruction that wrote one of its scalar registers:
+        // the ranges' ends are differences cut off at zero as signed numbers, which scalar instructions make (unsigned, a vector one did), and the assembly is tested for it.
+        // (s_nop 4 here instead: 8192 rows 1 % slower, 24 rows 4 %.) A load into LDS needs one behind the write of M0, a reserved register that the compiler keeps nothing in.
+        const srd_t sa = plain_srd(a + k, is ? a_bytes - k : 0u), sb = plain_srd(b + k, is ? static_cast<uint32_t>(max(static_cast<int>(b_bytes) - static_cast<int>(k), 0)) : 0u);
 #pragma unroll
         for (int i = 0; i < Tile::kLoads; ++i) {
             const bool of_b = i >= Tile::kLoads / 2;
             const uint32_t dst = __builtin_amdgcn_readfirstlane(to + (of_b ? kStage / 2 : 0) + i % (Tile::kLoads / 2) * 1024);
-            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(at[i]), "s"(of_b ? sb : sa) : "memory");
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(at[i]), "s"(of_b ? sb : sa) : "memory");
         }
     };
     const int wm = (wave & 1) * kWave, wn = (wave >> 1) * kWave;
