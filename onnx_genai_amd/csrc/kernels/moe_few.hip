@@ -4,9 +4,10 @@
 //   moe_few_down_kernel   y = base + sum over the active experts of weight * (h W2^T + bias)
 //
 // The weights' bytes bound it once there are enough of them, and before that the way to them: arguments, logits and weights are reached one after the other.
-// A lane holds 32 elements of K of a row of x in registers, in 16 dot products of two with 32 nibbles of each of several columns (v_dot2_f32_f16, v_dot2_f32_bf16:
-// 46 instructions for 16 bytes of weights and one row; the matrix core wants the nibbles turned between lanes and takes 71 with its corrections, for up to 16 rows).
-// A nibble q is the 16-bit float magic + q (magic = 1024 in f16, 128 in bf16; exact), and the products' sum starts from -(magic + zp) times the lane's sum of x.
+// A lane holds 32 elements of K of a row of x in registers and multiplies them with 32 nibbles of each of several columns: f16 in 16 dot products of two (v_dot2_f32_f16),
+// bf16 in f32 by 32 mixed-precision multiply-adds (v_fma_mix_f32). A weight enters as the f16 q - zp, which is exact, so that one of zero adds nothing however large its x
+// is. (As magic + q, with -(magic + zp) times the sum of x in front, a pair of weights takes one instruction less in f16 and two in bf16, and what is left of magic * x
+// shows: an x of 60000 at weights of zero put y off by 15 %. One token 17.7 us and 18.4 now, three tokens of 4096 and 14336 131 and 133.)
 // Measured: one token, 8 of 64 experts of 2048 and 1024 in bf16, 10.7 us up and 7.2 down (28 MB; an empty launch is 2 us, and routing 3 more before the first weights),
 // three tokens of 4096 and 14336 over 8 experts in f16 with zero points 78 and 58 us (3.9 and 2.6 TB/s).
 // LPC lanes stand side by side on K and read 16 LPC bytes of a column's row as the caller holds it; 64 / LPC columns are read at once.
@@ -37,21 +38,9 @@ __device__ __forceinline__ MoeTile<NM> moe_tile(const MoeMatrix& m, int expert, 
     return t;
 }
 
-typedef __attribute__((ext_vector_type(2))) _Float16 moe_half2_t;
-typedef __attribute__((ext_vector_type(2))) __bf16 moe_bf16x2_t;
-
-template <bool BF16>
-__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c)
-{
-    if constexpr (BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(moe_bf16x2_t, a), __builtin_bit_cast(moe_bf16x2_t, b), c, false);
-    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(moe_half2_t, a), __builtin_bit_cast(moe_half2_t, b), c, false);
-}
-
-// 32 elements of a row in the order of a dword's nibbles under a mask and shifts: 0 4 | 1 5 | 2 6 | 3 7 of each eight; and their sum.
-template <bool BF16>
+// 32 elements of a row in the order of a dword's nibbles under a mask and shifts: 0 4 | 1 5 | 2 6 | 3 7 of each eight.
 struct Elements32 {
     uint32_t v[16];
-    float sum;
 
     // `count` of them are there (a multiple of 8), the rest is zero
     __device__ __forceinline__ void load(const uint16_t* x, int count)
@@ -70,15 +59,6 @@ struct Elements32 {
     {
 #pragma unroll
         for (int j = 0; j < 4; ++j) put(j, ordered(make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3])));
-        add_up();
-    }
-    __device__ __forceinline__ void add_up()
-    {
-        constexpr uint32_t kOnes = BF16 ? 0x3f803f80u : 0x3c003c00u;
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i & 3] = dot2<BF16>(v[i], kOnes, s[i & 3]);
-        sum = (s[0] + s[1]) + (s[2] + s[3]);
     }
     static __device__ __forceinline__ uint4 ordered(const uint4& d)
     {
@@ -87,29 +67,81 @@ struct Elements32 {
     }
 };
 
-// `mask`: 0x000f000f in a vector register, which leaves room for the magic in a scalar one, so that each pair but the first is a shift and one and-or.
-template <bool BF16>
-__device__ __forceinline__ void nibbles32(const uint4& w, uint32_t mask, uint32_t (&out)[16])
+// 32 nibbles as f16 pairs q - z, exact. A nibble in the low four bits of an f16's ten is 1024 + q, in the next four 1024 + 16 q, which one packed multiply-add takes
+// to q - z: two of a dword's four pairs need no shift of their own.
+// What that takes, in registers: masks in vector ones and the magic in a scalar one make and, or one instruction.
+struct Unpacking {
+    uint32_t low = 0x000f000fu, high = 0x00f000f0u, magic = opaque_scalar(0x64006400u);
+    __device__ __forceinline__ Unpacking() { asm volatile("" : "+v"(low), "+v"(high)); }
+};
+__device__ __forceinline__ void weights32(const Unpacking& by, const uint4& w, uint32_t z, half2p_t (&out)[16])
 {
-    const uint32_t magic = opaque_scalar(BF16 ? 0x43004300u : 0x64006400u);
     uint32_t d[4] = {w.x, w.y, w.z, w.w};
     // unpacked for each row anew: kept for the next row, the nibbles of a wave's columns take 128 registers
     asm volatile("" : "+v"(d[0]), "+v"(d[1]), "+v"(d[2]), "+v"(d[3]));
+    // -(1024 + z) and -(64 + z): f16's steps there are 1 and 1/16
+    const half2p_t off = __builtin_bit_cast(half2p_t, 0xE400E400u + z * 0x00010001u), off_high = __builtin_bit_cast(half2p_t, 0xD400D400u + z * 0x00100010u);
+    const half2p_t sixteenth = __builtin_bit_cast(half2p_t, 0x2C002C00u);
+    auto pair = [&](uint32_t bits, uint32_t mask) { return __builtin_bit_cast(half2p_t, (bits & mask) | by.magic); };
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) out[4 * j + i] = ((d[j] >> (4 * i)) & mask) | magic;
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t upper = d[j] >> 8;
+        out[4 * j] = pair(d[j], by.low) + off;
+        out[4 * j + 1] = __builtin_elementwise_fma(pair(d[j], by.high), sixteenth, off_high);
+        out[4 * j + 2] = pair(upper, by.low) + off;
+        out[4 * j + 3] = __builtin_elementwise_fma(pair(upper, by.high), sixteenth, off_high);
+    }
 }
 
-// start + sum a (magic + q), in four chains
-template <bool BF16>
-__device__ __forceinline__ float dot32(const uint32_t (&a)[16], const uint32_t (&b)[16], float start)
-{
-    float s[4] = {start, 0.f, 0.f, 0.f};
+// A row's 32 elements as they are multiplied, and their product with 32 weights, in four chains. f16: dot products of two, for each part of a value.
+template <bool BF16, int NH>
+struct Factors32 {
+    uint32_t v[NH][16];
+    __device__ __forceinline__ explicit Factors32(const Elements32 (&a)[NH])
+    {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i & 3] = dot2<BF16>(a[i], b[i], s[i & 3]);
-    return (s[0] + s[1]) + (s[2] + s[3]);
-}
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[h][i] = a[h].v[i];
+    }
+    __device__ __forceinline__ float dot(const half2p_t (&q)[16]) const
+    {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i & 3] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2p_t, v[h][i]), q[i], s[i & 3], false);
+        return (s[0] + s[1]) + (s[2] + s[3]);
+    }
+};
+// bf16: in f32, the parts of a value joined, with the f16 weights in mixed-precision multiply-adds. (Weights widened to bf16 for dot products of two take a quarter
+// more instructions: one token of 8 of 64 experts 19.3 us, 18.4 so.)
+template <int NH>
+struct Factors32<true, NH> {
+    float v[32];
+    __device__ __forceinline__ explicit Factors32(const Elements32 (&a)[NH])
+    {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            v[2 * i] = __uint_as_float(a[0].v[i] << 16);
+            v[2 * i + 1] = __uint_as_float(a[0].v[i] & 0xffff0000u);
+            if constexpr (NH == 2) {
+                v[2 * i] += __uint_as_float(a[1].v[i] << 16);
+                v[2 * i + 1] += __uint_as_float(a[1].v[i] & 0xffff0000u);
+            }
+        }
+    }
+    __device__ __forceinline__ float dot(const half2p_t (&q)[16]) const
+    {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i & 1] = fmaf(static_cast<float>(q[i].x), v[2 * i], s[i & 1]);
+            s[2 + (i & 1)] = fmaf(static_cast<float>(q[i].y), v[2 * i + 1], s[2 + (i & 1)]);
+        }
+        return (s[0] + s[1]) + (s[2] + s[3]);
+    }
+};
 
 // The weights of NU times 64 / LPC columns: load u has column n0 + u (64 / LPC) + lane / LPC, bytes 16 (lane % LPC) on from a pass's begin.
 template <typename ST, bool ZP, int NU, int LPC>
@@ -138,23 +170,13 @@ struct FewColumns {
 
 // acc[u] += factor * scale * sum a (q - zp) for NH parts of a row
 template <bool BF16, typename ST, bool ZP, int NU, int LPC, int NH>
-__device__ __forceinline__ void few_multiply(const FewColumns<ST, ZP, NU, LPC>& c, const Elements32<BF16> (&a)[NH], int odd, float factor, float (&acc)[NU])
+__device__ __forceinline__ void few_multiply(const Unpacking& by, const FewColumns<ST, ZP, NU, LPC>& c, const Factors32<BF16, NH>& a, int odd, float factor, float (&acc)[NU])
 {
-    constexpr float kMagic = BF16 ? 128.f : 1024.f;
-    float sum = a[0].sum;
-    if constexpr (NH == 2) sum += a[1].sum;
-    const float plain = -(kMagic + 8.f) * sum;
-    uint32_t mask = 0x000f000fu;
-    asm volatile("" : "+v"(mask));
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-        uint32_t q[16];
-        nibbles32<BF16>(c.w[u], mask, q);
-        float start = plain;
-        if constexpr (ZP) start = (-kMagic - static_cast<float>((c.z[u] >> odd) & 15u)) * sum;
-        float d = dot32<BF16>(a[0].v, q, start);
-        if constexpr (NH == 2) d += dot32<BF16>(a[1].v, q, 0.f);
-        acc[u] = fmaf(factor * ScaleIo<ST>::to_f32(c.s[u], BF16), d, acc[u]);
+        half2p_t q[16];
+        weights32(by, c.w[u], ZP ? (c.z[u] >> odd) & 15u : 8u, q);
+        acc[u] = fmaf(factor * ScaleIo<ST>::to_f32(c.s[u], BF16), a.dot(q), acc[u]);
     }
 }
 
@@ -198,7 +220,7 @@ __global__ __launch_bounds__(256) void moe_few_up_kernel(MOE_FEW_FIRST, MoeUpCal
         for (unsigned piece = threadIdx.x; piece < pieces; piece += 256) {
             const unsigned l = piece / 4;
             const uint4 d = piece * 8 < static_cast<unsigned>(width) ? *reinterpret_cast<const uint4*>(x + static_cast<int64_t>(t) * width + piece * 8) : make_uint4(0, 0, 0, 0);
-            staged[((t * passes + l / LPC) * 4 + piece % 4) * LPC + l % LPC] = Elements32<BF16>::ordered(d);
+            staged[((t * passes + l / LPC) * 4 + piece % 4) * LPC + l % LPC] = Elements32::ordered(d);
         }
     if (ranks) rank_few(routing, logit, rows, experts, k, normalize);
     else route_few<4>(routing, logits, logits_dtype, rows, experts, k, normalize);
@@ -213,6 +235,7 @@ __global__ __launch_bounds__(256) void moe_few_up_kernel(MOE_FEW_FIRST, MoeUpCal
         __syncthreads();
     }
 
+    const Unpacking by;
     const int shift = 31 - __builtin_clz(p.m.block_size);
     MoeMatrix up = p.m;
     up.w[0] = p.m.w[1];
@@ -254,12 +277,12 @@ __global__ __launch_bounds__(256) void moe_few_up_kernel(MOE_FEW_FIRST, MoeUpCal
 #pragma unroll
         for (int t = 0; t < kFewRows; ++t) {
             if (!(chose >> t & 1)) continue;
-            Elements32<BF16> a[1];
+            Elements32 a[1];
 #pragma unroll
             for (int j = 0; j < 4; ++j) a[0].put(j, staged[((t * passes + pass) * 4 + j) * LPC + kl]);
-            a[0].add_up();
-            few_multiply<BF16, ST, ZP, NU, LPC, 1>(of_g, a, odd, 1.f, g[t]);
-            few_multiply<BF16, ST, ZP, NU, LPC, 1>(of_u, a, odd, 1.f, u[t]);
+            const Factors32<BF16, 1> factors(a);
+            few_multiply<BF16, ST, ZP, NU, LPC, 1>(by, of_g, factors, odd, 1.f, g[t]);
+            few_multiply<BF16, ST, ZP, NU, LPC, 1>(by, of_u, factors, odd, 1.f, u[t]);
         }
         if (pass != static_cast<int>(passes) - 1) return next(now);
         // the tile's sums; lane i of a column's lanes keeps column i's
@@ -302,7 +325,7 @@ __global__ __launch_bounds__(512) void moe_few_down_kernel(const MoeFewTable* ta
     constexpr int NU = LPC / 8, kCols = 8, kPass = LPC * 32;
     struct Item {
         FewColumns<ST, ZP, NU, LPC> c;
-        Elements32<BF16> a[2];
+        Elements32 a[2];
     };
     __shared__ float sums[8][kFewRows][kCols];
     __shared__ float weight[kFewPairs][kFewRows];
@@ -314,6 +337,7 @@ __global__ __launch_bounds__(512) void moe_few_down_kernel(const MoeFewTable* ta
     for (int i = threadIdx.x; i < slots; i += blockDim.x) chosen[i] = table->expert[i];
     const int active = table->active;
     __syncthreads();
+    const Unpacking by;
     const int n0 = static_cast<int>(blockIdx.x) * kCols, live = min(p.m.n - n0, kCols);
     const int shift = 31 - __builtin_clz(p.m.block_size), width = static_cast<int>(p.ip), passes = static_cast<int>(static_cast<unsigned>(width + kPass - 1) / kPass);
     struct Place {
@@ -334,7 +358,7 @@ __global__ __launch_bounds__(512) void moe_few_down_kernel(const MoeFewTable* ta
         while (t < kFewRows - 1 && !(weight[slot][t] > 0.f)) ++t;
         return __builtin_amdgcn_readfirstlane(t);
     };
-    auto rows_of = [&](int slot, int t, int at, Elements32<BF16> (&a)[2]) {
+    auto rows_of = [&](int slot, int t, int at, Elements32 (&a)[2]) {
         const uint16_t* const h = p.h + (static_cast<int64_t>(slot) * kFewRows + t) * (2 * p.ip) + at;
         a[0].load(h, width - at);
         a[1].load(h + p.ip, width - at);
@@ -358,7 +382,7 @@ __global__ __launch_bounds__(512) void moe_few_down_kernel(const MoeFewTable* ta
             if (t != first) rows_of(slot, t, at, of.a);
             of.a[0].order();
             of.a[1].order();
-            few_multiply<BF16, ST, ZP, NU, LPC, 2>(of.c, of.a, odd, w, acc[t]);
+            few_multiply<BF16, ST, ZP, NU, LPC, 2>(by, of.c, Factors32<BF16, 2>(of.a), odd, w, acc[t]);
         }
     };
     if (now.slot < active) {
