@@ -320,7 +320,7 @@ void nxrt_rocm_ep_graph_release(NxrtRocmEp* ep, NxrtRocmGraph* graph);
 /* Counters a harness reads to prove the provider, not a fallback, did the work
  * (the role of nxrt_ep_compiled_node_count in ep-cuda-plugin/src/lib.rs:345-372). */
 /* Counts the steps of calls that were run or recorded: one for a product, with all that it takes (quantized rows, expanded weights,
- * blocks of rows, slices of K), and one for each normalization, gather of act-order rows and SwiGLU epilogue beside it. A recorded
+ * blocks of rows, slices of K), one for each normalization, gather of act-order rows and SwiGLU epilogue beside it, and one for a call of a node. A recorded
  * call counts the same whether it is a launch of its own or shares one; replays do not count. */
 uint64_t nxrt_rocm_ep_kernel_launch_count(const NxrtRocmEp* ep);
 uint64_t nxrt_rocm_live_provider_count(void);

@@ -544,7 +544,6 @@ struct Int8Node final : NxrtRocmNode {
             args.a_float = at(*a);
         } else {
             if (rc == 0) rc = rocm_launch_quantize_rows(at(*a), static_cast<int>(a->dtype), args.m, s.k, reinterpret_cast<int8_t*>(w + l.codes), reinterpret_cast<float*>(w + l.scales), ep->stream);
-            ep->launches.fetch_add(1);
             args.a = reinterpret_cast<const int8_t*>(w + l.codes);
             args.a_scale = reinterpret_cast<const float*>(w + l.scales);
         }

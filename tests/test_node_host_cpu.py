@@ -1,0 +1,39 @@
+"""What the operators beside MatMulNBits keep to on the host: counted steps, scratch, reasons. The GPU's functions are stood for."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from onnx_genai_amd import ep as E
+
+from .test_allocation_failure_cpu import host_only  # noqa: F401  (the fixture: the library's host sources without a GPU)
+
+HOLD = np.zeros(1 << 20, np.uint8)
+NONE = E.TensorView.absent()
+
+
+def view(dtype, shape, at=0):
+    return E.TensorView((HOLD.ctypes.data + 255) // 256 * 256 + at, dtype, shape)
+
+
+@pytest.fixture
+def provider(host_only):  # noqa: F811
+    p = E.RocmExecutionProvider(0)
+    yield p
+    p.shutdown()
+
+
+def int8_call(rows, dtype=E.F16, k=32):
+    scale = [view(E.F32, (rows,), 1 << 17)] if dtype == E.I8 else []
+    return [view(dtype, (rows, k)), view(E.I8, (8, k), 1 << 18), view(E.F32, (8,), 1 << 19)] + scale, [view(E.F16, (rows, 8), 3 << 18)]
+
+
+@pytest.mark.parametrize("dtype", [E.F16, E.F32, E.I8])
+@pytest.mark.parametrize("rows,k", [(1, 32), (3, 33), (40, 32), (500, 33)])
+def test_a_product_is_one_step(provider, rows, k, dtype):
+    """One for a product with all that it takes: quantized rows, padded rows, slices of K."""
+    kernel = provider.get_kernel({"K": k, "N": 8}, op_type="MatMulInt8")
+    before = provider.kernel_launch_count()
+    kernel.execute(*int8_call(rows, dtype, k))
+    assert provider.kernel_launch_count() == before + 1
+    kernel.release()
