@@ -227,9 +227,10 @@ uint64_t nxrt_rocm_matmul_nbits_retired_buffers(const NxrtRocmMatMulNBits* kerne
 /* ---- operators beside MatMulNBits: what stands between the quantized products of a decoder layer ---- */
 
 /* One node of one of the operators below. The contract is that of a MatMulNBits kernel: tensors contiguous and on the provider's GPU, an absent optional
- * tensor has data = NULL, calls run on the provider's stream in call order, one call at a time per node. No node copies or remembers its weights. Outputs may not overlap inputs unless said so. A node
- * keeps a reference on its provider. Calls may be recorded into a graph; a call that needs scratch takes the caller's workspace or the node's own,
- * which an eager call of that height has to have made before (nothing is allocated while a capture is open). Outgrown scratch stays until the node is released. */
+ * tensor has data = NULL, calls run on the provider's stream in call order, one call at a time per node. No node copies or remembers its weights. Outputs may not
+ * overlap inputs unless said so. A node keeps a reference on its provider. Calls may be recorded into a graph; a call that needs scratch takes the caller's workspace
+ * or the node's own, which an eager call of that height has to have made before (nothing is allocated while a capture is open). Outgrown scratch of the node's own is
+ * freed while the provider has opened no capture yet; from then on, since a graph may name it, it stays until the node is released. */
 typedef struct NxrtRocmNode NxrtRocmNode;
 
 /* com.microsoft::QMoE with activation_type "swiglu" (or "silu" with fc3): a mixture-of-experts layer over 4-bit weights, from router logits to the weighted sum.

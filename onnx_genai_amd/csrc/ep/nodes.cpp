@@ -236,6 +236,21 @@ struct NxrtRocmNode {
 
     std::string err(const std::string& m) const { return std::string(op()) + ": " + m; }
 
+    // Once the provider has recorded a graph, one may name the scratch, and it stays until the node is released. Before that it is freed when the stream has drained: a
+    // host whose prompts grow holds one scratch a node, not one a length.
+    void drop_scratch()
+    {
+        if (!scratch) return;
+        if (ep->captures.load() != 0) {
+            retired.push_back(scratch);
+        } else {
+            rocm_ffi_stream_sync(ep->stream);
+            rocm_ffi_free(scratch);
+        }
+        scratch = nullptr;
+        scratch_bytes = 0;
+    }
+
     // `need` bytes for this call: the caller's, or the node's own, grown where that may be.
     NxrtStatus find_scratch(uint64_t need, void* ws, uint64_t ws_bytes, void** out)
     {
@@ -253,7 +268,7 @@ struct NxrtRocmNode {
             void* fresh = nullptr;
             const int e = rocm_ffi_malloc(&fresh, need);
             if (e != 0) return hip_status(e, "workspace hipMalloc");
-            if (scratch) retired.push_back(scratch);
+            drop_scratch();
             scratch = fresh;
             scratch_bytes = need;
         }

@@ -37,3 +37,17 @@ def test_a_product_is_one_step(provider, rows, k, dtype):
     kernel.execute(*int8_call(rows, dtype, k))
     assert provider.kernel_launch_count() == before + 1
     kernel.release()
+
+
+def test_outgrown_scratch_is_freed_until_a_capture_was_opened(provider):
+    """Calls of growing length, as prompts are: while no graph can name the scratch, a node has one."""
+    kernel = provider.get_kernel({"K": 32, "N": 8}, op_type="MatMulInt8")
+    for rows in (4, 40, 400, 1000):
+        kernel.execute(*int8_call(rows))
+        assert kernel.retired_buffers() == 0
+    provider.capture_begin()
+    kernel.execute(*int8_call(1000))
+    provider.capture_end()
+    kernel.execute(*int8_call(2000))
+    assert kernel.retired_buffers() == 1                     # what the recorded call names
+    kernel.release()
