@@ -759,6 +759,7 @@ NxrtStatus create_node(const char* op, NxrtRocmEp* ep, const Attrs* attrs, NxrtR
 template <typename F>
 int supported(const char* op, char* reason, size_t reason_len, F&& problem) noexcept
 {
+    if (reason && reason_len) reason[0] = 0;
     try {
         const std::string why = problem();
         return why.empty() ? 1 : decline(std::string(op) + ": " + why, reason, reason_len);

@@ -51,3 +51,13 @@ def test_outgrown_scratch_is_freed_until_a_capture_was_opened(provider):
     kernel.execute(*int8_call(2000))
     assert kernel.retired_buffers() == 1                     # what the recorded call names
     kernel.release()
+
+
+@pytest.mark.parametrize("op_type,attrs", [("QMoE", {"k": 2, "block_size": 32}), ("MatMulInt8", {"K": 32, "N": 8}), ("GatedResidualNorm", {})])
+def test_no_reason_where_a_node_is_supported(provider, op_type, attrs):
+    """What the caller's buffer held before is no reason."""
+    a = E.make_node_attrs(op_type, attrs)
+    supports = getattr(provider.lib, f"nxrt_rocm_ep_supports_{E._NODE_OPS[op_type][1]}")
+    reason = C.create_string_buffer(b"left from before", 64)
+    assert supports(provider.handle, C.byref(a), None, 0, reason, 64) == 1 and reason.value == b""
+    assert supports(provider.handle, C.byref(a), None, 0, None, 0) == 1
