@@ -233,7 +233,8 @@ uint64_t nxrt_rocm_matmul_nbits_retired_buffers(const NxrtRocmMatMulNBits* kerne
  * freed while the provider has opened no capture yet; from then on, since a graph may name it, it stays until the node is released. */
 typedef struct NxrtRocmNode NxrtRocmNode;
 
-/* com.microsoft::QMoE with activation_type "swiglu" (or "silu" with fc3): a mixture-of-experts layer over 4-bit weights, from router logits to the weighted sum.
+/* com.microsoft::QMoE with activation_type "swiglu" (or "silu" with fc3; the struct has no activation_type: a host keeps nodes with another one, or with none, whose
+ * default is "relu", to itself): a mixture-of-experts layer over 4-bit weights, from router logits to the weighted sum.
  *   inputs: 0 input [.., H] Float16 / BFloat16; 1 router_probs [.., E] logits of any float type; 2 fc1_experts_weights [E, F, kb, block_size / 2] (or
  *           [E, F, kb * block_size / 2]) Uint8, 3 fc1_scales [E, F, kb], 4 fc1_experts_bias [E, F] or absent; 5, 6, 7 the same of fc2 ([E, H, ..] over I);
  *           8, 9, 10 of fc3 or absent; 11, 12, 13 zero points [E, F, ceil(kb / 2)] of fc1, fc2, fc3 or absent (8; fc1's come with fc3's).
@@ -242,8 +243,11 @@ typedef struct NxrtRocmNode NxrtRocmNode;
  *   swiglu_fusion 1: F = 2 I, gate and up rows alternate; 2: I gate rows, then I up rows; 0: F = I, gate in fc1 and up in fc3.
  * For token t: p = softmax(logits); S = the k experts of the largest logits, the lowest index first among equal ones, without those whose p is 0; w = p, or p over
  * its sum on S with normalize_routing_weights. h = g sigmoid(activation_alpha g) (u + activation_beta), g <= swiglu_limit, |u| <= swiglu_limit (g, u: the
- * products with bias), rounded to the input's type; y = sum over S of w (fc2 h + bias), summed in f32. A row whose logits are all -inf (padding) gives zeros and
- * reads no expert; a NaN or +inf among a row's logits gives NaN. An infinity or NaN in a row of `input` gives no finite value in that row.
+ * products with bias); y = sum over S of w (fc2 h + bias), summed in f32 and rounded once. With more than four tokens h is rounded to the input's type in between, and
+ * y's error is then about 1.4 times its own rounding's; with up to four tokens (and up to 256 experts, 128 choices in all and rows * ceil(H / 2048) <= 12) h keeps
+ * twice that type's bits, so that a token alone and the same token in a larger call may differ in their last bits. With Float16 an h beyond 65504 is an infinity
+ * in either. A row whose logits are all -inf (padding) gives zeros and reads no expert; a NaN or +inf among a row's logits gives NaN. An infinity or NaN in a row
+ * of `input` gives no finite value in that row, unless swiglu_limit takes each infinity back that comes of it.
  * Weights are exact (q - zp) * scale. block_size: a power of two >= 32. E <= 1024, k <= 64. Weights start at multiples of 16 bytes. */
 typedef struct NxrtRocmQMoEAttrs {
   uint32_t struct_size;
@@ -288,7 +292,7 @@ int nxrt_rocm_ep_supports_gated_residual_norm(const NxrtRocmEp* ep, const NxrtRo
                                               size_t reason_len);
 NxrtStatus nxrt_rocm_gated_residual_norm_create(NxrtRocmEp* ep, const NxrtRocmGatedResidualNormAttrs* attrs, NxrtRocmNode** out_node);
 
-/* As the functions of the same names for MatMulNBits. */
+/* As the functions of the same names for MatMulNBits; but which inputs are constant makes no difference to a node, which reads its weights as they are in each call. */
 void nxrt_rocm_node_set_constant_inputs(NxrtRocmNode* node, const uint8_t* is_constant, uint32_t n);
 NxrtStatus nxrt_rocm_node_workspace_requirement(const NxrtRocmNode* node, const NxrtTensorDesc* inputs, uint32_t n_inputs, NxrtRocmWorkspaceRequirement* out);
 NxrtStatus nxrt_rocm_node_execute(NxrtRocmNode* node, const NxrtRocmTensorView* inputs, uint32_t n_inputs, NxrtRocmTensorView* outputs, uint32_t n_outputs,

@@ -213,7 +213,6 @@ struct NxrtRocmNode {
     NxrtRocmEp* ep;
     std::mutex mu;                         // one call at a time: scratch, copies and variant are per node
     const char* variant = "none";
-    bool constant[kMaxInputs] = {};        // (no node copies its weights: what the host says is only kept)
     void* scratch = nullptr;
     uint64_t scratch_bytes = 0;
     std::vector<void*> retired;            // outgrown scratch that a recorded graph may still name
@@ -828,12 +827,7 @@ NxrtStatus nxrt_rocm_gated_residual_norm_create(NxrtRocmEp* ep, const NxrtRocmGa
     return create_node<GatedNormNode>("GatedResidualNorm", ep, attrs, out_node);
 }
 
-void nxrt_rocm_node_set_constant_inputs(NxrtRocmNode* node, const uint8_t* is_constant, uint32_t n)
-{
-    if (!node) return;
-    std::lock_guard<std::mutex> lock(node->mu);
-    for (uint32_t i = 0; i < kMaxInputs; ++i) node->constant[i] = is_constant && i < n && is_constant[i] != 0;
-}
+void nxrt_rocm_node_set_constant_inputs(NxrtRocmNode*, const uint8_t*, uint32_t) {}        // (no node copies its weights)
 
 NxrtStatus nxrt_rocm_node_workspace_requirement(const NxrtRocmNode* node, const NxrtTensorDesc* inputs, uint32_t n_inputs, NxrtRocmWorkspaceRequirement* out)
 {
