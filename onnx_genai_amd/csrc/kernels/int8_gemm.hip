@@ -136,8 +136,8 @@ __device__ __forceinline__ void store_scaled(const Int8Params& p, int64_t row, i
 // bytes as 16 columns). Two steps' loads are in flight.
 // FUSED (up to three rows of at most 32 KiB of codes): a is [m, k] of type T, and every workgroup makes the codes for itself, in LDS, while its first weights are on
 // their way: a launch of its own takes longer than a row's second and third trip from L2.
-// Measured: one row of 4096 -> 6144 with the quantizer inside 8.1 us (25 MB: 3.1 TB/s, an empty launch is 2 of them), 8 rows of 4096 -> 28672 23.5 us (5.0 TB/s),
-// 24 rows of 4096 -> 12288 13.7 us (3.7 TB/s).
+// Measured: one row of 4096 -> 6144 with the quantizer inside 8.2 us, three sets of operands in turn (25 MB: 3.1 TB/s, an empty launch is 2 of them); the same operands
+// each time, which the last-level cache then holds, 8 rows of 4096 -> 28672 23.5 us (5.0 TB/s), 24 rows of 4096 -> 12288 13.7 us (3.7 TB/s).
 template <int RT, int CT, typename T, bool BF16, bool FUSED>
 __global__ __launch_bounds__(512) void int8_rows_kernel(const int8_t* b_base, const void* a_base, int m, int n, int k, int steps, Int8Params p)
 {
@@ -600,7 +600,8 @@ Int8Plan plan_of(const RocmInt8Args& a)
     }
     return p;
 }
-// Whether the product quantizes its rows itself. us with and without, 4096 -> 6144: 1 row 6.7 and 8.9, 2 7.7 and 9.2, 3 8.5 and 9.3, 4 9.5 and 9.4; 4096 -> 14336: 1 row 11.8
+// Whether the product quantizes its rows itself. us of a call among others on the same operands (in the last-level cache: less than the kernel takes on others), with
+// and without, 4096 -> 6144: 1 row 6.7 and 8.9, 2 7.7 and 9.2, 3 8.5 and 9.3, 4 9.5 and 9.4; 4096 -> 14336: 1 row 11.8
 // and 15.0, 3 15.3 and 15.1, 4 17.0 and 15.8.
 bool fuses(const RocmInt8Args& a) { return a.m <= 3 && (a.a_dtype == ROCM_DT_F16 || a.a_dtype == ROCM_DT_BF16) && a.m * ((a.k + 127) / 128 * 128) <= 32768; }
 

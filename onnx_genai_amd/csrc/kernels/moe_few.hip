@@ -8,8 +8,8 @@
 // bf16 in f32 by 32 mixed-precision multiply-adds (v_fma_mix_f32). A weight enters as the f16 q - zp, which is exact, so that one of zero adds nothing however large its x
 // is. (As magic + q, with -(magic + zp) times the sum of x in front, a pair of weights takes one instruction less in f16 and two in bf16, and what is left of magic * x
 // shows: an x of 60000 at weights of zero put y off by 15 %. One token 17.7 us and 18.4 now, three tokens of 4096 and 14336 131 and 133.)
-// Measured: one token, 8 of 64 experts of 2048 and 1024 in bf16, 10.7 us up and 7.2 down (28 MB; an empty launch is 2 us, and routing 3 more before the first weights),
-// three tokens of 4096 and 14336 over 8 experts in f16 with zero points 78 and 58 us (3.9 and 2.6 TB/s).
+// Measured: one token, 8 of 64 experts of 2048 and 1024 in bf16, 12.6 us up and 7.4 down (28 MB; an empty launch is 2 us, and routing 3 more before the first weights),
+// three tokens of 4096 and 14336 over 8 experts in f16 with zero points 82 and 58 us (3.8 and 2.7 TB/s).
 // LPC lanes stand side by side on K and read 16 LPC bytes of a column's row as the caller holds it; 64 / LPC columns are read at once.
 #include "moe_route.hiph"
 

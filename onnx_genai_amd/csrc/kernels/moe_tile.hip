@@ -3,11 +3,12 @@
 // A wave has all rows of the tile and 32 columns of weights that no other wave has (16 of gate beside 16 of up), so that it unpacks them for itself, from
 // registers into the matrix core; only activations go through LDS, in the order in which a dword's nibbles come out (0 4 1 5 2 6 3 7 of each eight).
 // Weights enter the matrix core as q - zp, which is exact in 16 bits, and each block's sum is scaled in f32: no weight is rounded.
-// TM = 4 (prompts): the matrix cores and the vector instructions beside them bound it, 64 to scale a block's sums and 44 (bf16: 76) to
-// unpack 64 k for 512 cycles of products. TM = 1 (a few rows an expert): the weights' bytes, and a CU's path to memory, where 64 columns' scales take as long as
+// TM = 4 (prompts): 64 vector instructions scale a block's sums and 44 (bf16: 76) unpack 64 k beside 512 cycles of products. Neither unit is at its limit: of the SIMDs'
+// cycles vector instructions take 59 % up and 47 % down in bf16 with blocks of 128, products 39 and 34 %; in f16 with blocks of 32, 63 and 53 %, 32 and 29 %. The shares
+// add up to 81 to 98 %: two waves a SIMD, which meet at a barrier every 64 k, overlap the two little. TM = 1 (a few rows an expert): the weights' bytes, and a CU's path to memory, where 64 columns' scales take as long as
 // their weights.
 // Measured: TM = 1, 48 tokens of 8 out of 64 experts of 2048 and 1024, blocks of 64, 52 us up and 28 down (2.7 TB/s); TM = 4, 4096 tokens of those, blocks of 128, 405 us
-// up and 222 down (0.68 and 0.62 PFLOP/s; vector and matrix instructions together fill the issue slots, at 2.0 GHz), 777 tokens of 4 out of 16 experts of 2880, f16,
+// up and 222 down (0.68 and 0.62 PFLOP/s at 1.9 GHz), 777 tokens of 4 out of 16 experts of 2880, f16,
 // blocks of 32, 230 us up and 121 down (0.45 and 0.43 PFLOP/s; its tiles are 128 and 66 rows, a quarter of them absent). With a step's reads and unpacking in front of
 // its products, as the compiler places them, those were 414, 223, 252 and 142.
 // Weights rounded to 16 bits before the product save the scaling and half of the accumulators, so that a wave has 64 columns (777 tokens: 191 us up and 124 down; 4096
