@@ -75,7 +75,8 @@ typedef struct NxrtNegotiateResponse {
 enum { NXRT_DEVICE_CPU = 0, NXRT_DEVICE_CUDA = 1, NXRT_DEVICE_ROCM = 2 };
 
 /* onnx-runtime-ir/src/dtype.rs:9-37 — element types on the wire */
-enum { NXRT_DT_FLOAT32 = 1, NXRT_DT_UINT8 = 2, NXRT_DT_INT8 = 3, NXRT_DT_INT32 = 6, NXRT_DT_FLOAT16 = 10, NXRT_DT_BFLOAT16 = 16 };
+enum { NXRT_DT_FLOAT32 = 1, NXRT_DT_UINT8 = 2, NXRT_DT_INT8 = 3, NXRT_DT_INT32 = 6, NXRT_DT_INT64 = 7, NXRT_DT_FLOAT16 = 10, NXRT_DT_BFLOAT16 = 16,
+       NXRT_DT_FLOAT8E4M3FN = 17 };
 
 /* vtable.rs:55-66 */
 typedef struct NxrtTensorDesc {
