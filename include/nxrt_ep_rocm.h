@@ -292,6 +292,92 @@ int nxrt_rocm_ep_supports_gated_residual_norm(const NxrtRocmEp* ep, const NxrtRo
                                               size_t reason_len);
 NxrtStatus nxrt_rocm_gated_residual_norm_create(NxrtRocmEp* ep, const NxrtRocmGatedResidualNormAttrs* attrs, NxrtRocmNode** out_node);
 
+/* ---- a paged 8-bit cache of keys and values, from the qkv product to the o product ----
+ *
+ * One layer's cache: k_cache [P, KV, B, D] and v_cache [P, KV, D, B] of Int8 or Float8E4M3FN codes (both alike), k_scale and v_scale [P, KV] Float32, not negative. A page
+ * holds B tokens (16, 32, 64 or 128) of each of KV heads of D elements; the value of a code is code * scale of its page and head. Of the values a page holds
+ * the tokens of one element side by side.
+ * A call's new tokens are rows, T in all, those of a sequence behind one another: cumulative_lengths [N + 1] Int32, the first 0, sequence b has rows
+ * cumulative_lengths[b] up to cumulative_lengths[b + 1]; rows behind the last sequence belong to none. past_lengths [N] Int32: tokens of a sequence in front of them.
+ * block_table [N, W] Int32: token t of sequence b is slot t % B of page block_table[b, t / B].
+ * What these tensors hold is read on the GPU and not reported: lengths are taken into 0 .. T, past lengths into 0 .. W B, and a page outside 0 .. P - 1 holds no tokens.
+ * D: 64, 80, 96, 128 or 256 for CacheAttention, a multiple of 16 up to 256 for CacheAppend. W B < 2^30. */
+
+/* com.microsoft::RotaryEmbedding: pairs of a head's elements turned by their row's position.
+ *   inputs: 0 input [.., C] Float32 / Float16 / BFloat16, the heads of a row side by side; or, with rank 4, [N, H, S, D]; 1 position_ids Int64 / Int32, one for each row (of
+ *           rank 4: [N, S]), or one element, the position of the first row of each sequence (the last dimension but one counts its rows); 2 cos_cache, 3 sin_cache [M, R / 2]
+ *           of any float type, or both absent.
+ *   output: of the input's shape and type; it may be written over the input.
+ * D = head_size. The first num_heads heads of a row turn (0: all of C, which D then divides), what lies behind them passes through: packed queries, keys and values. R =
+ * rotary_embedding_dim (0: D), even, up to 512: elements of a head that turn; pairs (i, i + R / 2), or (2 i, 2 i + 1) with interleaved.
+ *   a' = a c - b s, b' = b c + a s; c, s = row position of the caches (a position that they do not have gives NaN), or magnitude * cos, sin(position * f_i) in 64 bits:
+ *   f_i = rope_theta^(-2 i / R); scaling 1 (linear): f_i / factor; 2 (llama3): f_i / factor below low_freq_factor turns within original_max_position, f_i above
+ *   high_freq_factor, in between a blend by turns; 3 (yarn): f_i / factor below beta_slow turns, f_i above beta_fast, in between a blend by pairs; magnitude =
+ *   attention_factor, by default 1, with yarn 0.1 ln(factor) + 1. Positions are exact up to 2^53. In f32, rounded once. */
+typedef struct NxrtRocmRotaryEmbeddingAttrs {
+  uint32_t struct_size;
+  uint32_t present;      /* bit i: 0 head_size (required), 1 num_heads (0), 2 rotary_embedding_dim (0), 3 interleaved (0), 4 scaling (0), 5 original_max_position (8192),
+                            6 rope_theta (10000), 7 factor (1), 8 low_freq_factor (1), 9 high_freq_factor (4), 10 beta_fast (32), 11 beta_slow (1), 12 attention_factor */
+  int64_t head_size, num_heads, rotary_embedding_dim, interleaved, scaling, original_max_position;
+  double rope_theta, factor, low_freq_factor, high_freq_factor, beta_fast, beta_slow, attention_factor;
+} NxrtRocmRotaryEmbeddingAttrs;
+int nxrt_rocm_ep_supports_rotary_embedding(const NxrtRocmEp* ep, const NxrtRocmRotaryEmbeddingAttrs* attrs, const NxrtTensorDesc* inputs, uint32_t n_inputs, char* reason,
+                                           size_t reason_len);
+NxrtStatus nxrt_rocm_rotary_embedding_create(NxrtRocmEp* ep, const NxrtRocmRotaryEmbeddingAttrs* attrs, NxrtRocmNode** out_node);
+
+/* CacheAppend: new tokens' keys and values into their pages.
+ *   inputs: 0 key [T, KV D] of a float type, 1 value of the same shape and type; or 0 packed rows [T, (num_heads + 2 KV) D], queries, keys, values, and 1 absent;
+ *           2 k_cache, 3 v_cache, 4 k_scale, 5 v_scale, 6 cumulative_lengths, 7 past_lengths, 8 block_table.
+ *   outputs: 0 k_cache, 1 v_cache, 2 k_scale, 3 v_scale: the inputs' own tensors, changed where they are.
+ * A page whose first token is new gets scale = max|x| / top over its new tokens (top: 127, or 448), code = x / scale to the nearest, ties to even; a scale of 0 gives codes
+ * 0. A page that has tokens gets scale' = max(scale, max|x| / top), and where that is larger, its codes become code * (scale / scale') to the nearest: each such
+ * step adds up to half a step of rounding to the tokens before. An infinity or a NaN makes the scale NaN and the new codes 0 (and those before), until the page begins
+ * again. Slots that no token has are left as they are. Two sequences may share pages, but not one that a call writes. */
+typedef struct NxrtRocmCacheAppendAttrs {
+  uint32_t struct_size;
+  uint32_t present;      /* bit i: 0 num_heads (0; read for packed rows), 1 kv_num_heads (required), 2 head_size (required) */
+  int64_t num_heads, kv_num_heads, head_size;
+} NxrtRocmCacheAppendAttrs;
+int nxrt_rocm_ep_supports_cache_append(const NxrtRocmEp* ep, const NxrtRocmCacheAppendAttrs* attrs, const NxrtTensorDesc* inputs, uint32_t n_inputs, char* reason, size_t reason_len);
+NxrtStatus nxrt_rocm_cache_append_create(NxrtRocmEp* ep, const NxrtRocmCacheAppendAttrs* attrs, NxrtRocmNode** out_node);
+
+/* CacheAttention: attention of the new tokens over their sequences' pages, which hold them already (CacheAppend goes before).
+ *   inputs: 0 query [T, num_heads D] Float16 / BFloat16, or packed rows [T, (num_heads + 2 KV) D], whose first columns are read; 1 k_cache, 2 v_cache, 3 k_scale, 4 v_scale,
+ *           5 cumulative_lengths, 6 past_lengths, 7 block_table.
+ *   output: [T, num_heads D] of the query's type; rows of no sequence are left as they are.
+ * Head h reads key head h / (num_heads / KV). New token i of sequence b sees slots t <= past_lengths[b] + i, with local_window_size the last so many of them (itself is one):
+ *   y = softmax(z) v,  z = scale (q . k), with softcap  softcap tanh(z / softcap);  scale 0 (the default): 1 / sqrt(D).
+ * A row that sees no slot is zero. Products, softmax and sums in f32 over f16 operands: codes exact, queries to 2^-22 of their row's largest, weights rounded to 11 bits. A page
+ * of scale NaN gives NaN to the rows that see it, and to no other; a NaN code of Float8E4M3FN (CacheAppend makes none) may reach rows that do not see its slot. */
+typedef struct NxrtRocmCacheAttentionAttrs {
+  uint32_t struct_size;
+  uint32_t present;      /* bit i: 0 num_heads, 1 kv_num_heads, 2 head_size (all required), 3 local_window_size (-1: none), 4 scale (0), 5 softcap (0: none) */
+  int64_t num_heads, kv_num_heads, head_size, local_window_size;
+  double scale, softcap;
+} NxrtRocmCacheAttentionAttrs;
+int nxrt_rocm_ep_supports_cache_attention(const NxrtRocmEp* ep, const NxrtRocmCacheAttentionAttrs* attrs, const NxrtTensorDesc* inputs, uint32_t n_inputs, char* reason,
+                                          size_t reason_len);
+NxrtStatus nxrt_rocm_cache_attention_create(NxrtRocmEp* ep, const NxrtRocmCacheAttentionAttrs* attrs, NxrtRocmNode** out_node);
+
+/* CachePages: the block table of the next step and the pages that move for it; or, with compact, a pool whose pages in use are its first ones.
+ *   inputs: 0 block_table [S, W] Int32, 1 lengths [S] Int32: tokens cached of each sequence; 2 parents [S] Int32 or absent (each its own): the sequence that slot i goes on from,
+ *           -1: none, the slot is free; 3 new_tokens [S] Int32 or absent (0): tokens that slot i is going to get; 4 .. 13 pools [L, P, ..] of any type: what moves with a page,
+ *           L layers of P pages each.
+ *   outputs: 0 next table [S, W] Int32, entries without a page -1; 1 next lengths [S] Int32: past_lengths of the next step; 2 moves [S, 2] ([P / 2, 2] with compact, in rising
+ *           order) Int32: from, to, or -1; 3 counts [2] Int32: pages in use, pages that were missing; 4 .. the pools, the inputs' own tensors.
+ * Slot i has the pages of its parent that are whole. A begun one stays with the lowest slot that continues it, if no slot has it as a whole page; the others get a copy in a
+ * fresh page. Fresh pages, copies first and then those that new_tokens need, are the lowest that no slot has, dealt out slot by slot. Where they run out, entries are -1 and
+ * count as missing (as do entries outside 0 .. P - 1); the inputs' table still stands then. No count is kept beside the table: a page is free if no slot has it.
+ * With compact (parents and new_tokens absent) the k-th page in use beyond the first n goes to the k-th free one among them, n the pages in use.
+ * S <= 1024, P <= 2^18, W page_size < 2^30. */
+typedef struct NxrtRocmCachePagesAttrs {
+  uint32_t struct_size;
+  uint32_t present;      /* bit i: 0 page_size (required; 1..=2^20), 1 compact (0) */
+  int64_t page_size, compact;
+} NxrtRocmCachePagesAttrs;
+int nxrt_rocm_ep_supports_cache_pages(const NxrtRocmEp* ep, const NxrtRocmCachePagesAttrs* attrs, const NxrtTensorDesc* inputs, uint32_t n_inputs, char* reason, size_t reason_len);
+NxrtStatus nxrt_rocm_cache_pages_create(NxrtRocmEp* ep, const NxrtRocmCachePagesAttrs* attrs, NxrtRocmNode** out_node);
+
 /* As the functions of the same names for MatMulNBits; but which inputs are constant makes no difference to a node, which reads its weights as they are in each call. */
 void nxrt_rocm_node_set_constant_inputs(NxrtRocmNode* node, const uint8_t* is_constant, uint32_t n);
 NxrtStatus nxrt_rocm_node_workspace_requirement(const NxrtRocmNode* node, const NxrtTensorDesc* inputs, uint32_t n_inputs, NxrtRocmWorkspaceRequirement* out);

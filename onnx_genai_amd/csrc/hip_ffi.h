@@ -408,6 +408,92 @@ const char* rocm_moe_variant(const RocmMoeArgs* args);
 /* workspace: rocm_moe_workspace_bytes() of device memory, 256-byte aligned, contents of no interest before or after. */
 int rocm_launch_moe(const RocmMoeArgs* args, void* workspace, rocm_stream_t stream);
 
+/* ---- the paged 8-bit cache ------------------------------------------------------------------------------------------------ */
+
+enum { ROCM_DT_I64 = 7, ROCM_DT_E4M3 = 17 };
+
+/* RotaryEmbedding (kernels/rotary.hip). Row r = (r / inner, r % inner) begins at (r / inner) * outer_step + (r % inner) * row_step elements; head h of it lies
+ * head_step elements further each; `extra` elements behind the last head pass through, as do those of a head from `part` on. x and y: the same layout, the same
+ * memory or apart. Any alignment of whole elements. */
+enum { ROCM_ROTARY_MAX_PAIRS = 256 };
+typedef struct RocmRotaryArgs {
+  const void* x;
+  void* y;
+  const void* positions;    /* [rows], or [1]: the position of row 0 of each run of `inner` rows */
+  const void* cos_cache;    /* [cache_rows, part / 2] of cache_dtype, or NULL: cosines and sines of position * turns[i] */
+  const void* sin_cache;
+  int64_t rows, inner, outer_step, row_step, head_step, extra, cache_rows;
+  int heads, head_size, part, interleaved, dtype, cache_dtype, positions_dtype, one_position;
+  double magnitude;
+  double turns[ROCM_ROTARY_MAX_PAIRS];   /* whole turns a position, of each pair */
+} RocmRotaryArgs;
+int rocm_launch_rotary(const RocmRotaryArgs* args, rocm_stream_t stream);
+
+/* The cache of one layer: codes of keys [pages, kv_heads, page, head_size] and values [pages, kv_heads, head_size, page] (int8 or e4m3), scales
+ * [pages, kv_heads]; codes at addresses of 16 bytes. Sequence b has rows ends[b] .. ends[b + 1] of the call's new tokens behind past[b] tokens; token t of it lies
+ * in page table[b * width + t / page]. What a table, ends or past say is never followed out of the tensors: pages outside 0 .. pages - 1 hold no tokens, and
+ * ends and past are taken into 0 .. rows and 0 .. width * page. width * page < 2^30. */
+typedef struct RocmCache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* ends;
+  const int32_t* past;
+  const int32_t* table;
+  int64_t pages;
+  int sequences, width, page, kv_heads, head_size, code_dtype;
+} RocmCache;
+enum { ROCM_CACHE_MAX_HEAD = 256, ROCM_CACHE_MAX_PAGE = 128 };
+
+/* CacheAppend (kernels/cache_append.hip). Rows of k and v are k_step and v_step elements apart. */
+typedef struct RocmCacheAppendArgs {
+  RocmCache cache;
+  const void* k;
+  const void* v;
+  int64_t rows, k_step, v_step;
+  int dtype;
+} RocmCacheAppendArgs;
+int rocm_launch_cache_append(const RocmCacheAppendArgs* args, rocm_stream_t stream);
+
+/* CacheAttention (kernels/cache_attention.hip). Rows of q are q_step elements apart, those of y heads * head_size. rows * heads < 2^30. */
+typedef struct RocmCacheAttentionArgs {
+  RocmCache cache;
+  const void* q;
+  void* y;
+  int64_t rows, q_step;
+  int heads, dtype;
+  int window;               /* tokens that a query sees, itself the last of them; 0: all before it */
+  float scale, softcap;     /* softcap 0: none */
+} RocmCacheAttentionArgs;
+int rocm_cache_attention_supports(int head_size);
+uint64_t rocm_cache_attention_workspace_bytes(const RocmCacheAttentionArgs* args);
+const char* rocm_cache_attention_variant(const RocmCacheAttentionArgs* args);
+/* workspace: rocm_cache_attention_workspace_bytes() of device memory, 256-byte aligned, contents of no interest before or after. */
+int rocm_launch_cache_attention(const RocmCacheAttentionArgs* args, void* workspace, rocm_stream_t stream);
+
+/* CachePages (kernels/cache_pages.hip). A pool has `layers` times `pages` pages of page_bytes each, one behind the other. */
+enum { ROCM_PAGES_MAX_POOLS = 10, ROCM_PAGES_MAX_SLOTS = 1024, ROCM_PAGES_MAX_PAGES = 1 << 18 };
+typedef struct RocmPool {
+  void* at;
+  int64_t layers, page_bytes;
+} RocmPool;
+typedef struct RocmCachePagesArgs {
+  const int32_t* table;     /* [slots, width] */
+  const int32_t* lengths;   /* [slots] */
+  const int32_t* parents;   /* [slots], or NULL: each its own */
+  const int32_t* grow;      /* [slots] tokens to come, or NULL: none */
+  int32_t* next;            /* [slots, width] */
+  int32_t* next_lengths;    /* [slots] */
+  int32_t* moves;           /* [slots, 2], with `compact` [pages / 2, 2] */
+  int32_t* counts;          /* [2]: pages in use, pages that were missing */
+  int64_t pages;
+  int slots, width, page, compact, pools;
+  RocmPool pool[ROCM_PAGES_MAX_POOLS];
+} RocmCachePagesArgs;
+uint64_t rocm_cache_pages_workspace_bytes(const RocmCachePagesArgs* args);
+int rocm_launch_cache_pages(const RocmCachePagesArgs* args, void* workspace, rocm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,468 @@
+// CacheAttention over few rows: o = softmax(scale q k^T) v of a sequence's new tokens over its pages, where a key head has up to a few dozen query rows.
+//
+// The cache's bytes bound it: each is read once for all rows of a tile. A wave takes 64 tokens at a time on its own, straight from memory into the operands of the
+// matrix instructions, without LDS. Scores are taken transposed, S^T = K Q^T: 16 tokens (rows) by 16 queries (columns) an instruction, over any order of tokens and of
+// head elements as long as both operands agree. So row m of key tile t is token 16 (m / 4) + 4 t + m % 4: a lane then holds the scores of 16 tokens in a row, which is
+// what it needs of them as the second operand of O^T = V^T P^T, with 16 tokens of one element a 16-byte load of the values' page. Nothing moves between lanes but
+// the maximum of a row. The 16 tokens lie in one page, which holds 16 at least, and their page's scale is one number a lane.
+//
+// Codes are exact in f16, as 8-bit integers and as e4m3. Queries go to f16 with their row's largest at 2^8 (what falls below f16's range is less than 2^-22 of it).
+// Weights p = exp(s - max) are held as p * 2^14 * (scale of the values' page / largest such scale so far) in f16: rounded to 11 bits, down to 2^-28 of the largest
+// weight, below that to 2^-38; sums and all products are in f32.
+#include "cache_attention.hiph"
+#include "mfma_common.hiph"
+#include "rows.hiph"
+
+namespace mnb {
+namespace {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kRows = 16;
+constexpr float kNone = -__builtin_huge_valf();
+constexpr float kWeightBits = 14.f;
+
+typedef __attribute__((ext_vector_type(8))) _Float16 half8_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 half2_t;
+typedef __attribute__((ext_vector_type(4))) float float4_t;
+
+// Sixteen codes as f16, exactly. int8: with its sign bit turned a byte is code + 128, which placed below 0x64 is the f16 code + 1152.
+template <bool E4M3>
+__device__ __forceinline__ void widen(const uint4& w, half8_t& lo, half8_t& hi)
+{
+    const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+    half2_t h[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (E4M3) {
+            h[2 * i] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d[i], 1.0f, false));
+            h[2 * i + 1] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d[i], 1.0f, true));
+        } else {
+            const half2_t off = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
+            const uint32_t u = d[i] ^ 0x80808080u;
+            h[2 * i] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off;
+            h[2 * i + 1] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off;
+        }
+    }
+    lo = half8_t{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
+    hi = half8_t{h[4].x, h[4].y, h[5].x, h[5].y, h[6].x, h[6].y, h[7].x, h[7].y};
+}
+
+// The largest of the four lanes 16 apart, in each of them.
+__device__ __forceinline__ float over_groups_max(float v)
+{
+    const uint32_t a = __float_as_uint(v);
+    const auto s = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    v = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    const uint32_t b = __float_as_uint(v);
+    const auto t = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+__device__ __forceinline__ float over_groups_sum(float v)
+{
+    const uint32_t a = __float_as_uint(v);
+    const auto s = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    const uint32_t b = __float_as_uint(v);
+    const auto t = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+}
+
+// A score before the softmax, in powers of two. `x` is the product scaled as the softmax wants it, or, with a softcap, as it is.
+__device__ __forceinline__ float capped(float x, float softcap)
+{
+    // cap * tanh(x / cap) * log2(e); tanh z = 1 - 2 / (e^2z + 1)
+    const float e = __builtin_amdgcn_exp2f(x * (2.885390082f / softcap));
+    return softcap * 1.442695041f * (1.0f - 2.0f / (e + 1.0f));
+}
+
+// f32 -> the tensor's 16-bit type
+__device__ __forceinline__ uint16_t narrow(float v, int dtype) { return dtype == ROCM_DT_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v); }
+
+template <int D>
+struct Queries {
+    static constexpr int kChunks = (D + 63) / 64;
+    half8_t q[kChunks][2];
+    float undo;                      // what a score is multiplied by for the row's own scale
+
+    // Row `n` of lane n, 16 elements from 64 c + 16 g of it in q[c].
+    __device__ __forceinline__ void load(const uint16_t* row, bool bf16, int g)
+    {
+        float x[kChunks][16];
+        float most = 0.f;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            const bool there = row && c * 64 + g * 16 < D;
+            Bytes16 raw[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            if (there) {
+                raw[0] = *reinterpret_cast<const Bytes16*>(row + c * 64 + g * 16);
+                raw[1] = *reinterpret_cast<const Bytes16*>(row + c * 64 + g * 16 + 8);
+            }
+            const uint32_t d[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[c][2 * i] = bf16 ? __uint_as_float(d[i] << 16) : f16_bits_to_f32(static_cast<uint16_t>(d[i]));
+                x[c][2 * i + 1] = bf16 ? __uint_as_float(d[i] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(d[i] >> 16));
+                most = fmaxf(most, fmaxf(fabsf(x[c][2 * i]), fabsf(x[c][2 * i + 1])));
+            }
+        }
+        most = over_groups_max(most);
+        // (an infinity or a NaN stays one: the exponent of neither is asked for; a row of zeros has any)
+        int e = most > 0.f && most < __builtin_huge_valf() ? static_cast<int>((__float_as_uint(most) >> 23) & 0xff) - 127 : 0;
+        e = e < -110 ? -110 : e;
+        const float factor = __uint_as_float(static_cast<uint32_t>(127 + 8 - e) << 23);
+        undo = __uint_as_float(static_cast<uint32_t>(127 - 8 + e) << 23);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) q[c][i >> 3][i & 7] = static_cast<_Float16>(x[c][i] * factor);
+    }
+};
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(kThreads) void attention_few_kernel(AttentionParams p)
+{
+    constexpr int kChunks = (D + 63) / 64, kTiles = D / 16;
+    __shared__ float results[kWaves][kRows][D + 4];
+    __shared__ float2 sums[kWaves][kRows];
+    const RocmCache& c = p.a.cache;
+    const int head = blockIdx.x % c.kv_heads;
+    Piece w;
+    if (!piece_at(p, blockIdx.x / c.kv_heads, &w)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int context = context_of(c, w.s);
+
+    // the lane's query row
+    const int first_row = w.tile * kRows, rows = w.s.rows * p.group - first_row < kRows ? w.s.rows * p.group - first_row : kRows;
+    const int token = (first_row + n) / p.group, member = first_row + n - token * p.group;
+    const int own = w.s.past + token;                                        // the row's own slot
+    const bool row_there = n < rows;
+    const uint16_t* const q_row = static_cast<const uint16_t*>(p.a.q) + static_cast<int64_t>(w.s.first + token) * p.a.q_step + (head * p.group + member) * D;
+    Queries<D> q;
+    q.load(row_there ? q_row : nullptr, p.a.dtype == ROCM_DT_BF16, g);
+    const float row_scale = q.undo * p.scale;
+    // tokens that every row of the tile sees, and those that some row does
+    const int first_own = w.s.past + first_row / p.group, last_own = w.s.past + (first_row + rows - 1) / p.group;
+    const int window = p.a.window;
+
+    float4_t o[kTiles];
+#pragma unroll
+    for (int u = 0; u < kTiles; ++u) o[u] = float4_t{0.f, 0.f, 0.f, 0.f};
+    float top = kNone, sum = 0.f, reference = 0.f;
+
+    // The page of 16 tokens of a step: sub-block n / 4 for the lane's keys, g for its values and scales; -1: none. Tokens behind the context have none either.
+    const int page_bits = __builtin_ctz(c.page);
+    auto page_id = [&](int group, int sub) {
+        const int t = group * kGroup + sub * 16;
+        return t < context ? page_of(c, w.b, t >> page_bits) : -1;
+    };
+    struct Step {
+        uint4 k[4][kChunks], v[kTiles];
+        float ks, vs;
+        int live;                                    // tokens of sub-block g that there are
+    };
+    const int64_t page_bytes = static_cast<int64_t>(c.page) * D;
+    const uint8_t *const k_base = static_cast<const uint8_t*>(c.k), *const v_base = static_cast<const uint8_t*>(c.v);
+    auto load_keys = [&](int group, int page, Step& s) {
+        const int64_t at = (static_cast<int64_t>(page < 0 ? 0 : page) * c.kv_heads + head) * page_bytes;
+        const int slot = ((group * kGroup + (n >> 2) * 16) & (c.page - 1)) + (n & 3);
+        const uint8_t* const from = k_base + at + slot * D + g * 16;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) {
+                s.k[t][i] = make_uint4(0, 0, 0, 0);
+                if (D % 64 == 0 || i * 64 + g * 16 < D) s.k[t][i] = *reinterpret_cast<const uint4*>(from + t * 4 * D + i * 64);
+            }
+    };
+    auto load_values = [&](int group, int page, Step& s) {
+        const int64_t index = static_cast<int64_t>(page < 0 ? 0 : page) * c.kv_heads + head;
+        const uint8_t* const from = v_base + index * page_bytes + n * c.page + ((group * kGroup + g * 16) & (c.page - 1));
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u) s.v[u] = *reinterpret_cast<const uint4*>(from + u * 16 * c.page);
+    };
+    auto load_scales = [&](int group, int page, Step& s) {
+        const int64_t index = static_cast<int64_t>(page < 0 ? 0 : page) * c.kv_heads + head;
+        s.ks = c.k_scale[index];
+        s.vs = c.v_scale[index];
+        s.live = page < 0 ? 0 : clamped(context - (group * kGroup + g * 16), 0, 16);
+    };
+
+    Step s;
+    int at = w.span.lo + wave, key_page = -1, value_page = -1;
+    if (at < w.span.hi) {
+        key_page = page_id(at, n >> 2);
+        value_page = page_id(at, g);
+        load_keys(at, key_page, s);
+        load_scales(at, value_page, s);
+        load_values(at, value_page, s);
+        key_page = page_id(at + kWaves, n >> 2);
+        value_page = page_id(at + kWaves, g);
+    }
+    for (; at < w.span.hi; at += kWaves) {
+        const int t0 = at * kGroup;
+        // scores: lane (n, g) gets token t0 + 16 g + 4 t + i of row n in score[t][i]
+        float4_t score[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            score[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) {
+                half8_t lo, hi;
+                widen<E4M3>(s.k[t][i], lo, hi);
+                score[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, q.q[i][0], score[t], 0, 0, 0);
+                score[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, q.q[i][1], score[t], 0, 0, 0);
+            }
+        }
+        const int live = s.live;
+        const float key_scale = s.ks * row_scale, value_scale = s.vs;
+        // the next step's keys, scales and page numbers while this one goes on
+        const bool more = at + kWaves < w.span.hi;
+        if (more) {
+            load_keys(at + kWaves, key_page, s);
+            load_scales(at + kWaves, value_page, s);
+        }
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = score[e >> 2][e & 3] * key_scale;
+        if (p.a.softcap > 0.f) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = capped(x[e], p.a.softcap);
+        }
+        const bool masked = __ballot(live < 16) != 0 || t0 + kGroup - 1 > first_own || (window > 0 && t0 <= last_own - window);
+        uint32_t seen = 0xffffu;                     // bit e: the row sees token e of the lane's
+        if (masked) {
+            const int here = t0 + g * 16;
+            const int hi = own - here + 1 < live ? own - here + 1 : live, lo = window > 0 ? own - window + 1 - here : 0;
+            seen = hi > 0 ? 0xffffu >> (16 - (hi < 16 ? hi : 16)) : 0u;
+            if (lo > 0) seen &= lo < 16 ? 0xffffu << lo : 0u;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = (seen >> e) & 1 ? x[e] : kNone;
+        }
+        float most = x[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) most = fmaxf(most, x[e]);
+        most = fmaxf(top, over_groups_max(most));
+        const float zero = most == kNone ? 0.f : most;                          // (a row that has seen nothing yet)
+        const float shrink = __builtin_amdgcn_exp2f(top - zero);
+        top = most;
+        const float before = reference;
+        reference = fmaxf(reference, over_groups_max(live ? value_scale : 0.f));
+        // weights relative to the largest page scale so far
+        const float relative = reference > 0.f ? value_scale / reference : 0.f;
+        const float again = shrink * (reference > before ? before / reference : 1.f);
+        sum *= shrink;
+        float part = 0.f;
+        half8_t weights[2];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            float y = __builtin_amdgcn_exp2f(x[e] - (zero - kWeightBits));
+            if (masked) y = (seen >> e) & 1 ? y : 0.f;
+            part += y;
+            weights[e >> 3][e & 7] = static_cast<_Float16>(masked && !((seen >> e) & 1) ? 0.f : y * relative);
+        }
+        sum += part;
+        if (__ballot(again != 1.f)) {
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u) o[u] *= again;
+        }
+        if (masked && __ballot(live < 16)) {
+            // what lies behind the context may be anything
+            uint32_t keep[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int left = live - 4 * j;
+                keep[j] = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left);
+            }
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u) s.v[u] = make_uint4(s.v[u].x & keep[0], s.v[u].y & keep[1], s.v[u].z & keep[2], s.v[u].w & keep[3]);
+        }
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u) {
+            half8_t lo, hi;
+            widen<E4M3>(s.v[u], lo, hi);
+            o[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, weights[0], o[u], 0, 0, 0);
+            o[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, weights[1], o[u], 0, 0, 0);
+        }
+        if (more) {
+            load_values(at + kWaves, value_page, s);
+            key_page = page_id(at + 2 * kWaves, n >> 2);
+            value_page = page_id(at + 2 * kWaves, g);
+        }
+    }
+
+    // the waves' results: o[u][i] is element 16 u + 4 g + i of row n
+    sum = over_groups_sum(sum);
+#pragma unroll
+    for (int u = 0; u < kTiles; ++u) *reinterpret_cast<float4_t*>(&results[wave][n][u * 16 + g * 4]) = o[u] * reference;
+    if (g == 0) sums[wave][n] = make_float2(top, sum);
+    __syncthreads();
+    constexpr int kQuads = D / 4;
+    const int64_t out_step = static_cast<int64_t>(p.a.heads) * D;
+    for (int i = threadIdx.x; i < rows * kQuads; i += kThreads) {
+        const int row = i / kQuads, e = (i - row * kQuads) * 4;
+        float most = kNone;
+#pragma unroll
+        for (int j = 0; j < kWaves; ++j) most = fmaxf(most, sums[j][row].x);
+        const float zero = most == kNone ? 0.f : most;
+        float total = 0.f;
+        float4_t all = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kWaves; ++j) {
+            const float f = __builtin_amdgcn_exp2f(sums[j][row].x - zero);
+            total += sums[j][row].y * f;
+            all += *reinterpret_cast<const float4_t*>(&results[j][row][e]) * f;
+        }
+        if (w.slot >= 0) {
+            const int64_t place = (static_cast<int64_t>(w.slot) * c.kv_heads + head) * kRows + row;
+            *reinterpret_cast<float4_t*>(p.partial + place * D + e) = all;
+            if (e == 0) p.partial_sums[place] = make_float2(most, total);
+        } else {
+            // a row that sees nothing is zero
+            const float inverse = total == 0.f ? 0.f : 1.0f / total;
+            const int r = first_row + row, tk = r / p.group;
+            uint16_t* const to = static_cast<uint16_t*>(p.a.y) + static_cast<int64_t>(w.s.first + tk) * out_step + (head * p.group + r - tk * p.group) * D + e;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[j] = narrow(all[j] * inverse, p.a.dtype);
+        }
+    }
+}
+
+// The pieces of a tile joined: a workgroup for two rows, its waves a quarter of the pieces each, in an order that is always the same.
+__global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionParams p, int d)
+{
+    __shared__ float results[kWaves][2][ROCM_CACHE_MAX_HEAD];
+    __shared__ float2 sums[kWaves][2];
+    const RocmCache& c = p.a.cache;
+    const int head = blockIdx.x % c.kv_heads;
+    Piece w;
+    if (!tile_to_join(p, blockIdx.x / c.kv_heads, &w)) return;
+    const int first_row = w.tile * p.tile_rows, left = w.s.rows * p.group - first_row, rows = left < p.tile_rows ? left : p.tile_rows;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int which = lane >> 5, row = blockIdx.y * 2 + which;
+    if (static_cast<int>(blockIdx.y) * 2 >= rows) return;
+    const int from_row = row < rows ? row : rows - 1;
+    float most = kNone, total = 0.f, all[ROCM_CACHE_MAX_HEAD / 32];
+#pragma unroll
+    for (int j = 0; j < ROCM_CACHE_MAX_HEAD / 32; ++j) all[j] = 0.f;
+    for (int i = wave; i < w.pieces; i += kWaves) {
+        const int64_t place = (static_cast<int64_t>(w.slot + i) * c.kv_heads + head) * p.tile_rows + from_row;
+        const float2 s = p.partial_sums[place];
+        const float now = fmaxf(most, s.x), zero = now == kNone ? 0.f : now;
+        const float old = __builtin_amdgcn_exp2f(most - zero), fresh = __builtin_amdgcn_exp2f(s.x - zero);
+        total = total * old + s.y * fresh;
+        most = now;
+#pragma unroll
+        for (int j = 0; j < ROCM_CACHE_MAX_HEAD / 32; ++j) {
+            const int e = (lane & 31) + 32 * j;
+            if (e < d) all[j] = all[j] * old + p.partial[place * d + e] * fresh;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < ROCM_CACHE_MAX_HEAD / 32; ++j) {
+        const int e = (lane & 31) + 32 * j;
+        if (e < d) results[wave][which][e] = all[j];
+    }
+    if ((lane & 31) == 0) sums[wave][which] = make_float2(most, total);
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * d; i += kThreads) {
+        const int r = i / d, e = i - r * d, out_row = static_cast<int>(blockIdx.y) * 2 + r;
+        if (out_row >= rows) continue;
+        float peak = kNone;
+#pragma unroll
+        for (int j = 0; j < kWaves; ++j) peak = fmaxf(peak, sums[j][r].x);
+        const float zero = peak == kNone ? 0.f : peak;
+        float sum = 0.f, value = 0.f;
+#pragma unroll
+        for (int j = 0; j < kWaves; ++j) {
+            const float f = __builtin_amdgcn_exp2f(sums[j][r].x - zero);
+            sum += sums[j][r].y * f;
+            value += results[j][r][e] * f;
+        }
+        const int row_of_all = first_row + out_row, tk = row_of_all / p.group;
+        const int64_t to = static_cast<int64_t>(w.s.first + tk) * p.a.heads * d + (head * p.group + row_of_all - tk * p.group) * d + e;
+        static_cast<uint16_t*>(p.a.y)[to] = narrow(sum == 0.f ? 0.f : value / sum, p.a.dtype);
+    }
+}
+
+struct Plan {
+    bool ok;
+    int tile_rows, target, least;
+    int64_t tiles, pieces;          // most that a call of these sizes has, for one key head
+    uint64_t sums_at, bytes;
+};
+
+Plan plan_of(const RocmCacheAttentionArgs& a)
+{
+    Plan plan{};
+    const RocmCache& c = a.cache;
+    if (a.rows <= 0 || c.sequences <= 0 || c.kv_heads < 1 || a.heads < c.kv_heads || a.heads % c.kv_heads != 0 || !rocm_cache_attention_supports(c.head_size) || a.rows >= (1 << 30) || c.page < 16 ||
+        c.page > ROCM_CACHE_MAX_PAGE || (c.page & (c.page - 1)) != 0 || c.width < 1 || static_cast<int64_t>(c.width) * c.page >= (1 << 30))
+        return plan;
+    const int group = a.heads / c.kv_heads;
+    if (a.rows * group >= (1 << 30)) return plan;
+    plan.tile_rows = kRows;
+    plan.tiles = a.rows * group / plan.tile_rows + (a.rows < c.sequences ? a.rows : c.sequences);
+    // Pieces until there are four workgroups for each CU, none shorter than the 256 tokens that a workgroup's waves take in one step.
+    const int64_t wanted = 4 * static_cast<int64_t>(rocm_ffi_compute_units()) / c.kv_heads;
+    plan.least = kWaves;
+    if (plan.tiles < wanted && static_cast<int64_t>(c.width) * c.page > kGroup * plan.least) plan.target = static_cast<int>(wanted > 0 ? wanted : 1);
+    plan.pieces = plan.tiles + plan.target;
+    const uint64_t places = 2 * static_cast<uint64_t>(plan.target) * c.kv_heads * plan.tile_rows;
+    plan.sums_at = (places * c.head_size * 4 + 255) / 256 * 256;
+    plan.bytes = plan.target ? plan.sums_at + (places * 8 + 255) / 256 * 256 : 0;
+    plan.ok = plan.pieces * c.kv_heads < (1 << 24);
+    return plan;
+}
+
+template <bool E4M3>
+hipError_t launch_few(const AttentionParams& p, dim3 grid, hipStream_t s)
+{
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, p);
+        return hipGetLastError();
+    };
+    switch (p.a.cache.head_size) {
+        case 64: return go(attention_few_kernel<64, E4M3>);
+        case 80: return go(attention_few_kernel<80, E4M3>);
+        case 96: return go(attention_few_kernel<96, E4M3>);
+        case 128: return go(attention_few_kernel<128, E4M3>);
+        case 256: return go(attention_few_kernel<256, E4M3>);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace
+}  // namespace mnb
+
+extern "C" int rocm_cache_attention_supports(int head_size) { return head_size == 64 || head_size == 80 || head_size == 96 || head_size == 128 || head_size == 256; }
+
+extern "C" uint64_t rocm_cache_attention_workspace_bytes(const RocmCacheAttentionArgs* args) { return mnb::plan_of(*args).bytes; }
+
+extern "C" const char* rocm_cache_attention_variant(const RocmCacheAttentionArgs* args) { return mnb::plan_of(*args).target ? "cache_attention_pieces" : "cache_attention"; }
+
+extern "C" int rocm_launch_cache_attention(const RocmCacheAttentionArgs* args, void* workspace, rocm_stream_t stream)
+{
+    using namespace mnb;
+    if (args->rows <= 0 || args->cache.sequences <= 0) return 0;
+    const Plan plan = plan_of(*args);
+    if (!plan.ok || (plan.bytes && !workspace)) return static_cast<int>(hipErrorInvalidValue);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    AttentionParams p{};
+    p.a = *args;
+    p.group = args->heads / args->cache.kv_heads;
+    p.tile_rows = plan.tile_rows;
+    p.target = plan.target;
+    p.least = plan.least;
+    p.slots = 2 * plan.target;
+    p.scale = args->softcap > 0.f ? args->scale : args->scale * 1.442695041f;
+    p.partial = static_cast<float*>(workspace);
+    p.partial_sums = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.sums_at);
+    const dim3 grid(static_cast<unsigned>(plan.pieces * args->cache.kv_heads));
+    hipError_t e = args->cache.code_dtype == ROCM_DT_E4M3 ? launch_few<true>(p, grid, s) : launch_few<false>(p, grid, s);
+    if (e == hipSuccess && plan.target) {
+        hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<unsigned>(plan.tiles * args->cache.kv_heads), static_cast<unsigned>((plan.tile_rows + 1) / 2)), dim3(kThreads), 0, s, p,
+                           args->cache.head_size);
+        e = hipGetLastError();
+    }
+    return static_cast<int>(e);
+}

@@ -1,0 +1,257 @@
+// CachePages: the block table of the next step, and the pages that have to move for it.
+//
+// A step: slot i goes on from sequence parents[i]. Whole pages are shared. A begun page is written by the step's new tokens, so it stays with one slot, the lowest that
+// continues it, unless it is a whole page of some other; every other one gets a fresh page and a copy. Fresh pages, for copies and for the tokens to come, are the
+// lowest that no slot holds, dealt out slot by slot. Nothing is kept between calls: what is in use is what the table says, and a slot is freed by giving it no parent.
+// Compacting: with n pages in use, the ones from n on, in rising order, go to the free ones below n, in rising order. No page is read and written by one call.
+//
+// Two launches. The first, one workgroup, holds a bit for each page in LDS and ranks pages and slots by sums over the workgroup; what it costs is its trips through
+// the tables. The second copies: a workgroup for 8 KB of a page, of each layer and pool; memory bounds it.
+#include "common.hiph"
+
+namespace mnb {
+namespace {
+
+constexpr int kThreads = 1024, kWaves = kThreads / 64, kCopyThreads = 256, kCopyBytes = 8192;
+
+struct PagesWorkspace {
+    int32_t* count;       // [1]: moves
+    int32_t* from;        // [pages]: sources of moves
+    int32_t* to;          // [pages]: and where they go
+    int32_t* list;        // [pages]: free pages by rank; compacting, where a page goes
+};
+
+// The sum over the threads below this one; `all`: over every thread. Two barriers.
+__device__ __forceinline__ int sum_below(int v, int* slots, int* all)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int upto = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int below = __shfl_up(upto, off, 64);
+        if (lane >= off) upto += below;
+    }
+    __syncthreads();
+    if (lane == 63) slots[wave] = upto;
+    __syncthreads();
+    int before = 0, total = 0;
+    for (int i = 0; i < kWaves; ++i) {
+        before += i < wave ? slots[i] : 0;
+        total += slots[i];
+    }
+    *all = total;
+    return before + upto - v;
+}
+
+__device__ __forceinline__ bool is_set(const uint32_t* bits, int page) { return (bits[page >> 5] >> (page & 31)) & 1; }
+__device__ __forceinline__ void set(uint32_t* bits, int page) { atomicOr(bits + (page >> 5), 1u << (page & 31)); }
+
+__global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, PagesWorkspace w)
+{
+    extern __shared__ uint32_t held[];                         // a bit for each page
+    __shared__ int parent[ROCM_PAGES_MAX_SLOTS], length[ROCM_PAGES_MAX_SLOTS], begun[ROCM_PAGES_MAX_SLOTS], start[ROCM_PAGES_MAX_SLOTS], keeps[ROCM_PAGES_MAX_SLOTS];
+    __shared__ int slots[kWaves], missing;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int pages = static_cast<int>(a.pages), words = (pages + 31) / 32, capacity = a.width * a.page;
+    auto page_at = [&](int slot, int j) {
+        const int p = a.table[static_cast<int64_t>(slot) * a.width + j];
+        return p >= 0 && p < pages ? p : -1;
+    };
+    for (int i = t; i < words; i += kThreads) held[i] = 0;
+    if (t == 0) missing = 0;
+    if (t < a.slots) {
+        const int p = a.parents && !a.compact ? a.parents[t] : t;
+        parent[t] = p >= 0 && p < a.slots ? p : -1;
+        const int n = parent[t] < 0 ? 0 : a.lengths[parent[t]];
+        length[t] = n < 0 ? 0 : n > capacity ? capacity : n;
+        // a begun page counts as one like the others where nothing forks
+        begun[t] = !a.compact && length[t] % a.page ? page_at(parent[t], length[t] / a.page) : -1;
+    }
+    __syncthreads();
+    auto whole = [&](int slot) { return a.compact ? (length[slot] + a.page - 1) / a.page : length[slot] / a.page; };
+    for (int i = wave; i < a.slots; i += kWaves) {
+        const int n = whole(i);
+        for (int j = lane; j < a.width; j += 64) {
+            const int p = j < n ? page_at(parent[i], j) : -1;
+            if (p >= 0) set(held, p);
+            else if (j < n) atomicAdd(&missing, 1);
+            a.next[static_cast<int64_t>(i) * a.width + j] = p;
+        }
+    }
+    __syncthreads();
+    // words of the bit map are dealt out in runs, so that ranks rise with the pages
+    const int run = (words + kThreads - 1) / kThreads, first = t * run, last = first + run < words ? first + run : words;
+    auto valid = [&](int word) { return 32 * word + 32 <= pages ? 0xffffffffu : (1u << (pages - 32 * word)) - 1; };
+
+    if (a.compact) {
+        int mine = 0, live;
+        for (int i = first; i < last; ++i) mine += __popc(held[i]);
+        sum_below(mine, slots, &live);
+        auto below = [&](int word) { return 32 * word + 32 <= live ? 0xffffffffu : 32 * word >= live ? 0u : (1u << (live - 32 * word)) - 1; };
+        int sources = 0, holes = 0, moves, unused;
+        for (int i = first; i < last; ++i) {
+            sources += __popc(held[i] & ~below(i));
+            holes += __popc(~held[i] & below(i));
+        }
+        int source = sum_below(sources, slots, &moves), hole = sum_below(holes, slots, &unused);
+        for (int i = first; i < last; ++i) {
+            for (uint32_t bits = held[i] & ~below(i); bits; bits &= bits - 1) w.from[source++] = 32 * i + __ffs(bits) - 1;
+            for (uint32_t bits = ~held[i] & below(i); bits; bits &= bits - 1) w.to[hole++] = 32 * i + __ffs(bits) - 1;
+        }
+        __syncthreads();
+        for (int i = t; i < moves; i += kThreads) w.list[w.from[i]] = w.to[i];
+        const int room = pages / 2;
+        for (int i = t; i < room; i += kThreads) {
+            a.moves[2 * i] = i < moves ? w.from[i] : -1;
+            a.moves[2 * i + 1] = i < moves ? w.to[i] : -1;
+        }
+        __syncthreads();
+        for (int i = wave; i < a.slots; i += kWaves) {
+            const int n = whole(i);
+            for (int j = lane; j < n; j += 64) {
+                const int p = page_at(i, j);
+                if (p >= live) a.next[static_cast<int64_t>(i) * a.width + j] = w.list[p];
+            }
+        }
+        if (t < a.slots) a.next_lengths[t] = length[t];
+        if (t == 0) {
+            *w.count = moves;
+            a.counts[0] = live;
+            a.counts[1] = missing;
+        }
+        return;
+    }
+
+    int need = 0, copies = 0;
+    const bool rest = t < a.slots && length[t] % a.page != 0;
+    bool keep = false;
+    if (t < a.slots) {
+        if (begun[t] >= 0) {
+            keep = !is_set(held, begun[t]);
+            for (int i = 0; i < t && keep; ++i) keep = begun[i] != begun[t];
+            copies = !keep;
+        }
+        const int more = a.grow && parent[t] >= 0 && a.grow[t] > 0 ? a.grow[t] : 0;
+        const int end = more < capacity - length[t] ? length[t] + more : capacity;
+        need = copies + (end + a.page - 1) / a.page - (length[t] + a.page - 1) / a.page;
+    }
+    __syncthreads();
+    if (keep) set(held, begun[t]);
+    int needed, free_pages, moves;
+    const int mine = sum_below(need, slots, &needed);
+    if (t < a.slots) {
+        start[t] = mine;
+        keeps[t] = keep;
+    }
+    int empty = 0;
+    for (int i = first; i < last; ++i) empty += __popc(~held[i] & valid(i));
+    int rank = sum_below(empty, slots, &free_pages);
+    for (int i = first; i < last && rank < needed; ++i)
+        for (uint32_t bits = ~held[i] & valid(i); bits && rank < needed; bits &= bits - 1) w.list[rank++] = 32 * i + __ffs(bits) - 1;
+    __syncthreads();
+    auto fresh = [&](int k) { return k < free_pages ? w.list[k] : -1; };
+    const int copy = copies ? fresh(mine) : -1;
+    const int place = sum_below(copy >= 0, slots, &moves);
+    if (t < a.slots) {
+        const int full = length[t] / a.page;
+        if (rest) {
+            const int p = keep ? begun[t] : copy;
+            a.next[static_cast<int64_t>(t) * a.width + full] = p;
+            if (p < 0) atomicAdd(&missing, 1);
+        }
+        a.moves[2 * t] = copy >= 0 ? begun[t] : -1;
+        a.moves[2 * t + 1] = copy;
+        if (copy >= 0) {
+            w.from[place] = begun[t];
+            w.to[place] = copy;
+        }
+        a.next_lengths[t] = length[t];
+    }
+    for (int i = wave; i < a.slots; i += kWaves) {
+        const int have = (length[i] + a.page - 1) / a.page, begins = start[i] + (begun[i] >= 0 && !keeps[i]);
+        const int ends = i + 1 < a.slots ? start[i + 1] : needed;
+        for (int k = begins + lane; k < ends; k += 64) {
+            const int p = fresh(k);
+            if (p < 0) atomicAdd(&missing, 1);
+            a.next[static_cast<int64_t>(i) * a.width + have + k - begins] = p;
+        }
+    }
+    __syncthreads();
+    if (t == 0) {
+        *w.count = moves;
+        a.counts[0] = pages - free_pages + (needed < free_pages ? needed : free_pages);
+        a.counts[1] = missing;
+    }
+}
+
+struct CopyPlan {
+    int pieces[ROCM_PAGES_MAX_POOLS];      // workgroups for one move, up to and with each pool
+};
+
+__global__ __launch_bounds__(kCopyThreads) void copy_kernel(RocmCachePagesArgs a, PagesWorkspace w, CopyPlan plan)
+{
+    int k = 0;
+    while (static_cast<int>(blockIdx.x) >= plan.pieces[k]) ++k;
+    const int index = blockIdx.x - (k ? plan.pieces[k - 1] : 0);
+    const RocmPool pool = a.pool[k];
+    const int parts = static_cast<int>((pool.page_bytes + kCopyBytes - 1) / kCopyBytes);
+    const int layer = index / parts;
+    const int64_t skip = static_cast<int64_t>(index - layer * parts) * kCopyBytes, left = pool.page_bytes - skip;
+    const int bytes = left < kCopyBytes ? static_cast<int>(left) : kCopyBytes;
+    uint8_t* const base = static_cast<uint8_t*>(pool.at) + static_cast<int64_t>(layer) * a.pages * pool.page_bytes + skip;
+    const bool wide = (reinterpret_cast<uintptr_t>(pool.at) | static_cast<uint64_t>(pool.page_bytes)) % 16 == 0;
+    const int moves = *w.count;
+    for (int m = blockIdx.y; m < moves; m += gridDim.y) {
+        const uint8_t* const from = base + w.from[m] * pool.page_bytes;
+        uint8_t* const to = base + w.to[m] * pool.page_bytes;
+        if (wide) {
+            constexpr int kEach = kCopyBytes / 16 / kCopyThreads;
+            uint4 v[kEach];
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int at = (threadIdx.x + i * kCopyThreads) * 16;
+                v[i] = at < bytes ? *reinterpret_cast<const uint4*>(from + at) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int at = (threadIdx.x + i * kCopyThreads) * 16;
+                if (at < bytes) *reinterpret_cast<uint4*>(to + at) = v[i];
+            }
+        } else {
+            for (int at = threadIdx.x; at < bytes; at += kCopyThreads) to[at] = from[at];
+        }
+    }
+}
+
+}  // namespace
+}  // namespace mnb
+
+extern "C" uint64_t rocm_cache_pages_workspace_bytes(const RocmCachePagesArgs* args) { return 256 + 3 * ((static_cast<uint64_t>(args->pages) * 4 + 255) / 256 * 256); }
+
+extern "C" int rocm_launch_cache_pages(const RocmCachePagesArgs* args, void* workspace, rocm_stream_t stream)
+{
+    using namespace mnb;
+    if (args->slots <= 0) return 0;
+    if (args->slots > ROCM_PAGES_MAX_SLOTS || args->pages < 1 || args->pages > ROCM_PAGES_MAX_PAGES || args->width < 1 || args->page < 1 || static_cast<int64_t>(args->width) * args->page >= (1 << 30) ||
+        args->pools < 0 || args->pools > ROCM_PAGES_MAX_POOLS || !workspace)
+        return static_cast<int>(hipErrorInvalidValue);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    uint8_t* const at = static_cast<uint8_t*>(workspace);
+    const uint64_t each = (static_cast<uint64_t>(args->pages) * 4 + 255) / 256 * 256;
+    const PagesWorkspace w{reinterpret_cast<int32_t*>(at), reinterpret_cast<int32_t*>(at + 256), reinterpret_cast<int32_t*>(at + 256 + each), reinterpret_cast<int32_t*>(at + 256 + 2 * each)};
+    CopyPlan plan{};
+    int64_t pieces = 0;
+    for (int i = 0; i < args->pools; ++i) {
+        pieces += args->pool[i].layers * ((args->pool[i].page_bytes + kCopyBytes - 1) / kCopyBytes);
+        if (pieces >= (1 << 20)) return static_cast<int>(hipErrorInvalidValue);
+        plan.pieces[i] = static_cast<int>(pieces);
+    }
+    for (int i = args->pools; i < ROCM_PAGES_MAX_POOLS; ++i) plan.pieces[i] = static_cast<int>(pieces);
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), static_cast<unsigned>((args->pages + 31) / 32 * 4), s, *args, w);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || pieces == 0) return static_cast<int>(e);
+    const int64_t most = args->compact ? args->pages / 2 : args->slots;
+    if (most == 0) return 0;
+    hipLaunchKernelGGL(copy_kernel, dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(most < 1024 ? most : 1024)), dim3(kCopyThreads), 0, s, *args, w, plan);
+    return static_cast<int>(hipGetLastError());
+}

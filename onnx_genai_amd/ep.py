@@ -23,9 +23,9 @@ try:
 except ModuleNotFoundError:      # a tree not built for this interpreter: every call is packed here and goes through ctypes
     _calls = None
 
-F32, U8, I8, I32, F16, BF16 = 1, 2, 3, 6, 10, 16
+F32, U8, I8, I32, I64, F16, BF16, F8E4M3 = 1, 2, 3, 6, 7, 10, 16, 17
 DEVICE_ROCM = 2
-_ITEM = {F32: 4, U8: 1, I8: 1, I32: 4, F16: 2, BF16: 2}
+_ITEM = {F32: 4, U8: 1, I8: 1, I32: 4, I64: 8, F16: 2, BF16: 2, F8E4M3: 1}
 
 LIB_PATH = os.environ.get("NXRT_ROCM_LIBRARY") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libnxrt_ep_rocm.so")
 
@@ -84,8 +84,29 @@ class GatedResidualNormAttrs(C.Structure):
                 ("layer_norm", C.c_int64)]
 
 
+class RotaryEmbeddingAttrs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("present", C.c_uint32), ("head_size", C.c_int64), ("num_heads", C.c_int64), ("rotary_embedding_dim", C.c_int64),
+                ("interleaved", C.c_int64), ("scaling", C.c_int64), ("original_max_position", C.c_int64), ("rope_theta", C.c_double), ("factor", C.c_double),
+                ("low_freq_factor", C.c_double), ("high_freq_factor", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("attention_factor", C.c_double)]
+
+
+class CacheAppendAttrs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("present", C.c_uint32), ("num_heads", C.c_int64), ("kv_num_heads", C.c_int64), ("head_size", C.c_int64)]
+
+
+class CacheAttentionAttrs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("present", C.c_uint32), ("num_heads", C.c_int64), ("kv_num_heads", C.c_int64), ("head_size", C.c_int64),
+                ("local_window_size", C.c_int64), ("scale", C.c_double), ("softcap", C.c_double)]
+
+
+class CachePagesAttrs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("present", C.c_uint32), ("page_size", C.c_int64), ("compact", C.c_int64)]
+
+
 # operators beside MatMulNBits: their attributes (bit i of `present` = the i-th of them) and the name in their entry points
-_NODE_OPS = {"QMoE": (QMoEAttrs, "qmoe"), "MatMulInt8": (MatMulInt8Attrs, "matmul_int8"), "GatedResidualNorm": (GatedResidualNormAttrs, "gated_residual_norm")}
+_NODE_OPS = {"QMoE": (QMoEAttrs, "qmoe"), "MatMulInt8": (MatMulInt8Attrs, "matmul_int8"), "GatedResidualNorm": (GatedResidualNormAttrs, "gated_residual_norm"),
+             "RotaryEmbedding": (RotaryEmbeddingAttrs, "rotary_embedding"), "CacheAppend": (CacheAppendAttrs, "cache_append"),
+             "CacheAttention": (CacheAttentionAttrs, "cache_attention"), "CachePages": (CachePagesAttrs, "cache_pages")}
 
 _ATTR_BITS = {"K": 0, "N": 1, "bits": 2, "block_size": 3, "accuracy_level": 4, "weight_prepacked": 5, "folded_bias": 6, "gate_up_swiglu": 7,
               "decomposed_silu": 8, "rmsnorm_prologue": 9, "rmsnorm_epsilon": 10}
@@ -417,7 +438,7 @@ class RocmExecutionProvider:
         return bool(ok), reason.value.decode()
 
     def get_kernel(self, attrs: dict, input_shapes=None, op_type: str = "MatMulNBits"):
-        """A kernel object for one node: MatMulNBits, or QMoE, MatMulInt8, GatedResidualNorm (include/nxrt_ep_rocm.h says what each takes)."""
+        """A kernel object for one node: MatMulNBits, or an operator of _NODE_OPS (include/nxrt_ep_rocm.h says what each takes)."""
         return MatMulNBitsKernel(self, attrs, input_shapes) if op_type == "MatMulNBits" else NodeKernel(self, op_type, attrs)
 
     # -- pieces -----------------------------------------------------------------------------------
@@ -630,7 +651,7 @@ class NodeKernel:
             pass
 
 
-_NP = {F32: np.float32, F16: np.float16, BF16: np.uint16, U8: np.uint8, I8: np.int8, I32: np.int32}
+_NP = {F32: np.float32, F16: np.float16, BF16: np.uint16, U8: np.uint8, I8: np.int8, I32: np.int32, I64: np.int64, F8E4M3: np.uint8}
 
 
 class DeviceOperands:
