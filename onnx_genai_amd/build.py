@@ -43,6 +43,7 @@ HIP_SOURCES = [
     "kernels/rotary.hip",
     "kernels/cache_append.hip",
     "kernels/cache_attention.hip",
+    "kernels/cache_attention_rows.hip",
     "kernels/cache_pages.hip",
 ]
 HOST_SOURCES = ["ep/provider.cpp", "ep/matmul_nbits.cpp", "ep/nodes.cpp", "ep/cache_nodes.cpp", "ep/nxrt_plugin.cpp", "ep/nxmem_plugin.cpp", "ep/ort_plugin.cpp"]

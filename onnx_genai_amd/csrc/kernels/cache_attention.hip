@@ -10,41 +10,11 @@
 // Weights p = exp(s - max) are held as p * 2^14 * (scale of the values' page / largest such scale so far) in f16: rounded to 11 bits, down to 2^-28 of the largest
 // weight, below that to 2^-38; sums and all products are in f32.
 #include "cache_attention.hiph"
-#include "mfma_common.hiph"
-#include "rows.hiph"
 
 namespace mnb {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kRows = 16;
-constexpr float kNone = -__builtin_huge_valf();
-constexpr float kWeightBits = 14.f;
-
-typedef __attribute__((ext_vector_type(8))) _Float16 half8_t;
-typedef __attribute__((ext_vector_type(2))) _Float16 half2_t;
-typedef __attribute__((ext_vector_type(4))) float float4_t;
-
-// Sixteen codes as f16, exactly. int8: with its sign bit turned a byte is code + 128, which placed below 0x64 is the f16 code + 1152.
-template <bool E4M3>
-__device__ __forceinline__ void widen(const uint4& w, half8_t& lo, half8_t& hi)
-{
-    const uint32_t d[4] = {w.x, w.y, w.z, w.w};
-    half2_t h[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (E4M3) {
-            h[2 * i] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d[i], 1.0f, false));
-            h[2 * i + 1] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d[i], 1.0f, true));
-        } else {
-            const half2_t off = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
-            const uint32_t u = d[i] ^ 0x80808080u;
-            h[2 * i] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off;
-            h[2 * i + 1] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off;
-        }
-    }
-    lo = half8_t{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
-    hi = half8_t{h[4].x, h[4].y, h[5].x, h[5].y, h[6].x, h[6].y, h[7].x, h[7].y};
-}
 
 // The largest of the four lanes 16 apart, in each of them.
 __device__ __forceinline__ float over_groups_max(float v)
@@ -65,17 +35,6 @@ __device__ __forceinline__ float over_groups_sum(float v)
     const auto t = __builtin_amdgcn_permlane32_swap(b, b, false, false);
     return __uint_as_float(t[0]) + __uint_as_float(t[1]);
 }
-
-// A score before the softmax, in powers of two. `x` is the product scaled as the softmax wants it, or, with a softcap, as it is.
-__device__ __forceinline__ float capped(float x, float softcap)
-{
-    // cap * tanh(x / cap) * log2(e); tanh z = 1 - 2 / (e^2z + 1)
-    const float e = __builtin_amdgcn_exp2f(x * (2.885390082f / softcap));
-    return softcap * 1.442695041f * (1.0f - 2.0f / (e + 1.0f));
-}
-
-// f32 -> the tensor's 16-bit type
-__device__ __forceinline__ uint16_t narrow(float v, int dtype) { return dtype == ROCM_DT_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v); }
 
 template <int D>
 struct Queries {
@@ -105,15 +64,12 @@ struct Queries {
             }
         }
         most = over_groups_max(most);
-        // (an infinity or a NaN stays one: the exponent of neither is asked for; a row of zeros has any)
-        int e = most > 0.f && most < __builtin_huge_valf() ? static_cast<int>((__float_as_uint(most) >> 23) & 0xff) - 127 : 0;
-        e = e < -110 ? -110 : e;
-        const float factor = __uint_as_float(static_cast<uint32_t>(127 + 8 - e) << 23);
-        undo = __uint_as_float(static_cast<uint32_t>(127 - 8 + e) << 23);
+        const QueryScale scale(most);
+        undo = scale.undo;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) q[c][i >> 3][i & 7] = static_cast<_Float16>(x[c][i] * factor);
+            for (int i = 0; i < 16; ++i) q[c][i >> 3][i & 7] = static_cast<_Float16>(x[c][i] * scale.factor);
     }
 };
 
@@ -385,7 +341,7 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionParam
 }
 
 struct Plan {
-    bool ok;
+    bool ok, many;
     int tile_rows, target, least;
     int64_t tiles, pieces;          // most that a call of these sizes has, for one key head
     uint64_t sums_at, bytes;
@@ -400,10 +356,12 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
         return plan;
     const int group = a.heads / c.kv_heads;
     if (a.rows * group >= (1 << 30)) return plan;
-    plan.tile_rows = kRows;
+    // From 32 rows a sequence on, on average, tiles share what they read of the cache through LDS.
+    plan.many = a.rows * group > 32 * static_cast<int64_t>(c.sequences);
+    plan.tile_rows = plan.many ? kManyRows : kRows;
     plan.tiles = a.rows * group / plan.tile_rows + (a.rows < c.sequences ? a.rows : c.sequences);
-    // Pieces until there are four workgroups for each CU, none shorter than the 256 tokens that a workgroup's waves take in one step.
-    const int64_t wanted = 4 * static_cast<int64_t>(rocm_ffi_compute_units()) / c.kv_heads;
+    // Pieces until there are four workgroups for each CU (two of many rows), none shorter than the 256 tokens that the waves of a workgroup of few rows take in one step.
+    const int64_t wanted = (plan.many ? 2 : 4) * static_cast<int64_t>(rocm_ffi_compute_units()) / c.kv_heads;
     plan.least = kWaves;
     if (plan.tiles < wanted && static_cast<int64_t>(c.width) * c.page > kGroup * plan.least) plan.target = static_cast<int>(wanted > 0 ? wanted : 1);
     plan.pieces = plan.tiles + plan.target;
@@ -438,7 +396,11 @@ extern "C" int rocm_cache_attention_supports(int head_size) { return head_size =
 
 extern "C" uint64_t rocm_cache_attention_workspace_bytes(const RocmCacheAttentionArgs* args) { return mnb::plan_of(*args).bytes; }
 
-extern "C" const char* rocm_cache_attention_variant(const RocmCacheAttentionArgs* args) { return mnb::plan_of(*args).target ? "cache_attention_pieces" : "cache_attention"; }
+extern "C" const char* rocm_cache_attention_variant(const RocmCacheAttentionArgs* args) 
+{
+    const mnb::Plan plan = mnb::plan_of(*args);
+    return plan.many ? plan.target ? "cache_attention_rows_pieces" : "cache_attention_rows" : plan.target ? "cache_attention_pieces" : "cache_attention";
+}
 
 extern "C" int rocm_launch_cache_attention(const RocmCacheAttentionArgs* args, void* workspace, rocm_stream_t stream)
 {
@@ -458,7 +420,7 @@ extern "C" int rocm_launch_cache_attention(const RocmCacheAttentionArgs* args, v
     p.partial = static_cast<float*>(workspace);
     p.partial_sums = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.sums_at);
     const dim3 grid(static_cast<unsigned>(plan.pieces * args->cache.kv_heads));
-    hipError_t e = args->cache.code_dtype == ROCM_DT_E4M3 ? launch_few<true>(p, grid, s) : launch_few<false>(p, grid, s);
+    hipError_t e = plan.many ? launch_attention_rows(p, grid, s) : args->cache.code_dtype == ROCM_DT_E4M3 ? launch_few<true>(p, grid, s) : launch_few<false>(p, grid, s);
     if (e == hipSuccess && plan.target) {
         hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<unsigned>(plan.tiles * args->cache.kv_heads), static_cast<unsigned>((plan.tile_rows + 1) / 2)), dim3(kThreads), 0, s, p,
                            args->cache.head_size);

@@ -1,0 +1,344 @@
+// CacheAttention over many rows: prompts and chunks of them.
+//
+// Matrix instructions bound it. A workgroup has 128 rows, 32 a wave, and goes through the tokens 64 at a time: the codes are read once for all rows, become f16 on their way into LDS
+// (exactly), and are read from there as operands. As over few rows the scores are taken transposed, S^T = K Q^T, 32 tokens by 32 rows an instruction, with the tokens of a
+// key tile in the order in which a lane's scores are the weights that it has to hand in for O^T = V^T P^T: row m of the instruction is token 16 (m / 16) + 8 ((m / 4) % 2) +
+// 4 ((m / 8) % 2) + m % 4. Keys lie in LDS a token a row, values an element a row, rows 16 bytes apart more than their data, which spreads 16 rows over all banks.
+// While a step is computed, the next one's codes are on their way into registers; they go to the other half of LDS behind it.
+//
+// A page's scales are numbers of 16 tokens each here, and stay out of the products over single scores: key scales enter a score's one multiply-add, value scales its exponent,
+// weight = 2^(score + log2(scale) - top), and their inverse the sum of 8 weights.
+#include "cache_attention.hiph"
+
+namespace mnb {
+namespace {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kWaveRows = 32;
+static_assert(kWaves * kWaveRows == kManyRows, "rows of a tile");
+constexpr float kLeastShare = 60.f;          // bits that a page's scale may lie below the largest one: what is further below counts as this
+
+typedef __attribute__((ext_vector_type(16))) float float16_t;
+typedef __attribute__((ext_vector_type(4))) float float4_t;
+
+template <int D>
+struct Tile {
+    static constexpr int kKeyPitch = D * 2 + 16, kValuePitch = kGroup * 2 + 16, kValueRows = (D + 31) / 32 * 32;
+    alignas(16) uint8_t k[kGroup * kKeyPitch];
+    alignas(16) uint8_t v[kValueRows * kValuePitch];
+    float key_scale[4], value_bits[4], value_inverse[4];       // of 16 tokens each; log2 and 1 / scale of the values
+    int there[4];
+};
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_kernel(AttentionParams p)
+{
+    constexpr int kSteps = D / 16, kOut = (D + 31) / 32, kPieces = 4 * D, kEach = (kPieces + kThreads - 1) / kThreads;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    Tile<D>* const tiles = reinterpret_cast<Tile<D>*>(lds);
+    const RocmCache& c = p.a.cache;
+    const int head = blockIdx.x % c.kv_heads;
+    Piece w;
+    if (!piece_at(p, blockIdx.x / c.kv_heads, &w)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const int context = context_of(c, w.s);
+    const bool bf16 = p.a.dtype == ROCM_DT_BF16;
+
+    // the lane's query row: half h has the elements 16 i + 8 h of it
+    const int first_row = w.tile * kManyRows + wave * kWaveRows, left = w.s.rows * p.group - first_row, rows = left < kWaveRows ? left : kWaveRows;
+    const int token = (first_row + n) / p.group, member = first_row + n - token * p.group;
+    const int own = w.s.past + token, last_seen = own < context ? own : context - 1;
+    half8_t q[kSteps];
+    float row_scale;
+    {
+        const uint16_t* const row = static_cast<const uint16_t*>(p.a.q) + static_cast<int64_t>(w.s.first + token) * p.a.q_step + (head * p.group + member) * D + 8 * h;
+        Bytes16 raw[kSteps];
+        float most = 0.f;
+        auto get = [&](int i, float (&x)[8]) {
+            const uint32_t d[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[2 * j] = bf16 ? __uint_as_float(d[j] << 16) : f16_bits_to_f32(static_cast<uint16_t>(d[j]));
+                x[2 * j + 1] = bf16 ? __uint_as_float(d[j] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(d[j] >> 16));
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            raw[i] = Bytes16{0, 0, 0, 0};
+            if (n < rows) raw[i] = *reinterpret_cast<const Bytes16*>(row + 16 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            float x[8];
+            get(i, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+        }
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        const QueryScale scale(most);
+        row_scale = scale.undo * p.scale;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            float x[8];
+            get(i, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[i][j] = static_cast<_Float16>(x[j] * scale.factor);
+        }
+    }
+    // tokens that every row of the wave sees, and those that some row does
+    const int first_own = w.s.past + first_row / p.group, last_own = w.s.past + (first_row + (rows > 0 ? rows : 1) - 1) / p.group;
+    const int window = p.a.window;
+
+    const int page_bits = __builtin_ctz(c.page);
+    const int64_t page_bytes = static_cast<int64_t>(c.page) * D;
+    auto page_id = [&](int group, int sub) {
+        const int t = group * kGroup + sub * 16;
+        return t < context ? page_of(c, w.b, t >> page_bits) : -1;
+    };
+    // a thread's 16-byte pieces of a step: piece i of the keys is 16 elements of token i / (D / 16), of the values 16 tokens of element i / 4
+    uint4 keys[kEach], values[kEach];
+    int key_page[kEach], value_page = -1, scale_page = -1;
+    float key_scale = 0.f, value_scale = 0.f;
+    auto find_pages = [&](int group) {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) key_page[j] = page_id(group, ((threadIdx.x + j * kThreads) / (D / 16)) >> 4 & 3);
+        value_page = page_id(group, threadIdx.x & 3);
+        scale_page = value_page;
+    };
+    auto load = [&](int group) {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const int i = threadIdx.x + j * kThreads;
+            if (kPieces % kThreads == 0 || i < kPieces) {
+                const int t = i / (D / 16), col = i - t * (D / 16);
+                const int64_t at = (static_cast<int64_t>(key_page[j] < 0 ? 0 : key_page[j]) * c.kv_heads + head) * page_bytes;
+                keys[j] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(c.k) + at + ((group * kGroup + t) & (c.page - 1)) * D + col * 16);
+                const int64_t from = (static_cast<int64_t>(value_page < 0 ? 0 : value_page) * c.kv_heads + head) * page_bytes;
+                values[j] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(c.v) + from + (i >> 2) * c.page + ((group * kGroup + (i & 3) * 16) & (c.page - 1)));
+            }
+        }
+        if (threadIdx.x < 4) {
+            const int64_t at = static_cast<int64_t>(scale_page < 0 ? 0 : scale_page) * c.kv_heads + head;
+            key_scale = c.k_scale[at];
+            value_scale = c.v_scale[at];
+        }
+    };
+    auto store = [&](int group, Tile<D>& tile, int at_page) {
+        const int live = at_page < 0 ? 0 : clamped(context - (group * kGroup + (threadIdx.x & 3) * 16), 0, 16);
+        if (__ballot(live < 16)) {
+            // what lies behind the context may be anything
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                uint32_t* const d = &values[j].x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int l = live - 4 * e;
+                    d[e] &= l >= 4 ? 0xffffffffu : l <= 0 ? 0u : 0xffffffffu >> (32 - 8 * l);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const int i = threadIdx.x + j * kThreads;
+            if (kPieces % kThreads == 0 || i < kPieces) {
+                const int t = i / (D / 16), col = i - t * (D / 16);
+                half8_t lo, hi;
+                widen<E4M3>(keys[j], lo, hi);
+                half8_t* const k = reinterpret_cast<half8_t*>(tile.k + t * Tile<D>::kKeyPitch + col * 32);
+                k[0] = lo;
+                k[1] = hi;
+                widen<E4M3>(values[j], lo, hi);
+                half8_t* const v = reinterpret_cast<half8_t*>(tile.v + (i >> 2) * Tile<D>::kValuePitch + (i & 3) * 32);
+                v[0] = lo;
+                v[1] = hi;
+            }
+        }
+        if (threadIdx.x < 4) {
+            tile.key_scale[threadIdx.x] = key_scale;
+            // a page of scale 0 (its codes are 0) weighs as the smallest scale does
+            const float scale = value_scale < 1.17549435e-38f ? 1.17549435e-38f : value_scale;
+            tile.value_bits[threadIdx.x] = at_page < 0 ? -126.f : __builtin_amdgcn_logf(scale);
+            tile.value_inverse[threadIdx.x] = 1.0f / scale;
+            tile.there[threadIdx.x] = at_page >= 0;
+        }
+    };
+
+    float16_t o[kOut];
+#pragma unroll
+    for (int u = 0; u < kOut; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[u][i] = 0.f;
+    float top = kNone, sum = 0.f, reference = -126.f;           // reference: log2 of the largest value scale so far
+
+    if (w.span.lo < w.span.hi) {
+        find_pages(w.span.lo);
+        load(w.span.lo);
+        const int page = value_page;
+        store(w.span.lo, tiles[0], page);
+        find_pages(w.span.lo + 1);
+    }
+    for (int at = w.span.lo, turn = 0; at < w.span.hi; ++at, turn ^= 1) {
+        __syncthreads();
+        const Tile<D>& tile = tiles[turn];
+        const bool more = at + 1 < w.span.hi;
+        const int page_ahead = value_page;
+        if (more) {
+            load(at + 1);
+            find_pages(at + 2);
+        }
+        const int t0 = at * kGroup;
+        const bool skipped = rows <= 0 || t0 > last_own || (window > 0 && t0 + kGroup - 1 <= first_own - window);
+        if (!skipped) {
+            // scores: lane (n, h) gets token 16 s + 8 h + j of row n in score[s / 2][8 (s % 2) + j]
+            float16_t score[2];
+            const int order = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) score[b][i] = 0.f;
+                const uint8_t* const from = tile.k + (b * 32 + order) * Tile<D>::kKeyPitch + h * 16;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) score[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(from + i * 32), q[i], score[b], 0, 0, 0);
+            }
+            float ks[4], bits[4], inverse[4];
+            int there = 15;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                ks[s] = tile.key_scale[s] * row_scale;
+                bits[s] = tile.value_bits[s];
+                inverse[s] = tile.value_inverse[s];
+                there &= tile.there[s] ? 15 : 15 ^ (1 << s);
+            }
+            if (p.a.softcap > 0.f) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) score[s >> 1][8 * (s & 1) + j] = capped(score[s >> 1][8 * (s & 1) + j] * ks[s], p.a.softcap);
+                    ks[s] = 1.f;
+                }
+            }
+            const bool masked = there != 15 || t0 + kGroup - 1 > first_own || t0 + kGroup > context || (window > 0 && t0 <= last_own - window);
+            const int hi = last_seen - t0 - 8 * h, lo = window > 0 ? own - window + 1 - t0 - 8 * h : -8;
+            auto seen = [&](int s, int j) { return 16 * s + j <= hi && 16 * s + j >= lo && ((there >> s) & 1); };
+            if (masked) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) score[s >> 1][8 * (s & 1) + j] = seen(s, j) ? score[s >> 1][8 * (s & 1) + j] : kNone;
+            }
+            float most = top;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                float m = score[s >> 1][8 * (s & 1)];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) m = fmaxf(m, score[s >> 1][8 * (s & 1) + j]);
+                most = fmaxf(most, m * ks[s]);
+            }
+            {
+                const uint32_t a = __float_as_uint(most);
+                const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+                most = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+            }
+            const float zero = most == kNone ? 0.f : most;                      // (a row that has seen nothing yet)
+            const float shrink = __builtin_amdgcn_exp2f(top - zero);
+            top = most;
+            const float before = reference;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) reference = fmaxf(reference, bits[s]);
+            const float largest = __builtin_amdgcn_exp2f(reference);
+            const float again = shrink * __builtin_amdgcn_exp2f(before - reference);
+            sum *= shrink;
+            half8_t weights[4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                // (a NaN scale stays one)
+                const float share = bits[s] < reference - kLeastShare ? -kLeastShare : bits[s] - reference;
+                const float off = zero - kWeightBits - share;
+                float part = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float y = __builtin_amdgcn_exp2f(fmaf(score[s >> 1][8 * (s & 1) + j], ks[s], -off));
+                    if (masked) y = seen(s, j) ? y : 0.f;
+                    part += y;
+                    weights[s][j] = static_cast<_Float16>(y);
+                }
+                sum = fmaf(part, fminf(largest * inverse[s], 1152921504606846976.f), sum);
+            }
+            if (__ballot(again != 1.f)) {
+#pragma unroll
+                for (int u = 0; u < kOut; ++u) o[u] *= again;
+            }
+#pragma unroll
+            for (int u = 0; u < kOut; ++u) {
+                const uint8_t* const from = tile.v + (u * 32 + n) * Tile<D>::kValuePitch + h * 16;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(from + s * 32), weights[s], o[u], 0, 0, 0);
+            }
+        }
+        if (more) store(at + 1, tiles[turn ^ 1], page_ahead);
+    }
+
+    // o[u][4 a + i] is element 32 u + 8 a + 4 h + i of row n
+    sum += __shfl_xor(sum, 32, 64);
+    if (n >= rows) return;
+    const float scale = reference <= -126.f ? 0.f : __builtin_amdgcn_exp2f(reference);
+    if (w.slot >= 0) {
+        const int64_t place = (static_cast<int64_t>(w.slot) * c.kv_heads + head) * kManyRows + wave * kWaveRows + n;
+#pragma unroll
+        for (int u = 0; u < kOut; ++u)
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const int e = u * 32 + a * 8 + h * 4;
+                if (D % 32 == 0 || e < D) *reinterpret_cast<float4_t*>(p.partial + place * D + e) = float4_t{o[u][4 * a], o[u][4 * a + 1], o[u][4 * a + 2], o[u][4 * a + 3]} * scale;
+            }
+        if (h == 0) p.partial_sums[place] = make_float2(top, sum);
+    } else {
+        // a row that sees nothing is zero
+        const float inverse = sum == 0.f ? 0.f : scale / sum;
+        uint16_t* const to = static_cast<uint16_t*>(p.a.y) + (static_cast<int64_t>(w.s.first + token) * p.a.heads + head * p.group + member) * D;
+#pragma unroll
+        for (int u = 0; u < kOut; ++u)
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const int e = u * 32 + a * 8 + h * 4;
+                if (D % 32 == 0 || e < D) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) to[e + i] = narrow(o[u][4 * a + i] * inverse, p.a.dtype);
+                }
+            }
+    }
+}
+
+template <int D, bool E4M3>
+hipError_t launch(const AttentionParams& p, dim3 grid, hipStream_t s)
+{
+    constexpr size_t kLds = 2 * sizeof(Tile<D>);
+    if (kLds > 65536) {              // more than a kernel gets without asking
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attention_rows_kernel<D, E4M3>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLds));
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((attention_rows_kernel<D, E4M3>), grid, dim3(kThreads), kLds, s, p);
+    return hipGetLastError();
+}
+
+template <bool E4M3>
+hipError_t launch_of(const AttentionParams& p, dim3 grid, hipStream_t s)
+{
+    switch (p.a.cache.head_size) {
+        case 64: return launch<64, E4M3>(p, grid, s);
+        case 80: return launch<80, E4M3>(p, grid, s);
+        case 96: return launch<96, E4M3>(p, grid, s);
+        case 128: return launch<128, E4M3>(p, grid, s);
+        case 256: return launch<256, E4M3>(p, grid, s);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace
+
+hipError_t launch_attention_rows(const AttentionParams& p, dim3 grid, hipStream_t stream)
+{
+    return p.a.cache.code_dtype == ROCM_DT_E4M3 ? launch_of<true>(p, grid, stream) : launch_of<false>(p, grid, stream);
+}
+
+}  // namespace mnb
