@@ -4,8 +4,8 @@
 //   begun page:  scale' = max(scale, max|x| / top); where that is larger, the codes before are recoded, code' = code * (scale / scale') to the nearest
 //
 // A page with an infinity or a NaN has no codes: its scale is NaN and stays it, its codes are 0. A workgroup has one head of one page, keys or values: the scale is a
-// maximum over all of it. Memory bounds a prompt: rows come in twice, the second time out of the caches, and codes leave in whole dwords. Values lie in a page with
-// the tokens of one element side by side, as the products that read them want them, and turn round in LDS.
+// maximum over all of it, and keeps its rows in registers from the maximum to the codes. Memory bounds a prompt. Values lie in a page with the tokens of one element
+// side by side, as the products that read them want them; a thread has four tokens of eight elements, and so whole dwords of either layout.
 #include <type_traits>
 
 #include "cache.hiph"
@@ -64,11 +64,11 @@ __device__ __forceinline__ uint32_t recoded(uint32_t w, float ratio)
 
 __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
-template <typename T, bool BF16, bool E4M3>
+// UNITS: units of four tokens by eight elements that a thread has at most.
+template <typename T, bool BF16, bool E4M3, int UNITS>
 __global__ __launch_bounds__(kThreads) void append_kernel(RocmCacheAppendArgs a)
 {
     __shared__ uint32_t slots_max[4];
-    extern __shared__ uint32_t turned[];                 // values: [head_size][page + 4] bytes
     const RocmCache& c = a.cache;
     const int page = c.page, head = blockIdx.y, d = c.head_size;
     const bool values = blockIdx.z != 0;
@@ -82,29 +82,53 @@ __global__ __launch_bounds__(kThreads) void append_kernel(RocmCacheAppendArgs a)
     const int begun = s.past % page;
     const int slot = k == 0 ? begun : 0;                 // the page's first new token
     const int passed = k == 0 ? 0 : k * page - begun;    // new tokens in pages before
-    const int count = s.rows - passed < page - slot ? s.rows - passed : page - slot;
+    const int end = slot + (s.rows - passed < page - slot ? s.rows - passed : page - slot);
     const int p = page_of(c, b, s.past / page + k);
     if (p < 0) return;
     const int64_t at = static_cast<int64_t>(p) * c.kv_heads + head;
     uint32_t* const codes = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(values ? c.v : c.k) + at * page * d);
     float* const scale_at = (values ? c.v_scale : c.k_scale) + at;
     const int64_t step = values ? a.v_step : a.k_step;
-    const T* const from = static_cast<const T*>(values ? a.v : a.k) + (s.first + passed) * step + head * d;
+    // row of slot 0 (which is in front of the page's first new token, or is it)
+    const T* const from = static_cast<const T*>(values ? a.v : a.k) + (s.first + passed - slot) * step + head * d;
 
-    const int pieces = d / 8, tokens = kThreads / pieces;        // pieces of eight elements in a row of the head, rows at once
-    const int row0 = threadIdx.x / pieces, piece = threadIdx.x - row0 * pieces;
+    // Unit u: slots 4 quad .. 4 quad + 3, elements 8 piece ... Keys leave as rows of a token, so pieces run first; values as rows of an element, four tokens to a
+    // dword, so quads do (four pieces first there too: 64 bytes of a row together).
+    const int pieces = d / 8, quad0 = slot / 4, quads = (end + 3) / 4 - quad0, units = pieces * quads;
+    auto place = [&](int u, int& quad, int& piece) {
+        if (!values) {
+            quad = u / pieces;
+            piece = u - quad * pieces;
+        } else {
+            piece = u / quads;
+            quad = u - piece * quads;
+        }
+        quad += quad0;
+    };
+    const float old = slot ? *scale_at : 0.f;
+    Eight<T, BF16> x[UNITS][4];
     uint32_t amax = 0;
-    if (row0 < tokens) {
-        for (int t = row0; t < count; t += tokens) {
-            Eight<T, BF16> x;
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) {
+        const int u = threadIdx.x + j * kThreads;
+        int quad = 0, piece = 0;
+        place(u, quad, piece);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int there = 4 * quad + t;
+            x[j][t].zero();
+            if (u < units && there >= slot && there < end) x[j][t].load(from + there * step + piece * 8);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
             float e[8];
-            x.load(from + t * step + piece * 8);
-            x.get(e);
+            x[j][t].get(e);
 #pragma unroll
             for (int i = 0; i < 8; ++i) amax = larger(amax, __float_as_uint(e[i]) & 0x7fffffffu);
         }
-    }
-    const float old = slot ? *scale_at : 0.f;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     amax = over_workgroup(amax, slots_max, wave, kThreads / 64, larger);
     float scale = amax >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(amax) / (E4M3 ? 448.0f : 127.0f);
@@ -125,40 +149,45 @@ __global__ __launch_bounds__(kThreads) void append_kernel(RocmCacheAppendArgs a)
                 const uint32_t w = codes[row * each + j], keep = left >= 4 ? 0u : 0xffffffffu << (8 * left);
                 codes[row * each + j] = (recoded<E4M3>(w, ratio) & ~keep) | (w & keep);
             }
+            __syncthreads();                             // (new codes go to bytes of the same dwords)
         }
     }
     const Coder<E4M3> coder(none ? 0.f : scale);
-    if (row0 < tokens) {
-        for (int t = row0; t < count; t += tokens) {
-            Eight<T, BF16> x;
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) {
+        const int u = threadIdx.x + j * kThreads;
+        if (u >= units) continue;
+        int quad, piece;
+        place(u, quad, piece);
+        uint32_t w[4][2];                                // of token t: eight codes
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
             float e[8];
-            x.load(from + t * step + piece * 8);
-            x.get(e);
-            const uint32_t lo = coder.four(e[0], e[1], e[2], e[3]), hi = coder.four(e[4], e[5], e[6], e[7]);
-            if (!values) {
-                uint2* const to = reinterpret_cast<uint2*>(codes + ((slot + t) * d + piece * 8) / 4);
-                *to = make_uint2(lo, hi);
-            } else {
-                uint8_t* const to = reinterpret_cast<uint8_t*>(turned) + slot + t;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) to[(piece * 8 + i) * (page + 4)] = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
-            }
+            x[j][t].get(e);
+            w[t][0] = coder.four(e[0], e[1], e[2], e[3]);
+            w[t][1] = coder.four(e[4], e[5], e[6], e[7]);
         }
-    }
-    if (!values) return;
-    // rows of one element: whole dwords of new tokens, and bytes where old ones (or nobody's) are in the same dword
-    __syncthreads();
-    const int first = slot / 4, words = (slot + count + 3) / 4 - first, each = page / 4, all = d * words;
-    for (int i = threadIdx.x; i < all; i += kThreads) {
-        const int row = i / words, j = first + (i - row * words);
-        const uint32_t w = turned[row * (each + 1) + j];
-        if (4 * j >= slot && 4 * j + 4 <= slot + count) {
-            codes[row * each + j] = w;
-        } else {
-            uint8_t* const to = reinterpret_cast<uint8_t*>(codes + row * each + j);
+        const bool whole = 4 * quad >= slot && 4 * quad + 4 <= end;
+        if (!values) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (4 * j + e >= slot && 4 * j + e < slot + count) to[e] = static_cast<uint8_t>(w >> (8 * e));
+            for (int t = 0; t < 4; ++t)
+                if (whole || (4 * quad + t >= slot && 4 * quad + t < end)) *reinterpret_cast<uint2*>(codes + ((4 * quad + t) * d + piece * 8) / 4) = make_uint2(w[t][0], w[t][1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                // byte i of each token's eight
+                const int sel = i & 3, half = i >> 2;
+                const uint32_t lo = __builtin_amdgcn_perm(w[1][half], w[0][half], (0x0c0c0400u + sel * 0x0101u)), hi = __builtin_amdgcn_perm(w[3][half], w[2][half], (0x0c0c0400u + sel * 0x0101u));
+                const uint32_t four = lo | hi << 16;
+                uint32_t* const to = codes + ((piece * 8 + i) * page + 4 * quad) / 4;
+                if (whole) {
+                    *to = four;
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        if (4 * quad + t >= slot && 4 * quad + t < end) reinterpret_cast<uint8_t*>(to)[t] = static_cast<uint8_t>(four >> (8 * t));
+                }
+            }
         }
     }
 }
@@ -178,15 +207,21 @@ extern "C" int rocm_launch_cache_append(const RocmCacheAppendArgs* args, rocm_st
     // a sequence with n tokens touches at most n / page + 2 pages, and at most n
     const int64_t pages = args->rows < c.sequences ? args->rows : args->rows / c.page + 2 * static_cast<int64_t>(c.sequences);
     const dim3 grid(static_cast<unsigned>(pages < args->rows ? pages : args->rows), static_cast<unsigned>(c.kv_heads), 2);
-    const unsigned lds = static_cast<unsigned>(c.head_size * (c.page + 4));
+    const int units = c.head_size / 8 * (c.page / 4);          // of a whole page; few new tokens fill the first of a thread's alone
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, s, *args);
+        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, *args);
         return static_cast<int>(hipGetLastError());
     };
     auto typed = [&](auto t, auto bf) {
         using T = decltype(t);
         constexpr bool BF16 = decltype(bf)::value;
-        return c.code_dtype == ROCM_DT_E4M3 ? go(append_kernel<T, BF16, true>) : go(append_kernel<T, BF16, false>);
+        auto coded = [&](auto e4m3) {
+            constexpr bool E4M3 = decltype(e4m3)::value;
+            if (units <= kThreads) return go(append_kernel<T, BF16, E4M3, 1>);
+            if (units <= 2 * kThreads) return go(append_kernel<T, BF16, E4M3, 2>);
+            return go(append_kernel<T, BF16, E4M3, 4>);
+        };
+        return c.code_dtype == ROCM_DT_E4M3 ? coded(std::true_type{}) : coded(std::false_type{});
     };
     if (args->dtype == ROCM_DT_F32) return typed(float{}, std::false_type{});
     if (args->dtype == ROCM_DT_BF16) return typed(uint16_t{}, std::true_type{});

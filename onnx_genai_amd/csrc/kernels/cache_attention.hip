@@ -277,67 +277,66 @@ __global__ __launch_bounds__(kThreads) void attention_few_kernel(AttentionParams
             const float inverse = total == 0.f ? 0.f : 1.0f / total;
             const int r = first_row + row, tk = r / p.group;
             uint16_t* const to = static_cast<uint16_t*>(p.a.y) + static_cast<int64_t>(w.s.first + tk) * out_step + (head * p.group + r - tk * p.group) * D + e;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) to[j] = narrow(all[j] * inverse, p.a.dtype);
+            store_four(to, all[0] * inverse, all[1] * inverse, all[2] * inverse, all[3] * inverse, p.a.dtype);
         }
     }
 }
 
-// The pieces of a tile joined: a workgroup for two rows, its waves a quarter of the pieces each, in an order that is always the same.
-__global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionParams p, int d)
+// The pieces of a tile joined, in an order that is always the same. A workgroup has some rows of it; what a piece counts for in a row is found first, by a wave over the pieces
+// of a row, so that the sums over the pieces wait for nothing but their loads.
+constexpr int kMostPieces = 1025;                    // of a tile: the target and one more
+__global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionParams p, int d, int rows_at_once)
 {
-    __shared__ float results[kWaves][2][ROCM_CACHE_MAX_HEAD];
-    __shared__ float2 sums[kWaves][2];
+    extern __shared__ __attribute__((aligned(16))) float shares[];      // [rows_at_once][pieces], then [threads][4]
     const RocmCache& c = p.a.cache;
     const int head = blockIdx.x % c.kv_heads;
     Piece w;
     if (!tile_to_join(p, blockIdx.x / c.kv_heads, &w)) return;
     const int first_row = w.tile * p.tile_rows, left = w.s.rows * p.group - first_row, rows = left < p.tile_rows ? left : p.tile_rows;
+    const int row0 = blockIdx.y * rows_at_once;
+    if (row0 >= rows) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int which = lane >> 5, row = blockIdx.y * 2 + which;
-    if (static_cast<int>(blockIdx.y) * 2 >= rows) return;
-    const int from_row = row < rows ? row : rows - 1;
-    float most = kNone, total = 0.f, all[ROCM_CACHE_MAX_HEAD / 32];
-#pragma unroll
-    for (int j = 0; j < ROCM_CACHE_MAX_HEAD / 32; ++j) all[j] = 0.f;
-    for (int i = wave; i < w.pieces; i += kWaves) {
-        const int64_t place = (static_cast<int64_t>(w.slot + i) * c.kv_heads + head) * p.tile_rows + from_row;
-        const float2 s = p.partial_sums[place];
-        const float now = fmaxf(most, s.x), zero = now == kNone ? 0.f : now;
-        const float old = __builtin_amdgcn_exp2f(most - zero), fresh = __builtin_amdgcn_exp2f(s.x - zero);
-        total = total * old + s.y * fresh;
-        most = now;
-#pragma unroll
-        for (int j = 0; j < ROCM_CACHE_MAX_HEAD / 32; ++j) {
-            const int e = (lane & 31) + 32 * j;
-            if (e < d) all[j] = all[j] * old + p.partial[place * d + e] * fresh;
+    const int64_t piece_step = static_cast<int64_t>(c.kv_heads) * p.tile_rows, first = (static_cast<int64_t>(w.slot) * c.kv_heads + head) * p.tile_rows;
+    for (int r = wave; r < rows_at_once; r += kWaves) {
+        const int row = row0 + r < rows ? row0 + r : rows - 1;
+        float most = kNone;
+        for (int i = lane; i < w.pieces; i += 64) most = fmaxf(most, p.partial_sums[first + i * piece_step + row].x);
+        most = over_wave(most, [](float x, float y) { return fmaxf(x, y); });
+        const float zero = most == kNone ? 0.f : most;
+        float sum = 0.f;
+        for (int i = lane; i < w.pieces; i += 64) {
+            const float2 s = p.partial_sums[first + i * piece_step + row];
+            const float share = __builtin_amdgcn_exp2f(s.x - zero);
+            sum += s.y * share;
+            shares[r * w.pieces + i] = share;
         }
+        sum = over_wave(sum, [](float x, float y) { return x + y; });
+        const float inverse = sum == 0.f ? 0.f : 1.0f / sum;
+        for (int i = lane; i < w.pieces; i += 64) shares[r * w.pieces + i] *= inverse;
     }
-#pragma unroll
-    for (int j = 0; j < ROCM_CACHE_MAX_HEAD / 32; ++j) {
-        const int e = (lane & 31) + 32 * j;
-        if (e < d) results[wave][which][e] = all[j];
-    }
-    if ((lane & 31) == 0) sums[wave][which] = make_float2(most, total);
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * d; i += kThreads) {
-        const int r = i / d, e = i - r * d, out_row = static_cast<int>(blockIdx.y) * 2 + r;
-        if (out_row >= rows) continue;
-        float peak = kNone;
-#pragma unroll
-        for (int j = 0; j < kWaves; ++j) peak = fmaxf(peak, sums[j][r].x);
-        const float zero = peak == kNone ? 0.f : peak;
-        float sum = 0.f, value = 0.f;
-#pragma unroll
-        for (int j = 0; j < kWaves; ++j) {
-            const float f = __builtin_amdgcn_exp2f(sums[j][r].x - zero);
-            sum += sums[j][r].y * f;
-            value += results[j][r][e] * f;
+    // a group of d / 4 threads has a row's elements, four each, over every so many pieces
+    const int quads = d / 4, groups = kThreads / quads, each = groups / rows_at_once;
+    const int group = threadIdx.x / quads, quad = threadIdx.x - group * quads, r = group / each, part = group - r * each;
+    float4_t* const sums = reinterpret_cast<float4_t*>(shares + (rows_at_once * w.pieces + 3) / 4 * 4);
+    float4_t all = {0.f, 0.f, 0.f, 0.f};
+    const bool busy = r < rows_at_once && row0 + r < rows;
+    if (busy) {
+        const float* const from = p.partial + (first + row0 + r) * d + quad * 4;
+        const float* const share = shares + r * w.pieces;
+#pragma unroll 8
+        for (int i = part; i < w.pieces; i += each) {
+            const float4_t v = *reinterpret_cast<const float4_t*>(from + i * piece_step * d);
+            const float f = share[i];
+            all += v * f;
         }
-        const int row_of_all = first_row + out_row, tk = row_of_all / p.group;
-        const int64_t to = static_cast<int64_t>(w.s.first + tk) * p.a.heads * d + (head * p.group + row_of_all - tk * p.group) * d + e;
-        static_cast<uint16_t*>(p.a.y)[to] = narrow(sum == 0.f ? 0.f : value / sum, p.a.dtype);
     }
+    sums[threadIdx.x] = all;
+    __syncthreads();
+    if (!busy || part != 0) return;
+    for (int i = 1; i < each; ++i) all += sums[threadIdx.x + i * quads];
+    const int row = first_row + row0 + r, tk = row / p.group;
+    store_four(static_cast<uint16_t*>(p.a.y) + (static_cast<int64_t>(w.s.first + tk) * p.a.heads + head * p.group + row - tk * p.group) * d + quad * 4, all[0], all[1], all[2], all[3], p.a.dtype);
 }
 
 struct Plan {
@@ -360,10 +359,12 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
     plan.many = a.rows * group > 32 * static_cast<int64_t>(c.sequences);
     plan.tile_rows = plan.many ? kManyRows : kRows;
     plan.tiles = a.rows * group / plan.tile_rows + (a.rows < c.sequences ? a.rows : c.sequences);
-    // Pieces until there are four workgroups for each CU (two of many rows), none shorter than the 256 tokens that the waves of a workgroup of few rows take in one step.
-    const int64_t wanted = (plan.many ? 2 : 4) * static_cast<int64_t>(rocm_ffi_compute_units()) / c.kv_heads;
-    plan.least = kWaves;
-    if (plan.tiles < wanted && static_cast<int64_t>(c.width) * c.page > kGroup * plan.least) plan.target = static_cast<int>(wanted > 0 ? wanted : 1);
+    // Pieces until there are two workgroups for each CU, as many as fit on it at once, none shorter than 1024 tokens (few rows: four steps of each wave; one piece
+    // of 1000 tokens and no launch to join takes less time than four) or 256.
+    int64_t wanted = 2 * static_cast<int64_t>(rocm_ffi_compute_units()) / c.kv_heads;
+    if (wanted > kMostPieces - 1) wanted = kMostPieces - 1;
+    plan.least = plan.many ? 4 : 16;
+    if (plan.tiles < wanted && static_cast<int64_t>(c.width) * c.page > kGroup * plan.least) plan.target = static_cast<int>(wanted);
     plan.pieces = plan.tiles + plan.target;
     const uint64_t places = 2 * static_cast<uint64_t>(plan.target) * c.kv_heads * plan.tile_rows;
     plan.sums_at = (places * c.head_size * 4 + 255) / 256 * 256;
@@ -422,8 +423,10 @@ extern "C" int rocm_launch_cache_attention(const RocmCacheAttentionArgs* args, v
     const dim3 grid(static_cast<unsigned>(plan.pieces * args->cache.kv_heads));
     hipError_t e = plan.many ? launch_attention_rows(p, grid, s) : args->cache.code_dtype == ROCM_DT_E4M3 ? launch_few<true>(p, grid, s) : launch_few<false>(p, grid, s);
     if (e == hipSuccess && plan.target) {
-        hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<unsigned>(plan.tiles * args->cache.kv_heads), static_cast<unsigned>((plan.tile_rows + 1) / 2)), dim3(kThreads), 0, s, p,
-                           args->cache.head_size);
+        // two groups of threads a row where tiles have many rows, all of them where they have few
+        const int d = args->cache.head_size, groups = kThreads / (d / 4), rows = plan.many ? groups / 2 : 1;
+        const unsigned lds = static_cast<unsigned>((rows * (plan.target + 1) + 3) / 4 * 16 + kThreads * 16);
+        hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<unsigned>(plan.tiles * args->cache.kv_heads), static_cast<unsigned>((plan.tile_rows + rows - 1) / rows)), dim3(kThreads), lds, s, p, d, rows);
         e = hipGetLastError();
     }
     return static_cast<int>(e);

@@ -301,10 +301,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
                 const int e = u * 32 + a * 8 + h * 4;
-                if (D % 32 == 0 || e < D) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) to[e + i] = narrow(o[u][4 * a + i] * inverse, p.a.dtype);
-                }
+                if (D % 32 == 0 || e < D) store_four(to + e, o[u][4 * a] * inverse, o[u][4 * a + 1] * inverse, o[u][4 * a + 2] * inverse, o[u][4 * a + 3] * inverse, p.a.dtype);
             }
     }
 }

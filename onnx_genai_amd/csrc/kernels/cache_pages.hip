@@ -6,7 +6,7 @@
 // Compacting: with n pages in use, the ones from n on, in rising order, go to the free ones below n, in rising order. No page is read and written by one call.
 //
 // Two launches. The first, one workgroup, holds a bit for each page in LDS and ranks pages and slots by sums over the workgroup; what it costs is its trips through
-// the tables. The second copies: a workgroup for 8 KB of a page, of each layer and pool; memory bounds it.
+// the tables. The second copies: a workgroup for 8 KB of a move: a part of a page, or its pages in several layers; memory bounds it.
 #include "common.hiph"
 
 namespace mnb {
@@ -186,41 +186,50 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
 
 struct CopyPlan {
     int pieces[ROCM_PAGES_MAX_POOLS];      // workgroups for one move, up to and with each pool
+    int layers[ROCM_PAGES_MAX_POOLS];      // layers of a workgroup: several of pools with small pages
 };
+
+// A pool's units of W bytes: those of one move that workgroup `index` of the pool has.
+template <typename W>
+__device__ __forceinline__ void copy_units(const RocmCachePagesArgs& a, const PagesWorkspace& w, const RocmPool& pool, int index, int layers, int moves)
+{
+    constexpr int kWhole = kCopyBytes / kCopyThreads / static_cast<int>(sizeof(W)), kEach = kWhole < 8 ? kWhole : 8;
+    const int parts = static_cast<int>((pool.page_bytes + kCopyBytes - 1) / kCopyBytes);          // of a page; 1 where layers > 1
+    const int layer0 = index / parts * layers;
+    const int64_t skip = static_cast<int64_t>(index % parts) * kCopyBytes, left = pool.page_bytes - skip;
+    const int units = static_cast<int>(left < kCopyBytes ? left : kCopyBytes) / static_cast<int>(sizeof(W));
+    const int these = pool.layers - layer0 < layers ? static_cast<int>(pool.layers - layer0) : layers, all = units * these;
+    // where a thread's units lie in a page of the pool's first layer
+    int64_t at[kEach];
+    for (int base = 0; base < all; base += kEach * kCopyThreads) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int u = base + threadIdx.x + i * kCopyThreads, layer = these > 1 ? u / units : 0;
+            at[i] = u < all ? (layer0 + layer) * a.pages * pool.page_bytes + skip + static_cast<int64_t>(u - layer * units) * static_cast<int>(sizeof(W)) : -1;
+        }
+        for (int m = blockIdx.y; m < moves; m += gridDim.y) {
+            const uint8_t* const from = static_cast<const uint8_t*>(pool.at) + w.from[m] * pool.page_bytes;
+            uint8_t* const to = static_cast<uint8_t*>(pool.at) + w.to[m] * pool.page_bytes;
+            W v[kEach];
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) v[i] = at[i] >= 0 ? *reinterpret_cast<const W*>(from + at[i]) : W{};
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                if (at[i] >= 0) *reinterpret_cast<W*>(to + at[i]) = v[i];
+        }
+    }
+}
 
 __global__ __launch_bounds__(kCopyThreads) void copy_kernel(RocmCachePagesArgs a, PagesWorkspace w, CopyPlan plan)
 {
     int k = 0;
     while (static_cast<int>(blockIdx.x) >= plan.pieces[k]) ++k;
-    const int index = blockIdx.x - (k ? plan.pieces[k - 1] : 0);
+    const int index = blockIdx.x - (k ? plan.pieces[k - 1] : 0), moves = *w.count;
     const RocmPool pool = a.pool[k];
-    const int parts = static_cast<int>((pool.page_bytes + kCopyBytes - 1) / kCopyBytes);
-    const int layer = index / parts;
-    const int64_t skip = static_cast<int64_t>(index - layer * parts) * kCopyBytes, left = pool.page_bytes - skip;
-    const int bytes = left < kCopyBytes ? static_cast<int>(left) : kCopyBytes;
-    uint8_t* const base = static_cast<uint8_t*>(pool.at) + static_cast<int64_t>(layer) * a.pages * pool.page_bytes + skip;
-    const bool wide = (reinterpret_cast<uintptr_t>(pool.at) | static_cast<uint64_t>(pool.page_bytes)) % 16 == 0;
-    const int moves = *w.count;
-    for (int m = blockIdx.y; m < moves; m += gridDim.y) {
-        const uint8_t* const from = base + w.from[m] * pool.page_bytes;
-        uint8_t* const to = base + w.to[m] * pool.page_bytes;
-        if (wide) {
-            constexpr int kEach = kCopyBytes / 16 / kCopyThreads;
-            uint4 v[kEach];
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int at = (threadIdx.x + i * kCopyThreads) * 16;
-                v[i] = at < bytes ? *reinterpret_cast<const uint4*>(from + at) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int at = (threadIdx.x + i * kCopyThreads) * 16;
-                if (at < bytes) *reinterpret_cast<uint4*>(to + at) = v[i];
-            }
-        } else {
-            for (int at = threadIdx.x; at < bytes; at += kCopyThreads) to[at] = from[at];
-        }
-    }
+    const uint64_t aligned = reinterpret_cast<uintptr_t>(pool.at) | static_cast<uint64_t>(pool.page_bytes);
+    if (aligned % 16 == 0) copy_units<uint4>(a, w, pool, index, plan.layers[k], moves);
+    else if (aligned % 4 == 0) copy_units<uint32_t>(a, w, pool, index, plan.layers[k], moves);
+    else copy_units<uint8_t>(a, w, pool, index, plan.layers[k], moves);
 }
 
 }  // namespace
@@ -242,7 +251,10 @@ extern "C" int rocm_launch_cache_pages(const RocmCachePagesArgs* args, void* wor
     CopyPlan plan{};
     int64_t pieces = 0;
     for (int i = 0; i < args->pools; ++i) {
-        pieces += args->pool[i].layers * ((args->pool[i].page_bytes + kCopyBytes - 1) / kCopyBytes);
+        const RocmPool& pool = args->pool[i];
+        const int64_t together = pool.page_bytes > 0 && pool.page_bytes < kCopyBytes ? kCopyBytes / pool.page_bytes : 1;
+        plan.layers[i] = static_cast<int>(together < pool.layers ? together : pool.layers > 0 ? pool.layers : 1);
+        pieces += (pool.layers + plan.layers[i] - 1) / plan.layers[i] * ((pool.page_bytes + kCopyBytes - 1) / kCopyBytes);
         if (pieces >= (1 << 20)) return static_cast<int>(hipErrorInvalidValue);
         plan.pieces[i] = static_cast<int>(pieces);
     }
