@@ -74,7 +74,7 @@ struct Queries {
 };
 
 template <int D, bool E4M3>
-__global__ __launch_bounds__(kThreads) void attention_few_kernel(AttentionParams p)
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_few_kernel(AttentionParams p)
 {
     constexpr int kChunks = (D + 63) / 64, kTiles = D / 16;
     __shared__ float results[kWaves][kRows][D + 4];
@@ -184,44 +184,55 @@ __global__ __launch_bounds__(kThreads) void attention_few_kernel(AttentionParams
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[e] = capped(x[e], p.a.softcap);
         }
-        const bool masked = __ballot(live < 16) != 0 || t0 + kGroup - 1 > first_own || (window > 0 && t0 <= last_own - window);
-        uint32_t seen = 0xffffu;                     // bit e: the row sees token e of the lane's
-        if (masked) {
+        half8_t weights[2];
+        float again;
+        // MASKED: some row does not see some token of the step; seen: bit e for the lane's row and token e of its
+        auto softmax = [&](auto masked, uint32_t seen) {
+            constexpr bool MASKED = decltype(masked)::value;
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = (seen >> e) & 1 ? x[e] : kNone;
+            }
+            float most = x[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) most = fmaxf(most, x[e]);
+            most = fmaxf(top, over_groups_max(most));
+            const float zero = most == kNone ? 0.f : most;                      // (a row that has seen nothing yet)
+            const float shrink = __builtin_amdgcn_exp2f(top - zero);
+            top = most;
+            const float before = reference;
+            reference = fmaxf(reference, over_groups_max(live ? value_scale : 0.f));
+            // weights relative to the largest page scale so far
+            const float relative = reference > 0.f ? value_scale / reference : 0.f;
+            again = shrink * (reference > before ? before / reference : 1.f);
+            sum *= shrink;
+            float part = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float y = __builtin_amdgcn_exp2f(x[e] - (zero - kWeightBits));
+                if constexpr (MASKED) y = (seen >> e) & 1 ? y : 0.f;
+                part += y;
+                float weight = y * relative;
+                if constexpr (MASKED) weight = (seen >> e) & 1 ? weight : 0.f;
+                weights[e >> 3][e & 7] = static_cast<_Float16>(weight);
+            }
+            sum += part;
+        };
+        const bool partial = __ballot(live < 16) != 0;
+        if (partial || t0 + kGroup - 1 > first_own || (window > 0 && t0 <= last_own - window)) {
             const int here = t0 + g * 16;
             const int hi = own - here + 1 < live ? own - here + 1 : live, lo = window > 0 ? own - window + 1 - here : 0;
-            seen = hi > 0 ? 0xffffu >> (16 - (hi < 16 ? hi : 16)) : 0u;
+            uint32_t seen = hi > 0 ? 0xffffu >> (16 - (hi < 16 ? hi : 16)) : 0u;
             if (lo > 0) seen &= lo < 16 ? 0xffffu << lo : 0u;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = (seen >> e) & 1 ? x[e] : kNone;
+            softmax(std::true_type{}, seen);
+        } else {
+            softmax(std::false_type{}, 0u);
         }
-        float most = x[0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) most = fmaxf(most, x[e]);
-        most = fmaxf(top, over_groups_max(most));
-        const float zero = most == kNone ? 0.f : most;                          // (a row that has seen nothing yet)
-        const float shrink = __builtin_amdgcn_exp2f(top - zero);
-        top = most;
-        const float before = reference;
-        reference = fmaxf(reference, over_groups_max(live ? value_scale : 0.f));
-        // weights relative to the largest page scale so far
-        const float relative = reference > 0.f ? value_scale / reference : 0.f;
-        const float again = shrink * (reference > before ? before / reference : 1.f);
-        sum *= shrink;
-        float part = 0.f;
-        half8_t weights[2];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            float y = __builtin_amdgcn_exp2f(x[e] - (zero - kWeightBits));
-            if (masked) y = (seen >> e) & 1 ? y : 0.f;
-            part += y;
-            weights[e >> 3][e & 7] = static_cast<_Float16>(masked && !((seen >> e) & 1) ? 0.f : y * relative);
-        }
-        sum += part;
         if (__ballot(again != 1.f)) {
 #pragma unroll
             for (int u = 0; u < kTiles; ++u) o[u] *= again;
         }
-        if (masked && __ballot(live < 16)) {
+        if (partial) {
             // what lies behind the context may be anything
             uint32_t keep[4];
 #pragma unroll

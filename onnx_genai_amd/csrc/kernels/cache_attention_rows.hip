@@ -29,10 +29,12 @@ struct Tile {
     int there[4];
 };
 
-template <int D, bool E4M3>
+// WIDE: pages of 64 tokens or more, so that a step lies in one.
+template <int D, bool E4M3, bool WIDE>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_kernel(AttentionParams p)
 {
     constexpr int kSteps = D / 16, kOut = (D + 31) / 32, kPieces = 4 * D, kEach = (kPieces + kThreads - 1) / kThreads;
+    constexpr int kPages = WIDE ? 1 : 4;                         // that a step's scales are of
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     Tile<D>* const tiles = reinterpret_cast<Tile<D>*>(lds);
     const RocmCache& c = p.a.cache;
@@ -95,40 +97,57 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
         const int t = group * kGroup + sub * 16;
         return t < context ? page_of(c, w.b, t >> page_bits) : -1;
     };
-    // a thread's 16-byte pieces of a step: piece i of the keys is 16 elements of token i / (D / 16), of the values 16 tokens of element i / 4
+    // A thread's 16-byte pieces of a step. Keys: piece i is 16 elements of token i / (D / 16). Values: 16 tokens of an element; of a wide page piece i is of element i / 4 and tokens
+    // 16 (i % 4) on, 64 bytes of an element together; else of element i % D and tokens 16 (i / D) on, so that a piece of keys and one of values are of the same 16 tokens, and
+    // with D a multiple of 64, all of a wave's pieces.
+    constexpr bool kOneOfWave = WIDE || D % 64 == 0;
     uint4 keys[kEach], values[kEach];
-    int key_page[kEach], value_page = -1, scale_page = -1;
+    int pages[kEach], scale_page = -1;                           // of the step to be loaded next, -1: none
     float key_scale = 0.f, value_scale = 0.f;
+    auto sub_of = [&](int j) {
+        const int i = threadIdx.x + j * kThreads;
+        if constexpr (WIDE) return static_cast<int>(threadIdx.x & 3);
+        else if constexpr (kOneOfWave) return (wave * 64 + j * kThreads) / D;
+        else return i / D & 3;
+    };
     auto find_pages = [&](int group) {
+        if constexpr (WIDE) {
+            scale_page = __builtin_amdgcn_readfirstlane(page_id(group, 0));
+        } else {
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) key_page[j] = page_id(group, ((threadIdx.x + j * kThreads) / (D / 16)) >> 4 & 3);
-        value_page = page_id(group, threadIdx.x & 3);
-        scale_page = value_page;
+            for (int j = 0; j < kEach; ++j) {
+                pages[j] = page_id(group, sub_of(j));
+                if constexpr (kOneOfWave) pages[j] = __builtin_amdgcn_readfirstlane(pages[j]);
+            }
+            scale_page = page_id(group, threadIdx.x & 3);
+        }
     };
     auto load = [&](int group) {
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
             const int i = threadIdx.x + j * kThreads;
             if (kPieces % kThreads == 0 || i < kPieces) {
-                const int t = i / (D / 16), col = i - t * (D / 16);
-                const int64_t at = (static_cast<int64_t>(key_page[j] < 0 ? 0 : key_page[j]) * c.kv_heads + head) * page_bytes;
-                keys[j] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(c.k) + at + ((group * kGroup + t) & (c.page - 1)) * D + col * 16);
-                const int64_t from = (static_cast<int64_t>(value_page < 0 ? 0 : value_page) * c.kv_heads + head) * page_bytes;
-                values[j] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(c.v) + from + (i >> 2) * c.page + ((group * kGroup + (i & 3) * 16) & (c.page - 1)));
+                const int page = WIDE ? scale_page : pages[j], sub = WIDE ? 0 : sub_of(j), skip = (group * kGroup + sub * 16) & (c.page - 1);
+                const int64_t at = (static_cast<int64_t>(page < 0 ? 0 : page) * c.kv_heads + head) * page_bytes;
+                const uint32_t within = static_cast<uint32_t>(i - sub * D);
+                keys[j] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(c.k) + at + skip * D + within * 16);
+                values[j] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(c.v) + at + skip + (WIDE ? (within >> 2) * static_cast<uint32_t>(c.page) + (within & 3) * 16 : within * static_cast<uint32_t>(c.page)));
             }
         }
-        if (threadIdx.x < 4) {
+        if (threadIdx.x < kPages) {
             const int64_t at = static_cast<int64_t>(scale_page < 0 ? 0 : scale_page) * c.kv_heads + head;
             key_scale = c.k_scale[at];
             value_scale = c.v_scale[at];
         }
     };
-    auto store = [&](int group, Tile<D>& tile, int at_page) {
-        const int live = at_page < 0 ? 0 : clamped(context - (group * kGroup + (threadIdx.x & 3) * 16), 0, 16);
-        if (__ballot(live < 16)) {
-            // what lies behind the context may be anything
+    // `there`: bit j, the page of the thread's pieces j was one; of_scale: that of its scales was
+    auto store = [&](int group, Tile<D>& tile, uint32_t there, bool of_scale) {
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) {
+        for (int j = 0; j < kEach; ++j) {
+            const int i = threadIdx.x + j * kThreads, sub = sub_of(j);
+            const int live = (there >> j) & 1 ? clamped(context - (group * kGroup + sub * 16), 0, 16) : 0;
+            if (WIDE ? !(there & 1) || (group + 1) * kGroup > context : __ballot(live < 16) != 0) {
+                // what lies behind the context may be anything
                 uint32_t* const d = &values[j].x;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -136,10 +155,6 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
                     d[e] &= l >= 4 ? 0xffffffffu : l <= 0 ? 0u : 0xffffffffu >> (32 - 8 * l);
                 }
             }
-        }
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const int i = threadIdx.x + j * kThreads;
             if (kPieces % kThreads == 0 || i < kPieces) {
                 const int t = i / (D / 16), col = i - t * (D / 16);
                 half8_t lo, hi;
@@ -148,19 +163,26 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
                 k[0] = lo;
                 k[1] = hi;
                 widen<E4M3>(values[j], lo, hi);
-                half8_t* const v = reinterpret_cast<half8_t*>(tile.v + (i >> 2) * Tile<D>::kValuePitch + (i & 3) * 32);
+                half8_t* const v = reinterpret_cast<half8_t*>(tile.v + (WIDE ? i >> 2 : i - sub * D) * Tile<D>::kValuePitch + sub * 32);
                 v[0] = lo;
                 v[1] = hi;
             }
         }
-        if (threadIdx.x < 4) {
+        if (threadIdx.x < kPages) {
             tile.key_scale[threadIdx.x] = key_scale;
             // a page of scale 0 (its codes are 0) weighs as the smallest scale does
             const float scale = value_scale < 1.17549435e-38f ? 1.17549435e-38f : value_scale;
-            tile.value_bits[threadIdx.x] = at_page < 0 ? -126.f : __builtin_amdgcn_logf(scale);
+            tile.value_bits[threadIdx.x] = of_scale ? __builtin_amdgcn_logf(scale) : -126.f;
             tile.value_inverse[threadIdx.x] = 1.0f / scale;
-            tile.there[threadIdx.x] = at_page >= 0;
+            tile.there[threadIdx.x] = of_scale;
         }
+    };
+    auto are_there = [&]() {
+        if constexpr (WIDE) return scale_page >= 0 ? ~0u : 0u;
+        uint32_t bits = 0;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) bits |= pages[j] >= 0 ? 1u << j : 0u;
+        return bits;
     };
 
     float16_t o[kOut];
@@ -173,15 +195,15 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
     if (w.span.lo < w.span.hi) {
         find_pages(w.span.lo);
         load(w.span.lo);
-        const int page = value_page;
-        store(w.span.lo, tiles[0], page);
+        store(w.span.lo, tiles[0], are_there(), scale_page >= 0);
         find_pages(w.span.lo + 1);
     }
     for (int at = w.span.lo, turn = 0; at < w.span.hi; ++at, turn ^= 1) {
         __syncthreads();
         const Tile<D>& tile = tiles[turn];
         const bool more = at + 1 < w.span.hi;
-        const int page_ahead = value_page;
+        const uint32_t there_ahead = are_there();
+        const bool scale_ahead = scale_page >= 0;
         if (more) {
             load(at + 1);
             find_pages(at + 2);
@@ -200,69 +222,81 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) score[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(from + i * 32), q[i], score[b], 0, 0, 0);
             }
-            float ks[4], bits[4], inverse[4];
+            float ks[kPages], bits[kPages], inverse[kPages];
             int there = 15;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
+            for (int s = 0; s < kPages; ++s) {
                 ks[s] = tile.key_scale[s] * row_scale;
                 bits[s] = tile.value_bits[s];
                 inverse[s] = tile.value_inverse[s];
-                there &= tile.there[s] ? 15 : 15 ^ (1 << s);
+                there &= tile.there[s] ? 15 : WIDE ? 0 : 15 ^ (1 << s);
             }
             if (p.a.softcap > 0.f) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) score[s >> 1][8 * (s & 1) + j] = capped(score[s >> 1][8 * (s & 1) + j] * ks[s], p.a.softcap);
-                    ks[s] = 1.f;
-                }
-            }
-            const bool masked = there != 15 || t0 + kGroup - 1 > first_own || t0 + kGroup > context || (window > 0 && t0 <= last_own - window);
-            const int hi = last_seen - t0 - 8 * h, lo = window > 0 ? own - window + 1 - t0 - 8 * h : -8;
-            auto seen = [&](int s, int j) { return 16 * s + j <= hi && 16 * s + j >= lo && ((there >> s) & 1); };
-            if (masked) {
-#pragma unroll
                 for (int s = 0; s < 4; ++s)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) score[s >> 1][8 * (s & 1) + j] = seen(s, j) ? score[s >> 1][8 * (s & 1) + j] : kNone;
-            }
-            float most = top;
+                    for (int j = 0; j < 8; ++j) score[s >> 1][8 * (s & 1) + j] = capped(score[s >> 1][8 * (s & 1) + j] * ks[s % kPages], p.a.softcap);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                float m = score[s >> 1][8 * (s & 1)];
-#pragma unroll
-                for (int j = 1; j < 8; ++j) m = fmaxf(m, score[s >> 1][8 * (s & 1) + j]);
-                most = fmaxf(most, m * ks[s]);
+                for (int s = 0; s < kPages; ++s) ks[s] = 1.f;
             }
-            {
-                const uint32_t a = __float_as_uint(most);
-                const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
-                most = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-            }
-            const float zero = most == kNone ? 0.f : most;                      // (a row that has seen nothing yet)
-            const float shrink = __builtin_amdgcn_exp2f(top - zero);
-            top = most;
-            const float before = reference;
-#pragma unroll
-            for (int s = 0; s < 4; ++s) reference = fmaxf(reference, bits[s]);
-            const float largest = __builtin_amdgcn_exp2f(reference);
-            const float again = shrink * __builtin_amdgcn_exp2f(before - reference);
-            sum *= shrink;
             half8_t weights[4];
+            float again;
+            // MASKED: some row of the wave does not see some token of the step; seen: bit 8 s + j for the lane's row and its tokens
+            auto softmax = [&](auto masked, uint32_t seen) {
+                constexpr bool MASKED = decltype(masked)::value;
+                if constexpr (MASKED) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                // (a NaN scale stays one)
-                const float share = bits[s] < reference - kLeastShare ? -kLeastShare : bits[s] - reference;
-                const float off = zero - kWeightBits - share;
-                float part = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float y = __builtin_amdgcn_exp2f(fmaf(score[s >> 1][8 * (s & 1) + j], ks[s], -off));
-                    if (masked) y = seen(s, j) ? y : 0.f;
-                    part += y;
-                    weights[s][j] = static_cast<_Float16>(y);
+                    for (int e = 0; e < 32; ++e) score[e >> 4][e & 15] = (seen >> e) & 1 ? score[e >> 4][e & 15] : kNone;
                 }
-                sum = fmaf(part, fminf(largest * inverse[s], 1152921504606846976.f), sum);
+                float most = top;
+#pragma unroll
+                for (int s = 0; s < 4; s += 4 / kPages) {
+                    float m = score[s >> 1][8 * (s & 1)];
+#pragma unroll
+                    for (int e = 8 * s + 1; e < 8 * s + 32 / kPages; ++e) m = fmaxf(m, score[e >> 4][e & 15]);
+                    most = fmaxf(most, m * ks[s % kPages]);
+                }
+                {
+                    const uint32_t a = __float_as_uint(most);
+                    const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+                    most = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+                }
+                const float zero = most == kNone ? 0.f : most;                  // (a row that has seen nothing yet)
+                const float shrink = __builtin_amdgcn_exp2f(top - zero);
+                top = most;
+                const float before = reference;
+#pragma unroll
+                for (int s = 0; s < kPages; ++s) reference = fmaxf(reference, bits[s]);
+                const float largest = __builtin_amdgcn_exp2f(reference);
+                again = shrink * __builtin_amdgcn_exp2f(before - reference);
+                sum *= shrink;
+#pragma unroll
+                for (int s = 0; s < 4; s += 4 / kPages) {
+                    // (a NaN scale stays one)
+                    const float share = bits[s % kPages] < reference - kLeastShare ? -kLeastShare : bits[s % kPages] - reference;
+                    const float off = zero - kWeightBits - share;
+                    float part = 0.f;
+#pragma unroll
+                    for (int e = 8 * s; e < 8 * s + 32 / kPages; ++e) {
+                        float y = __builtin_amdgcn_exp2f(fmaf(score[e >> 4][e & 15], ks[s % kPages], -off));
+                        if constexpr (MASKED) y = (seen >> e) & 1 ? y : 0.f;
+                        part += y;
+                        weights[e >> 3][e & 7] = static_cast<_Float16>(y);
+                    }
+                    sum = fmaf(part, fminf(largest * inverse[s % kPages], 1152921504606846976.f), sum);
+                }
+            };
+            if (there != 15 || t0 + kGroup - 1 > first_own || t0 + kGroup > context || (window > 0 && t0 <= last_own - window)) {
+                const int hi = last_seen - t0 - 8 * h, lo = window > 0 ? own - window + 1 - t0 - 8 * h : -8;
+                uint32_t seen = 0;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const int end = clamped(hi + 1 - 16 * s, 0, 8), begin = clamped(lo - 16 * s, 0, 8);
+                    if ((there >> s) & 1) seen |= ((1u << end) - 1u & ~((1u << begin) - 1u)) << (8 * s);
+                }
+                softmax(std::true_type{}, seen);
+            } else {
+                softmax(std::false_type{}, 0u);
             }
             if (__ballot(again != 1.f)) {
 #pragma unroll
@@ -275,7 +309,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
                 for (int s = 0; s < 4; ++s) o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(from + s * 32), weights[s], o[u], 0, 0, 0);
             }
         }
-        if (more) store(at + 1, tiles[turn ^ 1], page_ahead);
+        if (more) store(at + 1, tiles[turn ^ 1], there_ahead, scale_ahead);
     }
 
     // o[u][4 a + i] is element 32 u + 8 a + 4 h + i of row n
@@ -306,27 +340,27 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
     }
 }
 
-template <int D, bool E4M3>
+template <int D, bool E4M3, bool WIDE>
 hipError_t launch(const AttentionParams& p, dim3 grid, hipStream_t s)
 {
     constexpr size_t kLds = 2 * sizeof(Tile<D>);
     if (kLds > 65536) {              // more than a kernel gets without asking
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attention_rows_kernel<D, E4M3>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLds));
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attention_rows_kernel<D, E4M3, WIDE>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLds));
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((attention_rows_kernel<D, E4M3>), grid, dim3(kThreads), kLds, s, p);
+    hipLaunchKernelGGL((attention_rows_kernel<D, E4M3, WIDE>), grid, dim3(kThreads), kLds, s, p);
     return hipGetLastError();
 }
 
-template <bool E4M3>
+template <bool E4M3, bool WIDE>
 hipError_t launch_of(const AttentionParams& p, dim3 grid, hipStream_t s)
 {
     switch (p.a.cache.head_size) {
-        case 64: return launch<64, E4M3>(p, grid, s);
-        case 80: return launch<80, E4M3>(p, grid, s);
-        case 96: return launch<96, E4M3>(p, grid, s);
-        case 128: return launch<128, E4M3>(p, grid, s);
-        case 256: return launch<256, E4M3>(p, grid, s);
+        case 64: return launch<64, E4M3, WIDE>(p, grid, s);
+        case 80: return launch<80, E4M3, WIDE>(p, grid, s);
+        case 96: return launch<96, E4M3, WIDE>(p, grid, s);
+        case 128: return launch<128, E4M3, WIDE>(p, grid, s);
+        case 256: return launch<256, E4M3, WIDE>(p, grid, s);
         default: return hipErrorInvalidValue;
     }
 }
@@ -335,7 +369,9 @@ hipError_t launch_of(const AttentionParams& p, dim3 grid, hipStream_t s)
 
 hipError_t launch_attention_rows(const AttentionParams& p, dim3 grid, hipStream_t stream)
 {
-    return p.a.cache.code_dtype == ROCM_DT_E4M3 ? launch_of<true>(p, grid, stream) : launch_of<false>(p, grid, stream);
+    const bool wide = p.a.cache.page >= kGroup;
+    if (p.a.cache.code_dtype == ROCM_DT_E4M3) return wide ? launch_of<true, true>(p, grid, stream) : launch_of<true, false>(p, grid, stream);
+    return wide ? launch_of<false, true>(p, grid, stream) : launch_of<false, false>(p, grid, stream);
 }
 
 }  // namespace mnb
