@@ -7,8 +7,8 @@
 // the maximum of a row. The 16 tokens lie in one page, which holds 16 at least, and their page's scale is one number a lane.
 //
 // Codes are exact in f16, as 8-bit integers and as e4m3. Queries go to f16 with their row's largest at 2^8 (what falls below f16's range is less than 2^-22 of it).
-// Weights p = exp(s - max) are held as p * 2^14 * (scale of the values' page / largest such scale so far) in f16: rounded to 11 bits, down to 2^-28 of the largest
-// weight, below that to 2^-38; sums and all products are in f32.
+// Weights p = exp(s - max) are held as p * 2^11 * (scale of the values' page / largest such scale so far) in f16: rounded to 11 bits, down to 2^-25 of the largest
+// weight, below that to 2^-36 of it; sums and all products are in f32.
 #include "cache_attention.hiph"
 
 namespace mnb {
@@ -105,11 +105,13 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_few_kern
     for (int u = 0; u < kTiles; ++u) o[u] = float4_t{0.f, 0.f, 0.f, 0.f};
     float top = kNone, sum = 0.f, reference = 0.f;
 
-    // The page of 16 tokens of a step: sub-block n / 4 for the lane's keys, g for its values and scales; -1: none. Tokens behind the context have none either.
+    // The page of 16 tokens of a step: sub-block n / 4 for the lane's keys, g for its values and scales. A step's entries of the table are asked for a step before its keys.
     const int page_bits = __builtin_ctz(c.page);
-    auto page_id = [&](int group, int sub) {
-        const int t = group * kGroup + sub * 16;
-        return t < context ? page_of(c, w.b, t >> page_bits) : -1;
+    const int32_t* const table = c.table + static_cast<int64_t>(w.b) * c.width;
+    int key_entry = 0, value_entry = 0;
+    auto ask = [&](int group) {
+        key_entry = entry_of(c, table, page_bits, group * kGroup + (n >> 2) * 16);
+        value_entry = entry_of(c, table, page_bits, group * kGroup + g * 16);
     };
     struct Step {
         uint4 k[4][kChunks], v[kTiles];
@@ -144,15 +146,17 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_few_kern
     };
 
     Step s;
-    int at = w.span.lo + wave, key_page = -1, value_page = -1;
+    int at = w.span.lo + wave, value_page = -1;
+    auto find = [&](int group) {
+        value_page = page_from(c, value_entry, group * kGroup + g * 16, context);
+        return page_from(c, key_entry, group * kGroup + (n >> 2) * 16, context);
+    };
     if (at < w.span.hi) {
-        key_page = page_id(at, n >> 2);
-        value_page = page_id(at, g);
-        load_keys(at, key_page, s);
+        ask(at);
+        load_keys(at, find(at), s);
         load_scales(at, value_page, s);
+        ask(at + kWaves);
         load_values(at, value_page, s);
-        key_page = page_id(at + kWaves, n >> 2);
-        value_page = page_id(at + kWaves, g);
     }
     for (; at < w.span.hi; at += kWaves) {
         const int t0 = at * kGroup;
@@ -174,8 +178,9 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_few_kern
         // the next step's keys, scales and page numbers while this one goes on
         const bool more = at + kWaves < w.span.hi;
         if (more) {
-            load_keys(at + kWaves, key_page, s);
+            load_keys(at + kWaves, find(at + kWaves), s);
             load_scales(at + kWaves, value_page, s);
+            ask(at + 2 * kWaves);
         }
         float x[16];
 #pragma unroll
@@ -184,54 +189,51 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_few_kern
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[e] = capped(x[e], p.a.softcap);
         }
-        half8_t weights[2];
-        float again;
-        // MASKED: some row does not see some token of the step; seen: bit e for the lane's row and token e of its
-        auto softmax = [&](auto masked, uint32_t seen) {
-            constexpr bool MASKED = decltype(masked)::value;
-            if constexpr (MASKED) {
+        // where some row does not see some token: bit e of `seen` for the lane's row and token e of its
+        const bool partial = __ballot(live < 16) != 0, masked = partial || t0 + kGroup - 1 > first_own || (window > 0 && t0 <= last_own - window);
+        uint32_t seen = 0;
+        if (masked) {
+            const int here = t0 + g * 16;
+            const int end = clamped(own - here + 1, 0, live), begin = window > 0 ? clamped(own - window + 1 - here, 0, 16) : 0;
+            seen = ((1u << end) - 1u) & ~((1u << begin) - 1u);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = (seen >> e) & 1 ? x[e] : kNone;
-            }
-            float most = x[0];
+            for (int e = 0; e < 16; ++e) x[e] = (seen >> e) & 1 ? x[e] : kNone;
+        }
+        float most = x[0];
 #pragma unroll
-            for (int e = 1; e < 16; ++e) most = fmaxf(most, x[e]);
-            most = fmaxf(top, over_groups_max(most));
-            const float zero = most == kNone ? 0.f : most;                      // (a row that has seen nothing yet)
-            const float shrink = __builtin_amdgcn_exp2f(top - zero);
-            top = most;
-            const float before = reference;
-            reference = fmaxf(reference, over_groups_max(live ? value_scale : 0.f));
-            // weights relative to the largest page scale so far
-            const float relative = reference > 0.f ? value_scale / reference : 0.f;
-            again = shrink * (reference > before ? before / reference : 1.f);
+        for (int e = 1; e < 16; ++e) most = fmaxf(most, x[e]);
+        most = fmaxf(top, over_groups_max(most));
+        const float next = fmaxf(reference, over_groups_max(live ? value_scale : 0.f));
+        // What weights are relative to stays until something is kSlack bits above it: sums and values are seldom scaled again.
+        if (__ballot(most > top + kSlack || next > reference)) {
+            const float shrink = __builtin_amdgcn_exp2f(top - (most == kNone ? 0.f : most));
+            const float again = shrink * (next > reference ? reference / next : 1.f);
             sum *= shrink;
+            top = most;
+            reference = next;
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u) o[u] *= again;
+        }
+        const float zero = top == kNone ? 0.f : top;                            // (a row that has seen nothing yet)
+        // weights relative to the largest page scale so far
+        const float relative = reference > 0.f ? value_scale / reference : 0.f;
+        half8_t weights[2];
+        auto weigh = [&](auto some) {
             float part = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                float y = __builtin_amdgcn_exp2f(x[e] - (zero - kWeightBits));
-                if constexpr (MASKED) y = (seen >> e) & 1 ? y : 0.f;
+                float y = __builtin_amdgcn_exp2f(x[e] - (zero - kWeightBits)), weight = y * relative;
+                if constexpr (decltype(some)::value) {
+                    y = (seen >> e) & 1 ? y : 0.f;
+                    weight = (seen >> e) & 1 ? weight : 0.f;
+                }
                 part += y;
-                float weight = y * relative;
-                if constexpr (MASKED) weight = (seen >> e) & 1 ? weight : 0.f;
                 weights[e >> 3][e & 7] = static_cast<_Float16>(weight);
             }
             sum += part;
         };
-        const bool partial = __ballot(live < 16) != 0;
-        if (partial || t0 + kGroup - 1 > first_own || (window > 0 && t0 <= last_own - window)) {
-            const int here = t0 + g * 16;
-            const int hi = own - here + 1 < live ? own - here + 1 : live, lo = window > 0 ? own - window + 1 - here : 0;
-            uint32_t seen = hi > 0 ? 0xffffu >> (16 - (hi < 16 ? hi : 16)) : 0u;
-            if (lo > 0) seen &= lo < 16 ? 0xffffu << lo : 0u;
-            softmax(std::true_type{}, seen);
-        } else {
-            softmax(std::false_type{}, 0u);
-        }
-        if (__ballot(again != 1.f)) {
-#pragma unroll
-            for (int u = 0; u < kTiles; ++u) o[u] *= again;
-        }
+        if (masked) weigh(std::true_type{});
+        else weigh(std::false_type{});
         if (partial) {
             // what lies behind the context may be anything
             uint32_t keep[4];
@@ -250,11 +252,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_few_kern
             o[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, weights[0], o[u], 0, 0, 0);
             o[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, weights[1], o[u], 0, 0, 0);
         }
-        if (more) {
-            load_values(at + kWaves, value_page, s);
-            key_page = page_id(at + 2 * kWaves, n >> 2);
-            value_page = page_id(at + 2 * kWaves, g);
-        }
+        if (more) load_values(at + kWaves, value_page, s);
     }
 
     // the waves' results: o[u][i] is element 16 u + 4 g + i of row n

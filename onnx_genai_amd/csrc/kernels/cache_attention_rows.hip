@@ -93,16 +93,14 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 
     const int page_bits = __builtin_ctz(c.page);
     const int64_t page_bytes = static_cast<int64_t>(c.page) * D;
-    auto page_id = [&](int group, int sub) {
-        const int t = group * kGroup + sub * 16;
-        return t < context ? page_of(c, w.b, t >> page_bits) : -1;
-    };
     // A thread's 16-byte pieces of a step. Keys: piece i is 16 elements of token i / (D / 16). Values: 16 tokens of an element; of a wide page piece i is of element i / 4 and tokens
     // 16 (i % 4) on, 64 bytes of an element together; else of element i % D and tokens 16 (i / D) on, so that a piece of keys and one of values are of the same 16 tokens, and
     // with D a multiple of 64, all of a wave's pieces.
     constexpr bool kOneOfWave = WIDE || D % 64 == 0;
     uint4 keys[kEach], values[kEach];
-    int pages[kEach], scale_page = -1;                           // of the step to be loaded next, -1: none
+    const int32_t* const table = c.table + static_cast<int64_t>(w.b) * c.width;
+    int entries[kEach], scale_entry = 0;                         // of the table, for the step to be loaded next: asked for a step ahead, looked at when it begins
+    int pages[kEach], scale_page = -1;                           // -1: none
     float key_scale = 0.f, value_scale = 0.f;
     auto sub_of = [&](int j) {
         const int i = threadIdx.x + j * kThreads;
@@ -110,16 +108,23 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
         else if constexpr (kOneOfWave) return (wave * 64 + j * kThreads) / D;
         else return i / D & 3;
     };
+    auto ask = [&](int group) {
+        if constexpr (!WIDE) {
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) entries[j] = entry_of(c, table, page_bits, group * kGroup + sub_of(j) * 16);
+        }
+        scale_entry = entry_of(c, table, page_bits, group * kGroup + (WIDE ? 0 : threadIdx.x & 3) * 16);
+    };
     auto find_pages = [&](int group) {
+        scale_page = page_from(c, scale_entry, group * kGroup + (WIDE ? 0 : threadIdx.x & 3) * 16, context);
         if constexpr (WIDE) {
-            scale_page = __builtin_amdgcn_readfirstlane(page_id(group, 0));
+            scale_page = __builtin_amdgcn_readfirstlane(scale_page);
         } else {
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
-                pages[j] = page_id(group, sub_of(j));
+                pages[j] = page_from(c, entries[j], group * kGroup + sub_of(j) * 16, context);
                 if constexpr (kOneOfWave) pages[j] = __builtin_amdgcn_readfirstlane(pages[j]);
             }
-            scale_page = page_id(group, threadIdx.x & 3);
         }
     };
     auto load = [&](int group) {
@@ -190,23 +195,23 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
     for (int u = 0; u < kOut; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[u][i] = 0.f;
-    float top = kNone, sum = 0.f, reference = -126.f;           // reference: log2 of the largest value scale so far
+    float top = kNone, sum = 0.f, reference = -126.f, largest = 0.f;           // reference: log2 of the largest value scale so far
 
     if (w.span.lo < w.span.hi) {
+        ask(w.span.lo);
         find_pages(w.span.lo);
         load(w.span.lo);
+        ask(w.span.lo + 1);
         store(w.span.lo, tiles[0], are_there(), scale_page >= 0);
-        find_pages(w.span.lo + 1);
     }
     for (int at = w.span.lo, turn = 0; at < w.span.hi; ++at, turn ^= 1) {
         __syncthreads();
         const Tile<D>& tile = tiles[turn];
         const bool more = at + 1 < w.span.hi;
-        const uint32_t there_ahead = are_there();
-        const bool scale_ahead = scale_page >= 0;
         if (more) {
+            find_pages(at + 1);
             load(at + 1);
-            find_pages(at + 2);
+            ask(at + 2);
         }
         const int t0 = at * kGroup;
         const bool skipped = rows <= 0 || t0 > last_own || (window > 0 && t0 + kGroup - 1 <= first_own - window);
@@ -214,14 +219,16 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
             // scores: lane (n, h) gets token 16 s + 8 h + j of row n in score[s / 2][8 (s % 2) + j]
             float16_t score[2];
             const int order = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
+            const uint8_t* const key = tile.k + order * Tile<D>::kKeyPitch + h * 16;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+            for (int i = 0; i < 16; ++i) score[0][i] = score[1][i] = 0.f;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) score[b][i] = 0.f;
-                const uint8_t* const from = tile.k + (b * 32 + order) * Tile<D>::kKeyPitch + h * 16;
+            for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) score[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(from + i * 32), q[i], score[b], 0, 0, 0);
-            }
+                for (int b = 0; b < 2; ++b)
+                    score[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(key + b * 32 * Tile<D>::kKeyPitch + i * 32), q[i], score[b], 0, 0, 0);
+            __builtin_amdgcn_s_setprio(0);
             float ks[kPages], bits[kPages], inverse[kPages];
             int there = 15;
 #pragma unroll
@@ -239,37 +246,47 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 #pragma unroll
                 for (int s = 0; s < kPages; ++s) ks[s] = 1.f;
             }
-            half8_t weights[4];
-            float again;
-            // MASKED: some row of the wave does not see some token of the step; seen: bit 8 s + j for the lane's row and its tokens
-            auto softmax = [&](auto masked, uint32_t seen) {
-                constexpr bool MASKED = decltype(masked)::value;
-                if constexpr (MASKED) {
+            // where some row of the wave does not see some token: bit 8 s + j of `seen` for the lane's row and its tokens
+            const bool masked = there != 15 || t0 + kGroup - 1 > first_own || t0 + kGroup > context || (window > 0 && t0 <= last_own - window);
+            uint32_t seen = 0;
+            if (masked) {
+                const int hi = last_seen - t0 - 8 * h, lo = window > 0 ? own - window + 1 - t0 - 8 * h : -8;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) score[e >> 4][e & 15] = (seen >> e) & 1 ? score[e >> 4][e & 15] : kNone;
+                for (int s = 0; s < 4; ++s) {
+                    const int end = clamped(hi + 1 - 16 * s, 0, 8), begin = clamped(lo - 16 * s, 0, 8);
+                    if ((there >> s) & 1) seen |= (((1u << end) - 1u) & ~((1u << begin) - 1u)) << (8 * s);
                 }
-                float most = top;
 #pragma unroll
-                for (int s = 0; s < 4; s += 4 / kPages) {
-                    float m = score[s >> 1][8 * (s & 1)];
+                for (int e = 0; e < 32; ++e) score[e >> 4][e & 15] = (seen >> e) & 1 ? score[e >> 4][e & 15] : kNone;
+            }
+            float most = top, next = reference;
 #pragma unroll
-                    for (int e = 8 * s + 1; e < 8 * s + 32 / kPages; ++e) m = fmaxf(m, score[e >> 4][e & 15]);
-                    most = fmaxf(most, m * ks[s % kPages]);
-                }
-                {
-                    const uint32_t a = __float_as_uint(most);
-                    const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
-                    most = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-                }
-                const float zero = most == kNone ? 0.f : most;                  // (a row that has seen nothing yet)
-                const float shrink = __builtin_amdgcn_exp2f(top - zero);
-                top = most;
-                const float before = reference;
+            for (int s = 0; s < 4; s += 4 / kPages) {
+                float m = score[s >> 1][8 * (s & 1)];
 #pragma unroll
-                for (int s = 0; s < kPages; ++s) reference = fmaxf(reference, bits[s]);
-                const float largest = __builtin_amdgcn_exp2f(reference);
-                again = shrink * __builtin_amdgcn_exp2f(before - reference);
+                for (int e = 8 * s + 1; e < 8 * s + 32 / kPages; ++e) m = fmaxf(m, score[e >> 4][e & 15]);
+                most = fmaxf(most, m * ks[s % kPages]);
+                next = fmaxf(next, bits[s % kPages]);
+            }
+            {
+                const uint32_t a = __float_as_uint(most);
+                const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+                most = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+            }
+            // What weights are relative to stays until something is kSlack bits above it: sums and values are seldom scaled again.
+            if (__ballot(most > top + kSlack || next > reference)) {
+                const float shrink = __builtin_amdgcn_exp2f(top - (most == kNone ? 0.f : most));
+                const float again = shrink * __builtin_amdgcn_exp2f(reference - next);
                 sum *= shrink;
+                top = most;
+                reference = next;
+                largest = __builtin_amdgcn_exp2f(reference);
+#pragma unroll
+                for (int u = 0; u < kOut; ++u) o[u] *= again;
+            }
+            const float zero = top == kNone ? 0.f : top;                        // (a row that has seen nothing yet)
+            half8_t weights[4];
+            auto weigh = [&](auto some) {
 #pragma unroll
                 for (int s = 0; s < 4; s += 4 / kPages) {
                     // (a NaN scale stays one)
@@ -279,37 +296,25 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 #pragma unroll
                     for (int e = 8 * s; e < 8 * s + 32 / kPages; ++e) {
                         float y = __builtin_amdgcn_exp2f(fmaf(score[e >> 4][e & 15], ks[s % kPages], -off));
-                        if constexpr (MASKED) y = (seen >> e) & 1 ? y : 0.f;
+                        if constexpr (decltype(some)::value) y = (seen >> e) & 1 ? y : 0.f;
                         part += y;
                         weights[e >> 3][e & 7] = static_cast<_Float16>(y);
                     }
                     sum = fmaf(part, fminf(largest * inverse[s % kPages], 1152921504606846976.f), sum);
                 }
             };
-            if (there != 15 || t0 + kGroup - 1 > first_own || t0 + kGroup > context || (window > 0 && t0 <= last_own - window)) {
-                const int hi = last_seen - t0 - 8 * h, lo = window > 0 ? own - window + 1 - t0 - 8 * h : -8;
-                uint32_t seen = 0;
+            if (masked) weigh(std::true_type{});
+            else weigh(std::false_type{});
+            __builtin_amdgcn_s_setprio(1);
+            const uint8_t* const from = tile.v + n * Tile<D>::kValuePitch + h * 16;
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const int end = clamped(hi + 1 - 16 * s, 0, 8), begin = clamped(lo - 16 * s, 0, 8);
-                    if ((there >> s) & 1) seen |= ((1u << end) - 1u & ~((1u << begin) - 1u)) << (8 * s);
-                }
-                softmax(std::true_type{}, seen);
-            } else {
-                softmax(std::false_type{}, 0u);
-            }
-            if (__ballot(again != 1.f)) {
+            for (int s = 0; s < 4; ++s)
 #pragma unroll
-                for (int u = 0; u < kOut; ++u) o[u] *= again;
-            }
-#pragma unroll
-            for (int u = 0; u < kOut; ++u) {
-                const uint8_t* const from = tile.v + (u * 32 + n) * Tile<D>::kValuePitch + h * 16;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(from + s * 32), weights[s], o[u], 0, 0, 0);
-            }
+                for (int u = 0; u < kOut; ++u)
+                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(from + u * 32 * Tile<D>::kValuePitch + s * 32), weights[s], o[u], 0, 0, 0);
+            __builtin_amdgcn_s_setprio(0);
         }
-        if (more) store(at + 1, tiles[turn ^ 1], there_ahead, scale_ahead);
+        if (more) store(at + 1, tiles[turn ^ 1], are_there(), scale_page >= 0);
     }
 
     // o[u][4 a + i] is element 32 u + 8 a + 4 h + i of row n

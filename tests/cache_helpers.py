@@ -126,6 +126,8 @@ def attention64(cache, q, heads, *, scale=None, window=0, softcap=0.0, size=Fals
             continue
         k, v = cache.tokens(i, cache.past[i] + n)
         slot = np.arange(cache.past[i] + n)
+        page, place = cache.table[i, slot // cache.page], slot % cache.page
+        codes, top = decode(cache.v[page, :, :, place], cache.code), np.nanmax(cache.vs[page], 0)
         for r in range(n):
             own, row = cache.past[i] + r, cache.ends[i] + r
             seen = (slot <= own) & ((slot > own - window) if window else True)
@@ -138,9 +140,10 @@ def attention64(cache, q, heads, *, scale=None, window=0, softcap=0.0, size=Fals
                 w /= w.sum()
                 y[row, h] = w @ vv
                 # scores: products of f16 operands (a query's bits reach 2^-22 of its row's largest) summed in f32, then a few f32 steps; weights: a rounding to 11 bits,
-                # those of f32 and of the exponential, and what f16 loses below 2^-28 of the largest
+                # those of f32 and of the exponential; and half of f16's smallest step, 2^-25, of weights that are held times 2^11 or more (relative to the row's largest) and times
+                # their page's scale over the largest such scale: 2^-36 of a value whose page had that scale
                 off = scale * (np.abs(kk).sum(-1) * np.abs(qq).max() * 2.0 ** -22 + np.abs(kk) @ np.abs(qq) * (d + 8) * 2.0 ** -24).max() + 2.0 ** -20
-                slack[row, h] = (w * (2.0 ** -11 + 2 * off)) @ np.abs(vv) + 2.0 ** -38 * np.abs(vv).sum(0)
+                slack[row, h] = (w * (2.0 ** -11 + 2 * off)) @ np.abs(vv) + 2.0 ** -36 * top[h // group] * np.abs(codes[seen, h // group]).sum(0)
     return y, slack
 
 
