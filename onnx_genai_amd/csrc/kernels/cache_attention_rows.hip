@@ -20,6 +20,21 @@ constexpr float kLeastShare = 60.f;          // bits that a page's scale may lie
 typedef __attribute__((ext_vector_type(16))) float float16_t;
 typedef __attribute__((ext_vector_type(4))) float float4_t;
 
+// The order of N matrix instructions and the reads out of LDS of an operand each: reads stay kAhead in front, which covers what a read takes.
+constexpr int kAhead = 6;
+template <int N>
+__device__ __forceinline__ void reads_ahead()
+{
+    constexpr int kMatrix = 0x008, kRead = 0x100, kFirst = N < kAhead ? N : kAhead;
+    __builtin_amdgcn_sched_group_barrier(kRead, kFirst, 0);
+#pragma unroll
+    for (int i = 0; i < N - kFirst; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kMatrix, kFirst, 0);
+}
+
 template <int D>
 struct Tile {
     static constexpr int kKeyPitch = D * 2 + 16, kValuePitch = kGroup * 2 + 16, kValueRows = (D + 31) / 32 * 32;
@@ -228,6 +243,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
                     score[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(key + b * 32 * Tile<D>::kKeyPitch + i * 32), q[i], score[b], 0, 0, 0);
+            reads_ahead<2 * kSteps>();
             __builtin_amdgcn_s_setprio(0);
             float ks[kPages], bits[kPages], inverse[kPages];
             int there = 15;
@@ -312,6 +328,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 #pragma unroll
                 for (int u = 0; u < kOut; ++u)
                     o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(from + u * 32 * Tile<D>::kValuePitch + s * 32), weights[s], o[u], 0, 0, 0);
+            reads_ahead<4 * kOut>();
             __builtin_amdgcn_s_setprio(0);
         }
         if (more) store(at + 1, tiles[turn ^ 1], are_there(), scale_page >= 0);
