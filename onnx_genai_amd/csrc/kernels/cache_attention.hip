@@ -294,7 +294,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_few_kern
 // The pieces of a tile joined, in an order that is always the same. A workgroup has some rows of it; what a piece counts for in a row is found first, by a wave over the pieces
 // of a row, so that the sums over the pieces wait for nothing but their loads.
 constexpr int kMostPieces = 1025;                    // of a tile: the target and one more
-__global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionParams p, int d, int rows_at_once)
+__global__ __launch_bounds__(kThreads, 6) void attention_join_kernel(AttentionParams p, int d, int rows_at_once)
 {
     extern __shared__ __attribute__((aligned(16))) float shares[];      // [rows_at_once][pieces], then [threads][4]
     const RocmCache& c = p.a.cache;
@@ -306,8 +306,21 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionParam
     if (row0 >= rows) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t piece_step = static_cast<int64_t>(c.kv_heads) * p.tile_rows, first = (static_cast<int64_t>(w.slot) * c.kv_heads + head) * p.tile_rows;
-    for (int r = wave; r < rows_at_once; r += kWaves) {
-        const int row = row0 + r < rows ? row0 + r : rows - 1;
+    // a group of d / 4 threads has a row's elements, four each, over every so many pieces; the first of them are on their way before anything is known of their shares
+    const int quads = d / 4, groups = kThreads / quads, each = groups / rows_at_once;
+    const int group = threadIdx.x / quads, quad = threadIdx.x - group * quads, r = group / each, part = group - r * each;
+    const bool busy = r < rows_at_once && row0 + r < rows;
+    const float* const from = p.partial + (first + row0 + (busy ? r : 0)) * d + quad * 4;
+    constexpr int kEarly = 4;
+    float4_t early[kEarly];
+#pragma unroll
+    for (int j = 0; j < kEarly; ++j) {
+        const int i = part + j * each;
+        early[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+        if (busy && i < w.pieces) early[j] = *reinterpret_cast<const float4_t*>(from + i * piece_step * d);
+    }
+    for (int k = wave; k < rows_at_once; k += kWaves) {
+        const int row = row0 + k < rows ? row0 + k : rows - 1;
         float most = kNone;
         for (int i = lane; i < w.pieces; i += 64) most = fmaxf(most, p.partial_sums[first + i * piece_step + row].x);
         most = over_wave(most, [](float x, float y) { return fmaxf(x, y); });
@@ -317,24 +330,22 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionParam
             const float2 s = p.partial_sums[first + i * piece_step + row];
             const float share = __builtin_amdgcn_exp2f(s.x - zero);
             sum += s.y * share;
-            shares[r * w.pieces + i] = share;
+            shares[k * w.pieces + i] = share;
         }
         sum = over_wave(sum, [](float x, float y) { return x + y; });
         const float inverse = sum == 0.f ? 0.f : 1.0f / sum;
-        for (int i = lane; i < w.pieces; i += 64) shares[r * w.pieces + i] *= inverse;
+        for (int i = lane; i < w.pieces; i += 64) shares[k * w.pieces + i] *= inverse;
     }
     __syncthreads();
-    // a group of d / 4 threads has a row's elements, four each, over every so many pieces
-    const int quads = d / 4, groups = kThreads / quads, each = groups / rows_at_once;
-    const int group = threadIdx.x / quads, quad = threadIdx.x - group * quads, r = group / each, part = group - r * each;
     float4_t* const sums = reinterpret_cast<float4_t*>(shares + (rows_at_once * w.pieces + 3) / 4 * 4);
     float4_t all = {0.f, 0.f, 0.f, 0.f};
-    const bool busy = r < rows_at_once && row0 + r < rows;
     if (busy) {
-        const float* const from = p.partial + (first + row0 + r) * d + quad * 4;
         const float* const share = shares + r * w.pieces;
-#pragma unroll 8
-        for (int i = part; i < w.pieces; i += each) {
+#pragma unroll
+        for (int j = 0; j < kEarly; ++j)
+            if (part + j * each < w.pieces) all += early[j] * share[part + j * each];
+#pragma unroll 4
+        for (int i = part + kEarly * each; i < w.pieces; i += each) {
             const float4_t v = *reinterpret_cast<const float4_t*>(from + i * piece_step * d);
             const float f = share[i];
             all += v * f;
@@ -350,7 +361,7 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttentionParam
 
 struct Plan {
     bool ok, many;
-    int tile_rows, target, least;
+    int tile_rows, target, least, teams;
     int64_t tiles, pieces;          // most that a call of these sizes has, for one key head
     uint64_t sums_at, bytes;
 };
@@ -367,13 +378,21 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
     // From 32 rows a sequence on, on average, tiles share what they read of the cache through LDS.
     plan.many = a.rows * group > 32 * static_cast<int64_t>(c.sequences);
     plan.tile_rows = plan.many ? kManyRows : kRows;
-    plan.tiles = a.rows * group / plan.tile_rows + (a.rows < c.sequences ? a.rows : c.sequences);
-    // Pieces until there are two workgroups for each CU, as many as fit on it at once, none shorter than 1024 tokens (few rows: four steps of each wave; one piece
-    // of 1000 tokens and no launch to join takes less time than four) or 256.
-    int64_t wanted = 2 * static_cast<int64_t>(rocm_ffi_compute_units()) / c.kv_heads;
+    // 256 rows a tile, which halves what a row costs of the codes' way into LDS, once that gives two tiles for each CU; 128 rows with two teams of waves, which halves the steps that follow one
+    // another, where there is no more than one tile for each CU. (4096 tokens over 32 heads by 8: 175 us, in tiles of 128 206 us; 2400 new tokens, 28 by 4: 54 us, with two teams
+    // 68 us; 700 tokens, 32 by 32 heads of 80: 32 us with two teams, 43 us with one.)
+    const int64_t cus = rocm_ffi_compute_units(), per_head = a.rows * group;
+    const bool small = c.head_size <= 128;
+    if (plan.many && small && per_head * c.kv_heads >= 2 * kMostRows * cus) plan.tile_rows = kMostRows;
+    plan.teams = plan.many && small && per_head * c.kv_heads <= kManyRows * cus ? 2 : 1;
+    plan.tiles = per_head / plan.tile_rows + (a.rows < c.sequences ? a.rows : c.sequences);
+    // Pieces until there are as many workgroups as fit on the GPU at once: two for each CU, or one of 512 threads or heads of 256. None is shorter than 512 tokens, or 1024 in tiles of
+    // many rows: joining them costs about what so many take. (One of 8 chunks in a window of 1024, 1111 rows over 14 heads by 2: 31 us whole, 35 us in pieces of 512.)
+    const int64_t at_once = plan.many && (plan.teams == 2 || plan.tile_rows == kMostRows || !small) ? cus : 2 * cus;
+    int64_t wanted = at_once / c.kv_heads;
     if (wanted > kMostPieces - 1) wanted = kMostPieces - 1;
-    plan.least = plan.many ? 4 : 16;
-    if (plan.tiles < wanted && static_cast<int64_t>(c.width) * c.page > kGroup * plan.least) plan.target = static_cast<int>(wanted);
+    plan.least = plan.many ? 16 : 8;
+    if (plan.tiles < wanted && static_cast<int64_t>(c.width) * c.page >= kGroup * 2 * plan.least) plan.target = static_cast<int>(wanted);
     plan.pieces = plan.tiles + plan.target;
     const uint64_t places = 2 * static_cast<uint64_t>(plan.target) * c.kv_heads * plan.tile_rows;
     plan.sums_at = (places * c.head_size * 4 + 255) / 256 * 256;
@@ -425,6 +444,7 @@ extern "C" int rocm_launch_cache_attention(const RocmCacheAttentionArgs* args, v
     p.tile_rows = plan.tile_rows;
     p.target = plan.target;
     p.least = plan.least;
+    p.teams = plan.teams;
     p.slots = 2 * plan.target;
     p.scale = args->softcap > 0.f ? args->scale : args->scale * 1.442695041f;
     p.partial = static_cast<float*>(workspace);
@@ -432,8 +452,8 @@ extern "C" int rocm_launch_cache_attention(const RocmCacheAttentionArgs* args, v
     const dim3 grid(static_cast<unsigned>(plan.pieces * args->cache.kv_heads));
     hipError_t e = plan.many ? launch_attention_rows(p, grid, s) : args->cache.code_dtype == ROCM_DT_E4M3 ? launch_few<true>(p, grid, s) : launch_few<false>(p, grid, s);
     if (e == hipSuccess && plan.target) {
-        // two groups of threads a row where tiles have many rows, all of them where they have few
-        const int d = args->cache.head_size, groups = kThreads / (d / 4), rows = plan.many ? groups / 2 : 1;
+        // A row's pieces are many where there are few tiles: then all groups of threads have one row, else two groups each.
+        const int d = args->cache.head_size, groups = kThreads / (d / 4), rows = plan.tiles <= 2 ? 1 : groups / 2;
         const unsigned lds = static_cast<unsigned>((rows * (plan.target + 1) + 3) / 4 * 16 + kThreads * 16);
         hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<unsigned>(plan.tiles * args->cache.kv_heads), static_cast<unsigned>((plan.tile_rows + rows - 1) / rows)), dim3(kThreads), lds, s, p, d, rows);
         e = hipGetLastError();

@@ -13,8 +13,7 @@
 namespace mnb {
 namespace {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves, kWaveRows = 32;
-static_assert(kWaves * kWaveRows == kManyRows, "rows of a tile");
+constexpr int kWaveRows = 32;
 constexpr float kLeastShare = 60.f;          // bits that a page's scale may lie below the largest one: what is further below counts as this
 
 typedef __attribute__((ext_vector_type(16))) float float16_t;
@@ -45,9 +44,11 @@ struct Tile {
 };
 
 // WIDE: pages of 64 tokens or more, so that a step lies in one.
-template <int D, bool E4M3, bool WIDE>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_kernel(AttentionParams p)
+// TEAMS 2: two teams of waves over the same rows, each every other step, their results joined in LDS: where there are few workgroups, half as many steps follow one another.
+template <int D, bool E4M3, bool WIDE, int WAVES, int TEAMS>
+__global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) : 1) void attention_rows_kernel(AttentionParams p)
 {
+    constexpr int kThreads = 64 * WAVES, kRows = WAVES * kWaveRows;
     constexpr int kSteps = D / 16, kOut = (D + 31) / 32, kPieces = 4 * D, kEach = (kPieces + kThreads - 1) / kThreads;
     constexpr int kPages = WIDE ? 1 : 4;                         // that a step's scales are of
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -56,13 +57,14 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
     const int head = blockIdx.x % c.kv_heads;
     Piece w;
     if (!piece_at(p, blockIdx.x / c.kv_heads, &w)) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads) : 0, thread = threadIdx.x - team * kThreads;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int context = context_of(c, w.s);
     const bool bf16 = p.a.dtype == ROCM_DT_BF16;
 
     // the lane's query row: half h has the elements 16 i + 8 h of it
-    const int first_row = w.tile * kManyRows + wave * kWaveRows, left = w.s.rows * p.group - first_row, rows = left < kWaveRows ? left : kWaveRows;
+    const int first_row = w.tile * kRows + wave * kWaveRows, left = w.s.rows * p.group - first_row, rows = left < kWaveRows ? left : kWaveRows;
     const int token = (first_row + n) / p.group, member = first_row + n - token * p.group;
     const int own = w.s.past + token, last_seen = own < context ? own : context - 1;
     half8_t q[kSteps];
@@ -118,8 +120,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
     int pages[kEach], scale_page = -1;                           // -1: none
     float key_scale = 0.f, value_scale = 0.f;
     auto sub_of = [&](int j) {
-        const int i = threadIdx.x + j * kThreads;
-        if constexpr (WIDE) return static_cast<int>(threadIdx.x & 3);
+        const int i = thread + j * kThreads;
+        if constexpr (WIDE) return static_cast<int>(thread & 3);
         else if constexpr (kOneOfWave) return (wave * 64 + j * kThreads) / D;
         else return i / D & 3;
     };
@@ -128,10 +130,10 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 #pragma unroll
             for (int j = 0; j < kEach; ++j) entries[j] = entry_of(c, table, page_bits, group * kGroup + sub_of(j) * 16);
         }
-        scale_entry = entry_of(c, table, page_bits, group * kGroup + (WIDE ? 0 : threadIdx.x & 3) * 16);
+        scale_entry = entry_of(c, table, page_bits, group * kGroup + (WIDE ? 0 : thread & 3) * 16);
     };
     auto find_pages = [&](int group) {
-        scale_page = page_from(c, scale_entry, group * kGroup + (WIDE ? 0 : threadIdx.x & 3) * 16, context);
+        scale_page = page_from(c, scale_entry, group * kGroup + (WIDE ? 0 : thread & 3) * 16, context);
         if constexpr (WIDE) {
             scale_page = __builtin_amdgcn_readfirstlane(scale_page);
         } else {
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
     auto load = [&](int group) {
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            const int i = threadIdx.x + j * kThreads;
+            const int i = thread + j * kThreads;
             if (kPieces % kThreads == 0 || i < kPieces) {
                 const int page = WIDE ? scale_page : pages[j], sub = WIDE ? 0 : sub_of(j), skip = (group * kGroup + sub * 16) & (c.page - 1);
                 const int64_t at = (static_cast<int64_t>(page < 0 ? 0 : page) * c.kv_heads + head) * page_bytes;
@@ -154,7 +156,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
                 values[j] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(c.v) + at + skip + (WIDE ? (within >> 2) * static_cast<uint32_t>(c.page) + (within & 3) * 16 : within * static_cast<uint32_t>(c.page)));
             }
         }
-        if (threadIdx.x < kPages) {
+        if (thread < kPages) {
             const int64_t at = static_cast<int64_t>(scale_page < 0 ? 0 : scale_page) * c.kv_heads + head;
             key_scale = c.k_scale[at];
             value_scale = c.v_scale[at];
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
     auto store = [&](int group, Tile<D>& tile, uint32_t there, bool of_scale) {
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            const int i = threadIdx.x + j * kThreads, sub = sub_of(j);
+            const int i = thread + j * kThreads, sub = sub_of(j);
             const int live = (there >> j) & 1 ? clamped(context - (group * kGroup + sub * 16), 0, 16) : 0;
             if (WIDE ? !(there & 1) || (group + 1) * kGroup > context : __ballot(live < 16) != 0) {
                 // what lies behind the context may be anything
@@ -188,13 +190,13 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
                 v[1] = hi;
             }
         }
-        if (threadIdx.x < kPages) {
-            tile.key_scale[threadIdx.x] = key_scale;
+        if (thread < kPages) {
+            tile.key_scale[thread] = key_scale;
             // a page of scale 0 (its codes are 0) weighs as the smallest scale does
             const float scale = value_scale < 1.17549435e-38f ? 1.17549435e-38f : value_scale;
-            tile.value_bits[threadIdx.x] = of_scale ? __builtin_amdgcn_logf(scale) : -126.f;
-            tile.value_inverse[threadIdx.x] = 1.0f / scale;
-            tile.there[threadIdx.x] = of_scale;
+            tile.value_bits[thread] = of_scale ? __builtin_amdgcn_logf(scale) : -126.f;
+            tile.value_inverse[thread] = 1.0f / scale;
+            tile.there[thread] = of_scale;
         }
     };
     auto are_there = [&]() {
@@ -212,24 +214,26 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
         for (int i = 0; i < 16; ++i) o[u][i] = 0.f;
     float top = kNone, sum = 0.f, reference = -126.f, largest = 0.f;           // reference: log2 of the largest value scale so far
 
-    if (w.span.lo < w.span.hi) {
-        ask(w.span.lo);
-        find_pages(w.span.lo);
-        load(w.span.lo);
-        ask(w.span.lo + 1);
-        store(w.span.lo, tiles[0], are_there(), scale_page >= 0);
+    Tile<D>* const mine = tiles + 2 * team;
+    const int begin = w.span.lo + team;
+    if (begin < w.span.hi) {
+        ask(begin);
+        find_pages(begin);
+        load(begin);
+        ask(begin + TEAMS);
+        store(begin, mine[0], are_there(), scale_page >= 0);
     }
-    for (int at = w.span.lo, turn = 0; at < w.span.hi; ++at, turn ^= 1) {
+    for (int at = begin, turn = 0; at - team < w.span.hi; at += TEAMS, turn ^= 1) {
         __syncthreads();
-        const Tile<D>& tile = tiles[turn];
-        const bool more = at + 1 < w.span.hi;
+        const Tile<D>& tile = mine[turn];
+        const bool more = at + TEAMS < w.span.hi;
         if (more) {
-            find_pages(at + 1);
-            load(at + 1);
-            ask(at + 2);
+            find_pages(at + TEAMS);
+            load(at + TEAMS);
+            ask(at + 2 * TEAMS);
         }
         const int t0 = at * kGroup;
-        const bool skipped = rows <= 0 || t0 > last_own || (window > 0 && t0 + kGroup - 1 <= first_own - window);
+        const bool skipped = rows <= 0 || at >= w.span.hi || t0 > last_own || (window > 0 && t0 + kGroup - 1 <= first_own - window);
         if (!skipped) {
             // scores: lane (n, h) gets token 16 s + 8 h + j of row n in score[s / 2][8 (s % 2) + j]
             float16_t score[2];
@@ -237,14 +241,12 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
             const uint8_t* const key = tile.k + order * Tile<D>::kKeyPitch + h * 16;
 #pragma unroll
             for (int i = 0; i < 16; ++i) score[0][i] = score[1][i] = 0.f;
-            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int i = 0; i < kSteps; ++i)
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
                     score[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(key + b * 32 * Tile<D>::kKeyPitch + i * 32), q[i], score[b], 0, 0, 0);
             reads_ahead<2 * kSteps>();
-            __builtin_amdgcn_s_setprio(0);
             float ks[kPages], bits[kPages], inverse[kPages];
             int there = 15;
 #pragma unroll
@@ -321,7 +323,6 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
             };
             if (masked) weigh(std::true_type{});
             else weigh(std::false_type{});
-            __builtin_amdgcn_s_setprio(1);
             const uint8_t* const from = tile.v + n * Tile<D>::kValuePitch + h * 16;
 #pragma unroll
             for (int s = 0; s < 4; ++s)
@@ -329,17 +330,40 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
                 for (int u = 0; u < kOut; ++u)
                     o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(from + u * 32 * Tile<D>::kValuePitch + s * 32), weights[s], o[u], 0, 0, 0);
             reads_ahead<4 * kOut>();
-            __builtin_amdgcn_s_setprio(0);
         }
-        if (more) store(at + 1, tiles[turn ^ 1], are_there(), scale_page >= 0);
+        if (more) store(at + TEAMS, mine[turn ^ 1], are_there(), scale_page >= 0);
     }
 
     // o[u][4 a + i] is element 32 u + 8 a + 4 h + i of row n
     sum += __shfl_xor(sum, 32, 64);
+    float scale = reference <= -126.f ? 0.f : __builtin_amdgcn_exp2f(reference);
+    if constexpr (TEAMS > 1) {
+        // the second team's results through LDS, where its tiles were: four elements a lane, lanes side by side
+        float* const other = reinterpret_cast<float*>(tiles) + wave * (kOut * 16 + 2) * 64 + lane;
+        __syncthreads();
+        if (team == 1) {
+#pragma unroll
+            for (int u = 0; u < kOut; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) other[(u * 16 + i) * 64] = o[u][i] * scale;
+            other[kOut * 16 * 64] = top;
+            other[(kOut * 16 + 1) * 64] = sum;
+        }
+        __syncthreads();
+        if (team == 1) return;
+        const float their_top = other[kOut * 16 * 64], most = fmaxf(top, their_top), zero = most == kNone ? 0.f : most;
+        const float ours = __builtin_amdgcn_exp2f(top - zero), theirs = __builtin_amdgcn_exp2f(their_top - zero), factor = scale * ours;
+        sum = sum * ours + other[(kOut * 16 + 1) * 64] * theirs;
+        top = most;
+        scale = 1.f;
+#pragma unroll
+        for (int u = 0; u < kOut; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[u][i] = o[u][i] * factor + other[(u * 16 + i) * 64] * theirs;
+    }
     if (n >= rows) return;
-    const float scale = reference <= -126.f ? 0.f : __builtin_amdgcn_exp2f(reference);
     if (w.slot >= 0) {
-        const int64_t place = (static_cast<int64_t>(w.slot) * c.kv_heads + head) * kManyRows + wave * kWaveRows + n;
+        const int64_t place = (static_cast<int64_t>(w.slot) * c.kv_heads + head) * kRows + wave * kWaveRows + n;
 #pragma unroll
         for (int u = 0; u < kOut; ++u)
 #pragma unroll
@@ -362,27 +386,35 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
     }
 }
 
-template <int D, bool E4M3, bool WIDE>
+template <int D, bool E4M3, bool WIDE, int WAVES, int TEAMS>
 hipError_t launch(const AttentionParams& p, dim3 grid, hipStream_t s)
 {
-    constexpr size_t kLds = 2 * sizeof(Tile<D>);
+    constexpr size_t kLds = 2 * TEAMS * sizeof(Tile<D>);
+    static_assert(TEAMS == 1 || kLds >= static_cast<size_t>(WAVES) * ((D + 31) / 32 * 16 + 2) * 256, "room for a team's results");
+    const auto kernel = attention_rows_kernel<D, E4M3, WIDE, WAVES, TEAMS>;
     if (kLds > 65536) {              // more than a kernel gets without asking
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attention_rows_kernel<D, E4M3, WIDE>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLds));
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLds));
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((attention_rows_kernel<D, E4M3, WIDE>), grid, dim3(kThreads), kLds, s, p);
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * WAVES * TEAMS), kLds, s, p);
     return hipGetLastError();
 }
 
 template <bool E4M3, bool WIDE>
 hipError_t launch_of(const AttentionParams& p, dim3 grid, hipStream_t s)
 {
+    const bool most = p.tile_rows == kMostRows;
+    if ((!most && p.tile_rows != kManyRows) || (p.teams != 1 && (most || p.teams != 2))) return hipErrorInvalidValue;
+    auto sized = [&](auto size) {
+        constexpr int D = decltype(size)::value;
+        return most ? launch<D, E4M3, WIDE, 8, 1>(p, grid, s) : p.teams == 2 ? launch<D, E4M3, WIDE, 4, 2>(p, grid, s) : launch<D, E4M3, WIDE, 4, 1>(p, grid, s);
+    };
     switch (p.a.cache.head_size) {
-        case 64: return launch<64, E4M3, WIDE>(p, grid, s);
-        case 80: return launch<80, E4M3, WIDE>(p, grid, s);
-        case 96: return launch<96, E4M3, WIDE>(p, grid, s);
-        case 128: return launch<128, E4M3, WIDE>(p, grid, s);
-        case 256: return launch<256, E4M3, WIDE>(p, grid, s);
+        case 64: return sized(std::integral_constant<int, 64>{});
+        case 80: return sized(std::integral_constant<int, 80>{});
+        case 96: return sized(std::integral_constant<int, 96>{});
+        case 128: return sized(std::integral_constant<int, 128>{});
+        case 256: return most || p.teams == 2 ? hipErrorInvalidValue : launch<256, E4M3, WIDE, 4, 1>(p, grid, s);
         default: return hipErrorInvalidValue;
     }
 }
