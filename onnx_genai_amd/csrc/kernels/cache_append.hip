@@ -16,21 +16,24 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// x / scale as a code's byte. The quotient as RowScale has it; e4m3 needs it correctly rounded down to 2^-11, where the remainder is exact for scales of 2^-90 or more.
+// Scales from which the quotient that RowScale makes, corrected by its remainder, is the correctly rounded one: int8 needs it from 1/4 on (2^-101), e4m3 down to 2^-11 (2^-90).
 template <bool E4M3>
+constexpr float kLeastExact = E4M3 ? 8.0779357e-28f : 3.9443045e-31f;
+
+// x / scale as codes, to the nearest, ties to even. EXACT: the scale is kLeastExact or more, else the quotient is a division's, or 0 where the scale is not above 0. A quotient is at most a
+// rounding above the largest code, to which it goes.
+template <bool E4M3, bool EXACT>
 struct Coder {
-    RowScale s;
-    __device__ __forceinline__ explicit Coder(float scale)
-    {
-        s.scale = scale;
-        s.inverse = scale > 0.f ? 1.0f / scale : 0.f;
-    }
+    float scale, inverse;
+    __device__ __forceinline__ explicit Coder(float s) : scale(s), inverse(EXACT ? 1.0f / s : 0.f) {}
     __device__ __forceinline__ float quotient(float v) const
     {
-        float q = v * s.inverse;
-        q = fmaf(fmaf(-q, s.scale, v), s.inverse, q);
-        if (s.scale < 8.0779357e-28f) q = v / s.scale;
-        return s.scale > 0.f ? fminf(fmaxf(q, -448.f), 448.f) : 0.f;
+        if constexpr (EXACT) {
+            const float q = v * inverse;
+            return fmaf(fmaf(-q, scale, v), inverse, q);
+        } else {
+            return scale > 0.f ? v / scale : 0.f;
+        }
     }
     __device__ __forceinline__ uint32_t four(float a, float b, float c, float d) const
     {
@@ -38,10 +41,42 @@ struct Coder {
             int w = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(a), quotient(b), 0, false);
             return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(quotient(c), quotient(d), w, true));
         } else {
-            return (s.code(a) & 0xff) | (s.code(b) & 0xff) << 8 | (s.code(c) & 0xff) << 16 | static_cast<uint32_t>(s.code(d)) << 24;
+            // 1.5 * 2^23 + q has the nearest integer in its lowest bits
+            auto bits = [&](float v) { return __float_as_uint(as_f32(quotient(v)) + 12582912.0f); };
+            const uint32_t lo = __builtin_amdgcn_perm(bits(b), bits(a), 0x0c0c0400u), hi = __builtin_amdgcn_perm(bits(d), bits(c), 0x0c0c0400u);
+            return lo | hi << 16;
         }
     }
 };
+
+// The larger of the bits of |x| over eight elements and `most`: 16-bit types two at a time, as their bits order as the values do.
+template <typename T, bool BF16>
+__device__ __forceinline__ void larger_of(const Eight<T, BF16>& x, uint32_t& most)
+{
+    if constexpr (sizeof(T) == 2) {
+        typedef __attribute__((ext_vector_type(2))) unsigned short short2_t;
+        const uint32_t d[4] = {x.raw.x, x.raw.y, x.raw.z, x.raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(short2_t, most), __builtin_bit_cast(short2_t, d[i] & 0x7fff7fffu)));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t bits = __float_as_uint(x.raw[i]) & 0x7fffffffu;
+            most = bits > most ? bits : most;
+        }
+    }
+}
+template <typename T, bool BF16>
+__device__ __forceinline__ uint32_t as_f32_bits(uint32_t most)
+{
+    if constexpr (sizeof(T) == 2) {
+        const uint16_t m = static_cast<uint16_t>((most >> 16) > (most & 0xffff) ? most >> 16 : most);
+        return BF16 ? static_cast<uint32_t>(m) << 16 : __float_as_uint(f16_bits_to_f32(m));
+    } else {
+        return most;
+    }
+}
 
 // Four codes times `ratio` (<= 1), to the nearest; ratio 0 clears them.
 template <bool E4M3>
@@ -123,12 +158,8 @@ __global__ __launch_bounds__(kThreads) void append_kernel(RocmCacheAppendArgs a)
 #pragma unroll
     for (int j = 0; j < UNITS; ++j)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            float e[8];
-            x[j][t].get(e);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) amax = larger(amax, __float_as_uint(e[i]) & 0x7fffffffu);
-        }
+        for (int t = 0; t < 4; ++t) larger_of(x[j][t], amax);
+    amax = as_f32_bits<T, BF16>(amax);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     amax = over_workgroup(amax, slots_max, wave, kThreads / 64, larger);
     float scale = amax >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(amax) / (E4M3 ? 448.0f : 127.0f);
@@ -152,44 +183,56 @@ __global__ __launch_bounds__(kThreads) void append_kernel(RocmCacheAppendArgs a)
             __syncthreads();                             // (new codes go to bytes of the same dwords)
         }
     }
-    const Coder<E4M3> coder(none ? 0.f : scale);
+    auto write = [&](auto exact) {
+        const Coder<E4M3, decltype(exact)::value> coder(none ? 0.f : scale);
 #pragma unroll
-    for (int j = 0; j < UNITS; ++j) {
-        const int u = threadIdx.x + j * kThreads;
-        if (u >= units) continue;
-        int quad, piece;
-        place(u, quad, piece);
-        uint32_t w[4][2];                                // of token t: eight codes
+        for (int j = 0; j < UNITS; ++j) {
+            const int u = threadIdx.x + j * kThreads;
+            if (u >= units) continue;
+            int quad, piece;
+            place(u, quad, piece);
+            uint32_t w[4][2];                                // of token t: eight codes
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            float e[8];
-            x[j][t].get(e);
-            w[t][0] = coder.four(e[0], e[1], e[2], e[3]);
-            w[t][1] = coder.four(e[4], e[5], e[6], e[7]);
-        }
-        const bool whole = 4 * quad >= slot && 4 * quad + 4 <= end;
-        if (!values) {
+            for (int t = 0; t < 4; ++t) {
+                float e[8];
+                x[j][t].get(e);
+                w[t][0] = coder.four(e[0], e[1], e[2], e[3]);
+                w[t][1] = coder.four(e[4], e[5], e[6], e[7]);
+            }
+            const int begins = slot - 4 * quad > 0 ? slot - 4 * quad : 0, ends = end - 4 * quad < 4 ? end - 4 * quad : 4;          // new tokens of the four
+            if (!values) {
+                uint32_t* const to = codes + (4 * quad * d + piece * 8) / 4;
+                if (ends - begins == 4) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-                if (whole || (4 * quad + t >= slot && 4 * quad + t < end)) *reinterpret_cast<uint2*>(codes + ((4 * quad + t) * d + piece * 8) / 4) = make_uint2(w[t][0], w[t][1]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                // byte i of each token's eight
-                const int sel = i & 3, half = i >> 2;
-                const uint32_t lo = __builtin_amdgcn_perm(w[1][half], w[0][half], (0x0c0c0400u + sel * 0x0101u)), hi = __builtin_amdgcn_perm(w[3][half], w[2][half], (0x0c0c0400u + sel * 0x0101u));
-                const uint32_t four = lo | hi << 16;
-                uint32_t* const to = codes + ((piece * 8 + i) * page + 4 * quad) / 4;
-                if (whole) {
-                    *to = four;
+                    for (int t = 0; t < 4; ++t) *reinterpret_cast<uint2*>(to + t * d / 4) = make_uint2(w[t][0], w[t][1]);
                 } else {
+                    for (int t = begins; t < ends; ++t) {
+                        const uint32_t lo = t == 0 ? w[0][0] : t == 1 ? w[1][0] : t == 2 ? w[2][0] : w[3][0], hi = t == 0 ? w[0][1] : t == 1 ? w[1][1] : t == 2 ? w[2][1] : w[3][1];
+                        *reinterpret_cast<uint2*>(to + t * d / 4) = make_uint2(lo, hi);
+                    }
+                }
+            } else {
+                uint32_t four[8];                            // of element i: the codes of the four tokens
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        if (4 * quad + t >= slot && 4 * quad + t < end) reinterpret_cast<uint8_t*>(to)[t] = static_cast<uint8_t>(four >> (8 * t));
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t sel = 0x0c0c0400u + (i & 3) * 0x0101u;
+                    four[i] = __builtin_amdgcn_perm(w[1][i >> 2], w[0][i >> 2], sel) | __builtin_amdgcn_perm(w[3][i >> 2], w[2][i >> 2], sel) << 16;
+                }
+                uint8_t* const to = reinterpret_cast<uint8_t*>(codes) + piece * 8 * page + 4 * quad;
+                if (ends - begins == 4) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(to + i * page) = four[i];
+                } else {
+                    // (the other bytes of the dword are old tokens', or nobody's and to be left alone)
+                    for (int t = begins; t < ends; ++t)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) to[i * page + t] = static_cast<uint8_t>(four[i] >> (8 * t));
                 }
             }
         }
-    }
+    };
+    if (!none && scale >= kLeastExact<E4M3>) write(std::true_type{});
+    else write(std::false_type{});
 }
 
 }  // namespace

@@ -375,8 +375,9 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
         return plan;
     const int group = a.heads / c.kv_heads;
     if (a.rows * group >= (1 << 30)) return plan;
-    // From 32 rows a sequence on, on average, tiles share what they read of the cache through LDS.
-    plan.many = a.rows * group > 32 * static_cast<int64_t>(c.sequences);
+    // Beyond 64 rows a sequence, on average, tiles of many rows share what they read of the cache through LDS. (16 sequences of up to 4000 tokens, 64 rows a key head: 48 us in tiles of
+    // 16, 65 us in one of 128; 64 such sequences with 128 rows: 133 and 117 us.)
+    plan.many = a.rows * group > 64 * static_cast<int64_t>(c.sequences);
     plan.tile_rows = plan.many ? kManyRows : kRows;
     // 256 rows a tile, which halves what a row costs of the codes' way into LDS, once that gives two tiles for each CU; 128 rows with two teams of waves, which halves the steps that follow one
     // another, where there is no more than one tile for each CU. (4096 tokens over 32 heads by 8: 175 us, in tiles of 128 206 us; 2400 new tokens, 28 by 4: 54 us, with two teams

@@ -161,9 +161,9 @@ extern "C" int rocm_launch_rotary(const RocmRotaryArgs* args, rocm_stream_t stre
         plan.passed = (args->head_size - args->part + 7) / 8;
         plan.extra = static_cast<int>((args->extra + 7) / 8);
     }
-    // A row to a workgroup once there are rows for every CU; before that its heads are dealt out, each of which repeats the row's angles.
-    const int64_t cus = rocm_ffi_compute_units();
-    int64_t parts = args->rows >= cus ? 1 : (cus + args->rows - 1) / args->rows;
+    // A row to a workgroup once there are eight rows for each CU, as many as run on it at once; before that a row's heads are dealt out, and its angles repeated for each part.
+    const int64_t most = 8 * static_cast<int64_t>(rocm_ffi_compute_units());
+    int64_t parts = args->rows >= most ? 1 : (most + args->rows - 1) / args->rows;
     if (parts > args->heads) parts = args->heads;
     plan.heads_at_once = static_cast<int>((args->heads + parts - 1) / parts);
     const unsigned groups = static_cast<unsigned>((args->heads + plan.heads_at_once - 1) / plan.heads_at_once);
