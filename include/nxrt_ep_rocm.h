@@ -369,7 +369,7 @@ NxrtStatus nxrt_rocm_cache_attention_create(NxrtRocmEp* ep, const NxrtRocmCacheA
  * fresh page. Fresh pages, copies first and then those that new_tokens need, are the lowest that no slot has, dealt out slot by slot. Where they run out, entries are -1 and
  * count as missing (as do entries outside 0 .. P - 1); the inputs' table still stands then. No count is kept beside the table: a page is free if no slot has it.
  * With compact (parents and new_tokens absent) the k-th page in use beyond the first n goes to the k-th free one among them, n the pages in use.
- * S <= 1024, P <= 2^18, W page_size < 2^30. */
+ * S <= 1024, P <= 2^18, W page_size < 2^30, S W < 2^31. */
 typedef struct NxrtRocmCachePagesAttrs {
   uint32_t struct_size;
   uint32_t present;      /* bit i: 0 page_size (required; 1..=2^20), 1 compact (0) */

@@ -443,6 +443,7 @@ struct PagesNode final : NxrtRocmNode {
         const uint64_t slots = table->shape[0], width = table->shape[1];
         if (slots > ROCM_PAGES_MAX_SLOTS) c.fail("block_table may have up to " + std::to_string(ROCM_PAGES_MAX_SLOTS) + " sequences, got " + text(*table));
         if (!c.failed() && width * static_cast<uint64_t>(s.page_size) >= (uint64_t{1} << 30)) c.fail("block_table must have fewer than 2^30 tokens a sequence, got " + text(*table));
+        if (!c.failed() && slots * width > 0x7fffffff) c.fail("block_table must have fewer than 2^31 entries, got " + text(*table));
         RocmCachePagesArgs a{};
         auto whole = [&](uint32_t i, const char* name, bool needed) -> const int32_t* {
             const auto* v = c.input(i, name);

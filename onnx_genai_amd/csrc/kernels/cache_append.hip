@@ -101,7 +101,7 @@ __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > 
 
 // UNITS: units of four tokens by eight elements that a thread has at most.
 template <typename T, bool BF16, bool E4M3, int UNITS>
-__global__ __launch_bounds__(kThreads) void append_kernel(RocmCacheAppendArgs a)
+__global__ __launch_bounds__(kThreads, UNITS == 1 && sizeof(T) == 2 ? 8 : 1) void append_kernel(RocmCacheAppendArgs a)
 {
     __shared__ uint32_t slots_max[4];
     const RocmCache& c = a.cache;

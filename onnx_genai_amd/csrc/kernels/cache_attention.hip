@@ -41,21 +41,27 @@ struct Queries {
     static constexpr int kChunks = (D + 63) / 64;
     half8_t q[kChunks][2];
     float undo;                      // what a score is multiplied by for the row's own scale
+    Bytes16 raw[kChunks][2];
 
-    // Row `n` of lane n, 16 elements from 64 c + 16 g of it in q[c].
-    __device__ __forceinline__ void load(const uint16_t* row, bool bf16, int g)
+    // Row n of lane n, 16 elements from 64 c + 16 g of it in q[c]: asked for first, and looked at when the first keys are on their way.
+    __device__ __forceinline__ void ask(const uint16_t* row, int g)
+    {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            raw[c][0] = raw[c][1] = Bytes16{0, 0, 0, 0};
+            if (row && c * 64 + g * 16 < D) {
+                raw[c][0] = *reinterpret_cast<const Bytes16*>(row + c * 64 + g * 16);
+                raw[c][1] = *reinterpret_cast<const Bytes16*>(row + c * 64 + g * 16 + 8);
+            }
+        }
+    }
+    __device__ __forceinline__ void convert(bool bf16)
     {
         float x[kChunks][16];
         float most = 0.f;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-            const bool there = row && c * 64 + g * 16 < D;
-            Bytes16 raw[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-            if (there) {
-                raw[0] = *reinterpret_cast<const Bytes16*>(row + c * 64 + g * 16);
-                raw[1] = *reinterpret_cast<const Bytes16*>(row + c * 64 + g * 16 + 8);
-            }
-            const uint32_t d[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+            const uint32_t d[8] = {raw[c][0].x, raw[c][0].y, raw[c][0].z, raw[c][0].w, raw[c][1].x, raw[c][1].y, raw[c][1].z, raw[c][1].w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 x[c][2 * i] = bf16 ? __uint_as_float(d[i] << 16) : f16_bits_to_f32(static_cast<uint16_t>(d[i]));
@@ -63,8 +69,7 @@ struct Queries {
                 most = fmaxf(most, fmaxf(fabsf(x[c][2 * i]), fabsf(x[c][2 * i + 1])));
             }
         }
-        most = over_groups_max(most);
-        const QueryScale scale(most);
+        const QueryScale scale(over_groups_max(most));
         undo = scale.undo;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
@@ -73,12 +78,14 @@ struct Queries {
     }
 };
 
-template <int D, bool E4M3>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_few_kernel(AttentionParams p)
+template <int D, bool E4M3, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void attention_few_kernel(AttentionParams p)
 {
+    constexpr int kWaves = WAVES, kThreads = 64 * WAVES;
     constexpr int kChunks = (D + 63) / 64, kTiles = D / 16;
-    __shared__ float results[kWaves][kRows][D + 4];
-    __shared__ float2 sums[kWaves][kRows];
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    float (*const results)[kRows][D + 4] = reinterpret_cast<float (*)[kRows][D + 4]>(lds);                    // [kWaves]
+    float2 (*const sums)[kRows] = reinterpret_cast<float2 (*)[kRows]>(lds + kWaves * kRows * (D + 4));         // [kWaves]
     const RocmCache& c = p.a.cache;
     const int head = blockIdx.x % c.kv_heads;
     Piece w;
@@ -94,8 +101,6 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_few_kern
     const bool row_there = n < rows;
     const uint16_t* const q_row = static_cast<const uint16_t*>(p.a.q) + static_cast<int64_t>(w.s.first + token) * p.a.q_step + (head * p.group + member) * D;
     Queries<D> q;
-    q.load(row_there ? q_row : nullptr, p.a.dtype == ROCM_DT_BF16, g);
-    const float row_scale = q.undo * p.scale;
     // tokens that every row of the tile sees, and those that some row does
     const int first_own = w.s.past + first_row / p.group, last_own = w.s.past + (first_row + rows - 1) / p.group;
     const int window = p.a.window;
@@ -151,13 +156,16 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_few_kern
         value_page = page_from(c, value_entry, group * kGroup + g * 16, context);
         return page_from(c, key_entry, group * kGroup + (n >> 2) * 16, context);
     };
+    if (at < w.span.hi) ask(at);
+    q.ask(row_there ? q_row : nullptr, g);
     if (at < w.span.hi) {
-        ask(at);
         load_keys(at, find(at), s);
         load_scales(at, value_page, s);
         ask(at + kWaves);
         load_values(at, value_page, s);
     }
+    q.convert(p.a.dtype == ROCM_DT_BF16);
+    const float row_scale = q.undo * p.scale;
     for (; at < w.span.hi; at += kWaves) {
         const int t0 = at * kGroup;
         // scores: lane (n, g) gets token t0 + 16 g + 4 t + i of row n in score[t][i]
@@ -361,7 +369,7 @@ __global__ __launch_bounds__(kThreads, 6) void attention_join_kernel(AttentionPa
 
 struct Plan {
     bool ok, many;
-    int tile_rows, target, least, teams;
+    int tile_rows, target, least, whole, teams;
     int64_t tiles, pieces;          // most that a call of these sizes has, for one key head
     uint64_t sums_at, bytes;
 };
@@ -385,15 +393,19 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
     const int64_t cus = rocm_ffi_compute_units(), per_head = a.rows * group;
     const bool small = c.head_size <= 128;
     if (plan.many && small && per_head * c.kv_heads >= 2 * kMostRows * cus) plan.tile_rows = kMostRows;
-    plan.teams = plan.many && small && per_head * c.kv_heads <= kManyRows * cus ? 2 : 1;
     plan.tiles = per_head / plan.tile_rows + (a.rows < c.sequences ? a.rows : c.sequences);
+    // Few rows: eight waves a tile instead of four, by the same rule. (16 sequences, 16 rows a key head, 8 of them: 31 us, with four waves 33 us; with 64 rows, four tiles a head: 57 and 48 us.)
+    const int64_t least_tiles = plan.tiles - (a.rows < c.sequences ? a.rows : c.sequences), filled = least_tiles > c.sequences || a.rows < c.sequences ? least_tiles : c.sequences;
+    plan.teams = small && filled * c.kv_heads <= cus ? 2 : 1;
     // Pieces until there are as many workgroups as fit on the GPU at once: two for each CU, or one of 512 threads or heads of 256. None is shorter than 512 tokens, or 1024 in tiles of
-    // many rows: joining them costs about what so many take. (One of 8 chunks in a window of 1024, 1111 rows over 14 heads by 2: 31 us whole, 35 us in pieces of 512.)
-    const int64_t at_once = plan.many && (plan.teams == 2 || plan.tile_rows == kMostRows || !small) ? cus : 2 * cus;
+    // many rows, and contexts below 2048 stay whole: joining pieces costs about what so many tokens take. (One token after 1000: 9 us whole, 13 us in two pieces; four tokens after 4000
+    // with heads of 256: 31 us in pieces of 512 and more, 44 us in pieces of 1024 and more; three chunks in a window of 1024: 31 us whole, 35 us in pieces.)
+    const int64_t at_once = plan.teams == 2 || plan.tile_rows == kMostRows || (plan.many && !small) ? cus : 2 * cus;
     int64_t wanted = at_once / c.kv_heads;
     if (wanted > kMostPieces - 1) wanted = kMostPieces - 1;
     plan.least = plan.many ? 16 : 8;
-    if (plan.tiles < wanted && static_cast<int64_t>(c.width) * c.page >= kGroup * 2 * plan.least) plan.target = static_cast<int>(wanted);
+    plan.whole = 32;
+    if (plan.tiles < wanted && static_cast<int64_t>(c.width) * c.page > kGroup * (plan.whole - 1)) plan.target = static_cast<int>(wanted);
     plan.pieces = plan.tiles + plan.target;
     const uint64_t places = 2 * static_cast<uint64_t>(plan.target) * c.kv_heads * plan.tile_rows;
     plan.sums_at = (places * c.head_size * 4 + 255) / 256 * 256;
@@ -402,19 +414,32 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
     return plan;
 }
 
+template <int D, bool E4M3, int WAVES>
+hipError_t launch_tiles(const AttentionParams& p, dim3 grid, hipStream_t s)
+{
+    constexpr size_t kLds = WAVES * kRows * ((D + 4) * 4 + 8);
+    const auto kernel = attention_few_kernel<D, E4M3, WAVES>;
+    if (kLds > 65536) {              // more than a kernel gets without asking
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLds));
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * WAVES), kLds, s, p);
+    return hipGetLastError();
+}
+
 template <bool E4M3>
 hipError_t launch_few(const AttentionParams& p, dim3 grid, hipStream_t s)
 {
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, p);
-        return hipGetLastError();
+    auto sized = [&](auto size) {
+        constexpr int D = decltype(size)::value;
+        return p.teams == 2 ? launch_tiles<D, E4M3, 8>(p, grid, s) : launch_tiles<D, E4M3, 4>(p, grid, s);
     };
     switch (p.a.cache.head_size) {
-        case 64: return go(attention_few_kernel<64, E4M3>);
-        case 80: return go(attention_few_kernel<80, E4M3>);
-        case 96: return go(attention_few_kernel<96, E4M3>);
-        case 128: return go(attention_few_kernel<128, E4M3>);
-        case 256: return go(attention_few_kernel<256, E4M3>);
+        case 64: return sized(std::integral_constant<int, 64>{});
+        case 80: return sized(std::integral_constant<int, 80>{});
+        case 96: return sized(std::integral_constant<int, 96>{});
+        case 128: return sized(std::integral_constant<int, 128>{});
+        case 256: return p.teams == 2 ? hipErrorInvalidValue : launch_tiles<256, E4M3, 4>(p, grid, s);
         default: return hipErrorInvalidValue;
     }
 }
@@ -445,6 +470,7 @@ extern "C" int rocm_launch_cache_attention(const RocmCacheAttentionArgs* args, v
     p.tile_rows = plan.tile_rows;
     p.target = plan.target;
     p.least = plan.least;
+    p.whole = plan.whole;
     p.teams = plan.teams;
     p.slots = 2 * plan.target;
     p.scale = args->softcap > 0.f ? args->scale : args->scale * 1.442695041f;

@@ -67,41 +67,13 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
     const int first_row = w.tile * kRows + wave * kWaveRows, left = w.s.rows * p.group - first_row, rows = left < kWaveRows ? left : kWaveRows;
     const int token = (first_row + n) / p.group, member = first_row + n - token * p.group;
     const int own = w.s.past + token, last_seen = own < context ? own : context - 1;
-    half8_t q[kSteps];
-    float row_scale;
+    Bytes16 raw[kSteps];
     {
         const uint16_t* const row = static_cast<const uint16_t*>(p.a.q) + static_cast<int64_t>(w.s.first + token) * p.a.q_step + (head * p.group + member) * D + 8 * h;
-        Bytes16 raw[kSteps];
-        float most = 0.f;
-        auto get = [&](int i, float (&x)[8]) {
-            const uint32_t d[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[2 * j] = bf16 ? __uint_as_float(d[j] << 16) : f16_bits_to_f32(static_cast<uint16_t>(d[j]));
-                x[2 * j + 1] = bf16 ? __uint_as_float(d[j] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(d[j] >> 16));
-            }
-        };
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             raw[i] = Bytes16{0, 0, 0, 0};
             if (n < rows) raw[i] = *reinterpret_cast<const Bytes16*>(row + 16 * i);
-        }
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            float x[8];
-            get(i, x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
-        }
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
-        const QueryScale scale(most);
-        row_scale = scale.undo * p.scale;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            float x[8];
-            get(i, x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) q[i][j] = static_cast<_Float16>(x[j] * scale.factor);
         }
     }
     // tokens that every row of the wave sees, and those that some row does
@@ -207,6 +179,45 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
         return bits;
     };
 
+    // the first step's codes are on their way while the queries become operands
+    Tile<D>* const mine = tiles + 2 * team;
+    const int begin = w.span.lo + team;
+    if (begin < w.span.hi) {
+        ask(begin);
+        find_pages(begin);
+        load(begin);
+    }
+    half8_t q[kSteps];
+    float row_scale;
+    {
+        auto get = [&](int i, float (&x)[8]) {
+            const uint32_t d[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[2 * j] = bf16 ? __uint_as_float(d[j] << 16) : f16_bits_to_f32(static_cast<uint16_t>(d[j]));
+                x[2 * j + 1] = bf16 ? __uint_as_float(d[j] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(d[j] >> 16));
+            }
+        };
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            float x[8];
+            get(i, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+        }
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        const QueryScale scale(most);
+        row_scale = scale.undo * p.scale;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            float x[8];
+            get(i, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[i][j] = static_cast<_Float16>(x[j] * scale.factor);
+        }
+    }
+
     float16_t o[kOut];
 #pragma unroll
     for (int u = 0; u < kOut; ++u)
@@ -214,12 +225,7 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
         for (int i = 0; i < 16; ++i) o[u][i] = 0.f;
     float top = kNone, sum = 0.f, reference = -126.f, largest = 0.f;           // reference: log2 of the largest value scale so far
 
-    Tile<D>* const mine = tiles + 2 * team;
-    const int begin = w.span.lo + team;
     if (begin < w.span.hi) {
-        ask(begin);
-        find_pages(begin);
-        load(begin);
         ask(begin + TEAMS);
         store(begin, mine[0], are_there(), scale_page >= 0);
     }

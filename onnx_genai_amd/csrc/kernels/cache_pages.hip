@@ -12,7 +12,7 @@
 namespace mnb {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64, kCopyThreads = 256, kCopyBytes = 8192;
+constexpr int kThreads = 1024, kWaves = kThreads / 64, kCopyThreads = 256, kCopyBytes = 8192, kCopyGroups = 16;
 
 struct PagesWorkspace {
     int32_t* count;       // [1]: moves
@@ -21,26 +21,36 @@ struct PagesWorkspace {
     int32_t* list;        // [pages]: free pages by rank; compacting, where a page goes
 };
 
-// The sum over the threads below this one; `all`: over every thread. Two barriers.
-__device__ __forceinline__ int sum_below(int v, int* slots, int* all)
+// N sums over the threads below this one, and over every thread, at once. Two barriers.
+template <int N>
+__device__ __forceinline__ void sums_below(const int (&v)[N], int (*slots)[kWaves], int (&below)[N], int (&all)[N])
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int upto = v;
+    int upto[N];
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int below = __shfl_up(upto, off, 64);
-        if (lane >= off) upto += below;
+    for (int k = 0; k < N; ++k) {
+        upto[k] = v[k];
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int lower = __shfl_up(upto[k], off, 64);
+            if (lane >= off) upto[k] += lower;
+        }
     }
     __syncthreads();
-    if (lane == 63) slots[wave] = upto;
-    __syncthreads();
-    int before = 0, total = 0;
-    for (int i = 0; i < kWaves; ++i) {
-        before += i < wave ? slots[i] : 0;
-        total += slots[i];
+    if (lane == 63) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) slots[k][wave] = upto[k];
     }
-    *all = total;
-    return before + upto - v;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        below[k] = upto[k] - v[k];
+        all[k] = 0;
+        for (int i = 0; i < kWaves; ++i) {
+            below[k] += i < wave ? slots[k][i] : 0;
+            all[k] += slots[k][i];
+        }
+    }
 }
 
 __device__ __forceinline__ bool is_set(const uint32_t* bits, int page) { return (bits[page >> 5] >> (page & 31)) & 1; }
@@ -50,7 +60,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
 {
     extern __shared__ uint32_t held[];                         // a bit for each page
     __shared__ int parent[ROCM_PAGES_MAX_SLOTS], length[ROCM_PAGES_MAX_SLOTS], begun[ROCM_PAGES_MAX_SLOTS], start[ROCM_PAGES_MAX_SLOTS], keeps[ROCM_PAGES_MAX_SLOTS];
-    __shared__ int slots[kWaves], missing;
+    __shared__ int list[kThreads], slots[3][kWaves], missing;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int pages = static_cast<int>(a.pages), words = (pages + 31) / 32, capacity = a.width * a.page;
     auto page_at = [&](int slot, int j) {
@@ -69,14 +79,14 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
     }
     __syncthreads();
     auto whole = [&](int slot) { return a.compact ? (length[slot] + a.page - 1) / a.page : length[slot] / a.page; };
-    for (int i = wave; i < a.slots; i += kWaves) {
-        const int n = whole(i);
-        for (int j = lane; j < a.width; j += 64) {
-            const int p = j < n ? page_at(parent[i], j) : -1;
-            if (p >= 0) set(held, p);
-            else if (j < n) atomicAdd(&missing, 1);
-            a.next[static_cast<int64_t>(i) * a.width + j] = p;
-        }
+    // entries of all slots side by side: a short table is one trip to memory
+    const uint32_t entries = static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.width);
+    for (uint32_t e = t; e < entries; e += kThreads) {
+        const int i = static_cast<int>(e / static_cast<uint32_t>(a.width)), j = static_cast<int>(e - static_cast<uint32_t>(i) * a.width), n = whole(i);
+        const int p = j < n ? page_at(parent[i], j) : -1;
+        if (p >= 0) set(held, p);
+        else if (j < n) atomicAdd(&missing, 1);
+        a.next[e] = p;
     }
     __syncthreads();
     // words of the bit map are dealt out in runs, so that ranks rise with the pages
@@ -84,16 +94,19 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
     auto valid = [&](int word) { return 32 * word + 32 <= pages ? 0xffffffffu : (1u << (pages - 32 * word)) - 1; };
 
     if (a.compact) {
-        int mine = 0, live;
-        for (int i = first; i < last; ++i) mine += __popc(held[i]);
-        sum_below(mine, slots, &live);
+        int set_bits[1] = {0}, unused[1], all[1];
+        for (int i = first; i < last; ++i) set_bits[0] += __popc(held[i]);
+        sums_below(set_bits, slots, unused, all);
+        const int live = all[0];
         auto below = [&](int word) { return 32 * word + 32 <= live ? 0xffffffffu : 32 * word >= live ? 0u : (1u << (live - 32 * word)) - 1; };
-        int sources = 0, holes = 0, moves, unused;
+        int counts[2] = {0, 0}, at[2], both[2];                // sources and holes: as many of one as of the other
         for (int i = first; i < last; ++i) {
-            sources += __popc(held[i] & ~below(i));
-            holes += __popc(~held[i] & below(i));
+            counts[0] += __popc(held[i] & ~below(i));
+            counts[1] += __popc(~held[i] & below(i));
         }
-        int source = sum_below(sources, slots, &moves), hole = sum_below(holes, slots, &unused);
+        sums_below(counts, slots, at, both);
+        int source = at[0], hole = at[1];
+        const int moves = both[0];
         for (int i = first; i < last; ++i) {
             for (uint32_t bits = held[i] & ~below(i); bits; bits &= bits - 1) w.from[source++] = 32 * i + __ffs(bits) - 1;
             for (uint32_t bits = ~held[i] & below(i); bits; bits &= bits - 1) w.to[hole++] = 32 * i + __ffs(bits) - 1;
@@ -106,12 +119,10 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
             a.moves[2 * i + 1] = i < moves ? w.to[i] : -1;
         }
         __syncthreads();
-        for (int i = wave; i < a.slots; i += kWaves) {
-            const int n = whole(i);
-            for (int j = lane; j < n; j += 64) {
-                const int p = page_at(i, j);
-                if (p >= live) a.next[static_cast<int64_t>(i) * a.width + j] = w.list[p];
-            }
+        for (uint32_t e = t; e < entries; e += kThreads) {
+            const int i = static_cast<int>(e / static_cast<uint32_t>(a.width)), j = static_cast<int>(e - static_cast<uint32_t>(i) * a.width);
+            const int p = j < whole(i) ? page_at(i, j) : -1;
+            if (p >= live) a.next[e] = w.list[p];
         }
         if (t < a.slots) a.next_lengths[t] = length[t];
         if (t == 0) {
@@ -137,40 +148,50 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
     }
     __syncthreads();
     if (keep) set(held, begun[t]);
-    int needed, free_pages, moves;
-    const int mine = sum_below(need, slots, &needed);
+    __syncthreads();
+    int counts[3] = {need, 0, copies}, at[3], all[3];            // fresh pages wanted, pages that are free, copies
+    for (int i = first; i < last; ++i) counts[1] += __popc(~held[i] & valid(i));
+    sums_below(counts, slots, at, all);
+    const int mine = at[0], needed = all[0], free_pages = all[1], moves = all[2];
     if (t < a.slots) {
         start[t] = mine;
         keeps[t] = keep;
     }
-    int empty = 0;
-    for (int i = first; i < last; ++i) empty += __popc(~held[i] & valid(i));
-    int rank = sum_below(empty, slots, &free_pages);
+    int rank = at[1];
     for (int i = first; i < last && rank < needed; ++i)
-        for (uint32_t bits = ~held[i] & valid(i); bits && rank < needed; bits &= bits - 1) w.list[rank++] = 32 * i + __ffs(bits) - 1;
+        for (uint32_t bits = ~held[i] & valid(i); bits && rank < needed; bits &= bits - 1, ++rank) {
+            const int p = 32 * i + __ffs(bits) - 1;
+            if (rank < kThreads) list[rank] = p;
+            else w.list[rank] = p;
+        }
     __syncthreads();
-    auto fresh = [&](int k) { return k < free_pages ? w.list[k] : -1; };
-    const int copy = copies ? fresh(mine) : -1;
-    const int place = sum_below(copy >= 0, slots, &moves);
+    auto fresh = [&](int k) { return k >= free_pages ? -1 : k < kThreads ? list[k] : w.list[k]; };
+    constexpr int kOwn = 2;                                      // further pages that a slot's thread enters itself
     if (t < a.slots) {
-        const int full = length[t] / a.page;
+        const int copy = copies ? fresh(mine) : -1, have = (length[t] + a.page - 1) / a.page;
+        int32_t* const next = a.next + static_cast<int64_t>(t) * a.width;
         if (rest) {
             const int p = keep ? begun[t] : copy;
-            a.next[static_cast<int64_t>(t) * a.width + full] = p;
+            next[length[t] / a.page] = p;
+            if (p < 0) atomicAdd(&missing, 1);
+        }
+        for (int k = copies; k < need && k < copies + kOwn; ++k) {
+            const int p = fresh(mine + k);
+            next[have + k - copies] = p;
             if (p < 0) atomicAdd(&missing, 1);
         }
         a.moves[2 * t] = copy >= 0 ? begun[t] : -1;
         a.moves[2 * t + 1] = copy;
-        if (copy >= 0) {
-            w.from[place] = begun[t];
-            w.to[place] = copy;
+        if (copies) {
+            w.from[at[2]] = begun[t];
+            w.to[at[2]] = copy;                                  // (-1 where there was no page: nothing is copied)
         }
         a.next_lengths[t] = length[t];
     }
     for (int i = wave; i < a.slots; i += kWaves) {
         const int have = (length[i] + a.page - 1) / a.page, begins = start[i] + (begun[i] >= 0 && !keeps[i]);
         const int ends = i + 1 < a.slots ? start[i + 1] : needed;
-        for (int k = begins + lane; k < ends; k += 64) {
+        for (int k = begins + kOwn + lane; k < ends; k += 64) {
             const int p = fresh(k);
             if (p < 0) atomicAdd(&missing, 1);
             a.next[static_cast<int64_t>(i) * a.width + have + k - begins] = p;
@@ -207,15 +228,23 @@ __device__ __forceinline__ void copy_units(const RocmCachePagesArgs& a, const Pa
             const int u = base + threadIdx.x + i * kCopyThreads, layer = these > 1 ? u / units : 0;
             at[i] = u < all ? (layer0 + layer) * a.pages * pool.page_bytes + skip + static_cast<int64_t>(u - layer * units) * static_cast<int>(sizeof(W)) : -1;
         }
-        for (int m = blockIdx.y; m < moves; m += gridDim.y) {
-            const uint8_t* const from = static_cast<const uint8_t*>(pool.at) + w.from[m] * pool.page_bytes;
-            uint8_t* const to = static_cast<uint8_t*>(pool.at) + w.to[m] * pool.page_bytes;
-            W v[kEach];
+        // two moves at a time, their loads together
+        const int step = gridDim.y;
+        for (int m = blockIdx.y; m < moves; m += 2 * step) {
+            const bool second = m + step < moves;
+            const int other = second ? m + step : m;
+            const int64_t from[2] = {w.from[m] * pool.page_bytes, w.from[other] * pool.page_bytes};
+            const int to[2] = {w.to[m], second ? w.to[other] : -1};
+            W v[2][kEach];
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) v[i] = at[i] >= 0 ? *reinterpret_cast<const W*>(from + at[i]) : W{};
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int i = 0; i < kEach; ++i)
-                if (at[i] >= 0) *reinterpret_cast<W*>(to + at[i]) = v[i];
+                for (int i = 0; i < kEach; ++i) v[k][i] = at[i] >= 0 && to[k] >= 0 ? *reinterpret_cast<const W*>(static_cast<const uint8_t*>(pool.at) + from[k] + at[i]) : W{};
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < kEach; ++i)
+                    if (at[i] >= 0 && to[k] >= 0) *reinterpret_cast<W*>(static_cast<uint8_t*>(pool.at) + to[k] * pool.page_bytes + at[i]) = v[k][i];
         }
     }
 }
@@ -241,7 +270,7 @@ extern "C" int rocm_launch_cache_pages(const RocmCachePagesArgs* args, void* wor
 {
     using namespace mnb;
     if (args->slots <= 0) return 0;
-    if (args->slots > ROCM_PAGES_MAX_SLOTS || args->pages < 1 || args->pages > ROCM_PAGES_MAX_PAGES || args->width < 1 || args->page < 1 || static_cast<int64_t>(args->width) * args->page >= (1 << 30) ||
+    if (args->slots > ROCM_PAGES_MAX_SLOTS || args->pages < 1 || args->pages > ROCM_PAGES_MAX_PAGES || args->width < 1 || args->page < 1 || static_cast<int64_t>(args->width) * args->page >= (1 << 30) || static_cast<int64_t>(args->slots) * args->width > 0x7fffffff ||
         args->pools < 0 || args->pools > ROCM_PAGES_MAX_POOLS || !workspace)
         return static_cast<int>(hipErrorInvalidValue);
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -264,6 +293,8 @@ extern "C" int rocm_launch_cache_pages(const RocmCachePagesArgs* args, void* wor
     if (e != hipSuccess || pieces == 0) return static_cast<int>(e);
     const int64_t most = args->compact ? args->pages / 2 : args->slots;
     if (most == 0) return 0;
-    hipLaunchKernelGGL(copy_kernel, dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(most < 1024 ? most : 1024)), dim3(kCopyThreads), 0, s, *args, w, plan);
+    // workgroups for every CU several times over; each takes every so many of the moves, whose number only the GPU knows
+    const int64_t wanted = (kCopyGroups * static_cast<int64_t>(rocm_ffi_compute_units()) + pieces - 1) / pieces, rows = most < wanted ? most : wanted;
+    hipLaunchKernelGGL(copy_kernel, dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(rows < 65535 ? rows : 65535)), dim3(kCopyThreads), 0, s, *args, w, plan);
     return static_cast<int>(hipGetLastError());
 }

@@ -289,6 +289,8 @@ def test_pages_refusals(provider):
     refused(k, [table, lengths, parents, new, big], outs + [big], "a pool may have 1..=262144 pages")
     many = E.TensorView(HOLD.ctypes.data // 16 * 16 + 16, E.I32, (1025, 5))
     refused(k, [many, lengths, parents, new] + pools, outs + pools, "up to 1024 sequences")
+    refused(k, [E.TensorView(many.data, E.I32, (1000, 3000000)), lengths, parents, new] + pools, outs + pools, "fewer than 2^31 entries")
+    refused(k, [E.TensorView(many.data, E.I32, (2, 1 << 27)), lengths, parents, new] + pools, outs + pools, "fewer than 2^30 tokens a sequence")
     k.execute([E.TensorView(None, E.I32, (0, 5)), NONE, NONE, NONE, NONE], [NONE])
     k.release()
     k = provider.get_kernel({"page_size": 16, "compact": 1}, op_type="CachePages")
