@@ -116,8 +116,8 @@ def append32(cache, key, value):
             t += count
 
 
-def attention64(cache, q, heads, *, scale=None, window=0, softcap=0.0, size=False):
-    """[T, heads, head] in 64 bits, zero where nothing is seen; and how far off the kernel may be beside its last rounding: per element, from the roundings that it makes."""
+def attention64(cache, q, heads, *, scale=None, window=0, softcap=0.0, rows=None, of_heads=None):
+    """[T, heads, head] in 64 bits (of some rows and heads, if they are given), zero where nothing is seen; and how far off the kernel may be beside its last rounding: per element, from the roundings that it makes."""
     d, group = cache.head, heads // cache.kv_heads
     scale = scale or 1 / np.sqrt(d)
     y, slack = np.zeros((cache.rows, heads, d)), np.zeros((cache.rows, heads, d))
@@ -130,8 +130,10 @@ def attention64(cache, q, heads, *, scale=None, window=0, softcap=0.0, size=Fals
         codes, top = decode(cache.v[page, :, :, place], cache.code), np.nanmax(cache.vs[page], 0)
         for r in range(n):
             own, row = cache.past[i] + r, cache.ends[i] + r
+            if rows is not None and row not in rows:
+                continue
             seen = (slot <= own) & ((slot > own - window) if window else True)
-            for h in range(heads):
+            for h in of_heads or range(heads):
                 kk, vv, qq = k[seen, h // group], v[seen, h // group], q[row, h]
                 z = scale * (kk @ qq)
                 if softcap:

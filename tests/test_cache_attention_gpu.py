@@ -70,6 +70,32 @@ def test_chunks(ep, head, page, kv_heads, group, code, dtype):
     check(ep, cache, kv_heads * group, dtype, 2, extra=1, packed=True, offset=1)
 
 
+KINDS = {
+    # (new tokens of the sequences, past, heads, key heads): what the call's size makes of it on 256 CUs
+    "few_rows_four_waves": ([1] * 139 + [2], [17 * i % 300 for i in range(140)], 8, 2),
+    "tiles_of_128": ([900, 0, 203], [70, 5, 333], 64, 2),
+    "tiles_of_256": ([1500, 1, 650], [0, 900, 129], 64, 2),
+}
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("head,page,code,window", [(64, 16, E.I8, 0), (64, 64, E.F8E4M3, 0), (80, 32, E.I8, 100), (80, 128, E.F8E4M3, 0), (96, 64, E.I8, 0), (96, 16, E.F8E4M3, 0), (128, 16, E.F8E4M3, 77),
+                                                   (128, 64, E.I8, 0), (128, 128, E.F8E4M3, 500), (128, 32, E.I8, 0), (256, 16, E.I8, 0), (256, 64, E.F8E4M3, 0)])
+def test_tiles_of_every_kind(ep, kind, head, page, code, window):
+    """Calls large enough for the kernels of many tiles; some rows of every sequence, its first and last among them, against the definition."""
+    new, past, heads, kv_heads = KINDS[kind]
+    rng = np.random.default_rng(head + page)
+    cache = Cache(rng, new, past, code, kv_heads, head, page)
+    q = floats(rng, (cache.rows + 1, heads * head), E.F16)
+    got, variant = attend(ep, cache, q, E.F16, heads, extra=1, local_window_size=window or -1)
+    assert variant.startswith("cache_attention_rows") == (kind != "few_rows_four_waves")
+    rows = set(rng.integers(0, cache.rows, 12).tolist()) | {int(e) for e in cache.ends[:-1] if e < cache.rows} | {int(e) - 1 for e in cache.ends[1:]} if len(new) < 9 else set(range(0, cache.rows, 5))
+    of_heads = [0, heads // kv_heads - 1, heads - 1]
+    want, slack = attention64(cache, as64(q, E.F16).reshape(-1, heads, head), heads, window=window, rows=rows, of_heads=of_heads)
+    at = np.ix_(sorted(rows), of_heads)
+    near(got[at], want[at], slack[at], E.F16)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 64, 65, 127, 128, 129, 200, 257])
 @pytest.mark.parametrize("group", [1, 4])
 def test_prompt_lengths(ep, rows, group):
