@@ -301,7 +301,8 @@ NxrtStatus nxrt_rocm_gated_residual_norm_create(NxrtRocmEp* ep, const NxrtRocmGa
  * cumulative_lengths[b] up to cumulative_lengths[b + 1]; rows behind the last sequence belong to none. past_lengths [N] Int32: tokens of a sequence in front of them.
  * block_table [N, W] Int32: token t of sequence b is slot t % B of page block_table[b, t / B].
  * What these tensors hold is read on the GPU and not reported: lengths are taken into 0 .. T, past lengths into 0 .. W B, and a page outside 0 .. P - 1 holds no tokens.
- * D: 64, 80, 96, 128 or 256 for CacheAttention, a multiple of 16 up to 256 for CacheAppend. W B < 2^30. */
+ * D: 64, 80, 96, 128 or 256 for CacheAttention, a multiple of 16 up to 256 for CacheAppend. W B < 2^30, N KV < 2^20; T < 2^26 for CacheAppend, T num_heads < 2^29 for
+ * CacheAttention. */
 
 /* com.microsoft::RotaryEmbedding: pairs of a head's elements turned by their row's position.
  *   inputs: 0 input [.., C] Float32 / Float16 / BFloat16, the heads of a row side by side; or, with rank 4, [N, H, S, D]; 1 position_ids Int64 / Int32, one for each row (of

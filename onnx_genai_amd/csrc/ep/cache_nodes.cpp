@@ -91,6 +91,7 @@ struct RotaryNode final : NxrtRocmNode {
             const uint64_t heads = x->shape[1], length = x->shape[2];
             if (last != d) c.fail("input of rank 4 must have last dimension head_size=" + std::to_string(d) + ", got " + text(*x));
             if (!c.failed() && s.heads && heads != static_cast<uint64_t>(s.heads)) c.fail("input must have num_heads=" + std::to_string(s.heads) + " heads, got " + text(*x));
+            if (!c.failed() && heads > (1u << 20)) c.fail("input may have up to 2^20 heads, got " + text(*x));
             rows = x->shape[0] * length;
             a.inner = static_cast<int64_t>(length);
             a.outer_step = static_cast<int64_t>(heads * length * d);
@@ -192,7 +193,7 @@ struct CacheInputs {
         if (table->ndim != 2 || table->shape[1] < 1) return c.fail("block_table must have shape [N, W] with W >= 1, got " + text(*table));
         const uint64_t n = table->shape[0], width = table->shape[1];
         if (width * b >= (uint64_t{1} << 30)) return c.fail("block_table must have fewer than 2^30 slots a sequence, got " + text(*table));
-        if (n >= (1u << 24)) return c.fail("too many sequences: " + text(*table));
+        if (n >= (1u << 20) || n * kv_heads >= (1u << 20)) return c.fail("block_table must have fewer than 2^20 sequences times key heads, got " + text(*table));
         c.shape(ends, "cumulative_lengths", {n + 1});
         c.shape(past, "past_lengths", {n});
         if (c.failed()) return;
@@ -260,7 +261,7 @@ struct AppendNode final : NxrtRocmNode {
         const uint64_t kv = static_cast<uint64_t>(s.kv_heads * s.head_size), packed = static_cast<uint64_t>(s.heads * s.head_size) + 2 * kv;
         if (key->ndim != 2 || key->shape[1] != (value ? kv : packed))
             c.fail(std::string(value ? "key" : "packed rows (no value)") + " must have shape [T, " + std::to_string(value ? kv : packed) + "], got " + text(*key));
-        if (!c.failed() && key->shape[0] >= (1u << 30)) c.fail("too many rows: " + text(*key));
+        if (!c.failed() && key->shape[0] >= (1u << 26)) c.fail("too many rows: " + text(*key));
         c.dtype(value, "value", {key->dtype});
         if (value && !c.failed()) c.shape(value, "value", {key->shape[0], kv});
         const CacheInputs cache(c, 2);
@@ -335,7 +336,7 @@ struct AttentionNode final : NxrtRocmNode {
     {
         RocmCacheAttentionArgs a{};
         a.heads = static_cast<int>(s.heads);
-        a.window = s.window > 0 ? static_cast<int>(s.window) : 0;
+        a.window = s.window > 0 && s.window < (1 << 30) ? static_cast<int>(s.window) : 0;          // (no sequence has 2^30 slots)
         a.scale = static_cast<float>(s.scale);
         a.softcap = static_cast<float>(s.softcap);
         a.cache.kv_heads = static_cast<int>(s.kv_heads);
@@ -349,7 +350,7 @@ struct AttentionNode final : NxrtRocmNode {
             return make_status(NXRT_INVALID_ARGUMENT, err("workspace_requirement needs the shapes of query, k_cache and block_table"));
         RocmCacheAttentionArgs a = args();
         const int64_t page = in[1].dims[2];
-        if (rows * s.heads >= (int64_t{1} << 30) || sequences >= (1 << 24) || width < 1 || page < 1 || page > ROCM_CACHE_MAX_PAGE || width * page >= (int64_t{1} << 30))
+        if (rows >= (1 << 29) || rows * s.heads >= (int64_t{1} << 29) || sequences >= (1 << 20) || sequences * s.kv_heads >= (1 << 20) || width < 1 || page < 1 || page > ROCM_CACHE_MAX_PAGE || width * page >= (int64_t{1} << 30))
             return make_status(NXRT_INVALID_ARGUMENT, err("workspace_requirement got shapes that no call takes"));
         a.rows = rows;
         a.cache.sequences = static_cast<int>(sequences);
@@ -371,7 +372,7 @@ struct AttentionNode final : NxrtRocmNode {
         const uint64_t wide = static_cast<uint64_t>(s.heads * s.head_size), packed = wide + static_cast<uint64_t>(2 * s.kv_heads * s.head_size);
         if (q->ndim != 2 || (q->shape[1] != wide && q->shape[1] != packed))
             c.fail("query must have shape [T, " + std::to_string(wide) + "], or packed [T, " + std::to_string(packed) + "], got " + text(*q));
-        if (!c.failed() && q->shape[0] * static_cast<uint64_t>(s.heads) >= (uint64_t{1} << 30)) c.fail("too many rows: " + text(*q));
+        if (!c.failed() && (q->shape[0] >= (1u << 29) || q->shape[0] * static_cast<uint64_t>(s.heads) >= (1u << 29))) c.fail("too many rows: " + text(*q));
         const CacheInputs cache(c, 1);
         RocmCacheAttentionArgs a = args();
         if (!c.failed()) cache.check(c, static_cast<uint64_t>(s.kv_heads), static_cast<uint64_t>(s.head_size), &a.cache);

@@ -249,6 +249,7 @@ extern "C" int rocm_launch_cache_append(const RocmCacheAppendArgs* args, rocm_st
     hipStream_t s = static_cast<hipStream_t>(stream);
     // a sequence with n tokens touches at most n / page + 2 pages, and at most n
     const int64_t pages = args->rows < c.sequences ? args->rows : args->rows / c.page + 2 * static_cast<int64_t>(c.sequences);
+    if (pages >= (1 << 24)) return static_cast<int>(hipErrorInvalidValue);          // (a grid has fewer than 2^32 threads a side)
     const dim3 grid(static_cast<unsigned>(pages < args->rows ? pages : args->rows), static_cast<unsigned>(c.kv_heads), 2);
     const int units = c.head_size / 8 * (c.page / 4);          // of a whole page; few new tokens fill the first of a thread's alone
     auto go = [&](auto kernel) {

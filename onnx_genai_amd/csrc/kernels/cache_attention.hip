@@ -223,8 +223,8 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void attentio
             for (int u = 0; u < kTiles; ++u) o[u] *= again;
         }
         const float zero = top == kNone ? 0.f : top;                            // (a row that has seen nothing yet)
-        // weights relative to the largest page scale so far
-        const float relative = reference > 0.f ? value_scale / reference : 0.f;
+        // weights relative to the largest page scale so far, where there is one; a NaN stays one
+        const float relative = reference > 0.f ? value_scale / reference : value_scale * 0.f;
         half8_t weights[2];
         auto weigh = [&](auto some) {
             float part = 0.f;
@@ -410,7 +410,7 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
     const uint64_t places = 2 * static_cast<uint64_t>(plan.target) * c.kv_heads * plan.tile_rows;
     plan.sums_at = (places * c.head_size * 4 + 255) / 256 * 256;
     plan.bytes = plan.target ? plan.sums_at + (places * 8 + 255) / 256 * 256 : 0;
-    plan.ok = plan.pieces * c.kv_heads < (1 << 24);
+    plan.ok = plan.pieces * c.kv_heads < (1 << 23);          // (a grid has fewer than 2^32 threads, a workgroup up to 512)
     return plan;
 }
 
@@ -451,7 +451,7 @@ extern "C" int rocm_cache_attention_supports(int head_size) { return head_size =
 
 extern "C" uint64_t rocm_cache_attention_workspace_bytes(const RocmCacheAttentionArgs* args) { return mnb::plan_of(*args).bytes; }
 
-extern "C" const char* rocm_cache_attention_variant(const RocmCacheAttentionArgs* args) 
+extern "C" const char* rocm_cache_attention_variant(const RocmCacheAttentionArgs* args)
 {
     const mnb::Plan plan = mnb::plan_of(*args);
     return plan.many ? plan.target ? "cache_attention_rows_pieces" : "cache_attention_rows" : plan.target ? "cache_attention_pieces" : "cache_attention";

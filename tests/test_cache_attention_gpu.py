@@ -165,6 +165,36 @@ def test_nan_stays_with_the_rows_that_see_it(ep, new):
         near(got[~sees], want[~sees], slack[~sees], E.F16)
 
 
+@pytest.mark.parametrize("new", [[1], [90]])
+@pytest.mark.parametrize("which", ["ks", "vs"])
+def test_nothing_but_nan_pages(ep, which, new):
+    """Every page of one head has a scale of NaN: its rows are NaN, the other head's are as without it. And a scale of 0 is no NaN."""
+    rng = np.random.default_rng(24)
+    cache = Cache(rng, new, [700], E.I8, 2, 64, 16)
+    q = floats(rng, (cache.rows, 2 * 64), E.F16)
+    want, slack = attention64(cache, as64(q, E.F16).reshape(-1, 2, 64), 2)
+    getattr(cache, which)[:, 0] = np.nan
+    got, _ = attend(ep, cache, q, E.F16, 2)
+    assert np.isnan(as64(got[:, 0], E.F16)).all()
+    near(got[:, 1], want[:, 1], slack[:, 1], E.F16)
+    cache.ks[:, 0] = 0.02
+    cache.vs[:, 0] = 0.0
+    got, _ = attend(ep, cache, q, E.F16, 2)
+    assert not as64(got[:, 0], E.F16).any()
+
+
+@pytest.mark.parametrize("new", [[1, 1], [90, 3]])
+def test_the_widest_windows(ep, new):
+    """A window as long as anything can be, or longer, is none."""
+    rng = np.random.default_rng(25)
+    cache = Cache(rng, new, [130, 7], E.I8, 1, 64, 16)
+    q = floats(rng, (cache.rows, 2 * 64), E.F16)
+    plain, _ = attend(ep, cache, q, E.F16, 2)
+    for window in (1 << 29, (1 << 30) - 1, 1 << 30, (1 << 31) - 1):
+        got, _ = attend(ep, cache, q, E.F16, 2, local_window_size=window)
+        assert np.array_equal(got, plain), window
+
+
 def test_nan_and_infinite_queries(ep):
     rng = np.random.default_rng(15)
     for new in ([1, 1, 1, 1], [40, 9, 3, 1]):

@@ -163,6 +163,7 @@ def test_rotary_refusals(provider):
     k.release()
     k = provider.get_kernel({"head_size": 8}, op_type="RotaryEmbedding")
     refused(k, [at(E.F16, (4, 20)), p], [y], "must be a multiple of head_size=8")
+    refused(k, [E.TensorView(x.data, E.F16, (1, (1 << 20) + 1, 4, 8)), p], [y], "up to 2^20 heads")
     k.release()
 
 
@@ -195,6 +196,7 @@ CACHE_REFUSALS = [
     (6, lambda at: at(E.I32, (15,)), "block_table must have shape [N, W]"),
     (6, lambda at: at(E.I32, (3, 0)), "block_table must have shape [N, W]"),
     (6, lambda at: E.TensorView(HOLD.ctypes.data // 16 * 16 + 16, E.I32, (3, 1 << 26)), "fewer than 2^30 slots"),
+    (6, lambda at: E.TensorView(HOLD.ctypes.data // 16 * 16 + 16, E.I32, (1 << 19, 1)), "fewer than 2^20 sequences times key heads"),
     (6, lambda at: at(E.I32, (3, 5), strides=(8, 1)), "block_table must be contiguous"),
     (6, lambda at: at(E.I32, (3, 5), device_index=1), "block_table must live on ROCm device 0"),
 ]
@@ -236,6 +238,7 @@ def test_append_refusals(provider):
     refused(k, [key, value] + same, same[:4], "overlaps")
     inside = E.TensorView(views[0].data, E.F16, (6, 128))
     refused(k, [inside, value] + views, views[:4], "k_cache overlaps key")
+    refused(k, [E.TensorView(key.data, E.F16, (1 << 26, 128)), E.TensorView(value.data, E.F16, (1 << 26, 128))] + views, views[:4], "too many rows")
     refused(k, [key, value] + views[:6], views[:4], "expected 9..=9 inputs")
     k.execute([E.TensorView(None, E.F16, (0, 128)), NONE] + [NONE] * 7, [NONE] * 4)
     k.release()
@@ -254,7 +257,8 @@ def test_attention_refusals(provider):
     refused(k, [q] + views, [q], "output overlaps query")
     refused(k, [q] + views, [], "expected 1..=1 outputs")
     refused(k, [q] + views[:5], [y], "expected 8..=8 inputs")
-    refused(k, [E.TensorView(q.data, E.F16, (1 << 28, 256))] + views, [y], "too many rows")
+    for rows in (1 << 27, 1 << 28):
+        refused(k, [E.TensorView(q.data, E.F16, (rows, 256))] + views, [y], "too many rows")
     k.execute([E.TensorView(None, E.F16, (0, 256))] + [NONE] * 7, [NONE])
     k.release()
 
@@ -322,7 +326,8 @@ def test_workspace_requests(provider):
     descs = [((6, 256), E.F16)] + [(s, d) for s, d in CACHE]
     k = provider.get_kernel({"num_heads": 4, "kv_num_heads": 2, "head_size": 64}, op_type="CacheAttention")
     k.workspace_requirement(descs)
-    for bad, message in ((descs[:7], "needs the shapes"), (swapped(descs, 7, ((3, 1 << 26), E.I32)), "shapes that no call takes"), (swapped(descs, 0, ((1 << 28, 256), E.F16)), "shapes that no call takes")):
+    for bad, message in ((descs[:7], "needs the shapes"), (swapped(descs, 7, ((3, 1 << 26), E.I32)), "shapes that no call takes"), (swapped(descs, 0, ((1 << 28, 256), E.F16)), "shapes that no call takes"),
+                         (swapped(descs, 7, ((1 << 19, 1), E.I32)), "shapes that no call takes")):
         with pytest.raises(E.EpError, match=message):
             k.workspace_requirement(bad)
     k.release()
