@@ -15,6 +15,7 @@ namespace mnb {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kRows = 16;
+constexpr int kWhole = 32;                           // groups of 64 tokens below which a context stays whole
 
 // The largest of the four lanes 16 apart, in each of them.
 __device__ __forceinline__ float over_groups_max(float v)
@@ -383,15 +384,21 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
         return plan;
     const int group = a.heads / c.kv_heads;
     if (a.rows * group >= (1 << 30)) return plan;
-    // Beyond 64 rows a sequence, on average, tiles of many rows share what they read of the cache through LDS. (16 sequences of up to 4000 tokens, 64 rows a key head: 48 us in tiles of
-    // 16, 65 us in one of 128; 64 such sequences with 128 rows: 133 and 117 us.)
-    plan.many = a.rows * group > 64 * static_cast<int64_t>(c.sequences);
+    const int64_t cus = rocm_ffi_compute_units(), per_head = a.rows * group, capacity = static_cast<int64_t>(c.width) * c.page;
+    const bool small = c.head_size <= 128;
+    // Beyond 64 rows a sequence, on average, tiles of many rows share what they read of the cache through LDS, (16 sequences of up to 4000 tokens, 64 rows a key head: 48 us in tiles of
+    // 16, 65 us in one of 128; 64 such sequences with 128 rows: 139 and 117 us), unless there is little to do: where contexts are short or tiles few, a tile's own steps are what a call
+    // waits for, and tiles of 16 deal them out to more waves. That holds for up to four tiles of 16 for each CU (two with heads of 256, one of which fills a CU) where contexts stay whole,
+    // and for so much work in all where they are cut. (Prompts of 256 tokens, 32 heads by 8: 11 us in tiles of 16, 17 us in tiles of 128; 1000 tokens in a window of 1024, 14 heads of 64 by 2:
+    // 22 and 32 us; but 1024 tokens, 32 by 8: 49 and 33 us. 128 tokens after 3000: 26 and 38 us, after 6000: 45 and 41 us, after 16000: 95 and 63 us. Heads of 256, 64 tokens after 5000: 47 and
+    // 76 us, 256 tokens: 116 and 83 us.)
+    const int64_t fine = (per_head + kRows - 1) / kRows * c.kv_heads, seen = a.window > 0 && a.window < capacity ? a.window : capacity, busy = (small ? 2 : 1) * cus;
+    const bool little = fine <= 2 * busy && (seen <= kGroup * kWhole || fine * seen <= 3000 * busy);
+    plan.many = per_head > 64 * static_cast<int64_t>(c.sequences) && !little;
     plan.tile_rows = plan.many ? kManyRows : kRows;
     // 256 rows a tile, which halves what a row costs of the codes' way into LDS, once that gives two tiles for each CU; 128 rows with two teams of waves, which halves the steps that follow one
     // another, where there is no more than one tile for each CU. (4096 tokens over 32 heads by 8: 175 us, in tiles of 128 206 us; 2400 new tokens, 28 by 4: 54 us, with two teams
     // 68 us; 700 tokens, 32 by 32 heads of 80: 32 us with two teams, 43 us with one.)
-    const int64_t cus = rocm_ffi_compute_units(), per_head = a.rows * group;
-    const bool small = c.head_size <= 128;
     if (plan.many && small && per_head * c.kv_heads >= 2 * kMostRows * cus) plan.tile_rows = kMostRows;
     plan.tiles = per_head / plan.tile_rows + (a.rows < c.sequences ? a.rows : c.sequences);
     // Few rows: eight waves a tile instead of four, by the same rule. (16 sequences, 16 rows a key head, 8 of them: 31 us, with four waves 33 us; with 64 rows, four tiles a head: 57 and 48 us.)
@@ -404,8 +411,8 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
     int64_t wanted = at_once / c.kv_heads;
     if (wanted > kMostPieces - 1) wanted = kMostPieces - 1;
     plan.least = plan.many ? 16 : 8;
-    plan.whole = 32;
-    if (plan.tiles < wanted && static_cast<int64_t>(c.width) * c.page > kGroup * (plan.whole - 1)) plan.target = static_cast<int>(wanted);
+    plan.whole = kWhole;
+    if (plan.tiles < wanted && capacity > kGroup * (kWhole - 1)) plan.target = static_cast<int>(wanted);
     plan.pieces = plan.tiles + plan.target;
     const uint64_t places = 2 * static_cast<uint64_t>(plan.target) * c.kv_heads * plan.tile_rows;
     plan.sums_at = (places * c.head_size * 4 + 255) / 256 * 256;

@@ -43,6 +43,9 @@ def same_values(got, want, code):
     return np.array_equal(decode(got, code), decode(want, code), equal_nan=True)
 
 
+LEAST_SLOTS = [0]                   # that a sequence's table has, beyond what it needs: entries without a page
+
+
 class Cache:
     """A cache with pages at random places of the pool, one more than needed; slots and pages without tokens hold what would show (NaN codes, NaN scales)."""
 
@@ -50,7 +53,7 @@ class Cache:
         self.new, self.past, self.code, self.kv_heads, self.head, self.page = list(new), list(past), code, kv_heads, head, page
         need = [-(-(a + b) // page) for a, b in zip(new, past)]
         pages = sum(need) + 1
-        self.table = np.full((len(new), width or max(max(need, default=1), 1)), -7, np.int32)
+        self.table = np.full((len(new), max(width or max(max(need, default=1), 1), LEAST_SLOTS[0] // page)), -7, np.int32)
         order = rng.permutation(pages)
         at = 0
         for i, n in enumerate(need):

@@ -4,10 +4,18 @@ import pytest
 
 from onnx_genai_amd import ep as E
 
+from . import cache_helpers
 from .cache_helpers import Cache, attention64, floats
 from .node_helpers import EPS, Device, as64
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["short_table", "long_table"])
+def table(request, monkeypatch):
+    """Few rows in all go in small tiles where the table is short, and prompts of 65 rows and more in large ones where it has room for a million tokens."""
+    monkeypatch.setattr(cache_helpers, "LEAST_SLOTS", [(1 << 20) * (request.param == "long_table")])
+    return request.param
 
 
 def attend(ep, cache, q, dtype, heads, *, offset=0, packed=False, extra=0, views=None, dev=None, **attrs):
@@ -63,7 +71,7 @@ def test_single_tokens(ep, head, page, kv_heads, group, code, dtype):
 @pytest.mark.parametrize("dtype", [E.F16, E.BF16])
 @pytest.mark.parametrize("code", [E.I8, E.F8E4M3])
 @pytest.mark.parametrize("head,page,kv_heads,group", [(64, 16, 2, 7), (128, 64, 2, 4), (80, 32, 1, 1), (96, 128, 1, 3), (256, 64, 1, 2), (128, 32, 1, 48)])
-def test_chunks(ep, head, page, kv_heads, group, code, dtype):
+def test_chunks(ep, table, head, page, kv_heads, group, code, dtype):
     """Prompts and chunks behind a past, ragged, with tiles that begin inside a token's heads."""
     rng = np.random.default_rng(head + page)
     cache = Cache(rng, [70, 1, 0, 33, 5], [0, 100, 3, 129, 64], code, kv_heads, head, page, width=20)
@@ -98,22 +106,23 @@ def test_tiles_of_every_kind(ep, kind, head, page, code, window):
 
 @pytest.mark.parametrize("rows", [1, 2, 64, 65, 127, 128, 129, 200, 257])
 @pytest.mark.parametrize("group", [1, 4])
-def test_prompt_lengths(ep, rows, group):
+def test_prompt_lengths(ep, table, rows, group):
     rng = np.random.default_rng(rows)
     cache = Cache(rng, [rows], [0], E.I8, 1, 64, 16)
-    check(ep, cache, group, E.F16, 3)
+    variant = check(ep, cache, group, E.F16, 3)
+    assert variant.startswith("cache_attention_rows") == (table == "long_table" and rows * group > 64)
 
 
 @pytest.mark.parametrize("window", [1, 2, 16, 63, 64, 65, 100, 1000])
-@pytest.mark.parametrize("new", [[1, 1, 1], [40, 1, 90]])
-def test_windows(ep, new, window):
+@pytest.mark.parametrize("new,heads", [([1, 1, 1], 6), ([40, 1, 90], 6), ([40, 1, 90], 132)])
+def test_windows(ep, new, heads, window):
     rng = np.random.default_rng(window)
     cache = Cache(rng, new, [200, 0, 65], E.F8E4M3, 2, 64, 32)
-    check(ep, cache, 6, E.BF16, 4, window=window)
+    assert check(ep, cache, heads, E.BF16, 4, window=window).startswith("cache_attention_rows") == (heads == 132)
 
 
 @pytest.mark.parametrize("new", [[1, 1], [150, 7]])
-def test_softcap_and_scale(ep, new):
+def test_softcap_and_scale(ep, table, new):
     rng = np.random.default_rng(11)
     cache = Cache(rng, new, [200, 30], E.I8, 2, 128, 64)
     check(ep, cache, 8, E.F16, 5, sd=4.0, softcap=5.0)
@@ -123,7 +132,7 @@ def test_softcap_and_scale(ep, new):
 
 @pytest.mark.parametrize("new", [[1, 1], [150, 7]])
 @pytest.mark.parametrize("sd", [0.0, 1e-30, 1e-6, 30.0, 1e4])
-def test_sizes_of_queries(ep, sd, new):
+def test_sizes_of_queries(ep, table, sd, new):
     """From queries of zeros (even attention) to scores of thousands (one token takes all)."""
     rng = np.random.default_rng(12)
     cache = Cache(rng, new, [100, 30], E.I8, 1, 64, 16)
@@ -132,7 +141,7 @@ def test_sizes_of_queries(ep, sd, new):
 
 @pytest.mark.parametrize("code", [E.I8, E.F8E4M3])
 @pytest.mark.parametrize("new", [[1, 1], [150, 3]])
-def test_scales_of_pages(ep, new, code):
+def test_scales_of_pages(ep, table, new, code):
     """Pages whose scales differ by orders of magnitude, some zero: keys of zeros, values of zeros, both."""
     rng = np.random.default_rng(13)
     cache = Cache(rng, new, [300, 70], code, 2, 64, 16)
@@ -146,20 +155,20 @@ def test_scales_of_pages(ep, new, code):
     check(ep, cache, 4, E.BF16, 10)
 
 
-@pytest.mark.parametrize("new", [[1, 1, 1], [90, 3, 40]])
-def test_nan_stays_with_the_rows_that_see_it(ep, new):
+@pytest.mark.parametrize("new,heads", [([1, 1, 1], 4), ([90, 3, 40], 4), ([90, 3, 40], 132)])
+def test_nan_stays_with_the_rows_that_see_it(ep, new, heads):
     """A page of scale NaN, keys or values: rows that see it are NaN, others (before it, outside their window, of other heads and sequences) are as without it."""
     rng = np.random.default_rng(14)
     for which in ("ks", "vs"):
         cache = Cache(rng, new, [100, 70, 30], E.I8, 2, 64, 16)
-        q = floats(rng, (cache.rows, 4 * 64), E.F16)
-        want, slack = attention64(cache, as64(q, E.F16).reshape(-1, 4, 64), 4, window=40)
+        q = floats(rng, (cache.rows, heads * 64), E.F16)
+        want, slack = attention64(cache, as64(q, E.F16).reshape(-1, heads, 64), heads, window=40)
         bad = 6 if new[0] == 1 else 8                     # a page of the first sequence: all of its queries see page 6; some are before page 8, others are past it
         getattr(cache, which)[cache.table[0, bad], 0] = np.nan
-        got, _ = attend(ep, cache, q, E.F16, 4, local_window_size=40)
+        got, _ = attend(ep, cache, q, E.F16, heads, local_window_size=40)
         own = 100 + np.arange(new[0])
         sees = np.zeros(got.shape[:2], bool)
-        sees[:new[0], :2] = ((own >= 16 * bad) & (own - 40 < 16 * bad + 15))[:, None]
+        sees[:new[0], :heads // 2] = ((own >= 16 * bad) & (own - 40 < 16 * bad + 15))[:, None]
         assert sees.any() and not sees.all()
         assert np.isnan(as64(got, E.F16)[sees]).all()
         near(got[~sees], want[~sees], slack[~sees], E.F16)
@@ -167,7 +176,7 @@ def test_nan_stays_with_the_rows_that_see_it(ep, new):
 
 @pytest.mark.parametrize("new", [[1], [90]])
 @pytest.mark.parametrize("which", ["ks", "vs"])
-def test_nothing_but_nan_pages(ep, which, new):
+def test_nothing_but_nan_pages(ep, table, which, new):
     """Every page of one head has a scale of NaN: its rows are NaN, the other head's are as without it. And a scale of 0 is no NaN."""
     rng = np.random.default_rng(24)
     cache = Cache(rng, new, [700], E.I8, 2, 64, 16)
@@ -195,7 +204,7 @@ def test_the_widest_windows(ep, new):
         assert np.array_equal(got, plain), window
 
 
-def test_nan_and_infinite_queries(ep):
+def test_nan_and_infinite_queries(ep, table):
     rng = np.random.default_rng(15)
     for new in ([1, 1, 1, 1], [40, 9, 3, 1]):
         cache = Cache(rng, new, [100, 70, 30, 0], E.I8, 1, 64, 16)
@@ -211,18 +220,19 @@ def test_nan_and_infinite_queries(ep):
 
 
 @pytest.mark.parametrize("new", [[1, 1, 1], [70, 40, 40]])
-def test_pages_that_are_not_there(ep, new):
+def test_pages_that_are_not_there(ep, table, new):
     """Entries outside the pool hold no tokens: the rest of the context is what a row sees; a row that sees none is zero. Past lengths beyond the table end with it."""
     rng = np.random.default_rng(16)
     cache = Cache(rng, new, [160, 160, 160], E.F8E4M3, 1, 64, 16)
     q = floats(rng, (cache.rows, 2 * 64), E.F16)
-    views_of = lambda dev, table, past: cache.views(dev)[:5] + [dev.view(np.asarray(past, np.int32), E.I32), dev.view(table, E.I32)]  # noqa: E731
-    table = cache.table.copy()
-    table[0, 1::2] = [-1, cache.k.shape[0], 2 ** 31 - 1, -2 ** 31, -5, -1, -1][:len(table[0, 1::2])]
-    table[1] = -1
+    views_of = lambda dev, entries, past: cache.views(dev)[:5] + [dev.view(np.asarray(past, np.int32), E.I32), dev.view(entries, E.I32)]  # noqa: E731
+    entries = cache.table.copy()
+    odd = entries[0, 1:15:2]
+    odd[:] = [-1, cache.k.shape[0], 2 ** 31 - 1, -2 ** 31, -5, -1, -1][:len(odd)]
+    entries[1] = -1
     dev = Device(ep)
     try:
-        got, _ = attend(ep, cache, q, E.F16, 2, views=views_of(dev, table, cache.past_lengths), dev=dev)
+        got, _ = attend(ep, cache, q, E.F16, 2, views=views_of(dev, entries, cache.past_lengths), dev=dev)
     finally:
         dev.free()
     # the definition over the tokens that are there
@@ -282,7 +292,7 @@ def test_weights_far_below_the_largest(ep):
 
 
 @pytest.mark.parametrize("new", [[1, 1], [150, 7]])
-def test_shared_pages(ep, new):
+def test_shared_pages(ep, table, new):
     """Two sequences over the same prompt's pages."""
     rng = np.random.default_rng(20)
     cache = Cache(rng, new, [128, 128], E.I8, 1, 64, 64)
