@@ -111,8 +111,8 @@ __global__ __launch_bounds__(kThreads, UNITS == 1 && sizeof(T) == 2 ? 8 : 1) voi
         const Sequence s = sequence_of(c, b, static_cast<int>(a.rows));
         return s.rows ? (s.past % page + s.rows + page - 1) / page : 0;
     };
-    int b, k, unused;
-    if (!find_piece(c.sequences, blockIdx.x, pages_of, [](int) { return 0; }, &b, &k, &unused)) return;
+    int b, k;
+    if (!find_piece(c.sequences, blockIdx.x, pages_of, &b, &k)) return;
     const Sequence s = sequence_of(c, b, static_cast<int>(a.rows));
     const int begun = s.past % page;
     const int slot = k == 0 ? begun : 0;                 // the page's first new token

@@ -88,22 +88,22 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void attentio
     float (*const results)[kRows][D + 4] = reinterpret_cast<float (*)[kRows][D + 4]>(lds);                    // [kWaves]
     float2 (*const sums)[kRows] = reinterpret_cast<float2 (*)[kRows]>(lds + kWaves * kRows * (D + 4));         // [kWaves]
     const RocmCache& c = p.a.cache;
-    const int head = blockIdx.x % c.kv_heads;
     Piece w;
-    if (!piece_at(p, blockIdx.x / c.kv_heads, &w)) return;
+    if (!piece_at(p, blockIdx.x, &w)) return;
+    const int head = w.head;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int context = context_of(c, w.s);
 
     // the lane's query row
     const int first_row = w.tile * kRows, rows = w.s.rows * p.group - first_row < kRows ? w.s.rows * p.group - first_row : kRows;
-    const int token = (first_row + n) / p.group, member = first_row + n - token * p.group;
+    const int token = p.by_group.of(first_row + n), member = first_row + n - token * p.group;
     const int own = w.s.past + token;                                        // the row's own slot
     const bool row_there = n < rows;
     const uint16_t* const q_row = static_cast<const uint16_t*>(p.a.q) + static_cast<int64_t>(w.s.first + token) * p.a.q_step + (head * p.group + member) * D;
     Queries<D> q;
     // tokens that every row of the tile sees, and those that some row does
-    const int first_own = w.s.past + first_row / p.group, last_own = w.s.past + (first_row + rows - 1) / p.group;
+    const int first_own = w.s.past + p.by_group.of(first_row), last_own = w.s.past + p.by_group.of(first_row + rows - 1);
     const int window = p.a.window;
 
     float4_t o[kTiles];
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void attentio
         } else {
             // a row that sees nothing is zero
             const float inverse = total == 0.f ? 0.f : 1.0f / total;
-            const int r = first_row + row, tk = r / p.group;
+            const int r = first_row + row, tk = p.by_group.of(r);
             uint16_t* const to = static_cast<uint16_t*>(p.a.y) + static_cast<int64_t>(w.s.first + tk) * out_step + (head * p.group + r - tk * p.group) * D + e;
             store_four(to, all[0] * inverse, all[1] * inverse, all[2] * inverse, all[3] * inverse, p.a.dtype);
         }
@@ -309,68 +309,69 @@ __global__ __launch_bounds__(kThreads, 6) void attention_join_kernel(AttentionPa
     const RocmCache& c = p.a.cache;
     const int head = blockIdx.x % c.kv_heads;
     Piece w;
-    if (!tile_to_join(p, blockIdx.x / c.kv_heads, &w)) return;
+    if (!tile_to_join(p, p.by_heads.of(blockIdx.x), &w)) return;
     const int first_row = w.tile * p.tile_rows, left = w.s.rows * p.group - first_row, rows = left < p.tile_rows ? left : p.tile_rows;
-    const int row0 = blockIdx.y * rows_at_once;
-    if (row0 >= rows) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t piece_step = static_cast<int64_t>(c.kv_heads) * p.tile_rows, first = (static_cast<int64_t>(w.slot) * c.kv_heads + head) * p.tile_rows;
     // a group of d / 4 threads has a row's elements, four each, over every so many pieces; the first of them are on their way before anything is known of their shares
     const int quads = d / 4, groups = kThreads / quads, each = groups / rows_at_once;
     const int group = threadIdx.x / quads, quad = threadIdx.x - group * quads, r = group / each, part = group - r * each;
-    const bool busy = r < rows_at_once && row0 + r < rows;
-    const float* const from = p.partial + (first + row0 + (busy ? r : 0)) * d + quad * 4;
-    constexpr int kEarly = 4;
-    float4_t early[kEarly];
-#pragma unroll
-    for (int j = 0; j < kEarly; ++j) {
-        const int i = part + j * each;
-        early[j] = float4_t{0.f, 0.f, 0.f, 0.f};
-        if (busy && i < w.pieces) early[j] = *reinterpret_cast<const float4_t*>(from + i * piece_step * d);
-    }
-    for (int k = wave; k < rows_at_once; k += kWaves) {
-        const int row = row0 + k < rows ? row0 + k : rows - 1;
-        float most = kNone;
-        for (int i = lane; i < w.pieces; i += 64) most = fmaxf(most, p.partial_sums[first + i * piece_step + row].x);
-        most = over_wave(most, [](float x, float y) { return fmaxf(x, y); });
-        const float zero = most == kNone ? 0.f : most;
-        float sum = 0.f;
-        for (int i = lane; i < w.pieces; i += 64) {
-            const float2 s = p.partial_sums[first + i * piece_step + row];
-            const float share = __builtin_amdgcn_exp2f(s.x - zero);
-            sum += s.y * share;
-            shares[k * w.pieces + i] = share;
-        }
-        sum = over_wave(sum, [](float x, float y) { return x + y; });
-        const float inverse = sum == 0.f ? 0.f : 1.0f / sum;
-        for (int i = lane; i < w.pieces; i += 64) shares[k * w.pieces + i] *= inverse;
-    }
-    __syncthreads();
     float4_t* const sums = reinterpret_cast<float4_t*>(shares + (rows_at_once * w.pieces + 3) / 4 * 4);
-    float4_t all = {0.f, 0.f, 0.f, 0.f};
-    if (busy) {
-        const float* const share = shares + r * w.pieces;
+    for (int row0 = blockIdx.y * rows_at_once; row0 < rows; row0 += gridDim.y * rows_at_once) {
+        const bool busy = r < rows_at_once && row0 + r < rows;
+        const float* const from = p.partial + (first + row0 + (busy ? r : 0)) * d + quad * 4;
+        constexpr int kEarly = 4;
+        float4_t early[kEarly];
 #pragma unroll
-        for (int j = 0; j < kEarly; ++j)
-            if (part + j * each < w.pieces) all += early[j] * share[part + j * each];
+        for (int j = 0; j < kEarly; ++j) {
+            const int i = part + j * each;
+            early[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+            if (busy && i < w.pieces) early[j] = *reinterpret_cast<const float4_t*>(from + i * piece_step * d);
+        }
+        for (int k = wave; k < rows_at_once; k += kWaves) {
+            const int row = row0 + k < rows ? row0 + k : rows - 1;
+            float most = kNone;
+            for (int i = lane; i < w.pieces; i += 64) most = fmaxf(most, p.partial_sums[first + i * piece_step + row].x);
+            most = over_wave(most, [](float x, float y) { return fmaxf(x, y); });
+            const float zero = most == kNone ? 0.f : most;
+            float sum = 0.f;
+            for (int i = lane; i < w.pieces; i += 64) {
+                const float2 s = p.partial_sums[first + i * piece_step + row];
+                const float share = __builtin_amdgcn_exp2f(s.x - zero);
+                sum += s.y * share;
+                shares[k * w.pieces + i] = share;
+            }
+            sum = over_wave(sum, [](float x, float y) { return x + y; });
+            const float inverse = sum == 0.f ? 0.f : 1.0f / sum;
+            for (int i = lane; i < w.pieces; i += 64) shares[k * w.pieces + i] *= inverse;
+        }
+        __syncthreads();
+        float4_t all = {0.f, 0.f, 0.f, 0.f};
+        if (busy) {
+            const float* const share = shares + r * w.pieces;
+#pragma unroll
+            for (int j = 0; j < kEarly; ++j)
+                if (part + j * each < w.pieces) all += early[j] * share[part + j * each];
 #pragma unroll 4
-        for (int i = part + kEarly * each; i < w.pieces; i += each) {
-            const float4_t v = *reinterpret_cast<const float4_t*>(from + i * piece_step * d);
-            const float f = share[i];
-            all += v * f;
+            for (int i = part + kEarly * each; i < w.pieces; i += each) {
+                const float4_t v = *reinterpret_cast<const float4_t*>(from + i * piece_step * d);
+                const float f = share[i];
+                all += v * f;
+            }
+        }
+        sums[threadIdx.x] = all;
+        __syncthreads();
+        if (busy && part == 0) {
+            for (int i = 1; i < each; ++i) all += sums[threadIdx.x + i * quads];
+            const int row = first_row + row0 + r, tk = p.by_group.of(row);
+            store_four(static_cast<uint16_t*>(p.a.y) + (static_cast<int64_t>(w.s.first + tk) * p.a.heads + head * p.group + row - tk * p.group) * d + quad * 4, all[0], all[1], all[2], all[3], p.a.dtype);
         }
     }
-    sums[threadIdx.x] = all;
-    __syncthreads();
-    if (!busy || part != 0) return;
-    for (int i = 1; i < each; ++i) all += sums[threadIdx.x + i * quads];
-    const int row = first_row + row0 + r, tk = row / p.group;
-    store_four(static_cast<uint16_t*>(p.a.y) + (static_cast<int64_t>(w.s.first + tk) * p.a.heads + head * p.group + row - tk * p.group) * d + quad * 4, all[0], all[1], all[2], all[3], p.a.dtype);
 }
 
 struct Plan {
     bool ok, many;
-    int tile_rows, target, least, whole, teams;
+    int tile_rows, target, least, whole, teams, most;
     int64_t tiles, pieces;          // most that a call of these sizes has, for one key head
     uint64_t sums_at, bytes;
 };
@@ -412,7 +413,10 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
     if (wanted > kMostPieces - 1) wanted = kMostPieces - 1;
     plan.least = plan.many ? 16 : 8;
     plan.whole = kWhole;
-    if (plan.tiles < wanted && capacity > kGroup * (kWhole - 1)) plan.target = static_cast<int>(wanted);
+    // what a window lets the rows of a tile see (one more token than its rows have: it may begin inside a token's heads)
+    const int64_t tokens = (plan.tile_rows + group - 1) / group + 1;
+    plan.most = a.window > 0 ? static_cast<int>((a.window + tokens + kGroup - 2) / kGroup + 1) : 1 << 24;
+    if (plan.tiles < wanted && capacity > kGroup * (kWhole - 1) && plan.most >= kWhole) plan.target = static_cast<int>(wanted);
     plan.pieces = plan.tiles + plan.target;
     const uint64_t places = 2 * static_cast<uint64_t>(plan.target) * c.kv_heads * plan.tile_rows;
     plan.sums_at = (places * c.head_size * 4 + 255) / 256 * 256;
@@ -475,8 +479,12 @@ extern "C" int rocm_launch_cache_attention(const RocmCacheAttentionArgs* args, v
     p.a = *args;
     p.group = args->heads / args->cache.kv_heads;
     p.tile_rows = plan.tile_rows;
+    p.tile_bits = __builtin_ctz(plan.tile_rows);
+    p.by_group = Divisor(p.group);
+    p.by_heads = Divisor(args->cache.kv_heads);
     p.target = plan.target;
-    p.least = plan.least;
+    p.least_bits = __builtin_ctz(plan.least);
+    p.most = plan.most;
     p.whole = plan.whole;
     p.teams = plan.teams;
     p.slots = 2 * plan.target;
@@ -488,8 +496,10 @@ extern "C" int rocm_launch_cache_attention(const RocmCacheAttentionArgs* args, v
     if (e == hipSuccess && plan.target) {
         // A row's pieces are many where there are few tiles: then all groups of threads have one row, else two groups each.
         const int d = args->cache.head_size, groups = kThreads / (d / 4), rows = plan.tiles <= 2 ? 1 : groups / 2;
+        // a few workgroups for each CU, which go on to further rows: most tiles may have nothing to join
+        const int64_t all = plan.tiles * args->cache.kv_heads, most = (plan.tile_rows + rows - 1) / rows, wanted = (8 * static_cast<int64_t>(rocm_ffi_compute_units()) + all - 1) / all;
         const unsigned lds = static_cast<unsigned>((rows * (plan.target + 1) + 3) / 4 * 16 + kThreads * 16);
-        hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<unsigned>(plan.tiles * args->cache.kv_heads), static_cast<unsigned>((plan.tile_rows + rows - 1) / rows)), dim3(kThreads), lds, s, p, d, rows);
+        hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<unsigned>(all), static_cast<unsigned>(wanted < most ? wanted : most)), dim3(kThreads), lds, s, p, d, rows);
         e = hipGetLastError();
     }
     return static_cast<int>(e);

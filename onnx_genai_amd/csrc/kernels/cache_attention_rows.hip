@@ -54,9 +54,9 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     Tile<D>* const tiles = reinterpret_cast<Tile<D>*>(lds);
     const RocmCache& c = p.a.cache;
-    const int head = blockIdx.x % c.kv_heads;
     Piece w;
-    if (!piece_at(p, blockIdx.x / c.kv_heads, &w)) return;
+    if (!piece_at(p, blockIdx.x, &w)) return;
+    const int head = w.head;
     const int team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads) : 0, thread = threadIdx.x - team * kThreads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const int n = lane & 31, h = lane >> 5;
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
 
     // the lane's query row: half h has the elements 16 i + 8 h of it
     const int first_row = w.tile * kRows + wave * kWaveRows, left = w.s.rows * p.group - first_row, rows = left < kWaveRows ? left : kWaveRows;
-    const int token = (first_row + n) / p.group, member = first_row + n - token * p.group;
+    const int token = p.by_group.of(first_row + n), member = first_row + n - token * p.group;
     const int own = w.s.past + token, last_seen = own < context ? own : context - 1;
     Bytes16 raw[kSteps];
     {
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
         }
     }
     // tokens that every row of the wave sees, and those that some row does
-    const int first_own = w.s.past + first_row / p.group, last_own = w.s.past + (first_row + (rows > 0 ? rows : 1) - 1) / p.group;
+    const int first_own = w.s.past + p.by_group.of(first_row), last_own = w.s.past + p.by_group.of(first_row + (rows > 0 ? rows : 1) - 1);
     const int window = p.a.window;
 
     const int page_bits = __builtin_ctz(c.page);
