@@ -333,7 +333,7 @@ NxrtStatus nxrt_rocm_rotary_embedding_create(NxrtRocmEp* ep, const NxrtRocmRotar
  * A page whose first token is new gets scale = max|x| / top over its new tokens (top: 127, or 448), code = x / scale to the nearest, ties to even; a scale of 0 gives codes
  * 0. A page that has tokens gets scale' = max(scale, max|x| / top), and where that is larger, its codes become code * (scale / scale') to the nearest: each such
  * step adds up to half a step of rounding to the tokens before. An infinity or a NaN makes the scale NaN and the new codes 0 (and those before), until the page begins
- * again. Slots that no token has are left as they are. Two sequences may share pages, but not one that a call writes. */
+ * again. Slots that no token has are left as they are. Two sequences may share pages, but a page that a call writes stands in one place of one table row only. */
 typedef struct NxrtRocmCacheAppendAttrs {
   uint32_t struct_size;
   uint32_t present;      /* bit i: 0 num_heads (0; read for packed rows), 1 kv_num_heads (required), 2 head_size (required) */

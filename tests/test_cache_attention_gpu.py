@@ -273,6 +273,20 @@ def test_pieces_of_long_contexts(ep, new, past, window):
     assert check(ep, cache, 4, E.F16, 18, window=window).endswith("pieces") == (window != 1500)
 
 
+@pytest.mark.parametrize("new,past,heads,kv_heads,page,variant", [([3, 9], [5000, 2500], 30, 10, 64, "cache_attention_pieces"), ([1, 0, 30, 2], [2300, 9, 4100, 40], 12, 3, 16, "cache_attention_pieces"),
+                                                                  ([300], [9000], 12, 3, 64, "cache_attention_rows_pieces"), ([290, 3, 1], [6500, 7000, 1], 30, 10, 32, "cache_attention_rows_pieces")])
+def test_pieces_of_several_tiles_and_heads(ep, new, past, heads, kv_heads, page, variant):
+    """Tiles, pieces and key heads in numbers that no power of two divides; some rows against the definition."""
+    rng = np.random.default_rng(heads + past[0])
+    cache = Cache(rng, new, past, E.I8, kv_heads, 64, page)
+    q = floats(rng, (cache.rows, heads * 64), E.F16)
+    got, used = attend(ep, cache, q, E.F16, heads)
+    assert used == variant
+    rows = set(rng.integers(0, cache.rows, 10).tolist()) | {int(e) - 1 for e in cache.ends[1:]}
+    want, slack = attention64(cache, as64(q, E.F16).reshape(-1, heads, 64), heads, rows=rows)
+    near(got[sorted(rows)], want[sorted(rows)], slack[sorted(rows)], E.F16)
+
+
 def test_weights_far_below_the_largest(ep):
     """One token at the top and thousands far below it, whose weights together count: none of them is lost to f16."""
     rng = np.random.default_rng(19)
