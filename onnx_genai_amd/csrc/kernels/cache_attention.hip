@@ -395,8 +395,8 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
     // 16, 65 us in one of 128; 64 such sequences with 128 rows: 139 and 117 us), unless there is little to do: where contexts are short or tiles few, a tile's own steps are what a call
     // waits for, and tiles of 16 deal them out to more waves. That holds for up to four tiles of 16 for each CU (two with heads of 256, one of which fills a CU) where contexts stay whole,
     // and for so much work in all where they are cut. (Prompts of 256 tokens, 32 heads by 8: 11 us in tiles of 16, 17 us in tiles of 128; 1000 tokens in a window of 1024, 14 heads of 64 by 2:
-    // 22 and 32 us; but 1024 tokens, 32 by 8: 49 and 33 us. 128 tokens after 3000: 26 and 38 us, after 6000: 45 and 41 us, after 16000: 95 and 63 us. Heads of 256, 64 tokens after 5000: 47 and
-    // 76 us, 256 tokens: 116 and 83 us.)
+    // 20 and 32 us; but 1024 tokens, 32 by 8: 49 and 32 us. 128 tokens after 3000: 25 and 36 us, after 6000: 45 and 38 us, after 16000: 95 and 59 us. Heads of 256, 64 tokens after 5000: 44 and
+    // 72 us, 256 tokens: 107 and 78 us.)
     const int64_t fine = (per_head + kRows - 1) / kRows * c.kv_heads, seen = a.window > 0 && a.window < capacity ? a.window : capacity, busy = (small ? 2 : 1) * cus;
     const bool little = fine <= 2 * busy && (seen <= kGroup * kWhole || fine * seen <= 3000 * busy);
     plan.many = per_head > 64 * static_cast<int64_t>(c.sequences) && !little;
@@ -407,12 +407,12 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
     if (plan.many && small && per_head * c.kv_heads >= 2 * kMostRows * cus) plan.tile_rows = kMostRows;
     plan.tiles = per_head / plan.tile_rows + (a.rows < c.sequences ? a.rows : c.sequences);
     // Few rows: eight waves a tile instead of four, by the same rule. (16 sequences, 16 rows a key head, 8 of them: 31 us, with four waves 33 us; with 64 rows, four tiles a head: 57 and 48 us.)
-    const int64_t least_tiles = plan.tiles - (a.rows < c.sequences ? a.rows : c.sequences), filled = least_tiles > c.sequences || a.rows < c.sequences ? least_tiles : c.sequences;
+    const int64_t busy_sequences = a.rows < c.sequences ? a.rows : c.sequences, full_tiles = per_head / plan.tile_rows, filled = full_tiles > busy_sequences ? full_tiles : busy_sequences;
     plan.teams = small && filled * c.kv_heads <= cus ? 2 : 1;
     // Pieces until there are as many workgroups as fit on the GPU at once: two for each CU, or one of 512 threads or heads of 256. None is shorter than 512 tokens, or 1024 in tiles of
     // many rows, and contexts below 2048 stay whole: joining pieces costs about what so many tokens take. (One token after 1000: 9 us whole, 13 us in two pieces; four tokens after 4000
-    // with heads of 256: 31 us in pieces of 512 and more, 44 us in pieces of 1024 and more; three chunks in a window of 1024: 31 us whole, 35 us in pieces.)
-    const int64_t at_once = plan.teams == 2 || plan.tile_rows == kMostRows || (plan.many && !small) ? cus : 2 * cus;
+    // with heads of 256: 31 us in pieces of 512 and more, 44 us in pieces of 1024 and more.)
+    const int64_t at_once = plan.teams == 2 || plan.tile_rows == kMostRows || !small ? cus : 2 * cus;
     int64_t wanted = at_once / c.kv_heads;
     if (wanted > kMostPieces - 1) wanted = kMostPieces - 1;
     plan.least = plan.many ? 16 : 8;
@@ -420,7 +420,7 @@ Plan plan_of(const RocmCacheAttentionArgs& a)
     // what a window lets the rows of a tile see (one more token than its rows have: it may begin inside a token's heads)
     const int64_t tokens = (plan.tile_rows + group - 1) / group + 1;
     plan.most = a.window > 0 ? static_cast<int>((a.window + tokens + kGroup - 2) / kGroup + 1) : 1 << 24;
-    if (plan.tiles < wanted && capacity > kGroup * (kWhole - 1) && plan.most >= kWhole) plan.target = static_cast<int>(wanted);
+    if (filled < wanted && capacity > kGroup * (kWhole - 1) && plan.most >= kWhole) plan.target = static_cast<int>(wanted);
     plan.pieces = plan.tiles + plan.target;
     const uint64_t places = 2 * static_cast<uint64_t>(plan.target) * c.kv_heads * plan.tile_rows;
     plan.sums_at = (places * c.head_size * 4 + 255) / 256 * 256;
