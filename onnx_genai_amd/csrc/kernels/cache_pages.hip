@@ -63,7 +63,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
 {
     extern __shared__ uint32_t held[];                         // a bit for each page
     __shared__ int parent[ROCM_PAGES_MAX_SLOTS], length[ROCM_PAGES_MAX_SLOTS], begun[ROCM_PAGES_MAX_SLOTS], start[ROCM_PAGES_MAX_SLOTS], keeps[ROCM_PAGES_MAX_SLOTS];
-    __shared__ int list[kThreads], slots[3][kWaves], missing;
+    __shared__ int list[kThreads], slots[3][kWaves], missing, made;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int pages = static_cast<int>(a.pages), words = (pages + 31) / 32, capacity = a.width * a.page;
     auto page_at = [&](int slot, int j) {
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
         return p >= 0 && p < pages ? p : -1;
     };
     for (int i = t; i < words; i += kThreads) held[i] = 0;
-    if (t == 0) missing = 0;
+    if (t == 0) missing = made = 0;
     if (t < a.slots) {
         const int p = a.parents && !a.compact ? a.parents[t] : t;
         parent[t] = p >= 0 && p < a.slots ? p : -1;
@@ -193,9 +193,11 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
         }
         a.moves[2 * t] = copy >= 0 ? begun[t] : -1;
         a.moves[2 * t + 1] = copy;
-        if (copies) {
+        // Copies that got a page alone: fresh pages are dealt out in the order of the slots, so those are the first copies, and there are no more of them than pages.
+        if (copy >= 0) {
             w.from[at[2]] = begun[t];
-            w.to[at[2]] = copy;                                  // (-1 where there was no page: nothing is copied)
+            w.to[at[2]] = copy;
+            if (needed > free_pages) atomicAdd(&made, 1);
         }
         a.next_lengths[t] = length[t];
     }
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
     }
     __syncthreads();
     if (t == 0) {
-        *w.count = moves;
+        *w.count = needed > free_pages ? made : moves;
         a.counts[0] = pages - free_pages + (needed < free_pages ? needed : free_pages);
         a.counts[1] = missing;
     }
