@@ -368,7 +368,8 @@ NxrtStatus nxrt_rocm_cache_attention_create(NxrtRocmEp* ep, const NxrtRocmCacheA
  *           order) Int32: from, to, or -1; 3 counts [2] Int32: pages in use, pages that were missing; 4 .. the pools, the inputs' own tensors.
  * Slot i has the pages of its parent that are whole. A begun one stays with the lowest slot that continues it, if no slot has it as a whole page; the others get a copy in a
  * fresh page. Fresh pages, copies first and then those that new_tokens need, are the lowest that no slot has, dealt out slot by slot. Where they run out, entries are -1 and
- * count as missing (as do entries outside 0 .. P - 1); the inputs' table still stands then. No count is kept beside the table: a page is free if no slot has it.
+ * count as missing (as do entries outside 0 .. P - 1), and no page that the inputs' table has is written, so that it still stands: a copy into one is not made, its entry and move are -1.
+ * No count is kept beside the table: a page is free if no slot has it.
  * With compact (parents and new_tokens absent) the k-th page in use beyond the first n goes to the k-th free one among them, n the pages in use.
  * S <= 1024, P <= 2^18, W page_size < 2^30, S W < 2^31. */
 typedef struct NxrtRocmCachePagesAttrs {

@@ -20,7 +20,7 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64, kCopyThreads = 256, kCopy
 struct PagesWorkspace {
     int32_t* count;       // [1]: moves
     int32_t* from;        // [pages]: sources of moves
-    int32_t* to;          // [pages]: and where they go
+    int32_t* to;          // [pages]: and where they go; -1: nowhere
     int32_t* list;        // [pages]: free pages by rank; compacting, where a page goes
 };
 
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
 {
     extern __shared__ uint32_t held[];                         // a bit for each page
     __shared__ int parent[ROCM_PAGES_MAX_SLOTS], length[ROCM_PAGES_MAX_SLOTS], begun[ROCM_PAGES_MAX_SLOTS], start[ROCM_PAGES_MAX_SLOTS], keeps[ROCM_PAGES_MAX_SLOTS];
-    __shared__ int list[kThreads], slots[3][kWaves], missing, made;
+    __shared__ int list[kThreads], slots[3][kWaves], missing, made, refused;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int pages = static_cast<int>(a.pages), words = (pages + 31) / 32, capacity = a.width * a.page;
     auto page_at = [&](int slot, int j) {
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
         return p >= 0 && p < pages ? p : -1;
     };
     for (int i = t; i < words; i += kThreads) held[i] = 0;
-    if (t == 0) missing = made = 0;
+    if (t == 0) missing = made = refused = 0;
     if (t < a.slots) {
         const int p = a.parents && !a.compact ? a.parents[t] : t;
         parent[t] = p >= 0 && p < a.slots ? p : -1;
@@ -176,10 +176,22 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
             else w.list[rank] = p;
         }
     __syncthreads();
+    // Where pages run out, the inputs' table is what the caller goes on with: no page that it has is written. A copy into one is not made, and its entry is missing.
+    const bool run_out = needed > free_pages;
+    if (run_out) {
+        for (int i = t; i < words; i += kThreads) held[i] = 0;
+        __syncthreads();
+        for (uint32_t e = t; e < entries; e += kThreads) {
+            const int i = static_cast<int>(e / static_cast<uint32_t>(a.width)), j = static_cast<int>(e - static_cast<uint32_t>(i) * a.width), n = a.lengths[i];
+            const int p = n > 0 && j < ((n > capacity ? capacity : n) + a.page - 1) / a.page ? page_at(i, j) : -1;
+            if (p >= 0) set(held, p);
+        }
+        __syncthreads();
+    }
     auto fresh = [&](int k) { return k >= free_pages ? -1 : k < kThreads ? list[k] : w.list[k]; };
     constexpr int kOwn = 2;                                      // further pages that a slot's thread enters itself
     if (t < a.slots) {
-        const int copy = copies ? fresh(mine) : -1, have = (length[t] + a.page - 1) / a.page;
+        const int dealt = copies ? fresh(mine) : -1, copy = run_out && dealt >= 0 && is_set(held, dealt) ? -1 : dealt, have = (length[t] + a.page - 1) / a.page;
         int32_t* const next = a.next + static_cast<int64_t>(t) * a.width;
         if (rest) {
             const int p = keep ? begun[t] : copy;
@@ -194,10 +206,11 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
         a.moves[2 * t] = copy >= 0 ? begun[t] : -1;
         a.moves[2 * t + 1] = copy;
         // Copies that got a page alone: fresh pages are dealt out in the order of the slots, so those are the first copies, and there are no more of them than pages.
-        if (copy >= 0) {
+        if (dealt >= 0) {
             w.from[at[2]] = begun[t];
             w.to[at[2]] = copy;
-            if (needed > free_pages) atomicAdd(&made, 1);
+            if (run_out) atomicAdd(&made, 1);
+            if (copy < 0) atomicAdd(&refused, 1);
         }
         a.next_lengths[t] = length[t];
     }
@@ -212,8 +225,8 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
     }
     __syncthreads();
     if (t == 0) {
-        *w.count = needed > free_pages ? made : moves;
-        a.counts[0] = pages - free_pages + (needed < free_pages ? needed : free_pages);
+        *w.count = run_out ? made : moves;
+        a.counts[0] = pages - free_pages + (run_out ? free_pages - refused : needed);
         a.counts[1] = missing;
     }
 }

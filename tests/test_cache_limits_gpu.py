@@ -49,3 +49,53 @@ def test_more_copies_than_pages(ep, slots, pages, longer):
     expected = pool.copy()
     expected[:, made[:, 1]] = pool[:, made[:, 0]]
     assert np.array_equal(after, expected)
+
+
+def held_by(table, lengths, page):
+    return {int(p) for row, n in zip(table, lengths) for p in row[:-(-int(n) // page)]}
+
+
+def without_the_old(want, table, lengths, parents, page):
+    """A step that runs out of pages, by the definition: copies into pages that the inputs' table has are not made."""
+    next_table, next_lengths, moves, counts = (x.copy() for x in want)
+    old = held_by(table, lengths, page)
+    for i, (_, to) in enumerate(moves):
+        if to >= 0 and int(to) in old:
+            next_table[i, next_lengths[i] // page] = -1
+            moves[i] = -1
+            counts += [-1, 1]
+    return next_table, next_lengths, moves, counts
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("slots,width,pages", [(6, 5, 22), (40, 6, 150), (300, 3, 500)])
+def test_the_table_of_before_stands_where_pages_run_out(ep, slots, width, pages, seed):
+    rng = np.random.default_rng(seed)
+    page, order, at = 16, rng.permutation(pages), 0
+    table, lengths = np.full((slots, width), -1, np.int32), np.zeros(slots, np.int32)
+    for i in range(slots):                                     # sequences until the pool is all but full
+        n = int(min(rng.integers(0, width), pages - 2 - at))
+        table[i, :n] = order[at:at + n]
+        lengths[i] = max(0, n * page - int(rng.integers(0, page)))
+        at += n
+    parents, grow = rng.integers(0, max(1, slots // 3), slots), np.full(slots, 3 * page)
+    pool = rng.integers(0, 256, (3, pages, 52), dtype=np.uint8)
+    got, after = step_pages(ep, table, lengths, parents, grow, page, pool)
+    plain = pages_step(table, lengths, parents, grow, page, pages)
+    want = plain
+    if plain[3][1]:                                            # (some of the smaller tables have pages enough)
+        want = without_the_old(plain, table, lengths, parents, page)
+        old = sorted(held_by(table, lengths, page))
+        assert np.array_equal(after[:, old], pool[:, old]), "bytes of the table of before"
+    for name, g, w in zip(("table", "lengths", "moves", "counts"), got, want):
+        assert np.array_equal(g, w), name
+    expected = pool.copy()
+    made = want[2][want[2][:, 1] >= 0]
+    expected[:, made[:, 1]] = pool[:, made[:, 0]]
+    assert np.array_equal(after, expected)
+    # other parents, and no growth, from the same table
+    again = np.where(np.arange(slots) < 2, np.arange(slots), -1)
+    got, last = step_pages(ep, table, lengths, again, None, page, after)
+    want = pages_step(table, lengths, again, np.zeros(slots), page, pages)
+    for name, g, w in zip(("table", "lengths", "moves", "counts"), got, want):
+        assert np.array_equal(g, w), name
