@@ -371,7 +371,7 @@ NxrtStatus nxrt_rocm_cache_attention_create(NxrtRocmEp* ep, const NxrtRocmCacheA
  * count as missing (as do entries outside 0 .. P - 1), and no page that the inputs' table has is written, so that it still stands: a copy into one is not made, its entry and move are -1.
  * No count is kept beside the table: a page is free if no slot has it.
  * With compact (parents and new_tokens absent) the k-th page in use beyond the first n goes to the k-th free one among them, n the pages in use.
- * S <= 1024, P <= 2^18, W page_size < 2^30, S W < 2^31. */
+ * Without slots (S = 0) counts are 0 and moves -1, and the other tensors may be absent. S <= 1024, P <= 2^18, W page_size < 2^30, S W < 2^31. */
 typedef struct NxrtRocmCachePagesAttrs {
   uint32_t struct_size;
   uint32_t present;      /* bit i: 0 page_size (required; 1..=2^20), 1 compact (0) */

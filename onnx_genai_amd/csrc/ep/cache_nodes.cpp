@@ -432,11 +432,34 @@ struct PagesNode final : NxrtRocmNode {
         *bytes = rocm_cache_pages_workspace_bytes(&a);
         return ok();
     }
+    // No page is in use and none moves; whoever asks for counts and moves has to find that. None of the other tensors needs memory behind it.
+    NxrtStatus without_slots(Call& c)
+    {
+        const auto* moves = s.compact ? c.output(2, "moves") : nullptr;
+        const auto* counts = c.output(3, "counts");
+        c.dtype(counts, "counts", {NXRT_DT_INT32});
+        c.shape(counts, "counts", {2});
+        c.dtype(moves, "moves", {NXRT_DT_INT32});
+        if (moves && !c.failed() && (moves->ndim != 2 || moves->shape[0] > ROCM_PAGES_MAX_PAGES / 2)) c.fail("moves must have shape [P / 2, 2], got " + text(*moves));
+        if (moves && !c.failed()) c.shape(moves, "moves", {moves->shape[0], 2});
+        c.check_overlap();
+        if (c.failed()) return c.status();
+        if (!counts && !moves) return ok();
+        RocmCachePagesArgs a{};
+        a.compact = static_cast<int>(s.compact);
+        a.counts = counts ? reinterpret_cast<int32_t*>(at(*counts)) : nullptr;
+        a.moves = moves ? reinterpret_cast<int32_t*>(at(*moves)) : nullptr;
+        a.pages = moves ? static_cast<int64_t>(2 * moves->shape[0]) : 0;
+        const NxrtStatus st = ep->bind();
+        if (st.code != NXRT_OK) return st;
+        ep->launches.fetch_add(1);
+        return launched(rocm_launch_cache_pages(&a, nullptr, ep->stream));
+    }
     NxrtStatus execute(const NxrtRocmTensorView* in, uint32_t n_in, NxrtRocmTensorView* out, uint32_t n_out, void* ws, uint64_t ws_bytes) override
     {
         Call c(op(), *ep, in, n_in, out, n_out);
         c.arity(5, 4 + ROCM_PAGES_MAX_POOLS, 4 + ROCM_PAGES_MAX_POOLS);
-        if (!c.failed() && no_rows(in, n_in)) return ok();
+        if (!c.failed() && no_rows(in, n_in)) return without_slots(c);
         const auto* table = c.required(c.input(0, "block_table"), "block_table");
         c.dtype(table, "block_table", {NXRT_DT_INT32});
         if (!c.failed() && (table->ndim != 2 || table->shape[1] < 1)) c.fail("block_table must have shape [S, W] with W >= 1, got " + text(*table));

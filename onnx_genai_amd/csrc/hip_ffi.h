@@ -491,6 +491,7 @@ typedef struct RocmCachePagesArgs {
   int slots, width, page, compact, pools;
   RocmPool pool[ROCM_PAGES_MAX_POOLS];
 } RocmCachePagesArgs;
+/* Without slots: counts 0 and moves -1, those of them that are not NULL; no workspace. */
 uint64_t rocm_cache_pages_workspace_bytes(const RocmCachePagesArgs* args);
 int rocm_launch_cache_pages(const RocmCachePagesArgs* args, void* workspace, rocm_stream_t stream);
 

@@ -231,6 +231,12 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(RocmCachePagesArgs a, Pa
     }
 }
 
+__global__ __launch_bounds__(kThreads) void no_slots_kernel(int32_t* counts, int32_t* moves, int room)
+{
+    if (counts && threadIdx.x < 2) counts[threadIdx.x] = 0;
+    for (int i = threadIdx.x; moves && i < 2 * room; i += kThreads) moves[i] = -1;
+}
+
 struct CopyPlan {
     int pieces[ROCM_PAGES_MAX_POOLS];      // workgroups for one move, up to and with each pool
     int layers[ROCM_PAGES_MAX_POOLS];      // layers of a workgroup: several of pools with small pages
@@ -295,11 +301,14 @@ extern "C" uint64_t rocm_cache_pages_workspace_bytes(const RocmCachePagesArgs* a
 extern "C" int rocm_launch_cache_pages(const RocmCachePagesArgs* args, void* workspace, rocm_stream_t stream)
 {
     using namespace mnb;
-    if (args->slots <= 0) return 0;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (args->slots <= 0) {
+        hipLaunchKernelGGL(no_slots_kernel, dim3(1), dim3(kThreads), 0, s, args->counts, args->moves, static_cast<int>(args->pages / 2));
+        return static_cast<int>(hipGetLastError());
+    }
     if (args->slots > ROCM_PAGES_MAX_SLOTS || args->pages < 1 || args->pages > ROCM_PAGES_MAX_PAGES || args->width < 1 || args->page < 1 || static_cast<int64_t>(args->width) * args->page >= (1 << 30) || static_cast<int64_t>(args->slots) * args->width > 0x7fffffff ||
         args->pools < 0 || args->pools > ROCM_PAGES_MAX_POOLS || !workspace)
         return static_cast<int>(hipErrorInvalidValue);
-    hipStream_t s = static_cast<hipStream_t>(stream);
     uint8_t* const at = static_cast<uint8_t*>(workspace);
     const uint64_t each = (static_cast<uint64_t>(args->pages) * 4 + 255) / 256 * 256;
     const PagesWorkspace w{reinterpret_cast<int32_t*>(at), reinterpret_cast<int32_t*>(at + 256), reinterpret_cast<int32_t*>(at + 256 + each), reinterpret_cast<int32_t*>(at + 256 + 2 * each)};

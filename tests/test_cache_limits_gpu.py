@@ -99,3 +99,22 @@ def test_the_table_of_before_stands_where_pages_run_out(ep, slots, width, pages,
     want = pages_step(table, lengths, again, np.zeros(slots), page, pages)
     for name, g, w in zip(("table", "lengths", "moves", "counts"), got, want):
         assert np.array_equal(g, w), name
+
+
+@pytest.mark.parametrize("compact", [0, 1])
+def test_counts_of_no_slots(ep, compact):
+    dev = Device(ep)
+    try:
+        kernel = ep.get_kernel({"page_size": 16, "compact": compact}, op_type="CachePages")
+        none = E.TensorView.absent()
+        pool = dev.view(np.arange(2 * 9 * 5, dtype=np.uint8).reshape(2, 9, 5), E.U8)
+        counts, read = dev.output((2,), E.I32)
+        moves, read_moves = dev.output((4, 2) if compact else (1, 2), E.I32)
+        kernel.execute([E.TensorView(None, E.I32, (0, 4)), none, none, none, pool], [none, none, moves if compact else none, counts, pool])
+        ep.sync()
+        assert read().tolist() == [0, 0]
+        if compact:
+            assert (read_moves() == -1).all()
+        kernel.release()
+    finally:
+        dev.free()
