@@ -338,7 +338,8 @@ struct AttentionNode final : NxrtRocmNode {
         a.heads = static_cast<int>(s.heads);
         a.window = s.window > 0 && s.window < (1 << 30) ? static_cast<int>(s.window) : 0;          // (no sequence has 2^30 slots)
         a.scale = static_cast<float>(s.scale);
-        a.softcap = static_cast<float>(s.softcap);
+        // (a cap below f32's normal numbers makes scores alike, as the smallest of these does; 0 would be none)
+        a.softcap = s.softcap > 0.0 ? std::max(static_cast<float>(s.softcap), std::numeric_limits<float>::min()) : 0.f;
         a.cache.kv_heads = static_cast<int>(s.kv_heads);
         a.cache.head_size = static_cast<int>(s.head_size);
         return a;

@@ -464,7 +464,7 @@ typedef struct RocmCacheAttentionArgs {
   int64_t rows, q_step;
   int heads, dtype;
   int window;               /* tokens that a query sees, itself the last of them; 0: all before it */
-  float scale, softcap;     /* softcap 0: none */
+  float scale, softcap;     /* softcap 0: none, else a normal number */
 } RocmCacheAttentionArgs;
 int rocm_cache_attention_supports(int head_size);
 uint64_t rocm_cache_attention_workspace_bytes(const RocmCacheAttentionArgs* args);

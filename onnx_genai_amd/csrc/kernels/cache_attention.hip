@@ -200,7 +200,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void attentio
         for (int e = 0; e < 16; ++e) x[e] = score[e >> 2][e & 3] * key_scale;
         if (p.a.softcap > 0.f) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = capped(x[e], p.a.softcap);
+            for (int e = 0; e < 16; ++e) x[e] = capped(x[e], p.a.softcap, p.cap_inverse);
         }
         // where some row does not see some token: bit e of `seen` for the lane's row and token e of its
         const bool partial = __ballot(live < 16) != 0, masked = partial || t0 + kGroup - 1 > first_own || (window > 0 && t0 <= last_own - window);
@@ -492,6 +492,7 @@ extern "C" int rocm_launch_cache_attention(const RocmCacheAttentionArgs* args, v
     p.whole = plan.whole;
     p.teams = plan.teams;
     p.slots = 2 * plan.target;
+    p.cap_inverse = args->softcap > 0.f ? 1.0f / args->softcap : 0.f;
     p.scale = args->softcap > 0.f ? args->scale : args->scale * 1.442695041f;
     p.partial = static_cast<float*>(workspace);
     p.partial_sums = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.sums_at);

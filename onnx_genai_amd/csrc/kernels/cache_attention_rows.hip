@@ -270,7 +270,7 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
 #pragma unroll
                 for (int s = 0; s < 4; ++s)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) score[s >> 1][8 * (s & 1) + j] = capped(score[s >> 1][8 * (s & 1) + j] * ks[s % kPages], p.a.softcap);
+                    for (int j = 0; j < 8; ++j) score[s >> 1][8 * (s & 1) + j] = capped(score[s >> 1][8 * (s & 1) + j] * ks[s % kPages], p.a.softcap, p.cap_inverse);
 #pragma unroll
                 for (int s = 0; s < kPages; ++s) ks[s] = 1.f;
             }

@@ -1,0 +1,64 @@
+"""CacheAttention over the whole range of scores, scales and values, with an allowance that goes by what a row sees."""
+import numpy as np
+import pytest
+
+from onnx_genai_amd import ep as E
+
+from . import cache_helpers
+from .cache_helpers import Cache, decode, floats
+from .node_helpers import as64
+from .test_cache_attention_gpu import attend, near
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["short_table", "long_table"])
+def table(request, monkeypatch):
+    monkeypatch.setattr(cache_helpers, "LEAST_SLOTS", [(1 << 20) * (request.param == "long_table")])
+    return request.param
+
+
+def attention_seen(cache, q, heads, *, window=0, softcap=0.0):
+    """attention64, with an allowance that goes by what a row sees: weights are rounded to 11 bits, and to 2^-36 of the row's largest product of a weight and its page's scale."""
+    d, group = cache.head, heads // cache.kv_heads
+    y, slack = np.zeros((cache.rows, heads, d)), np.zeros((cache.rows, heads, d))
+    for i, n in enumerate(cache.new):
+        if not n:
+            continue
+        k, v = cache.tokens(i, cache.past[i] + n)
+        slot = np.arange(cache.past[i] + n)
+        page, place = cache.table[i, slot // cache.page], slot % cache.page
+        codes, scales = decode(cache.v[page, :, :, place], cache.code), cache.vs[page].astype(np.float64)
+        for r in range(n):
+            own, row = cache.past[i] + r, cache.ends[i] + r
+            seen = (slot <= own) & ((slot > own - window) if window else True)
+            for h in range(heads):
+                g = h // group
+                kk, vv, qq = k[seen, g], v[seen, g], q[row, h]
+                z = (kk @ qq) / np.sqrt(d)
+                if softcap:
+                    z = softcap * np.tanh(z / softcap)
+                w = np.exp(z - z.max())
+                w /= w.sum()
+                y[row, h] = w @ vv
+                # as in attention64; softcap: a few f32 roundings of the score, each 2^-24 of it
+                off = (np.abs(kk).sum(-1) * np.abs(qq).max() * 2.0 ** -22 + np.abs(kk) @ np.abs(qq) * (d + 8) * 2.0 ** -24).max() / np.sqrt(d) + 2.0 ** -20 + np.abs(z).max() * 2.0 ** -20 * bool(softcap)
+                slack[row, h] = (w * (2.0 ** -11 + 2 * off)) @ np.abs(vv) + 2.0 ** -36 * (w * scales[seen, g]).max() * np.abs(codes[seen, g]).sum(0)
+    return y, slack
+
+
+def check_seen(ep, cache, heads, dtype, seed, *, sd=1.0, window=0, softcap=0.0):
+    q = floats(np.random.default_rng(seed), (cache.rows, heads * cache.head), dtype, sd)
+    got, variant = attend(ep, cache, q, dtype, heads, local_window_size=window or -1, softcap=softcap)
+    with np.errstate(invalid="ignore", over="ignore"):
+        want, slack = attention_seen(cache, as64(q, dtype).reshape(-1, heads, cache.head), heads, window=window, softcap=softcap)
+    near(got, want, slack, dtype)
+    return variant
+
+
+@pytest.mark.parametrize("softcap", [1e-46, 1e-39, 1e-20, 1e-3, 0.3, 3.0, 30.0, 1e3, 1e4, 1e6, 1e8, 1e20, 3e38])
+@pytest.mark.parametrize("new", [[1, 1], [150, 7]])
+def test_softcaps_of_every_size(ep, table, new, softcap):
+    """From caps that make attention even to caps that are none."""
+    cache = Cache(np.random.default_rng(31), new, [200, 30], E.I8, 1, 64, 64)
+    check_seen(ep, cache, 4, E.F16, 32, sd=3.0, softcap=softcap)
