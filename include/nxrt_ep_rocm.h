@@ -330,8 +330,8 @@ NxrtStatus nxrt_rocm_rotary_embedding_create(NxrtRocmEp* ep, const NxrtRocmRotar
  *   inputs: 0 key [T, KV D] of a float type, 1 value of the same shape and type; or 0 packed rows [T, (num_heads + 2 KV) D], queries, keys, values, and 1 absent;
  *           2 k_cache, 3 v_cache, 4 k_scale, 5 v_scale, 6 cumulative_lengths, 7 past_lengths, 8 block_table.
  *   outputs: 0 k_cache, 1 v_cache, 2 k_scale, 3 v_scale: the inputs' own tensors, changed where they are.
- * A page whose first token is new gets scale = max|x| / top over its new tokens (top: 127, or 448), code = x / scale to the nearest, ties to even; a scale of 0 gives codes
- * 0. A page that has tokens gets scale' = max(scale, max|x| / top), and where that is larger, its codes become code * (scale / scale') to the nearest: each such
+ * A page whose first token is new gets scale = max|x| / top over its new tokens (top: 127, or 448), code = x / scale to the nearest, ties to even, at most top; a scale of 0 gives
+ * codes 0. A page that has tokens gets scale' = max(scale, max|x| / top), and where that is larger, its codes become code * (scale / scale') to the nearest: each such
  * step adds up to half a step of rounding to the tokens before. An infinity or a NaN makes the scale NaN and the new codes 0 (and those before), until the page begins
  * again. Slots that no token has are left as they are. Two sequences may share pages, but a page that a call writes stands in one place of one table row only. */
 typedef struct NxrtRocmCacheAppendAttrs {

@@ -23,8 +23,8 @@ constexpr int kThreads = 256;
 template <bool E4M3>
 constexpr float kLeastExact = E4M3 ? 8.0779357e-28f : 3.9443045e-31f;
 
-// x / scale as codes, to the nearest, ties to even. EXACT: the scale is kLeastExact or more, else the quotient is a division's, or 0 where the scale is not above 0. A quotient is at most a
-// rounding above the largest code, to which it goes.
+// x / scale as codes, to the nearest, ties to even. EXACT: the scale is kLeastExact or more, and a quotient is at most a rounding above the largest code, to which it goes. Else the quotient is a
+// division's, or 0 where the scale is not above 0; and a scale of so few of the smallest f32 steps that it is rounded by much gives quotients far above the largest code, which end there.
 template <bool E4M3, bool EXACT>
 struct Coder {
     float scale, inverse;
@@ -35,7 +35,8 @@ struct Coder {
             const float q = v * inverse;
             return fmaf(fmaf(-q, scale, v), inverse, q);
         } else {
-            return scale > 0.f ? v / scale : 0.f;
+            constexpr float kTop = E4M3 ? 448.0f : 127.0f;
+            return scale > 0.f ? fminf(fmaxf(v / scale, -kTop), kTop) : 0.f;
         }
     }
     __device__ __forceinline__ uint32_t four(float a, float b, float c, float d) const
