@@ -268,10 +268,11 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void attentio
         if (more) load_values(at + kWaves, value_page, s);
     }
 
-    // the waves' results: o[u][i] is element 16 u + 4 g + i of row n
+    // the waves' results, means of what each has seen, which no value is beyond: o[u][i] is element 16 u + 4 g + i of row n
     sum = over_groups_sum(sum);
+    const float own_inverse = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
-    for (int u = 0; u < kTiles; ++u) *reinterpret_cast<float4_t*>(&results[wave][n][u * 16 + g * 4]) = o[u] * reference;
+    for (int u = 0; u < kTiles; ++u) *reinterpret_cast<float4_t*>(&results[wave][n][u * 16 + g * 4]) = o[u] * own_inverse * reference;
     if (g == 0) sums[wave][n] = make_float2(top, sum);
     __syncthreads();
     constexpr int kQuads = D / 4;
@@ -282,24 +283,25 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void attentio
 #pragma unroll
         for (int j = 0; j < kWaves; ++j) most = fmaxf(most, sums[j][row].x);
         const float zero = most == kNone ? 0.f : most;
-        float total = 0.f;
-        float4_t all = {0.f, 0.f, 0.f, 0.f};
+        float total = 0.f, share[kWaves];
 #pragma unroll
         for (int j = 0; j < kWaves; ++j) {
-            const float f = __builtin_amdgcn_exp2f(sums[j][row].x - zero);
-            total += sums[j][row].y * f;
-            all += *reinterpret_cast<const float4_t*>(&results[j][row][e]) * f;
+            share[j] = sums[j][row].y * __builtin_amdgcn_exp2f(sums[j][row].x - zero);
+            total += share[j];
         }
+        // a row that sees nothing is zero
+        const float inverse = total == 0.f ? 0.f : 1.0f / total;
+        float4_t all = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kWaves; ++j) all += *reinterpret_cast<const float4_t*>(&results[j][row][e]) * (share[j] * inverse);
         if (w.slot >= 0) {
             const int64_t place = (static_cast<int64_t>(w.slot) * c.kv_heads + head) * kRows + row;
             *reinterpret_cast<float4_t*>(p.partial + place * D + e) = all;
             if (e == 0) p.partial_sums[place] = make_float2(most, total);
         } else {
-            // a row that sees nothing is zero
-            const float inverse = total == 0.f ? 0.f : 1.0f / total;
             const int r = first_row + row, tk = p.by_group.of(r);
             uint16_t* const to = static_cast<uint16_t*>(p.a.y) + static_cast<int64_t>(w.s.first + tk) * out_step + (head * p.group + r - tk * p.group) * D + e;
-            store_four(to, all[0] * inverse, all[1] * inverse, all[2] * inverse, all[3] * inverse, p.a.dtype);
+            store_four(to, all[0], all[1], all[2], all[3], p.a.dtype);
         }
     }
 }
@@ -341,8 +343,8 @@ __global__ __launch_bounds__(kThreads, 6) void attention_join_kernel(AttentionPa
             float sum = 0.f;
             for (int i = lane; i < w.pieces; i += 64) {
                 const float2 s = p.partial_sums[first + i * piece_step + row];
-                const float share = __builtin_amdgcn_exp2f(s.x - zero);
-                sum += s.y * share;
+                const float share = s.y * __builtin_amdgcn_exp2f(s.x - zero);
+                sum += share;
                 shares[k * w.pieces + i] = share;
             }
             sum = over_wave(sum, [](float x, float y) { return x + y; });

@@ -344,9 +344,13 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
         if (more) store(at + TEAMS, mine[turn ^ 1], are_there(), scale_page >= 0);
     }
 
-    // o[u][4 a + i] is element 32 u + 8 a + 4 h + i of row n
+    // o[u][4 a + i] is element 32 u + 8 a + 4 h + i of row n; from here on a mean of what the row has seen, which no value is beyond. A row that sees nothing is zero.
     sum += __shfl_xor(sum, 32, 64);
-    float scale = reference <= -126.f ? 0.f : __builtin_amdgcn_exp2f(reference);
+    {
+        const float inverse = sum == 0.f ? 0.f : 1.0f / sum, scale = reference <= -126.f ? 0.f : __builtin_amdgcn_exp2f(reference);
+#pragma unroll
+        for (int u = 0; u < kOut; ++u) o[u] = o[u] * inverse * scale;
+    }
     if constexpr (TEAMS > 1) {
         // the second team's results through LDS, where its tiles were: four elements a lane, lanes side by side
         float* const other = reinterpret_cast<float*>(tiles) + wave * (kOut * 16 + 2) * 64 + lane;
@@ -355,21 +359,23 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
 #pragma unroll
             for (int u = 0; u < kOut; ++u)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) other[(u * 16 + i) * 64] = o[u][i] * scale;
+                for (int i = 0; i < 16; ++i) other[(u * 16 + i) * 64] = o[u][i];
             other[kOut * 16 * 64] = top;
             other[(kOut * 16 + 1) * 64] = sum;
         }
         __syncthreads();
         if (team == 1) return;
         const float their_top = other[kOut * 16 * 64], most = fmaxf(top, their_top), zero = most == kNone ? 0.f : most;
-        const float ours = __builtin_amdgcn_exp2f(top - zero), theirs = __builtin_amdgcn_exp2f(their_top - zero), factor = scale * ours;
-        sum = sum * ours + other[(kOut * 16 + 1) * 64] * theirs;
+        float ours = sum * __builtin_amdgcn_exp2f(top - zero), theirs = other[(kOut * 16 + 1) * 64] * __builtin_amdgcn_exp2f(their_top - zero);
+        sum = ours + theirs;
         top = most;
-        scale = 1.f;
+        const float inverse = sum == 0.f ? 0.f : 1.0f / sum;
+        ours *= inverse;
+        theirs *= inverse;
 #pragma unroll
         for (int u = 0; u < kOut; ++u)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[u][i] = o[u][i] * factor + other[(u * 16 + i) * 64] * theirs;
+            for (int i = 0; i < 16; ++i) o[u][i] = o[u][i] * ours + other[(u * 16 + i) * 64] * theirs;
     }
     if (n >= rows) return;
     if (w.slot >= 0) {
@@ -379,19 +385,17 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
                 const int e = u * 32 + a * 8 + h * 4;
-                if (D % 32 == 0 || e < D) *reinterpret_cast<float4_t*>(p.partial + place * D + e) = float4_t{o[u][4 * a], o[u][4 * a + 1], o[u][4 * a + 2], o[u][4 * a + 3]} * scale;
+                if (D % 32 == 0 || e < D) *reinterpret_cast<float4_t*>(p.partial + place * D + e) = float4_t{o[u][4 * a], o[u][4 * a + 1], o[u][4 * a + 2], o[u][4 * a + 3]};
             }
         if (h == 0) p.partial_sums[place] = make_float2(top, sum);
     } else {
-        // a row that sees nothing is zero
-        const float inverse = sum == 0.f ? 0.f : scale / sum;
         uint16_t* const to = static_cast<uint16_t*>(p.a.y) + (static_cast<int64_t>(w.s.first + token) * p.a.heads + head * p.group + member) * D;
 #pragma unroll
         for (int u = 0; u < kOut; ++u)
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
                 const int e = u * 32 + a * 8 + h * 4;
-                if (D % 32 == 0 || e < D) store_four(to + e, o[u][4 * a] * inverse, o[u][4 * a + 1] * inverse, o[u][4 * a + 2] * inverse, o[u][4 * a + 3] * inverse, p.a.dtype);
+                if (D % 32 == 0 || e < D) store_four(to + e, o[u][4 * a], o[u][4 * a + 1], o[u][4 * a + 2], o[u][4 * a + 3], p.a.dtype);
             }
     }
 }

@@ -62,3 +62,22 @@ def test_softcaps_of_every_size(ep, table, new, softcap):
     """From caps that make attention even to caps that are none."""
     cache = Cache(np.random.default_rng(31), new, [200, 30], E.I8, 1, 64, 64)
     check_seen(ep, cache, 4, E.F16, 32, sd=3.0, softcap=softcap)
+
+
+KINDS = [([1, 1], [200, 30]), ([150, 7], [200, 30]), ([300], [10]), ([1], [5000]), ([70], [3000])]          # few rows, more, two teams of waves, pieces of either
+
+
+def check_values_of_size(ep, new, past, size):
+    cache = Cache(np.random.default_rng(38), new, past, E.I8, 1, 64, 64)
+    cache.vs[:] = np.where(np.isnan(cache.vs), cache.vs, np.float32(size))
+    q = floats(np.random.default_rng(39), (cache.rows, 2 * 64), E.BF16)
+    got, _ = attend(ep, cache, q, E.BF16, 2)
+    want, slack = attention_seen(cache, as64(q, E.BF16).reshape(-1, 2, 64), 2)
+    near(got, want, slack + 2.0 ** -133 * (1 + 2.0 ** -3), E.BF16)           # half a step of bf16's smallest numbers is 2^-134, of f32's on the way 2^-150 each
+
+
+@pytest.mark.parametrize("size", [1e-36, 1e33, 2.4e36])
+@pytest.mark.parametrize("new,past", KINDS)
+def test_values_as_large_as_they_can_be(ep, table, new, past, size):
+    """Values up to the largest that bf16 has are no infinities on the way, nor are small ones nothing."""
+    check_values_of_size(ep, new, past, size)
