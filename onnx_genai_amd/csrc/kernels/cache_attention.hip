@@ -7,8 +7,8 @@
 // the maximum of a row. The 16 tokens lie in one page, which holds 16 at least, and their page's scale is one number a lane.
 //
 // Codes are exact in f16, as 8-bit integers and as e4m3. Queries go to f16 with their row's largest at 2^8 (what falls below f16's range is less than 2^-22 of it).
-// Weights p = exp(s - max) are held as p * 2^11 * (scale of the values' page / largest such scale so far) in f16: rounded to 11 bits, down to 2^-25 of the largest
-// weight, below that to 2^-36 of it; sums and all products are in f32.
+// Weights p = exp(s - max) become operands as p times the scale of the values' page, relative to the largest such product that the row has seen, in f16: rounded to 11 bits, below 2^-25 of the
+// largest to 2^-36 of it. Sums of p itself and all products are in f32.
 //
 // One token each of 64 sequences of up to 8192, 32 query heads by 8 of 128 (538 MB): 119 to 124 us, 4.3 to 4.5 TB/s. One token after 131071 (268 MB): 55 us with its join, 4.9 TB/s; a GPU-wide copy reaches
 // 5.2 TB/s. With little to read the trips to memory count: lengths, table, keys and scales; one token after 1000 takes 10.5 us. A tile of 32 rows, which would read a code once for twice the
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void attentio
     float4_t o[kTiles];
 #pragma unroll
     for (int u = 0; u < kTiles; ++u) o[u] = float4_t{0.f, 0.f, 0.f, 0.f};
-    float top = kNone, sum = 0.f, reference = 0.f;
+    float top = kNone, sum = 0.f, reference = kNone;         // reference: log2 of the product that operands are relative to
 
     // The page of 16 tokens of a step: sub-block n / 4 for the lane's keys, g for its values and scales. A step's entries of the table are asked for a step before its keys.
     const int page_bits = __builtin_ctz(c.page);
@@ -215,12 +215,14 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void attentio
         float most = x[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) most = fmaxf(most, x[e]);
+        // (the scale's power of two, which is below it by less than a bit, will do; a scale of 0 or NaN, and what the row does not see, have no part in it)
+        const float product = value_scale > 0.f ? most + static_cast<float>(__builtin_amdgcn_frexp_expf(value_scale) - 1) : kNone;
         most = fmaxf(top, over_groups_max(most));
-        const float next = fmaxf(reference, over_groups_max(live ? value_scale : 0.f));
-        // What weights are relative to stays until something is kSlack bits above it: sums and values are seldom scaled again.
-        if (__ballot(most > top + kSlack || next > reference)) {
+        const float next = fmaxf(reference, over_groups_max(product));
+        // What weights and operands are relative to stays until something is kSlack bits above it: sums and values are seldom scaled again.
+        if (__ballot(most > top + kSlack || next > reference + (kSlack - 1.f))) {
             const float shrink = __builtin_amdgcn_exp2f(top - (most == kNone ? 0.f : most));
-            const float again = shrink * (next > reference ? reference / next : 1.f);
+            const float again = __builtin_amdgcn_exp2f(reference - (next == kNone ? 0.f : next));
             sum *= shrink;
             top = most;
             reference = next;
@@ -228,8 +230,9 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void attentio
             for (int u = 0; u < kTiles; ++u) o[u] *= again;
         }
         const float zero = top == kNone ? 0.f : top;                            // (a row that has seen nothing yet)
-        // weights relative to the largest page scale so far, where there is one; a NaN stays one
-        const float relative = reference > 0.f ? value_scale / reference : value_scale * 0.f;
+        // what makes a weight an operand; a NaN stays one. In two steps, as 2^(zero - reference) alone may be beyond f32, and the whole of it for a page whose weights are next to nothing
+        const float step = __builtin_amdgcn_exp2f(reference == kNone ? 0.f : fminf(0.5f * (zero - reference), 120.f)), product_of_one = value_scale * step * step;
+        const float relative = product_of_one > 3e38f ? 3e38f : product_of_one;
         half8_t weights[2];
         auto weigh = [&](auto some) {
             float part = 0.f;
@@ -270,9 +273,9 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void attentio
 
     // the waves' results, means of what each has seen, which no value is beyond: o[u][i] is element 16 u + 4 g + i of row n
     sum = over_groups_sum(sum);
-    const float own_inverse = sum == 0.f ? 0.f : 1.0f / sum;
+    const float own_inverse = sum == 0.f ? 0.f : 1.0f / sum, back = reference == kNone ? 0.f : __builtin_amdgcn_exp2f(0.5f * (reference - top));
 #pragma unroll
-    for (int u = 0; u < kTiles; ++u) *reinterpret_cast<float4_t*>(&results[wave][n][u * 16 + g * 4]) = o[u] * own_inverse * reference;
+    for (int u = 0; u < kTiles; ++u) *reinterpret_cast<float4_t*>(&results[wave][n][u * 16 + g * 4]) = o[u] * own_inverse * back * back;
     if (g == 0) sums[wave][n] = make_float2(top, sum);
     __syncthreads();
     constexpr int kQuads = D / 4;

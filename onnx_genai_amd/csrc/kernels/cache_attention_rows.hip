@@ -7,7 +7,7 @@
 // While a step is computed, the next one's codes are on their way into registers; they go to the other half of LDS behind it.
 //
 // A page's scales are numbers of 16 tokens each here, and stay out of the products over single scores: key scales enter a score's one multiply-add, value scales its exponent,
-// weight = 2^(score + log2(scale) - top), and their inverse the sum of 8 weights. (A page of values with a scale below 2^-126 counts as one of 2^-126.)
+// operand = 2^(score + log2(scale) - reference), and their inverse the sum of 8 operands. The reference is the largest score + log2(scale) that a row has seen, so operands are rounded as over few rows.
 //
 // 8192 tokens, 32 query heads by 8 of 128, each token after those before it: 580 to 600 us, 920 to 950 TFLOP/s; the library's product of f16 matrices reaches 1150. What is left are the vector
 // instructions of the softmax, about as many cycles as the products and hardly overlapped with them, since a wave's products wait for its own weights: their issue alone is four fifths of the time.
@@ -18,7 +18,8 @@ namespace mnb {
 namespace {
 
 constexpr int kWaveRows = 32;
-constexpr float kLeastShare = 60.f;          // bits that a page's scale may lie below the largest one: what is further below counts as this
+constexpr float kLeastShare = 60.f;          // bits by which a page's largest operands may lie below the reference: what is further below, and so 0 in f16, counts as this, for the sum's sake
+constexpr float kLeastBits = -1000.f;        // log2 of a scale of 0
 
 typedef __attribute__((ext_vector_type(16))) float float16_t;
 typedef __attribute__((ext_vector_type(4))) float float4_t;
@@ -43,7 +44,7 @@ struct Tile {
     static constexpr int kKeyPitch = D * 2 + 16, kValuePitch = kGroup * 2 + 16, kValueRows = (D + 31) / 32 * 32;
     alignas(16) uint8_t k[kGroup * kKeyPitch];
     alignas(16) uint8_t v[kValueRows * kValuePitch];
-    float key_scale[4], value_bits[4], value_inverse[4];       // of 16 tokens each; log2 and 1 / scale of the values
+    float key_scale[4], value_bits[4];       // of 16 tokens each; log2 of the values' scale
     int there[4];
 };
 
@@ -168,10 +169,10 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
         }
         if (thread < kPages) {
             tile.key_scale[thread] = key_scale;
-            // a page of scale 0 (its codes are 0) weighs as the smallest scale does
-            const float scale = value_scale < 1.17549435e-38f ? 1.17549435e-38f : value_scale;
-            tile.value_bits[thread] = of_scale ? __builtin_amdgcn_logf(scale) : -126.f;
-            tile.value_inverse[thread] = 1.0f / scale;
+            // (the logarithm knows normal numbers only; one of NaN stays one)
+            const bool low = value_scale < 5.42101086e-20f;
+            const float bits = __builtin_amdgcn_logf(low ? value_scale * 18446744073709551616.f : value_scale) - (low ? 64.f : 0.f);
+            tile.value_bits[thread] = !of_scale || bits < kLeastBits ? kLeastBits : bits;
             tile.there[thread] = of_scale;
         }
     };
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
     for (int u = 0; u < kOut; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[u][i] = 0.f;
-    float top = kNone, sum = 0.f, reference = -126.f, largest = 0.f;           // reference: log2 of the largest value scale so far
+    float top = kNone, sum = 0.f, reference = kNone;
 
     if (begin < w.span.hi) {
         ask(begin + TEAMS);
@@ -257,13 +258,12 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
                 for (int b = 0; b < 2; ++b)
                     score[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t*>(key + b * 32 * Tile<D>::kKeyPitch + i * 32), q[i], score[b], 0, 0, 0);
             reads_ahead<2 * kSteps>();
-            float ks[kPages], bits[kPages], inverse[kPages];
+            float ks[kPages], bits[kPages];
             int there = 15;
 #pragma unroll
             for (int s = 0; s < kPages; ++s) {
                 ks[s] = tile.key_scale[s] * row_scale;
                 bits[s] = tile.value_bits[s];
-                inverse[s] = tile.value_inverse[s];
                 there &= tile.there[s] ? 15 : WIDE ? 0 : 15 ^ (1 << s);
             }
             if (p.a.softcap > 0.f) {
@@ -294,31 +294,31 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
 #pragma unroll
                 for (int e = 8 * s + 1; e < 8 * s + 32 / kPages; ++e) m = fmaxf(m, score[e >> 4][e & 15]);
                 most = fmaxf(most, m * ks[s % kPages]);
-                next = fmaxf(next, bits[s % kPages]);
+                next = fmaxf(next, fmaf(m, ks[s % kPages], bits[s % kPages]));
             }
             {
-                const uint32_t a = __float_as_uint(most);
-                const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+                const uint32_t a = __float_as_uint(most), b = __float_as_uint(next);
+                const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false), q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
                 most = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+                next = fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
             }
-            // What weights are relative to stays until something is kSlack bits above it: sums and values are seldom scaled again.
-            if (__ballot(most > top + kSlack || next > reference)) {
+            // What sums and operands are relative to stays until something is kSlack bits above it: sums and values are seldom scaled again.
+            if (__ballot(most > top + kSlack || next > reference + kSlack)) {
                 const float shrink = __builtin_amdgcn_exp2f(top - (most == kNone ? 0.f : most));
-                const float again = shrink * __builtin_amdgcn_exp2f(reference - next);
+                const float again = __builtin_amdgcn_exp2f(reference - (next == kNone ? 0.f : next));
                 sum *= shrink;
                 top = most;
                 reference = next;
-                largest = __builtin_amdgcn_exp2f(reference);
 #pragma unroll
                 for (int u = 0; u < kOut; ++u) o[u] *= again;
             }
-            const float zero = top == kNone ? 0.f : top;                        // (a row that has seen nothing yet)
+            const float zero = top == kNone ? 0.f : top, behind = reference == kNone ? 0.f : zero - reference;          // (a row that has seen nothing yet)
             half8_t weights[4];
             auto weigh = [&](auto some) {
 #pragma unroll
                 for (int s = 0; s < 4; s += 4 / kPages) {
                     // (a NaN scale stays one)
-                    const float share = bits[s % kPages] < reference - kLeastShare ? -kLeastShare : bits[s % kPages] - reference;
+                    const float all = bits[s % kPages] + behind, share = all < -kLeastShare ? -kLeastShare : all;
                     const float off = zero - kWeightBits - share;
                     float part = 0.f;
 #pragma unroll
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
                         part += y;
                         weights[e >> 3][e & 7] = static_cast<_Float16>(y);
                     }
-                    sum = fmaf(part, fminf(largest * inverse[s % kPages], 1152921504606846976.f), sum);
+                    sum = fmaf(part, fminf(__builtin_amdgcn_exp2f(-share), 1152921504606846976.f), sum);          // (no row's sum is NaN for a page that it does not see)
                 }
             };
             if (masked) weigh(std::true_type{});
@@ -347,9 +347,9 @@ __global__ __launch_bounds__(64 * WAVES * TEAMS, D <= 128 ? 8 / (WAVES * TEAMS) 
     // o[u][4 a + i] is element 32 u + 8 a + 4 h + i of row n; from here on a mean of what the row has seen, which no value is beyond. A row that sees nothing is zero.
     sum += __shfl_xor(sum, 32, 64);
     {
-        const float inverse = sum == 0.f ? 0.f : 1.0f / sum, scale = reference <= -126.f ? 0.f : __builtin_amdgcn_exp2f(reference);
+        const float inverse = sum == 0.f ? 0.f : 1.0f / sum, back = reference == kNone ? 0.f : __builtin_amdgcn_exp2f(0.5f * (reference - top));          // (by halves: either may be beyond f32)
 #pragma unroll
-        for (int u = 0; u < kOut; ++u) o[u] = o[u] * inverse * scale;
+        for (int u = 0; u < kOut; ++u) o[u] = o[u] * inverse * back * back;
     }
     if constexpr (TEAMS > 1) {
         // the second team's results through LDS, where its tiles were: four elements a lane, lanes side by side

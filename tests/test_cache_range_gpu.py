@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 from onnx_genai_amd import ep as E
+from onnx_genai_amd import synth
 
 from . import cache_helpers
 from .cache_helpers import Cache, decode, floats
@@ -80,4 +81,44 @@ def check_values_of_size(ep, new, past, size):
 @pytest.mark.parametrize("new,past", KINDS)
 def test_values_as_large_as_they_can_be(ep, table, new, past, size):
     """Values up to the largest that bf16 has are no infinities on the way, nor are small ones nothing."""
+    check_values_of_size(ep, new, past, size)
+
+
+@pytest.mark.parametrize("code", [E.I8, E.F8E4M3])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("new,bits", [([1, 1], 30), ([150, 70], 30), ([150, 70], 60), ([150, 70], 100)])
+def test_scales_of_pages_that_a_row_does_not_see(ep, table, new, bits, page, code):
+    """Every third page of values has a scale far above the others': rows in front of the first, or with a window behind the last, are as without it."""
+    cache = Cache(np.random.default_rng(33), new, [40, 100], code, 1, 64, page)
+    for i in range(2):
+        live = -(-(cache.past[i] + new[i]) // page)
+        cache.vs[cache.table[i, 2:live:3]] *= np.float32(2.0 ** bits)
+    check_seen(ep, cache, 4, E.BF16, 34)
+    check_seen(ep, cache, 4, E.BF16, 35, window=20)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [150, 7]])
+@pytest.mark.parametrize("bits", [12, 20, 30, 60, 90])
+def test_small_pages_that_take_all(ep, table, new, bits):
+    """The page that takes nearly all of the weight has by far the smallest scale: its values come out with their digits."""
+    cache = Cache(np.random.default_rng(36), new, [200, 96], E.I8, 1, 64, 16)
+    # keys: the first page's stand out in element 0
+    cache.k[:, :, :, 0] = 0
+    for i in range(2):
+        cache.k[cache.table[i, 0], :, :, 0] = 100
+        cache.ks[cache.table[i, 0]] = 0.02
+        cache.vs[cache.table[i, 0]] *= np.float32(2.0 ** -bits)
+    q = np.zeros((cache.rows, 2, 64), np.float32)
+    q[:, :, 0] = 4 * bits                                        # scores of the first page: bits nats
+    q[:, :, 1:] = np.random.default_rng(37).standard_normal((cache.rows, 2, 63)) * 0.1
+    q = synth.to_dtype(q.reshape(cache.rows, -1), E.BF16)
+    got, _ = attend(ep, cache, q, E.BF16, 2)
+    want, slack = attention_seen(cache, as64(q, E.BF16).reshape(-1, 2, 64), 2)
+    near(got, want, slack, E.BF16)
+
+
+@pytest.mark.parametrize("size", [1e-43, 1e-39])
+@pytest.mark.parametrize("new,past", KINDS)
+def test_scales_below_the_normal_numbers(ep, table, new, past, size):
+    """Pages of values whose scale is one of f32's subnormal numbers."""
     check_values_of_size(ep, new, past, size)
