@@ -349,7 +349,8 @@ NxrtStatus nxrt_rocm_cache_append_create(NxrtRocmEp* ep, const NxrtRocmCacheAppe
  * Head h reads key head h / (num_heads / KV). New token i of sequence b sees slots t <= past_lengths[b] + i, with local_window_size the last so many of them (itself is one):
  *   y = softmax(z) v,  z = scale (q . k), with softcap  softcap tanh(z / softcap);  scale 0 (the default): 1 / sqrt(D).
  * A row that sees no slot is zero. Products, softmax and sums in f32 over f16 operands: codes exact, queries to 2^-22 of their row's largest, weights times
- * their page's scale rounded to 11 bits, or to 2^-36 of the largest such product that the row sees. A page of scale NaN gives NaN to the rows that see it, and to no other; a NaN code of Float8E4M3FN (CacheAppend makes none) may reach rows that do not see its slot. */
+ * their page's scale rounded to 11 bits, or to 2^-36 of the largest such product that the row sees. A page of scale NaN gives NaN to the rows that see it, and to no other;
+ * a NaN code of Float8E4M3FN (CacheAppend makes none) may reach rows that do not see its slot. */
 typedef struct NxrtRocmCacheAttentionAttrs {
   uint32_t struct_size;
   uint32_t present;      /* bit i: 0 num_heads, 1 kv_num_heads, 2 head_size (all required), 3 local_window_size (-1: none), 4 scale (0), 5 softcap (0: none) */

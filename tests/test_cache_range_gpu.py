@@ -122,3 +122,13 @@ def test_small_pages_that_take_all(ep, table, new, bits):
 def test_scales_below_the_normal_numbers(ep, table, new, past, size):
     """Pages of values whose scale is one of f32's subnormal numbers."""
     check_values_of_size(ep, new, past, size)
+
+
+@pytest.mark.parametrize("sequences", [65, 100, 130])
+def test_pieces_among_many_sequences(ep, sequences):
+    """More sequences than a wave looks at at once, some of them long enough to be cut."""
+    rng = np.random.default_rng(sequences)
+    past = rng.integers(0, 60, sequences)
+    past[[3, 64, sequences - 1]] = [4000, 2600, 5100]
+    cache = Cache(rng, rng.integers(0, 3, sequences).clip(0, 2) | (past > 1000), past, E.I8, 1, 64, 32)
+    assert check_seen(ep, cache, 2, E.F16, 40) == "cache_attention_pieces"
