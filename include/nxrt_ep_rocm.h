@@ -314,7 +314,7 @@ NxrtStatus nxrt_rocm_gated_residual_norm_create(NxrtRocmEp* ep, const NxrtRocmGa
  *   a' = a c - b s, b' = b c + a s; c, s = row position of the caches (a position that they do not have gives NaN), or magnitude * cos, sin(position * f_i) in 64 bits:
  *   f_i = rope_theta^(-2 i / R); scaling 1 (linear): f_i / factor; 2 (llama3): f_i / factor below low_freq_factor turns within original_max_position, f_i above
  *   high_freq_factor, in between a blend by turns; 3 (yarn): f_i / factor below beta_slow turns, f_i above beta_fast, in between a blend by pairs; magnitude =
- *   attention_factor, by default 1, with yarn 0.1 ln(factor) + 1. Positions are exact up to 2^53. In f32, rounded once. */
+ *   attention_factor, by default 1, with yarn and a factor above 1  0.1 ln(factor) + 1. Positions are exact up to 2^53. In f32, rounded once. */
 typedef struct NxrtRocmRotaryEmbeddingAttrs {
   uint32_t struct_size;
   uint32_t present;      /* bit i: 0 head_size (required), 1 num_heads (0), 2 rotary_embedding_dim (0), 3 interleaved (0), 4 scaling (0), 5 original_max_position (8192),

@@ -36,7 +36,7 @@ RotarySettings settings_of(const NxrtRocmRotaryEmbeddingAttrs* attrs)
     const double factor = NODE_ATTR_PRESENT(a, 7, factor) ? a.factor : 1.0;
     const double low = NODE_ATTR_PRESENT(a, 8, low_freq_factor) ? a.low_freq_factor : 1.0, high = NODE_ATTR_PRESENT(a, 9, high_freq_factor) ? a.high_freq_factor : 4.0;
     const double fast = NODE_ATTR_PRESENT(a, 10, beta_fast) ? a.beta_fast : 32.0, slow = NODE_ATTR_PRESENT(a, 11, beta_slow) ? a.beta_slow : 1.0;
-    s.magnitude = NODE_ATTR_PRESENT(a, 12, attention_factor) ? a.attention_factor : s.scaling == 3 ? 0.1 * std::log(factor) + 1.0 : 1.0;
+    s.magnitude = NODE_ATTR_PRESENT(a, 12, attention_factor) ? a.attention_factor : s.scaling == 3 && factor > 1.0 ? 0.1 * std::log(factor) + 1.0 : 1.0;
     if (s.head_size < 2 || s.head_size > (1 << 16)) s.problem = "head_size must be 2..=65536, got " + std::to_string(s.head_size);
     else if (s.heads < 0 || s.heads > (1 << 20)) s.problem = "num_heads must be 0..=2^20, got " + std::to_string(s.heads);
     else if (s.part < 2 || s.part > s.head_size || s.part % 2 != 0 || s.part > 2 * ROCM_ROTARY_MAX_PAIRS)
