@@ -20,8 +20,10 @@ def check(ep, f, magnitude, attrs):
     got, _ = run(ep, x, E.F32, positions, {"head_size": 64, "scaling": 3, **attrs})
     x64 = as64(x, E.F32).reshape(9, 2, 64)
     want = turned(x64, cos, sin, 64, 0).reshape(9, -1)
-    size = turned(np.abs(x64), np.abs(cos) + np.abs(sin), -np.abs(cos) - np.abs(sin), 64, 0).reshape(9, -1) + np.abs(x64).reshape(9, -1)
-    near(got, want, np.abs(size), E.F32)
+    # an element is a c - b s or b c + a s: of its terms, cosines and sines are off by 2^-24 of theirs, products and their sum by as much again
+    pair = np.abs(x64) + np.abs(np.roll(x64, 32, -1))
+    size = (pair * np.tile(np.abs(cos) + np.abs(sin), 2)[:, None]).reshape(9, -1)
+    near(got, want, size, E.F32)
 
 
 @pytest.mark.parametrize("factor", [1e-5, 0.5, 1.0, 1.5, 40.0])
