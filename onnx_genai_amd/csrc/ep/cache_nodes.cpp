@@ -51,7 +51,7 @@ RotarySettings settings_of(const NxrtRocmRotaryEmbeddingAttrs* attrs)
     else if (!std::isfinite(s.magnitude)) s.problem = "attention_factor must be finite";
     if (!s.problem.empty()) return s;
     const double turn = 6.283185307179586476925, context = static_cast<double>(original);
-    // yarn: the pair that makes so many turns within the first context
+    // yarn: the pair that makes so many turns within the first context (below 0: none does)
     auto pair = [&](double turns) { return static_cast<double>(s.part) * std::log(context / (turns * turn)) / (2.0 * std::log(theta)); };
     const double first = std::max(std::floor(pair(fast)), 0.0), last = std::min(std::ceil(pair(slow)), static_cast<double>(s.part - 1));
     for (int64_t i = 0; i < s.part / 2; ++i) {
@@ -59,7 +59,7 @@ RotarySettings settings_of(const NxrtRocmRotaryEmbeddingAttrs* attrs)
         double kept = 1.0;                // of the frequency as it is, against the slower one
         if (s.scaling == 1) kept = 0.0;
         if (s.scaling == 2) kept = std::min(1.0, std::max(0.0, (context * f / turn - low) / (high - low)));
-        if (s.scaling == 3) kept = 1.0 - std::min(1.0, std::max(0.0, (static_cast<double>(i) - first) / std::max(last - first, 0.001)));
+        if (s.scaling == 3) kept = last < 0.0 ? 0.0 : 1.0 - std::min(1.0, std::max(0.0, (static_cast<double>(i) - first) / std::max(last - first, 0.001)));
         f = f / factor * (1.0 - kept) + f * kept;
         s.turns.push_back(f / turn);
     }

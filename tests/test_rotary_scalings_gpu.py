@@ -31,3 +31,9 @@ def test_magnitude_of_yarn(ep, factor):
     """0.1 ln(factor) + 1 for contexts that are stretched; nothing is amplified or turned round where they are not."""
     f, _ = frequencies(64, scaling=3, factor=factor, original=4096)
     check(ep, f, 0.1 * np.log(factor) + 1 if factor > 1 else 1.0, {"factor": factor, "original_max_position": 4096})
+
+
+@pytest.mark.parametrize("original", [1, 3, 4])
+def test_yarn_where_no_pair_turns_once(ep, original):
+    """Within so short a context every pair makes fewer than beta_slow turns: all of them are slowed, the first one too."""
+    check(ep, 10000.0 ** (-np.arange(0, 64, 2) / 64) / 8, 0.1 * np.log(8) + 1, {"factor": 8.0, "original_max_position": original})
