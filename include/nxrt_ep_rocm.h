@@ -298,7 +298,7 @@ NxrtStatus nxrt_rocm_gated_residual_norm_create(NxrtRocmEp* ep, const NxrtRocmGa
  * holds B tokens (16, 32, 64 or 128) of each of KV heads of D elements; the value of a code is code * scale of its page and head. Of the values a page holds
  * the tokens of one element side by side.
  * A call's new tokens are rows, T in all, those of a sequence behind one another: cumulative_lengths [N + 1] Int32, the first 0, sequence b has rows
- * cumulative_lengths[b] up to cumulative_lengths[b + 1]; rows behind the last sequence belong to none. past_lengths [N] Int32: tokens of a sequence in front of them.
+ * cumulative_lengths[b] up to cumulative_lengths[b + 1]; rows behind the last sequence belong to none (without sequences, N = 0, all of them, and a call does nothing). past_lengths [N] Int32: tokens of a sequence in front of them.
  * block_table [N, W] Int32: token t of sequence b is slot t % B of page block_table[b, t / B].
  * What these tensors hold is read on the GPU and not reported: lengths are taken into 0 .. T, past lengths into 0 .. W B, and a page outside 0 .. P - 1 holds no tokens.
  * D: 64, 80, 96, 128 or 256 for CacheAttention, a multiple of 16 up to 256 for CacheAppend. W B < 2^30, N KV < 2^20; T < 2^26 for CacheAppend, T num_heads < 2^29 for

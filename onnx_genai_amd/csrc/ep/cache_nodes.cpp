@@ -159,6 +159,9 @@ struct RotaryNode final : NxrtRocmNode {
 
 // ---- what the cache's nodes read alike -----------------------------------------------------------------------------------
 
+// A call whose block table (input i) has no sequences has nothing to do, as one without rows, and none of its tensors needs memory behind it.
+bool no_sequences(const NxrtRocmTensorView* in, uint32_t n_in, uint32_t i) { return i < n_in && in[i].ndim == 2 && in[i].shape && in[i].shape[0] == 0; }
+
 // Inputs `first` (k_cache, v_cache, k_scale, v_scale, cumulative_lengths, past_lengths, block_table) of a call over `rows` new tokens.
 struct CacheInputs {
     const NxrtRocmTensorView *k, *v, *k_scale, *v_scale, *ends, *past, *table;
@@ -253,7 +256,7 @@ struct AppendNode final : NxrtRocmNode {
     {
         Call c(op(), *ep, in, n_in, out, n_out);
         c.arity(9, 9, 4);
-        if (!c.failed() && no_rows(in, n_in)) return ok();
+        if (!c.failed() && (no_rows(in, n_in) || no_sequences(in, n_in, 8))) return ok();
         const auto* key = c.required(c.input(0, "key"), "key");
         c.dtype(key, "key", {NXRT_DT_FLOAT32, NXRT_DT_FLOAT16, NXRT_DT_BFLOAT16});
         const auto* value = c.input(1, "value");
@@ -366,7 +369,7 @@ struct AttentionNode final : NxrtRocmNode {
     {
         Call c(op(), *ep, in, n_in, out, n_out);
         c.arity(8, 8, 1);
-        if (!c.failed() && no_rows(in, n_in)) return ok();
+        if (!c.failed() && (no_rows(in, n_in) || no_sequences(in, n_in, 7))) return ok();
         const auto* q = c.required(c.input(0, "query"), "query");
         c.dtype(q, "query", {NXRT_DT_FLOAT16, NXRT_DT_BFLOAT16});
         if (c.failed()) return c.status();

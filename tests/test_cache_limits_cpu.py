@@ -4,7 +4,7 @@ import pytest
 from onnx_genai_amd import ep as E
 
 from .test_allocation_failure_cpu import host_only  # noqa: F401  (the fixture: the library's host sources without a GPU)
-from .test_cache_nodes_cpu import NONE, Places, provider, refused  # noqa: F401  (provider: a fixture)
+from .test_cache_nodes_cpu import NONE, Places, cache_views, provider, refused  # noqa: F401  (provider: a fixture)
 
 
 @pytest.mark.parametrize("compact", [0, 1])
@@ -25,3 +25,18 @@ def test_pages_without_slots(provider, compact):  # noqa: F811
         refused(k, [table] + [NONE] * 4, [NONE, NONE, at(E.I32, (8,)), counts], "moves must have shape [P / 2, 2]")
         refused(k, [table] + [NONE] * 4, [NONE, NONE, E.TensorView(counts.data, E.I32, (4, 2)), counts], "counts overlaps moves")
     k.release()
+
+
+def test_rows_without_sequences(provider):  # noqa: F811
+    """A padded batch in which no sequence is left: nothing to do, and the empty table and lengths have no memory."""
+    at = Places()
+    views = cache_views(at)[:4] + [at(E.I32, (1,)), E.TensorView(None, E.I32, (0,)), E.TensorView(None, E.I32, (0, 5))]
+    before = provider.kernel_launch_count()
+    k = provider.get_kernel({"kv_num_heads": 2, "head_size": 64}, op_type="CacheAppend")
+    k.execute([at(E.F16, (6, 128)), at(E.F16, (6, 128))] + views, views[:4])
+    refused(k, [at(E.F16, (6, 128)), at(E.F16, (6, 128))] + views[:6] + [E.TensorView(None, E.I32, (5,))], views[:4], "past_lengths is required")
+    k.release()
+    k = provider.get_kernel({"num_heads": 4, "kv_num_heads": 2, "head_size": 64}, op_type="CacheAttention")
+    k.execute([at(E.F16, (6, 256))] + views, [at(E.F16, (6, 256))])
+    k.release()
+    assert provider.kernel_launch_count() == before
