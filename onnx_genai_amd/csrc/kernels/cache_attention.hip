@@ -11,7 +11,7 @@
 // largest to 2^-36 of it. Sums of p itself and all products are in f32.
 //
 // One token each of 64 sequences of up to 8192, 32 query heads by 8 of 128 (538 MB): 119 to 124 us, 4.3 to 4.5 TB/s. One token after 131071 (268 MB): 55 us with its join, 4.9 TB/s; a GPU-wide copy reaches
-// 5.2 TB/s. With little to read the trips to memory count: lengths, table, keys and scales; one token after 1000 takes 10.5 us. A tile of 32 rows, which would read a code once for twice the
+// 5.2 TB/s. With little to read the trips to memory count: lengths, table, keys and scales; one token after 1000 takes 9 to 10 us. A tile of 32 rows, which would read a code once for twice the
 // rows, was built for heads of up to 128 and left out: it needs more than the 256 registers that two waves a SIMD leave it (32 rows after up to 4000 tokens: 145 us against 99).
 #include "cache_attention.hiph"
 

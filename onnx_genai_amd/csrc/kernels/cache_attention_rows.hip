@@ -9,9 +9,10 @@
 // A page's scales are numbers of 16 tokens each here, and stay out of the products over single scores: key scales enter a score's one multiply-add, value scales its exponent,
 // operand = 2^(score + log2(scale) - reference), and their inverse the sum of 8 operands. The reference is the largest score + log2(scale) that a row has seen, so operands are rounded as over few rows.
 //
-// 8192 tokens, 32 query heads by 8 of 128, each token after those before it: 580 to 600 us, 920 to 950 TFLOP/s; the library's product of f16 matrices reaches 1150. What is left are the vector
+// 8192 tokens, 32 query heads by 8 of 128, each token after those before it: 595 to 605 us, 910 to 925 TFLOP/s; the library's product of f16 matrices reaches 1150. What is left are the vector
 // instructions of the softmax, about as many cycles as the products and hardly overlapped with them, since a wave's products wait for its own weights: their issue alone is four fifths of the time.
-// On the way: 16 rows a workgroup 1891 us, 128 rows 926, a path of its own for steps without masks 700, table entries a step ahead 688, reads out of LDS six products ahead 650, 256 rows 587.
+// On the way: 16 rows a workgroup 1891 us, 128 rows 926, a path of its own for steps without masks 700, table entries a step ahead 688, reads out of LDS six products ahead 650, 256 rows 587;
+// operands relative to what a row sees, and not to pages that it does not, 597.
 #include "cache_attention.hiph"
 
 namespace mnb {

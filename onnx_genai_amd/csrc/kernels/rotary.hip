@@ -164,7 +164,7 @@ extern "C" int rocm_launch_rotary(const RocmRotaryArgs* args, rocm_stream_t stre
         plan.extra = static_cast<int>((args->extra + 7) / 8);
     }
     // A row to a workgroup once there are eight rows for each CU, as many as run on it at once; before that a row's heads are dealt out, and its angles repeated for each part. (777 rows of
-    // 64 heads of 80: 8.1 us, with a row to a workgroup 8.7.)
+    // 64 heads of 80: 8.1 us with three workgroups a row, some of which run in a second round, with one a row 8.7; two were not timed.)
     const int64_t most = 8 * static_cast<int64_t>(rocm_ffi_compute_units());
     int64_t parts = args->rows >= most ? 1 : (most + args->rows - 1) / args->rows;
     if (parts > args->heads) parts = args->heads;
